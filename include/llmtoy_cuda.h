@@ -548,6 +548,125 @@ lt_status lt_sample_step(lt_ctx *ctx, const float *dev_logits, uint32_t n, const
 /* DefaultPrng.init(seed): the four xoshiro256++ words from SplitMix64 (host). */
 void lt_rng_seed(uint64_t seed, uint64_t state_out[4]);
 
+/* ── batched serving over a paged cache ──────────────────────────────────────
+ * No counterpart in the reference, which decodes one sequence over a
+ * contiguous cache: many sequences share one pool of pages per layer.
+ * Position j of sequence s is slot j % page_size of page
+ * page_table[s][j / page_size]; pages may be shared between sequences (a
+ * common prefix) as long as nobody appends to or evicts from them.  The
+ * tables, lengths and positions are device arrays, so one captured graph
+ * serves every step; max_len / max_q are host bounds on them (they size scratch
+ * and grids).  Scratch comes from the context arena: run an op once with the
+ * largest sizes before capturing it.
+ *
+ * A page id >= n_pages, a length past max_len or past the table, a query range
+ * outside total_q / max_q is reported by lt_sync as LT_EINVAL; nothing outside
+ * the given buffers is read or written, the results concerned are unspecified.
+ * Page-table entries past a sequence's length are never read; cache slots past
+ * it, or outside every query's window, may hold anything, infinities and NaN
+ * included.  K and V of visible positions must be finite. */
+typedef struct lt_paged_kv {
+    uint32_t n_kv_heads, head_dim;  /* head_dim 64, 128 or 256 */
+    uint32_t kv_f16;                /* 1: IEEE f16 elements, 0: f32 */
+    uint32_t page_size;             /* slots per page, any number >= 1 */
+    uint32_t n_pages;               /* pages in the pool */
+    uint32_t max_pages;             /* entries per page-table row */
+    /* Elements between pages, slots and KV heads; each row of head_dim values
+     * is contiguous.  All 0: [page][slot][head][head_dim].  In bytes each must
+     * be a multiple of 16, as must the pool addresses. */
+    uint64_t page_stride, slot_stride, head_stride;
+    void *dev_k, *dev_v;
+} lt_paged_kv;
+
+/* lt_attn_prep for ntok tokens of any sequences: dev_qkv[ntok][nq + 2 nkv] is
+ * only read; the queries (normalised, rotated to dev_pos[t]) go to
+ * dev_q[ntok][nq], K and V of token t to position dev_slot[t] (NULL:
+ * dev_pos[t]) of sequence dev_seq[t] < n_seq.  Two tokens of one call must not
+ * share a slot.  Of cfg the head counts, rope_*, eps and v_norm are used; the
+ * counts and head_dim must agree with kv's. */
+lt_status lt_paged_append(lt_ctx *ctx, const lt_attn_cfg *cfg, const lt_paged_kv *kv, const float *dev_qkv,
+                          uint32_t ntok, const float *dev_q_norm, const float *dev_k_norm, const uint32_t *dev_seq,
+                          const uint32_t *dev_pos, const uint32_t *dev_slot, const uint32_t *dev_page_table,
+                          uint32_t n_seq, float *dev_q);
+
+/* Attention over a paged cache.  The score of the query at position i and the
+ * key at position j of one head is
+ *   s = scale * q.k;  s = softcap * tanh(s / softcap)  (softcap != 0)
+ *   s = s - slope[head] * |i - j|                      (dev_slopes given)
+ * and the softmax runs over the keys that the query sees:
+ *   decode: j < len, and i - j < window (window != 0), with i = len - 1;
+ *   prompt: also j <= i or j < prefix[s] (causal != 0), with i = len - n + r for
+ *           row r of the sequence's n, and docs[s][j] == docs[s][i]
+ *           (docs given).
+ * A query that sees no key gives zeros.  After lt_kv_evict, positions are slots
+ * of what was kept: distances and windows count those. */
+typedef struct lt_paged_attn_cfg {
+    uint32_t n_heads;               /* query head h reads KV head h / (n_heads / n_kv_heads) */
+    uint32_t window;                /* 0: none */
+    uint32_t causal;                /* prompt only */
+    float scale, softcap;           /* softcap 0: none */
+    const float *dev_slopes;        /* [n_heads] or NULL */
+    uint64_t q_stride, out_stride;  /* floats between rows of q and out; 0: n_heads * head_dim */
+} lt_paged_attn_cfg;
+
+/* One query per sequence: dev_out[s] over the dev_lens[s] cached positions.
+ * dev_mass (nullable) [n_seq][n_kv_heads][mass_stride]: += the sum of the
+ * normalised weights of the KV head's query heads, for every position seen (what
+ * lt_kv_evict ranks by). */
+lt_status lt_paged_attn_decode(lt_ctx *ctx, const lt_paged_attn_cfg *cfg, const lt_paged_kv *kv, const float *dev_q,
+                               uint32_t n_seq, const uint32_t *dev_page_table, const uint32_t *dev_lens,
+                               uint32_t max_len, float *dev_mass, uint64_t mass_stride, float *dev_out);
+
+/* Several queries per sequence: rows dev_cu_q[s] .. dev_cu_q[s + 1] - 1 of
+ * dev_q and dev_out belong to sequence s, are its last positions and are
+ * already cached (lt_paged_append).  dev_cu_q has n_seq + 1 ascending entries up
+ * to total_q; at most max_q rows per sequence.  dev_prefix (nullable) [n_seq];
+ * dev_docs (nullable) [n_seq][doc_stride]: a number per cached position. */
+lt_status lt_paged_attn_prompt(lt_ctx *ctx, const lt_paged_attn_cfg *cfg, const lt_paged_kv *kv, const float *dev_q,
+                               uint32_t n_seq, const uint32_t *dev_cu_q, uint32_t total_q, uint32_t max_q,
+                               const uint32_t *dev_page_table, const uint32_t *dev_lens, uint32_t max_len,
+                               const uint32_t *dev_prefix, const uint32_t *dev_docs, uint64_t doc_stride,
+                               float *dev_out);
+
+/* Eviction by accumulated attention weight.  A sequence of more than budget
+ * positions keeps, per KV head, its newest `recent` and of the others the
+ * budget - recent with the largest dev_mass (the lowest position first among
+ * equals; NaN counts as the largest), in their order; K, V and mass of the i-th
+ * kept position move to slot i.  A shorter sequence keeps everything.
+ *   dev_dst_table NULL or dev_page_table: within the sequence's own pages (they
+ *   must not be shared); else into these pages ([n_seq][max_pages], none of
+ *   them a source page), and the old pages stay as they are.
+ * Outputs: dev_lens_out[n_seq] (may be dev_lens), dev_mass_out[n_seq][n_kv]
+ * [mass_out_stride] (may be dev_mass with its stride; slots past the kept ones
+ * are not written), dev_kept (nullable) [n_seq][n_kv][budget] the kept
+ * positions. */
+lt_status lt_kv_evict(lt_ctx *ctx, const lt_paged_kv *kv, uint32_t n_seq, const uint32_t *dev_page_table,
+                      const uint32_t *dev_lens, uint32_t max_len, const float *dev_mass, uint64_t mass_stride,
+                      uint32_t budget, uint32_t recent, const uint32_t *dev_dst_table, uint32_t *dev_lens_out,
+                      float *dev_mass_out, uint64_t mass_out_stride, uint32_t *dev_kept);
+
+/* What a request asks of one row of logits (device array, one per row).
+ * For a token that occurs c > 0 times in the row's history:
+ *   x = (x > 0 ? x / repetition : x * repetition) - (c * frequency + presence)
+ * then x += bias (of a token listed twice the last entry counts), then -inf
+ * where bit token % 32 of word token / 32 of the mask row is clear.  Ids past
+ * the vocabulary are skipped.  A row whose mask leaves nothing is all -inf. */
+#define LT_NO_MASK 0xffffffffu
+typedef struct lt_logit_rule {
+    float repetition, frequency, presence;  /* 1, 0, 0: none */
+    uint32_t history_first, history_len;    /* range of dev_history */
+    uint32_t bias_first, bias_len;          /* range of dev_bias_ids / dev_bias_values */
+    uint32_t mask_row;                      /* row of dev_masks, or LT_NO_MASK */
+} lt_logit_rule;
+
+/* dev_out[row][t] (may be dev_logits) for n_rows rows of n logits; dev_masks has
+ * (n + 31) / 32 words per row.  History, bias and mask arrays may be NULL when
+ * no rule names a range or row of theirs. */
+lt_status lt_logits_process(lt_ctx *ctx, const float *dev_logits, uint32_t n, uint32_t n_rows,
+                            const lt_logit_rule *dev_rules, const uint32_t *dev_history,
+                            const uint32_t *dev_bias_ids, const float *dev_bias_values, const uint32_t *dev_masks,
+                            float *dev_out);
+
 /* ── host-buffer entry points (synchronous) ─────────────────────────────────
  * Same semantics with HOST vectors, copies included: the shape of the
  * reference's own CPU calls, for callers that keep activations on the host. */

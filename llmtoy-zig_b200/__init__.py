@@ -43,7 +43,8 @@ EXPORTS = [
     "lt_sample_step", "lt_rng_seed", "lt_quantize_q8_1", "lt_dequant_q8_1", "lt_moe_block_scaled",
     "lt_qmatvec_multi", "lt_noalloc_status", "lt_selftest_wait",
     "lt_stack_create", "lt_stack_run", "lt_stack_free", "lt_ep_unique_id", "lt_ep_init", "lt_ep_free",
-    "lt_moe_ffn_ep",
+    "lt_moe_ffn_ep", "lt_paged_append", "lt_paged_attn_decode", "lt_paged_attn_prompt", "lt_kv_evict",
+    "lt_logits_process",
 ]
 
 
@@ -71,6 +72,31 @@ class TailIn(ctypes.Structure):
     """lt_ffn_tail_in: the previous Gemma 4 layer's FFN tail, fused into the next attention block."""
     _fields_ = [("f", ctypes.c_void_p), ("w1", ctypes.c_void_p), ("m", ctypes.c_void_p), ("w2", ctypes.c_void_p),
                 ("w", ctypes.c_void_p), ("los", ctypes.c_float), ("eps", ctypes.c_float)]
+
+
+class PagedKV(ctypes.Structure):
+    """lt_paged_kv: one layer's pool of cache pages (strides in elements, all 0: contiguous)."""
+    _fields_ = [("n_kv_heads", ctypes.c_uint32), ("head_dim", ctypes.c_uint32), ("kv_f16", ctypes.c_uint32),
+                ("page_size", ctypes.c_uint32), ("n_pages", ctypes.c_uint32), ("max_pages", ctypes.c_uint32),
+                ("page_stride", ctypes.c_uint64), ("slot_stride", ctypes.c_uint64), ("head_stride", ctypes.c_uint64),
+                ("k", ctypes.c_void_p), ("v", ctypes.c_void_p)]
+
+
+class PagedAttnCfg(ctypes.Structure):
+    """lt_paged_attn_cfg: what a score is and which keys a query sees."""
+    _fields_ = [("n_heads", ctypes.c_uint32), ("window", ctypes.c_uint32), ("causal", ctypes.c_uint32),
+                ("scale", ctypes.c_float), ("softcap", ctypes.c_float), ("slopes", ctypes.c_void_p),
+                ("q_stride", ctypes.c_uint64), ("out_stride", ctypes.c_uint64)]
+
+
+class LogitRule(ctypes.Structure):
+    """lt_logit_rule: 32 bytes per row of logits, in device memory."""
+    _fields_ = [("repetition", ctypes.c_float), ("frequency", ctypes.c_float), ("presence", ctypes.c_float),
+                ("history_first", ctypes.c_uint32), ("history_len", ctypes.c_uint32), ("bias_first", ctypes.c_uint32),
+                ("bias_len", ctypes.c_uint32), ("mask_row", ctypes.c_uint32)]
+
+
+NO_MASK = 0xFFFFFFFF  # LogitRule.mask_row of a row without a grammar
 
 
 class SampleParams(ctypes.Structure):
@@ -168,6 +194,13 @@ def load_library() -> ctypes.CDLL:
         "lt_attn_block_split": (I, [P, ctypes.POINTER(AttnCfg), P, P, F, P, P, P, P, P, P, P, P, P, P, P,
                                     ctypes.POINTER(TailIn), P]),
         "lt_prefetch_next": (I, [P, P, P]),
+        "lt_paged_append": (I, [P, ctypes.POINTER(AttnCfg), ctypes.POINTER(PagedKV), P, U32, P, P, P, P, P, P, U32, P]),
+        "lt_paged_attn_decode": (I, [P, ctypes.POINTER(PagedAttnCfg), ctypes.POINTER(PagedKV), P, U32, P, P, U32, P, U64,
+                                     P]),
+        "lt_paged_attn_prompt": (I, [P, ctypes.POINTER(PagedAttnCfg), ctypes.POINTER(PagedKV), P, U32, P, U32, U32, P, P,
+                                     U32, P, P, U64, P]),
+        "lt_kv_evict": (I, [P, ctypes.POINTER(PagedKV), U32, P, P, U32, P, U64, U32, U32, P, P, P, U64, P]),
+        "lt_logits_process": (I, [P, P, U32, U32, P, P, P, P, P, P]),
         "lt_quant_matvec_host": (I, [P, P, P, U32, P, U64, U64]),
         "lt_moe_forward_host": (I, [P, P, P, P, P, I, I, P, P, U32, U32, P, P, P]),
     }
@@ -469,6 +502,40 @@ class Context:
     def greedy_step(self, logits, n: int, tokens, pos, n_prompt) -> None:
         """n_prompt: a device word (the prompt length of the token stream)."""
         self._check(self.lib.lt_greedy_step(self.ptr, _ptr(logits), n, _ptr(tokens), _ptr(pos), _ptr(n_prompt)))
+
+    # -- batched serving over a paged cache ---------------------------------
+    def paged_append(self, cfg: AttnCfg, kv: PagedKV, qkv, ntok: int, q_norm, k_norm, seq, pos, slot, page_table,
+                     n_seq: int, q) -> None:
+        """qkv[ntok][nq + 2 nkv]: rotated queries to q[ntok][nq], K and V into the cache at slot (None: pos) of seq."""
+        self._check(self.lib.lt_paged_append(self.ptr, ctypes.byref(cfg), ctypes.byref(kv), _ptr(qkv), ntok, _ptr(q_norm),
+                                             _ptr(k_norm), _ptr(seq), _ptr(pos), _ptr(slot), _ptr(page_table), n_seq,
+                                             _ptr(q)))
+
+    def paged_attn_decode(self, cfg: PagedAttnCfg, kv: PagedKV, q, n_seq: int, page_table, lens, max_len: int, out,
+                          mass=None, mass_stride: int = 0) -> None:
+        """One query per sequence; mass[n_seq][n_kv][mass_stride] += the attention weights when given."""
+        self._check(self.lib.lt_paged_attn_decode(self.ptr, ctypes.byref(cfg), ctypes.byref(kv), _ptr(q), n_seq,
+                                                  _ptr(page_table), _ptr(lens), max_len, _ptr(mass), mass_stride,
+                                                  _ptr(out)))
+
+    def paged_attn_prompt(self, cfg: PagedAttnCfg, kv: PagedKV, q, n_seq: int, cu_q, total_q: int, max_q: int, page_table,
+                          lens, max_len: int, out, prefix=None, docs=None, doc_stride: int = 0) -> None:
+        """Rows cu_q[s] .. cu_q[s + 1] - 1 of q are the last positions of sequence s."""
+        self._check(self.lib.lt_paged_attn_prompt(self.ptr, ctypes.byref(cfg), ctypes.byref(kv), _ptr(q), n_seq,
+                                                  _ptr(cu_q), total_q, max_q, _ptr(page_table), _ptr(lens), max_len,
+                                                  _ptr(prefix), _ptr(docs), doc_stride, _ptr(out)))
+
+    def kv_evict(self, kv: PagedKV, n_seq: int, page_table, lens, max_len: int, mass, mass_stride: int, budget: int,
+                 recent: int, dst_table, lens_out, mass_out, mass_out_stride: int, kept=None) -> None:
+        """Keep budget positions per KV head, by accumulated weight; dst_table None: within the sequence's pages."""
+        self._check(self.lib.lt_kv_evict(self.ptr, ctypes.byref(kv), n_seq, _ptr(page_table), _ptr(lens), max_len,
+                                         _ptr(mass), mass_stride, budget, recent, _ptr(dst_table), _ptr(lens_out),
+                                         _ptr(mass_out), mass_out_stride, _ptr(kept)))
+
+    def logits_process(self, logits, n: int, n_rows: int, rules, history, bias_ids, bias_values, masks, out) -> None:
+        """Penalties, biases and grammar masks on n_rows rows of logits; rules: n_rows LogitRule on the device."""
+        self._check(self.lib.lt_logits_process(self.ptr, _ptr(logits), n, n_rows, _ptr(rules), _ptr(history),
+                                               _ptr(bias_ids), _ptr(bias_values), _ptr(masks), _ptr(out)))
 
     # -- kernel timing / graph capture -------------------------------------
     def profile(self, on: bool) -> None:

@@ -261,6 +261,30 @@ lt_status launched(lt_ctx *ctx, cudaError_t e, const char *what) {
 
 }  // namespace
 
+int lt::ctx_enter(lt_ctx *ctx) { return enter(ctx); }
+
+int lt::ctx_fail(lt_ctx *ctx, int status, const char *fmt, ...) {
+    if (ctx) {
+        char buf[512];
+        va_list ap;
+        va_start(ap, fmt);
+        vsnprintf(buf, sizeof buf, fmt, ap);
+        va_end(ap);
+        ctx->err = buf;
+    }
+    return status;
+}
+
+int lt::ctx_scratch(lt_ctx *ctx, size_t bytes, uint8_t **out) {
+    const lt_status st = ensure_scratch(ctx, bytes);
+    *out = ctx->scratch;
+    return st;
+}
+
+int lt::ctx_launched(lt_ctx *ctx, cudaError_t e, const char *what) { return launched(ctx, e, what); }
+
+lt::LaunchCfg lt::ctx_cfg(lt_ctx *ctx) { return cfg_of(ctx); }
+
 extern "C" {
 
 int lt_api_version(void) { return LT_API_VERSION; }

@@ -1,0 +1,270 @@
+// lt_evict.cu — eviction from a paged cache by accumulated attention weight.
+//
+// Per sequence of n > budget positions and per KV head: the newest `recent`
+// positions stay, and of the others the budget - recent with the largest
+// accumulated weight (the lowest position first among equals).  What stays keeps
+// its order; its K and V rows and its weights move to slots 0 .. budget - 1.
+//
+// k_evict_select: one CTA per (sequence, KV head).  The weights become
+// order-preserving 32-bit keys; three passes of 11, 11 and 10 bits narrow the
+// budget-th largest key down (histograms in shared memory), and one ordered
+// pass writes what stays: a kept position's slot is the number of larger keys
+// before it plus the equal ones before it, as far as equal ones are taken.
+// k_evict_move: the rows.  Bound: memory.  Into other pages any order will do
+// and every row is its own work.  Within the same pages row i comes from a
+// position >= i, so a CTA that goes up in steps, reading a step before it writes
+// it, never overwrites what a later step reads; 32-byte columns of the rows are
+// independent of each other and give the parallelism.
+#include "lt_paged.cuh"
+
+namespace lt {
+
+constexpr int kSelThreads = 1024;
+constexpr int kSelPer = 4;
+constexpr int kSelBins = 2048;
+constexpr int kMoveThreads = 256;
+constexpr int kMoveRows = 64;
+
+// Ascending with the weight; NaN counts as the largest, -0 as 0.
+LT_DEVINL uint32_t mass_key(float m) {
+    if (m != m) return 0xffffffffu;
+    const uint32_t u = __float_as_uint(m + 0.0f);
+    return (u >> 31) ? ~u : u | 0x80000000u;
+}
+
+// Exclusive sum over the block of one packed value per thread.
+LT_DEVINL uint64_t block_excl(uint64_t v, uint64_t *s_warp, uint64_t *total) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    uint64_t x = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint64_t y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+    }
+    __syncthreads();  // the last call's reads are over
+    if (lane == 31) s_warp[warp] = x;
+    __syncthreads();
+    if (warp == 0) {
+        uint64_t w = s_warp[lane];
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint64_t y = __shfl_up_sync(0xffffffffu, w, o);
+            if (lane >= o) w += y;
+        }
+        s_warp[lane] = w;
+    }
+    __syncthreads();
+    *total = s_warp[31];
+    return x - v + (warp ? s_warp[warp - 1] : 0);
+}
+
+__global__ void __launch_bounds__(kSelThreads) k_evict_select(EvictArgs a) {
+    __shared__ uint32_t s_hist[kSelBins];
+    __shared__ uint64_t s_warp[32];
+    __shared__ uint32_t s_bin, s_left;
+    pdl_launch_dependents();
+    pdl_wait();
+    const uint32_t h = blockIdx.x, s = blockIdx.y, tid = threadIdx.x;
+    const uint64_t pair = (uint64_t)s * a.kv.n_kv + h;
+    uint32_t n = a.lens[s];
+    if (n > a.max_len || (n + a.kv.page_size - 1) / a.kv.page_size > a.kv.max_pages) {
+        if (tid == 0) atomicExch(a.err, DEV_ERR_BAD_INDEX);
+        n = min((uint64_t)a.max_len, (uint64_t)a.kv.max_pages * a.kv.page_size);
+    }
+    const uint32_t keep = min(n, a.budget);
+    const float *mass = a.mass + pair * a.mass_stride;
+    float *mass_out = a.mass_out + pair * a.mass_out_stride;
+    uint32_t *kept = a.kept + pair * a.budget;
+    if (h == 0 && tid == 0) a.new_len[s] = keep;
+    const uint32_t old = n > a.budget ? n - a.recent : 0;  // positions that compete
+    uint32_t want = n > a.budget ? a.budget - a.recent : 0;
+
+    // the want-th largest key among the first `old`, bits from the top
+    uint32_t prefix = 0, done = 0;
+    for (int pass = 0; pass < 3 && want; pass++) {
+        const int bits = pass == 2 ? 10 : 11, shift = 32 - (int)done - bits, bins = 1 << bits;
+        for (int i = tid; i < kSelBins; i += kSelThreads) s_hist[i] = 0;
+        __syncthreads();
+        for (uint32_t j0 = 0; j0 < old; j0 += kSelThreads * 8) {
+            float m[8];
+#pragma unroll
+            for (int u = 0; u < 8; u++) {
+                const uint32_t j = j0 + u * kSelThreads + tid;
+                m[u] = j < old ? mass[j] : 0.0f;
+            }
+#pragma unroll
+            for (int u = 0; u < 8; u++) {
+                const uint32_t k = mass_key(m[u]);
+                if (j0 + u * kSelThreads + tid < old && (done == 0 || k >> (32 - done) == prefix))
+                    atomicAdd(&s_hist[(k >> shift) & (bins - 1)], 1u);
+            }
+        }
+        __syncthreads();
+        // bins from the top: thread t takes bins - 1 - 2 t and the one below
+        const int b0 = bins - 1 - 2 * (int)tid, b1 = b0 - 1;
+        const uint32_t c0 = b0 >= 0 ? s_hist[b0] : 0, c1 = b1 >= 0 ? s_hist[b1] : 0;
+        uint64_t total;
+        const uint32_t before = (uint32_t)block_excl((uint64_t)c0 + c1, s_warp, &total);
+        if (before < want && want <= before + c0) {
+            s_bin = b0;
+            s_left = want - before;
+        } else if (before + c0 < want && want <= before + c0 + c1) {
+            s_bin = b1;
+            s_left = want - before - c0;
+        }
+        __syncthreads();
+        prefix = (prefix << bits) | s_bin;
+        want = s_left;
+        done += bits;
+        __syncthreads();
+    }
+    // want now counts the keys equal to prefix that stay
+    const bool any = n > a.budget && a.budget > a.recent;
+    uint32_t greater = 0, equal = 0;  // so far
+    for (uint32_t j0 = 0; j0 < n; j0 += kSelThreads * kSelPer) {
+        const uint32_t j = j0 + tid * kSelPer;
+        float m[kSelPer];
+        uint32_t gt = 0, eq = 0;  // bit u: element j + u
+#pragma unroll
+        for (int u = 0; u < kSelPer; u++) {
+            m[u] = j + u < n ? mass[j + u] : 0.0f;
+            const uint32_t k = mass_key(m[u]);
+            if (j + u < n) {
+                if (j + u >= old)
+                    gt |= 1u << u;  // newest, or nothing is evicted
+                else if (any && k > prefix)
+                    gt |= 1u << u;
+                else if (any && k == prefix)
+                    eq |= 1u << u;
+            }
+        }
+        uint64_t total;
+        const uint64_t before = block_excl(((uint64_t)__popc(gt) << 32) | __popc(eq), s_warp, &total);
+        uint32_t g = greater + (uint32_t)(before >> 32), e = equal + (uint32_t)before;
+#pragma unroll
+        for (int u = 0; u < kSelPer; u++) {
+            const bool is_eq = eq >> u & 1u;
+            if ((gt >> u & 1u) || (is_eq && e < want)) {
+                const uint32_t to = g + min(e, want);
+                kept[to] = j + u;
+                mass_out[to] = m[u];
+            }
+            g += gt >> u & 1u;
+            e += is_eq;
+        }
+        greater += (uint32_t)(total >> 32);
+        equal += (uint32_t)total;
+    }
+}
+
+// Byte offset of a position of sequence s in the pool; false: a bad page id.
+LT_DEVINL bool evict_offset(const EvictArgs &a, const uint32_t *table, uint32_t s, uint32_t j, uint32_t h, uint64_t &off) {
+    const uint32_t p = j / a.kv.page_size;
+    const uint32_t page = p < a.kv.max_pages ? table[(uint64_t)s * a.kv.max_pages + p] : a.kv.n_pages;
+    if (page >= a.kv.n_pages) {
+        atomicExch(a.err, DEV_ERR_BAD_INDEX);
+        return false;
+    }
+    off = paged_offset(a.kv, page, j, h);
+    return true;
+}
+
+// Into other pages: grid (row steps, n_kv, n_seq); 16 bytes per thread at a time.
+__global__ void __launch_bounds__(kMoveThreads) k_evict_move(EvictArgs a) {
+    __shared__ uint64_t s_from[kMoveRows], s_to[kMoveRows];
+    pdl_launch_dependents();
+    pdl_wait();
+    const uint32_t h = blockIdx.y, s = blockIdx.z, i0 = blockIdx.x * kMoveRows, tid = threadIdx.x;
+    const uint32_t keep = a.new_len[s];
+    if (h == 0 && i0 == 0 && tid == 0) a.lens_out[s] = keep;
+    if (i0 >= keep) return;
+    const uint32_t rows = min((uint32_t)kMoveRows, keep - i0);
+    const uint64_t pair = (uint64_t)s * a.kv.n_kv + h;
+    if (tid < rows) {
+        uint64_t f = ~0ull, t = ~0ull;
+        const bool ok = evict_offset(a, a.table, s, a.kept[pair * a.budget + i0 + tid], h, f) &&
+                        evict_offset(a, a.dst_table, s, i0 + tid, h, t);
+        s_from[tid] = ok ? f : ~0ull;
+        s_to[tid] = t;
+    }
+    __syncthreads();
+    const uint32_t lanes = a.kv.hd * (a.kv.f16 ? 2 : 4) / 16;  // 8 .. 64, a power of two
+    const uint32_t col = tid % lanes * 16, step = kMoveThreads / lanes;
+    for (uint32_t r0 = tid / lanes; r0 < rows; r0 += 4 * step) {
+        uint4 k[4], v[4];
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            const uint32_t r = r0 + u * step;
+            if (r < rows && s_from[r] != ~0ull) {
+                k[u] = *reinterpret_cast<const uint4 *>(a.kv.k + s_from[r] + col);
+                v[u] = *reinterpret_cast<const uint4 *>(a.kv.v + s_from[r] + col);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            const uint32_t r = r0 + u * step;
+            if (r < rows && s_from[r] != ~0ull) {
+                *reinterpret_cast<uint4 *>(a.kv.k + s_to[r] + col) = k[u];
+                *reinterpret_cast<uint4 *>(a.kv.v + s_to[r] + col) = v[u];
+            }
+        }
+    }
+}
+
+// Within the same pages: grid (32-byte columns of K, then of V; n_kv, n_seq).
+__global__ void __launch_bounds__(kMoveThreads) k_evict_move_in_place(EvictArgs a) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const uint32_t h = blockIdx.y, s = blockIdx.z, tid = threadIdx.x;
+    const uint32_t cols = a.kv.hd * (a.kv.f16 ? 2 : 4) / 32;
+    uint8_t *base = blockIdx.x < cols ? a.kv.k : a.kv.v;
+    const uint32_t byte = blockIdx.x % cols * 32 + (tid & 1) * 16;
+    const uint32_t keep = a.new_len[s];
+    if (h == 0 && blockIdx.x == 0 && tid == 0) a.lens_out[s] = keep;
+    const uint32_t *kept = a.kept + ((uint64_t)s * a.kv.n_kv + h) * a.budget;
+    constexpr int U = 4, R = kMoveThreads / 2;
+    for (uint32_t i0 = 0; i0 < keep; i0 += R * U) {
+        uint4 x[U];
+        uint64_t to[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const uint32_t i = i0 + u * R + tid / 2;
+            to[u] = ~0ull;
+            if (i < keep && kept[i] != i) {
+                uint64_t f, t;
+                if (evict_offset(a, a.table, s, kept[i], h, f) && evict_offset(a, a.table, s, i, h, t)) {
+                    x[u] = *reinterpret_cast<const uint4 *>(base + f + byte);
+                    to[u] = t;
+                }
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            if (to[u] != ~0ull) *reinterpret_cast<uint4 *>(base + to[u] + byte) = x[u];
+        __syncthreads();
+    }
+}
+
+size_t evict_scratch(const EvictArgs &a, bool have_kept) {
+    const size_t lens = ((size_t)a.n_seq * 4 + 255) & ~(size_t)255;
+    return lens + (have_kept ? 0 : (size_t)a.n_seq * a.kv.n_kv * a.budget * 4);
+}
+
+cudaError_t launch_evict(const LaunchCfg &c, EvictArgs a, uint8_t *scratch) {
+    a.new_len = (uint32_t *)scratch;
+    if (!a.kept) a.kept = (uint32_t *)(scratch + (((size_t)a.n_seq * 4 + 255) & ~(size_t)255));
+    a.err = c.dev_err;
+    cudaError_t e = launch_k(c, "evict_select", k_evict_select, dim3(a.kv.n_kv, a.n_seq), dim3(kSelThreads), 0, a);
+    if (e != cudaSuccess) return e;
+    if (a.in_place) {
+        const uint32_t cols = a.kv.hd * (a.kv.f16 ? 2 : 4) / 32;
+        return launch_k(c, "evict_move", k_evict_move_in_place, dim3(2 * cols, a.kv.n_kv, a.n_seq), dim3(kMoveThreads),
+                        0, a);
+    }
+    const uint32_t most = min(a.budget, a.max_len);
+    return launch_k(c, "evict_move", k_evict_move, dim3((most + kMoveRows - 1) / kMoveRows, a.kv.n_kv, a.n_seq),
+                    dim3(kMoveThreads), 0, a);
+}
+
+}  // namespace lt

@@ -14,6 +14,14 @@ namespace lt {
 int ctx_device(const lt_ctx *ctx);
 cudaStream_t ctx_stream(const lt_ctx *ctx);
 
+// What entry points in other files need of the context: device selection and
+// a cleared error, a failure with its message, the arena and the counters
+// (grown outside capture only), launch settings, a launch's outcome.
+int ctx_enter(lt_ctx *ctx);
+int ctx_fail(lt_ctx *ctx, int status, const char *fmt, ...);
+int ctx_scratch(lt_ctx *ctx, size_t bytes, uint8_t **out);
+int ctx_launched(lt_ctx *ctx, cudaError_t e, const char *what);
+
 // A weight matrix as the kernels see it: GGUF rows at a 16-byte pitch.
 struct DevMat {
     const uint8_t *data;
@@ -71,6 +79,8 @@ struct LaunchCfg {
     Profiler *prof;  // nullptr or disabled: no timing
 };
 
+LaunchCfg ctx_cfg(lt_ctx *ctx);
+
 constexpr int kRouterMaxE = 256;  // experts per router (top-k runs in one warp)
 
 bool type_supported(uint32_t t);
@@ -127,6 +137,79 @@ cudaError_t launch_attn_prep(const LaunchCfg &c, const AttnGeom &g, float *qkv, 
                              const float *k_norm, const uint32_t *pos, void *kc, void *vc);
 cudaError_t launch_attn_decode(const LaunchCfg &c, const AttnGeom &g, const float *q, const void *kc,
                                const void *vc, const uint32_t *pos, float *out, float *part, uint32_t *counters);
+
+// A paged K/V cache (lt_paged.cuh); strides in bytes.
+struct PagedKvDev {
+    uint8_t *k, *v;
+    uint64_t page_stride, slot_stride, head_stride;
+    uint32_t n_kv, hd, f16;
+    uint32_t page_size, n_pages, max_pages;
+};
+
+// Rotated keys, values and queries of ntok tokens into / for a paged cache
+// (lt_paged_append.cu): launch_attn_prep's arithmetic per token.
+struct PagedAppendArgs {
+    PagedKvDev kv;
+    uint32_t n_heads, rope_neox, v_norm, n_seq, ntok;
+    float theta, eps;
+    const float *qkv, *q_norm, *k_norm;
+    const uint32_t *seq, *pos, *slot, *table;
+    float *q;
+    uint32_t heads_per_cta;  // head vectors per CTA, set by the launcher
+    int *err;
+};
+cudaError_t launch_paged_append(const LaunchCfg &c, PagedAppendArgs a);
+
+// Attention over a paged cache (lt_paged_attn.cu): one query per sequence
+// (cu == nullptr) or the queries cu[s] .. cu[s + 1] - 1 of each sequence.
+struct PagedAttnArgs {
+    PagedKvDev kv;
+    uint32_t n_heads, group, n_seq, max_len, max_q, total_q;
+    uint32_t window, causal, doc_stride;
+    float scale, softcap;
+    const float *slopes, *q;
+    uint64_t q_stride, out_stride;  // floats between rows
+    const uint32_t *cu, *table, *lens, *prefix, *docs;
+    float *mass;                    // [n_seq][n_kv][mass_stride] or nullptr
+    uint64_t mass_stride;
+    float *out;
+    // scratch, set by the launcher
+    float *part_o, *part_ml, *unit_ml, *scores;
+    uint32_t *unit_info;
+    uint32_t row_blocks;            // 8-row blocks per (sequence, KV head) at most
+    int *err;
+};
+size_t paged_attn_scratch(const PagedAttnArgs &a, int num_sms);
+cudaError_t launch_paged_attn(const LaunchCfg &c, PagedAttnArgs a, uint8_t *scratch);
+
+// Eviction from a paged cache (lt_evict.cu).
+struct EvictArgs {
+    PagedKvDev kv;
+    uint32_t n_seq, max_len, budget, recent;
+    const uint32_t *table, *lens, *dst_table;
+    const float *mass;
+    uint64_t mass_stride, mass_out_stride;
+    uint32_t *lens_out, *kept;
+    float *mass_out;
+    uint32_t *new_len;              // [n_seq] scratch
+    int in_place;
+    int *err;
+};
+size_t evict_scratch(const EvictArgs &a, bool have_kept);
+cudaError_t launch_evict(const LaunchCfg &c, EvictArgs a, uint8_t *scratch);
+
+// Rules on logits (lt_logits.cu).  The rule struct is lt_logit_rule.
+struct LogitArgs {
+    const float *logits;
+    uint32_t n, n_rows;
+    uint64_t in_stride, out_stride;
+    const void *rules;
+    const uint32_t *history, *bias_ids;
+    const float *bias_values;
+    const uint32_t *masks;
+    float *out;
+};
+cudaError_t launch_logits(const LaunchCfg &c, const LogitArgs &a);
 
 // The attention half of a decoder layer for one token in one persistent
 // kernel (lt_attn_block.cu): out = x + wo . attention(rope(norm(W_qkv .

@@ -1,0 +1,104 @@
+// lt_paged.cuh — what the paged-cache kernels share: the cache descriptor and
+// its addressing, the descriptors of an attention call, warp-level matrix
+// products on two-term operands, and small numeric helpers.
+//
+// A paged cache is one pool of pages for K and one for V.  Page p holds
+// page_size slots; position j of sequence s lives in slot j % page_size of page
+// table[s][j / page_size].  Strides are in bytes here and 64-bit throughout:
+// a pool of long contexts passes 4 GiB.
+#pragma once
+
+#include "lt_launch.cuh"
+
+namespace lt {
+
+// Byte offset of position j of a sequence (its page-table row `row`) for head
+// h, or ~0 when the page id lies outside the pool (the caller reports it).
+LT_DEVINL uint64_t paged_offset(const PagedKvDev &kv, uint32_t page, uint32_t j, uint32_t h) {
+    return (uint64_t)page * kv.page_stride + (uint64_t)(j % kv.page_size) * kv.slot_stride +
+           (uint64_t)h * kv.head_stride;
+}
+
+LT_DEVINL float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// 16-byte asynchronous copy to shared memory; zero-fills when !take (the
+// source is then not read).
+LT_DEVINL void cp_async16(uint32_t dst, const void *src, bool take) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(take ? 16 : 0) : "memory");
+}
+LT_DEVINL void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+LT_DEVINL void cp_async_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// Four 8x8 b16 matrices; lane l gives the address of row l % 8 of matrix l / 8.
+LT_DEVINL void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+LT_DEVINL void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+LT_DEVINL float4 lds128(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(addr)
+                 : "memory");
+    return v;
+}
+
+// C[16x8] += A[16x16] B[16x8], f16 operands, f32 sums.
+LT_DEVINL void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// C[16x8] += A[16x8] B[8x8], tf32 operands, f32 sums.
+LT_DEVINL void mma_tf32(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+LT_DEVINL uint32_t to_tf32(float x) {
+    uint32_t y;
+    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(y) : "f"(x));
+    return y;
+}
+// x = hi + lo with hi and lo in tf32 (11 significant bits each).
+LT_DEVINL void split_tf32(float x, uint32_t &hi, uint32_t &lo) {
+    hi = to_tf32(x);
+    lo = to_tf32(x - __uint_as_float(hi));
+}
+// Two values as packed f16 pairs: hi the nearest f16, lo the rest's nearest.
+LT_DEVINL void split_f16x2(float x, float y, uint32_t &hi, uint32_t &lo) {
+    const __half2 h = __floats2half2_rn(x, y);
+    const float2 f = __half22float2(h);
+    const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
+    hi = *reinterpret_cast<const uint32_t *>(&h);
+    lo = *reinterpret_cast<const uint32_t *>(&l);
+}
+
+// Score of one (query, key) pair in units of log2: the scaled product, capped
+// by cap * tanh(s / cap), minus slope * |distance|.  f is the row's factor on
+// the raw product: scale * log2(e) without a cap, scale / cap with one.
+LT_DEVINL float score_log2(float dot, float f, float cap, float slope, float dist) {
+    constexpr float kLog2e = 1.4426950408889634f;
+    float s = dot * f;
+    if (cap != 0.0f) s = tanhf(s) * (cap * kLog2e);
+    return fmaf(-slope * kLog2e, dist, s);
+}
+
+}  // namespace lt

@@ -1,0 +1,755 @@
+// lt_paged_attn.cu — attention over a paged cache: one new token per sequence,
+// and (prompts over f32 caches, a few tokens) several.
+//
+// For query row r = (token, head) at position i and the visible keys j:
+//   s_j = score(q_r . k_j)  (scale, cap, distance bias: score_log2)
+//   out_r = sum_j 2^(s_j - m) v_j / sum_j 2^(s_j - m),  m = max_j s_j
+// in one pass over the keys with the running maximum m and sum l; rows that see
+// no key give zero.  With `mass`, sum_r of the normalised weights is added to
+// mass[kv head][j].
+//
+// Bound: memory (K and V are read once per 8 query heads of a KV head).
+// - Work is (sequence, KV head, 8 rows) x tiles of the sequence's keys, counted
+//   through one after the other; every CTA takes an equal share of the tiles,
+//   wherever it begins and ends, so lengths may differ as they like.  A unit
+//   that several CTAs share leaves partial (m, l, sum) records, which
+//   k_paged_join adds up in CTA order: the result does not depend on timing.
+// - Each warp owns 16 keys of a tile (8 for f32 caches) and a ring of kStages
+//   such blocks in shared memory, filled by 16-byte asynchronous copies; rows sit
+//   at padded pitches so that matrix loads meet no bank conflict.
+// - The products run on the tensor cores without losing the f32 queries: a row
+//   goes in as two f16 terms (22 bits) in rows r and r + 8 of a 16-row
+//   operand, and so do the softmax weights; the two halves of the accumulator
+//   add up to the f32 product.  f32 caches use tf32 the same way, with K and V
+//   split into two terms as well.  A query row is scaled by a power of two so
+//   that its f16 terms neither overflow nor vanish.
+#include "lt_paged.cuh"
+
+namespace lt {
+
+constexpr int kPaWarps = 4, kPaThreads = kPaWarps * 32, kPaStages = 3, kPaRows = 8;
+constexpr int kMassThreads = 256, kMassKeys = 1024;
+
+template <int HD, bool F16>
+struct PaShape {
+    static constexpr int KB = F16 ? 16 : 8;                 // keys per warp and tile
+    static constexpr int TILE = KB * kPaWarps;
+    static constexpr int ROW = HD * (F16 ? 2 : 4);          // bytes
+    static constexpr int KP = ROW + (F16 ? 16 : 64), VP = ROW + 16;
+    static constexpr int BLOCK = KB * (KP + VP);
+    static constexpr int QSTEPS = F16 ? HD / 16 : HD / 8;   // k-steps of 512-byte operand fragments
+    static constexpr int RING = BLOCK * kPaStages * kPaWarps;
+    static constexpr int QBYTES = QSTEPS * 512;
+    static constexpr int MERGE = 2 * kPaRows * (HD + 2) * 4;
+    static constexpr int UNION = QBYTES > MERGE ? QBYTES : MERGE;
+    static constexpr int SMEM = RING + UNION + 16 * 8 * kPaWarps + 64;
+    static constexpr int CTAS = HD == 256 ? 1 : HD == 128 ? 2 : 3;
+};
+
+// A sequence's share of the work.
+struct PaSeq {
+    uint32_t len, nq, q0;   // cached positions, query tokens, first query row
+    uint32_t lo;            // first position any query sees
+    uint32_t blocks, tiles; // 8-row blocks per KV head, tiles per unit
+};
+
+template <bool PROMPT>
+LT_DEVINL PaSeq pa_seq(const PagedAttnArgs &a, uint32_t s, uint32_t tile, bool report) {
+    PaSeq q;
+    uint32_t n = a.lens[s];
+    const uint64_t cap = min((uint64_t)a.kv.max_pages * a.kv.page_size, (uint64_t)a.max_len);
+    bool bad = n > cap;
+    if (bad) n = (uint32_t)cap;
+    q.len = n;
+    if (PROMPT) {
+        const uint32_t c0 = a.cu[s], c1 = a.cu[s + 1];
+        const bool ok = c0 <= c1 && c1 <= a.total_q && c1 - c0 <= a.max_q;
+        bad |= !ok;
+        q.q0 = ok ? c0 : 0;
+        q.nq = ok ? c1 - c0 : 0;
+        const int64_t lo = (int64_t)n - q.nq - a.window + 1;
+        q.lo = a.window && lo > 0 ? (uint32_t)min(lo, (int64_t)n) : 0;
+        q.blocks = (uint32_t)(((uint64_t)q.nq * a.group + kPaRows - 1) / kPaRows);
+    } else {
+        q.q0 = s;
+        q.nq = 1;
+        q.lo = a.window && n > a.window ? n - a.window : 0;
+        q.blocks = (a.group + kPaRows - 1) / kPaRows;
+    }
+    q.tiles = max(1u, (n - q.lo + tile - 1) / tile);
+    if (bad && report) atomicExch(a.err, DEV_ERR_BAD_INDEX);
+    return q;
+}
+
+// Where a walk through the tiles stands.
+template <bool PROMPT>
+struct PaWalk {
+    uint32_t s, unit, tile;  // unit within the sequence: kv head * blocks + row block
+    PaSeq q;
+    uint32_t kh, rb;
+    uint32_t lo, hi;         // positions that this unit's rows can see
+
+    LT_DEVINL void set_unit(const PagedAttnArgs &a) {
+        kh = q.blocks ? unit / q.blocks : 0;
+        rb = q.blocks ? unit % q.blocks : 0;
+        lo = q.lo;
+        hi = q.len;
+        if (PROMPT) {
+            const uint32_t rows = q.nq * a.group;  // nq <= max_q: checked on the host not to overflow
+            const uint32_t t0 = rb * kPaRows / a.group, t1 = (min(rows, rb * kPaRows + kPaRows) - 1) / a.group;
+            const int64_t i0 = (int64_t)q.len - q.nq + t0, i1 = (int64_t)q.len - q.nq + t1;
+            if (a.causal) {
+                int64_t e = i1 + 1;
+                if (a.prefix) e = max(e, (int64_t)a.prefix[s]);
+                hi = (uint32_t)max((int64_t)0, min(e, (int64_t)q.len));
+            }
+            if (a.window) lo = (uint32_t)max((int64_t)q.lo, i0 - (int64_t)a.window + 1);
+        }
+    }
+    LT_DEVINL uint32_t units(const PagedAttnArgs &a) const { return q.blocks * a.kv.n_kv; }
+    // The next tile; the caller stops at the end of its share, which is never past the last sequence.
+    template <int TILE>
+    LT_DEVINL void next(const PagedAttnArgs &a) {
+        if (++tile < q.tiles) return;
+        tile = 0;
+        if (++unit >= units(a)) {
+            unit = 0;
+            do {
+                if (++s >= a.n_seq) {
+                    q.tiles = 0xffffffffu;
+                    return;
+                }
+                q = pa_seq<PROMPT>(a, s, TILE, false);
+            } while (q.blocks == 0);
+        }
+        set_unit(a);
+    }
+};
+
+// First tile of CTA c of G among T tiles, and the CTA that holds tile f.
+LT_DEVINL uint64_t pa_start(uint64_t T, uint32_t c, uint32_t G) { return T * c / G; }
+LT_DEVINL uint32_t pa_owner(uint64_t T, uint64_t f, uint32_t G) { return (uint32_t)(((f + 1) * G - 1) / T); }
+
+// A unit's place in the records: its first CTA and how many CTAs share it.
+LT_DEVINL uint64_t pa_unit(const PagedAttnArgs &a, uint32_t s, uint32_t kh, uint32_t rb) {
+    return ((uint64_t)s * a.kv.n_kv + kh) * a.row_blocks + rb;
+}
+
+template <int HD, bool F16, bool PROMPT>
+__global__ void __launch_bounds__(kPaThreads, PaShape<HD, F16>::CTAS) k_paged_attn(PagedAttnArgs a) {
+    using S = PaShape<HD, F16>;
+    constexpr int KB = S::KB, TILE = S::TILE, NB = HD / 8;
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ uint64_t s_scan[kPaWarps];
+    __shared__ uint64_t s_rem;
+    __shared__ uint32_t s_seq;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, j4 = lane & 3;
+    uint8_t *ring = smem + warp * (S::BLOCK * kPaStages);
+    uint8_t *qm = smem + S::RING;  // query fragments, then the merge records
+    uint64_t *offs = reinterpret_cast<uint64_t *>(smem + S::RING + S::UNION) + warp * 16;
+    float *rowf = reinterpret_cast<float *>(smem + S::RING + S::UNION + 16 * 8 * kPaWarps);
+    const uint32_t ring_u = smem_u32(ring), qm_u = smem_u32(qm);
+    const uint32_t c = blockIdx.x;
+    pdl_launch_dependents();
+    pdl_wait();
+
+    // the tiles of all sequences, and where this CTA's share begins
+    const uint32_t per = (a.n_seq + kPaThreads - 1) / kPaThreads;
+    const uint32_t sa = min(a.n_seq, tid * per), sb = min(a.n_seq, sa + per);
+    uint64_t mine = 0;
+#pragma unroll 4
+    for (uint32_t s = sa; s < sb; s++) {
+        const PaSeq q = pa_seq<PROMPT>(a, s, TILE, c == 0);
+        mine += (uint64_t)q.blocks * a.kv.n_kv * q.tiles;
+    }
+    uint64_t incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint64_t y = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += y;
+    }
+    if (lane == 31) s_scan[warp] = incl;
+    __syncthreads();
+    uint64_t T = 0, before = incl - mine;
+#pragma unroll
+    for (int w = 0; w < kPaWarps; w++) {
+        if (w < warp) before += s_scan[w];
+        T += s_scan[w];
+    }
+    // no more CTAs than tiles, so that every CTA of a unit leaves a record
+    const uint32_t G = (uint32_t)min((uint64_t)gridDim.x, T);
+    if (c >= G) return;
+    const uint64_t f0 = pa_start(T, c, G), f1 = pa_start(T, c + 1, G);
+    if (f0 >= before && f0 < before + mine) {
+        uint64_t rem = f0 - before;
+        for (uint32_t s = sa; s < sb; s++) {
+            const PaSeq q = pa_seq<PROMPT>(a, s, TILE, false);
+            const uint64_t w = (uint64_t)q.blocks * a.kv.n_kv * q.tiles;
+            if (rem < w) {
+                s_seq = s;
+                s_rem = rem;
+                break;
+            }
+            rem -= w;
+        }
+    }
+    __syncthreads();
+    PaWalk<PROMPT> cw, lw;  // the compute walk and the copies ahead of it
+    cw.s = s_seq;
+    cw.q = pa_seq<PROMPT>(a, cw.s, TILE, false);
+    cw.unit = (uint32_t)(s_rem / cw.q.tiles);
+    cw.tile = (uint32_t)(s_rem % cw.q.tiles);
+    cw.set_unit(a);
+    lw = cw;
+
+    // lane r < KB looks up row r of the block to copy next
+    uint32_t page = 0, key = 0;
+    bool take = false;
+    auto look = [&]() {
+        key = lw.q.lo + lw.tile * TILE + warp * KB + lane;
+        take = lane < KB && key < lw.hi && key >= lw.lo;
+        if (take) {
+            page = a.table[(uint64_t)lw.s * a.kv.max_pages + key / a.kv.page_size];
+        }
+    };
+    auto copy = [&](int stage) {
+        if (take && page >= a.kv.n_pages) {
+            take = false;
+            atomicExch(a.err, DEV_ERR_BAD_INDEX);
+        }
+        __syncwarp();
+        if (lane < KB) offs[lane] = take ? paged_offset(a.kv, page, key, lw.kh) : ~0ull;
+        __syncwarp();
+        constexpr int CH = S::ROW / 16, STEP = 32 / (CH < 32 ? CH : 32);
+        const uint32_t kdst = ring_u + stage * S::BLOCK, vdst = kdst + KB * S::KP;
+#pragma unroll
+        for (int r0 = 0; r0 < KB; r0 += STEP) {
+            const int r = r0 + (CH < 32 ? lane / CH : 0);
+            const uint64_t o = offs[r];
+            const bool t = o != ~0ull;
+#pragma unroll
+            for (int x0 = 0; x0 < CH; x0 += 32) {
+                const int x = x0 + (CH < 32 ? lane % CH : lane);
+                const uint64_t src = t ? o + x * 16 : 0;
+                cp_async16(kdst + r * S::KP + x * 16, a.kv.k + src, t);
+                cp_async16(vdst + r * S::VP + x * 16, a.kv.v + src, t);
+            }
+        }
+    };
+    const uint64_t nf = f1 - f0;
+    uint64_t ahead = 0;
+    look();
+#pragma unroll
+    for (int st = 0; st < kPaStages - 1; st++) {
+        if (ahead < nf) {
+            copy(st);
+            ahead++;
+            if (ahead < nf) {
+                lw.template next<TILE>(a);
+                look();
+            }
+        }
+        cp_async_commit();
+    }
+
+    uint64_t f = f0;
+    int stage = 0;
+    while (f < f1) {
+        // ── one segment: this CTA's tiles of one unit ──
+        const uint64_t left = cw.q.tiles - cw.tile;
+        const uint32_t seg = (uint32_t)min(left, f1 - f);
+        const uint64_t unit_f0 = f - cw.tile;
+        const uint32_t rows = min((uint32_t)kPaRows, cw.q.nq * a.group - cw.rb * kPaRows);
+        // queries to operand fragments: warp w takes rows 2 w and 2 w + 1
+#pragma unroll
+        for (int rr = 0; rr < 2; rr++) {
+            const uint32_t r = warp * 2 + rr;
+            float v[HD / 32];
+            const uint32_t R = cw.rb * kPaRows + r;
+            const float *src = a.q + (uint64_t)(cw.q.q0 + R / a.group) * a.q_stride + (uint64_t)(cw.kh * a.group + R % a.group) * HD;
+            float top = 0.0f;
+#pragma unroll
+            for (int e = 0; e < HD / 64; e++) {
+                const float2 t = r < rows ? *reinterpret_cast<const float2 *>(src + 64 * e + 2 * lane) : make_float2(0.0f, 0.0f);
+                v[2 * e] = t.x;
+                v[2 * e + 1] = t.y;
+                top = fmaxf(top, fmaxf(fabsf(t.x), fabsf(t.y)));
+            }
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            // the largest element lands in [2^8, 2^9)
+            float up = 1.0f;
+            if (F16 && top > 0.0f && top < INFINITY) {
+                const int ex = min(max(8 - (int)(__float_as_uint(top) >> 23) + 127, -126), 126);
+                up = __uint_as_float((uint32_t)(ex + 127) << 23);
+            }
+            if (lane == 0) rowf[r] = (a.softcap != 0.0f ? a.scale / a.softcap : a.scale * 1.4426950408889634f) / up;
+#pragma unroll
+            for (int e = 0; e < HD / 64; e++) {
+                const uint32_t k = 64 * e + 2 * lane;
+                if (F16) {
+                    uint32_t hi, lo;
+                    split_f16x2(v[2 * e] * up, v[2 * e + 1] * up, hi, lo);
+                    const uint32_t at = (k / 16) * 512 + (r * 4 + (k % 8) / 2) * 16 + ((k % 16) / 8) * 8;
+                    *reinterpret_cast<uint2 *>(qm + at) = make_uint2(hi, lo);
+                } else {
+                    // element 16 i + 4 j + c: fragment 2 i + c / 2, lane 4 r + j, registers 2 (c % 2) and + 1
+#pragma unroll
+                    for (int d = 0; d < 2; d++) {
+                        uint32_t hi, lo;
+                        split_tf32(v[2 * e + d], hi, lo);
+                        const uint32_t kk = k + d, cc = kk % 4;
+                        const uint32_t at = (2 * (kk / 16) + cc / 2) * 512 + (r * 4 + (kk % 16) / 4) * 16 + (cc & 1) * 8;
+                        *reinterpret_cast<uint2 *>(qm + at) = make_uint2(hi, lo);
+                    }
+                }
+            }
+        }
+        __syncthreads();
+        constexpr bool QREG = F16 && HD <= 128;
+        uint32_t qf[QREG ? S::QSTEPS : 1][4];
+        if constexpr (QREG) {
+#pragma unroll
+            for (int i = 0; i < S::QSTEPS; i++) {
+                const float4 t = lds128(qm_u + i * 512 + lane * 16);
+                qf[i][0] = __float_as_uint(t.x), qf[i][1] = __float_as_uint(t.y);
+                qf[i][2] = __float_as_uint(t.z), qf[i][3] = __float_as_uint(t.w);
+            }
+        }
+        // this thread's row g: factor, bias slope, what it sees
+        const uint32_t R = cw.rb * kPaRows + g;
+        const float rf = rowf[g];
+        const uint32_t head = cw.kh * a.group + R % a.group;
+        const float slope = a.slopes && (uint32_t)g < rows ? a.slopes[head] : 0.0f;
+        int64_t row_i = (int64_t)cw.q.len - cw.q.nq + R / a.group;
+        int64_t row_lo = cw.q.lo, row_hi = cw.q.len;
+        uint32_t my_doc = 0;
+        const uint32_t *docs = nullptr;
+        if (PROMPT) {
+            if (a.causal) {
+                row_hi = row_i + 1;
+                if (a.prefix) row_hi = max(row_hi, (int64_t)a.prefix[cw.s]);
+                row_hi = min(row_hi, (int64_t)cw.q.len);
+            }
+            row_lo = a.window ? row_i - (int64_t)a.window + 1 : 0;
+            if (a.docs) {
+                docs = a.docs + (uint64_t)cw.s * a.doc_stride;
+                if ((uint32_t)g < rows && row_i >= 0)
+                    my_doc = docs[row_i];
+                else
+                    row_hi = 0;
+            }
+        }
+        float o[NB][4];
+#pragma unroll
+        for (int n = 0; n < NB; n++) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
+        float m = -INFINITY, l = 0.0f;
+
+        for (uint32_t it = 0; it < seg; it++) {
+            cp_async_wait<kPaStages - 2>();
+            __syncwarp();
+            const uint32_t k0 = cw.q.lo + cw.tile * TILE + warp * KB;  // the block's first position
+            if (k0 < cw.hi && k0 + KB > cw.lo) {
+                const uint32_t kb = ring_u + stage * S::BLOCK, vb = kb + KB * S::KP;
+                constexpr int NS = KB / 4;  // scores per thread: keys k0 + 8 (n / 2) + 2 j4 + n % 2
+                float sc[NS];
+                if constexpr (F16) {
+                    float s0[4] = {}, s1[4] = {};
+                    const uint32_t ka = kb + ((lane >> 4) * 8 + (lane & 7)) * S::KP + ((lane >> 3) & 1) * 16;
+#pragma unroll
+                    for (int i = 0; i < S::QSTEPS; i++) {
+                        uint32_t b[4];
+                        ldsm4(b, ka + i * 32);
+                        uint32_t qa[4];
+                        if constexpr (QREG) {
+                            qa[0] = qf[i][0], qa[1] = qf[i][1], qa[2] = qf[i][2], qa[3] = qf[i][3];
+                        } else {
+                            const float4 t = lds128(qm_u + i * 512 + lane * 16);
+                            qa[0] = __float_as_uint(t.x), qa[1] = __float_as_uint(t.y);
+                            qa[2] = __float_as_uint(t.z), qa[3] = __float_as_uint(t.w);
+                        }
+                        mma_f16(s0, qa, b[0], b[1]);
+                        mma_f16(s1, qa, b[2], b[3]);
+                    }
+                    sc[0] = s0[0] + s0[2];
+                    sc[1] = s0[1] + s0[3];
+                    sc[2] = s1[0] + s1[2];
+                    sc[3] = s1[1] + s1[3];
+                } else {
+                    float s0[4] = {}, s1[4] = {};
+                    const uint32_t ka = kb + g * S::KP + j4 * 16;
+#pragma unroll 4
+                    for (int i = 0; i < HD / 16; i++) {
+                        const float4 t = lds128(ka + i * 64);
+                        const float kv4[4] = {t.x, t.y, t.z, t.w};
+                        uint32_t bh[4], bl[4];
+#pragma unroll
+                        for (int e = 0; e < 4; e++) split_tf32(kv4[e], bh[e], bl[e]);
+#pragma unroll
+                        for (int e = 0; e < 2; e++) {
+                            const float4 u = lds128(qm_u + (2 * i + e) * 512 + lane * 16);
+                            const uint32_t qa[4] = {__float_as_uint(u.x), __float_as_uint(u.y), __float_as_uint(u.z),
+                                                    __float_as_uint(u.w)};
+                            mma_tf32(s0, qa, bh[2 * e], bh[2 * e + 1]);
+                            mma_tf32(s1, qa, bl[2 * e], bl[2 * e + 1]);
+                        }
+                    }
+                    sc[0] = (s0[0] + s1[0]) + (s0[2] + s1[2]);
+                    sc[1] = (s0[1] + s1[1]) + (s0[3] + s1[3]);
+                }
+                float top = -INFINITY;
+#pragma unroll
+                for (int n = 0; n < NS; n++) {
+                    const uint32_t j = k0 + 8 * (n / 2) + 2 * j4 + (n & 1);
+                    sc[n] = score_log2(sc[n], rf, a.softcap, slope, fabsf((float)(row_i - (int64_t)j)));
+                    bool seen;
+                    if (PROMPT) {
+                        seen = (int64_t)j >= row_lo && (int64_t)j < row_hi;
+                        if (docs && seen) seen = docs[j] == my_doc;
+                    } else {
+                        seen = j < cw.q.len;
+                        if (a.mass && seen && (uint32_t)g < rows)
+                            a.scores[((uint64_t)cw.s * a.n_heads + head) * a.max_len + j] = sc[n];
+                    }
+                    if (!seen) sc[n] = -INFINITY;
+                    top = fmaxf(top, sc[n]);
+                }
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                const float mn = fmaxf(m, top);
+                if (__any_sync(0xffffffffu, mn > m)) {
+                    const float al = mn > m ? ex2(m - mn) : 1.0f;  // m = -inf: 0
+                    l *= al;
+#pragma unroll
+                    for (int n = 0; n < NB; n++) {
+                        o[n][0] *= al;
+                        o[n][1] *= al;
+                        o[n][2] *= al;
+                        o[n][3] *= al;
+                    }
+                    m = mn;
+                }
+                // weights scaled by 2^10 so that small ones keep their f16 bits; l carries the same factor
+                const float base = m == -INFINITY ? 0.0f : m - (F16 ? 10.0f : 0.0f);
+#pragma unroll
+                for (int n = 0; n < NS; n++) {
+                    sc[n] = ex2(sc[n] - base);
+                    l += sc[n];
+                }
+                if constexpr (F16) {
+                    uint32_t pa[4];
+                    split_f16x2(sc[0], sc[1], pa[0], pa[1]);
+                    split_f16x2(sc[2], sc[3], pa[2], pa[3]);
+                    const uint32_t va = vb + (((lane >> 3) & 1) * 8 + (lane & 7)) * S::VP + (lane >> 4) * 16;
+#pragma unroll
+                    for (int n = 0; n < NB; n += 2) {
+                        uint32_t b[4];
+                        ldsm4_t(b, va + n * 16);
+                        mma_f16(o[n], pa, b[0], b[1]);
+                        mma_f16(o[n + 1], pa, b[2], b[3]);
+                    }
+                } else {
+                    // operand index j4 is key 2 j4, index j4 + 4 key 2 j4 + 1; column g of product c is dim 32 i + 4 g + c
+                    uint32_t pa[4];
+                    split_tf32(sc[0], pa[0], pa[1]);
+                    split_tf32(sc[1], pa[2], pa[3]);
+                    const uint32_t va = vb + 2 * j4 * S::VP + g * 16;
+#pragma unroll
+                    for (int i = 0; i < HD / 32; i++) {
+                        const float4 t0 = lds128(va + i * 128), t1 = lds128(va + S::VP + i * 128);
+                        const float x0[4] = {t0.x, t0.y, t0.z, t0.w}, x1[4] = {t1.x, t1.y, t1.z, t1.w};
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            uint32_t h0, l0, h1, l1;
+                            split_tf32(x0[e], h0, l0);
+                            split_tf32(x1[e], h1, l1);
+                            mma_tf32(o[4 * i + e], pa, h0, h1);
+                            mma_tf32(o[4 * i + e], pa, l0, l1);
+                        }
+                    }
+                }
+            }
+            __syncwarp();
+            int fill = stage + kPaStages - 1;
+            if (fill >= kPaStages) fill -= kPaStages;
+            if (ahead < nf) {
+                copy(fill);
+                ahead++;
+                if (ahead < nf) {
+                    lw.template next<TILE>(a);
+                    look();
+                }
+            }
+            cp_async_commit();
+            if (++stage == kPaStages) stage = 0;
+            if (it + 1 < seg) cw.tile++;
+        }
+
+        // ── merge the warps: 2 and 3 into 0 and 1, then 1 into 0 ──
+        l += __shfl_xor_sync(0xffffffffu, l, 1);
+        l += __shfl_xor_sync(0xffffffffu, l, 2);
+#pragma unroll
+        for (int n = 0; n < NB; n++) {
+            o[n][0] += o[n][2];
+            o[n][1] += o[n][3];
+        }
+        auto dim = [&](int n, int e) { return F16 ? 8 * n + 2 * j4 + e : 32 * (n / 4) + 8 * j4 + 4 * e + n % 4; };
+        __syncthreads();  // every warp is done with the query fragments
+#pragma unroll
+        for (int half = kPaWarps / 2; half >= 1; half /= 2) {
+            float *rec = reinterpret_cast<float *>(qm) + (warp % half) * kPaRows * (HD + 2) + g * (HD + 2);
+            if (warp >= half && warp < 2 * half) {
+#pragma unroll
+                for (int n = 0; n < NB; n++) {
+                    rec[dim(n, 0)] = o[n][0];
+                    rec[dim(n, 1)] = o[n][1];
+                }
+                if (j4 == 0) {
+                    rec[HD] = m;
+                    rec[HD + 1] = l;
+                }
+            }
+            __syncthreads();
+            if (warp < half) {
+                const float m2 = rec[HD], mn = fmaxf(m, m2);
+                const float w1 = m == -INFINITY ? 0.0f : ex2(m - mn), w2 = m2 == -INFINITY ? 0.0f : ex2(m2 - mn);
+                l = l * w1 + rec[HD + 1] * w2;
+#pragma unroll
+                for (int n = 0; n < NB; n++) {
+                    o[n][0] = o[n][0] * w1 + rec[dim(n, 0)] * w2;
+                    o[n][1] = o[n][1] * w1 + rec[dim(n, 1)] * w2;
+                }
+                m = mn;
+            }
+            __syncthreads();
+        }
+        if (warp == 0) {
+            const uint32_t first = pa_owner(T, unit_f0, G), last = pa_owner(T, unit_f0 + cw.q.tiles - 1, G);
+            const uint64_t u = pa_unit(a, cw.s, cw.kh, cw.rb);
+            if (unit_f0 == f && lane == 0) {
+                a.unit_info[2 * u] = first;
+                a.unit_info[2 * u + 1] = last - first + 1;
+            }
+            if (first == last) {
+                const float inv = l > 0.0f ? __fdiv_rn(1.0f, l) : (l == 0.0f ? 0.0f : l);
+                if ((uint32_t)g < rows) {
+                    float *dst = a.out + (uint64_t)(cw.q.q0 + R / a.group) * a.out_stride + (uint64_t)head * HD;
+#pragma unroll
+                    for (int n = 0; n < NB; n++) {
+                        dst[dim(n, 0)] = o[n][0] * inv;
+                        dst[dim(n, 1)] = o[n][1] * inv;
+                    }
+                }
+                if (!PROMPT && a.mass && j4 == 0) {
+                    a.unit_ml[u * 16 + g] = m;
+                    a.unit_ml[u * 16 + 8 + g] = l;
+                }
+            } else {
+                const uint64_t p = 2 * (uint64_t)c + (unit_f0 == f ? 1 : 0);
+                float *dst = a.part_o + (p * kPaRows + g) * HD;
+#pragma unroll
+                for (int n = 0; n < NB; n++) {
+                    dst[dim(n, 0)] = o[n][0];
+                    dst[dim(n, 1)] = o[n][1];
+                }
+                if (j4 == 0) {
+                    a.part_ml[p * 16 + g] = m;
+                    a.part_ml[p * 16 + 8 + g] = l;
+                }
+            }
+        }
+        __syncthreads();  // the merge records are read before the next queries overwrite them
+        f += seg;
+        if (f < f1) cw.template next<TILE>(a);
+    }
+    cp_async_wait<0>();
+}
+
+// Partial p of a unit whose first CTA is `first`: that CTA's second record,
+// the later ones' first.
+LT_DEVINL uint64_t pa_part(uint32_t first, uint32_t p) { return 2 * (uint64_t)(first + p) + (p == 0 ? 1 : 0); }
+
+// Units that several CTAs share: grid (units, rows), one row per CTA.
+template <int HD, bool PROMPT>
+__global__ void __launch_bounds__(128) k_paged_join(PagedAttnArgs a) {
+    constexpr int LANES = HD / 4, GROUPS = 128 / LANES;
+    __shared__ float s_red[4], s_red2[4];
+    __shared__ float4 s_o[128];
+    pdl_launch_dependents();
+    pdl_wait();
+    const uint64_t u = blockIdx.x;
+    const uint32_t r = blockIdx.y, rb = (uint32_t)(u % a.row_blocks);
+    const uint32_t kh = (uint32_t)(u / a.row_blocks % a.kv.n_kv), s = (uint32_t)(u / a.row_blocks / a.kv.n_kv);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    uint32_t nq = 1, q0 = s;
+    if (PROMPT) {
+        const uint32_t c0 = a.cu[s], c1 = a.cu[s + 1];
+        if (!(c0 <= c1 && c1 <= a.total_q && c1 - c0 <= a.max_q)) return;
+        q0 = c0;
+        nq = c1 - c0;
+    }
+    const uint32_t R = rb * kPaRows + r;
+    if (R >= nq * a.group) return;
+    const uint32_t first = a.unit_info[2 * u], n = a.unit_info[2 * u + 1];
+    if (n < 2) return;
+    float m = -INFINITY;
+    for (uint32_t p = tid; p < n; p += 128) m = fmaxf(m, a.part_ml[pa_part(first, p) * 16 + r]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if (lane == 0) s_red[warp] = m;
+    __syncthreads();
+    m = fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3]));
+    const float ms = m == -INFINITY ? 0.0f : m;
+    float l = 0.0f;
+    for (uint32_t p = tid; p < n; p += 128) {
+        const float *ml = a.part_ml + pa_part(first, p) * 16 + r;
+        l += ml[8] * ex2(ml[0] - ms);
+    }
+    l = warp_sum(l);
+    if (lane == 0) s_red2[warp] = l;
+    const int grp = tid / LANES, x = tid % LANES;
+    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 8
+    for (uint32_t p = grp; p < n; p += GROUPS) {
+        const uint64_t k = pa_part(first, p);
+        const float w = ex2(a.part_ml[k * 16 + r] - ms);
+        const float4 v = *reinterpret_cast<const float4 *>(a.part_o + (k * kPaRows + r) * HD + 4 * x);
+        acc.x = fmaf(v.x, w, acc.x);
+        acc.y = fmaf(v.y, w, acc.y);
+        acc.z = fmaf(v.z, w, acc.z);
+        acc.w = fmaf(v.w, w, acc.w);
+    }
+    s_o[tid] = acc;
+    __syncthreads();
+    if (grp) return;
+    l = (s_red2[0] + s_red2[1]) + (s_red2[2] + s_red2[3]);
+#pragma unroll
+    for (int i = 1; i < GROUPS; i++) {
+        const float4 v = s_o[i * LANES + x];
+        acc.x += v.x;
+        acc.y += v.y;
+        acc.z += v.z;
+        acc.w += v.w;
+    }
+    const float inv = l > 0.0f ? __fdiv_rn(1.0f, l) : (l == 0.0f ? 0.0f : l);
+    float *dst = a.out + (uint64_t)(q0 + R / a.group) * a.out_stride + (uint64_t)(kh * a.group + R % a.group) * HD + 4 * x;
+    dst[0] = acc.x * inv;
+    dst[1] = acc.y * inv;
+    dst[2] = acc.z * inv;
+    dst[3] = acc.w * inv;
+}
+
+// mass[s][kv head][j] += sum over the KV head's query heads of 2^(score - m) / l.
+// Grid (key steps, n_kv, n_seq); one thread per key, so each cell has one writer.
+__global__ void __launch_bounds__(kMassThreads) k_paged_mass(PagedAttnArgs a) {
+    extern __shared__ float s_ml[];  // [group] maxima, [group] 1 / sum
+    pdl_launch_dependents();
+    pdl_wait();
+    const uint32_t kh = blockIdx.y, s = blockIdx.z, j0 = blockIdx.x * kMassKeys;
+    const PaSeq q = pa_seq<false>(a, s, 1, false);
+    if (j0 >= q.len || j0 + kMassKeys <= q.lo) return;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    for (uint32_t h = warp; h < a.group; h += kMassThreads / 32) {
+        const uint64_t u = pa_unit(a, s, kh, h / kPaRows);
+        const uint32_t r = h % kPaRows, first = a.unit_info[2 * u], n = a.unit_info[2 * u + 1];
+        float m = -INFINITY, l = 0.0f;
+        if (n < 2) {
+            m = a.unit_ml[u * 16 + r];
+            l = a.unit_ml[u * 16 + 8 + r];
+        } else {
+            for (uint32_t p = lane; p < n; p += 32) m = fmaxf(m, a.part_ml[pa_part(first, p) * 16 + r]);
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+            for (uint32_t p = lane; p < n; p += 32) {
+                const float *ml = a.part_ml + pa_part(first, p) * 16 + r;
+                l += ml[8] * ex2(ml[0] - (m == -INFINITY ? 0.0f : m));
+            }
+            l = warp_sum(l);
+        }
+        if (lane == 0) {
+            // the sums carry the weights' factor 2^10 on f16 caches
+            s_ml[h] = m == -INFINITY ? 0.0f : m - (a.kv.f16 ? 10.0f : 0.0f);
+            s_ml[a.group + h] = l > 0.0f ? 1.0f / l : 0.0f;
+        }
+    }
+    __syncthreads();
+    float *mass = a.mass + ((uint64_t)s * a.kv.n_kv + kh) * a.mass_stride;
+    const float *sc = a.scores + ((uint64_t)s * a.n_heads + kh * a.group) * a.max_len;
+    const uint32_t end = min(q.len, j0 + kMassKeys);
+    for (uint32_t j = max(q.lo, j0) + tid; j < end; j += kMassThreads) {
+        float w = 0.0f;
+#pragma unroll 8
+        for (uint32_t h = 0; h < a.group; h++) w = fmaf(ex2(sc[(uint64_t)h * a.max_len + j] - s_ml[h]), s_ml[a.group + h], w);
+        mass[j] += w;
+    }
+}
+
+namespace {
+
+size_t up256(size_t v) { return (v + 255) & ~(size_t)255; }
+
+struct PaScratch {
+    size_t part_o, part_ml, unit_ml, unit_info, scores, total;
+};
+PaScratch pa_layout(const PagedAttnArgs &a, uint32_t G) {
+    const uint64_t rows = (uint64_t)(a.cu ? a.max_q : 1) * a.group;
+    const uint64_t units = (uint64_t)a.n_seq * a.kv.n_kv * ((rows + kPaRows - 1) / kPaRows);
+    PaScratch s;
+    size_t off = 0;
+    auto take = [&](size_t b) {
+        const size_t at = off;
+        off += up256(b);
+        return at;
+    };
+    s.part_o = take((size_t)2 * G * kPaRows * a.kv.hd * 4);
+    s.part_ml = take((size_t)2 * G * 16 * 4);
+    s.unit_info = take(units * 8);
+    s.unit_ml = take(a.mass ? units * 64 : 0);
+    s.scores = take(a.mass ? (size_t)a.n_seq * a.n_heads * a.max_len * 4 : 0);
+    s.total = off;
+    return s;
+}
+
+uint32_t pa_grid(uint32_t hd, int num_sms) { return (uint32_t)num_sms * (hd == 256 ? 1 : hd == 128 ? 2 : 3); }
+
+template <int HD, bool F16, bool PROMPT>
+cudaError_t pa_launch(const LaunchCfg &c, const PagedAttnArgs &a, uint64_t units) {
+    cudaError_t e = launch_k(c, PROMPT ? "paged_attn_rows" : "paged_attn", k_paged_attn<HD, F16, PROMPT>,
+                             dim3(pa_grid(HD, c.num_sms)), dim3(kPaThreads), PaShape<HD, F16>::SMEM, a);
+    if (e != cudaSuccess) return e;
+    e = launch_k(c, "paged_join", k_paged_join<HD, PROMPT>, dim3((uint32_t)units, kPaRows), dim3(128), 0, a);
+    if (e != cudaSuccess || PROMPT || !a.mass) return e;
+    return launch_k(c, "paged_mass", k_paged_mass, dim3((a.max_len + kMassKeys - 1) / kMassKeys, a.kv.n_kv, a.n_seq),
+                    dim3(kMassThreads), 2 * a.group * sizeof(float), a);
+}
+
+template <bool F16, bool PROMPT>
+cudaError_t pa_launch_hd(const LaunchCfg &c, const PagedAttnArgs &a, uint64_t units) {
+    switch (a.kv.hd) {
+    case 64: return pa_launch<64, F16, PROMPT>(c, a, units);
+    case 128: return pa_launch<128, F16, PROMPT>(c, a, units);
+    case 256: return pa_launch<256, F16, PROMPT>(c, a, units);
+    default: return cudaErrorInvalidValue;
+    }
+}
+
+}  // namespace
+
+size_t paged_attn_scratch(const PagedAttnArgs &a, int num_sms) { return pa_layout(a, pa_grid(a.kv.hd, num_sms)).total; }
+
+cudaError_t launch_paged_attn(const LaunchCfg &c, PagedAttnArgs a, uint8_t *scratch) {
+    const PaScratch s = pa_layout(a, pa_grid(a.kv.hd, c.num_sms));
+    a.part_o = (float *)(scratch + s.part_o);
+    a.part_ml = (float *)(scratch + s.part_ml);
+    a.unit_info = (uint32_t *)(scratch + s.unit_info);
+    a.unit_ml = (float *)(scratch + s.unit_ml);
+    a.scores = (float *)(scratch + s.scores);
+    a.err = c.dev_err;
+    const uint64_t rows = (uint64_t)(a.cu ? a.max_q : 1) * a.group;
+    a.row_blocks = (uint32_t)((rows + kPaRows - 1) / kPaRows);
+    const uint64_t units = (uint64_t)a.n_seq * a.kv.n_kv * a.row_blocks;
+    if (a.cu) return a.kv.f16 ? pa_launch_hd<true, true>(c, a, units) : pa_launch_hd<false, true>(c, a, units);
+    return a.kv.f16 ? pa_launch_hd<true, false>(c, a, units) : pa_launch_hd<false, false>(c, a, units);
+}
+
+}  // namespace lt
