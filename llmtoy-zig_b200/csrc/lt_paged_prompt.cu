@@ -13,12 +13,17 @@
 //   warps 0-3, 4-7   softmax of row tile 0 and 1, a thread per row.  head_dim 256:
 //                    both on the one row tile, each half of the keys and of O.
 //   warp 8           issues the MMAs
-//   warps 9-11       bring K and V tiles from their pages (16-byte asynchronous
-//                    copies into 128-byte-swizzled rows) into a ring of stages
+//   warps 9-11       bring K and V tiles from their pages into a ring of stages of
+//                    128-byte-swizzled rows: tiles that lie wholly within the
+//                    sequence by TMA, a box per page and 64 columns; the ragged
+//                    ends, and pages that are no multiple of 8 slots, by 16-byte
+//                    asynchronous copies with zero fill
 // While one tile's softmax runs, the tensor cores work for the other: per tile
 // of keys the MMA order is PV0 QK0' PV1 QK1' (' the next keys).  S and P share
-// their columns of tensor memory; P lies as it is read: per 32 keys 16 columns
-// of high terms, then 16 of low ones, over the 32 columns of S they come from.
+// their columns of tensor memory; P lies as it is read: per 16 keys 8 columns
+// of high terms, then 8 of low ones, over the 16 columns of S they come from.
+#include <cuda.h>  // CUtensorMap (encoded through the runtime's driver entry point)
+
 #include "lt_paged.cuh"
 #include "lt_umma.cuh"
 
@@ -60,6 +65,28 @@ LT_DEVINL void tmem_st32(uint32_t taddr, const uint32_t (&v)[32]) {
         "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
         : "memory");
 }
+LT_DEVINL void tmem_ld16(uint32_t taddr, uint32_t (&v)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+          "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+        : "r"(taddr));
+}
+LT_DEVINL void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(
+            taddr),
+        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+        "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+        : "memory");
+}
+// Wait for this thread's TMEM loads; naming the loaded registers keeps their uses behind the wait.
+template <int N>
+LT_DEVINL void tmem_wait_ld(uint32_t (&v)[N]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < N; i++) asm volatile("" : "+r"(v[i]));
+}
 LT_DEVINL void tmem_st1(uint32_t taddr, float v) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(taddr), "r"(__float_as_uint(v)) : "memory");
 }
@@ -70,18 +97,33 @@ LT_DEVINL float tmem_ld1(uint32_t taddr) {
 }
 LT_DEVINL void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// D[tmem] (+)= A[tmem] * B, issued by one thread; A: 128 lanes, two f16 of K per column.
-LT_DEVINL void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-        " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d_tmem),
-        "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate));
-}
+// MMAs with descriptors as a changing low word and a constant high one, so that
+// the issuing thread adds a constant per product.  High word: see umma_desc_sw128.
+constexpr uint32_t kUmmaDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+LT_DEVINL uint32_t umma_lo(uint32_t saddr) { return ((saddr & 0x3FFFFu) >> 4) | (1u << 16); }
 // Operand whose rows run along K (V: one row of 64 N values per key): 64-wide
 // blocks of N lie `block` bytes apart, groups of 8 keys 1024 bytes.
-LT_DEVINL uint64_t umma_desc_sw128_mn(uint32_t saddr, uint32_t block) {
-    return (uint64_t)((saddr & 0x3FFFFu) >> 4) | ((uint64_t)(block >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
-           ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+LT_DEVINL uint32_t umma_lo_mn(uint32_t saddr, uint32_t block) { return ((saddr & 0x3FFFFu) >> 4) | ((block >> 4) << 16); }
+
+template <bool ACC>
+LT_DEVINL void umma_ss(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t idesc) {
+    asm volatile(
+        "{\n .reg .pred p;\n .reg .b64 a, b;\n setp.ne.b32 p, %5, 0;\n mov.b64 a, {%1, %4};\n mov.b64 b, {%2, %4};\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n}\n" ::"r"(d_tmem),
+        "r"(a_lo), "r"(b_lo), "r"(idesc), "n"(kUmmaDescHi), "n"(ACC ? 1 : 0));
+}
+// A in tensor memory: 128 lanes, two f16 of K per column.
+template <bool ACC>
+LT_DEVINL void umma_ts(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_lo, uint32_t idesc) {
+    asm volatile(
+        "{\n .reg .pred p;\n .reg .b64 b;\n setp.ne.b32 p, %5, 0;\n mov.b64 b, {%2, %4};\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n}\n" ::"r"(d_tmem),
+        "r"(a_tmem), "r"(b_lo), "r"(idesc), "n"(kUmmaDescHi), "n"(ACC ? 1 : 0));
+}
+LT_DEVINL bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(p));
+    return p != 0;
 }
 constexpr uint32_t kUmmaBTransposed = 1u << 16;  // instruction descriptor: B along N
 
@@ -100,6 +142,41 @@ template <int ID, int N>
 LT_DEVINL void named_sync() {
     asm volatile("bar.sync %0, %1;" ::"n"(ID), "n"(N) : "memory");
 }
+
+// K and V pools as [page][head][slot][head_dim] tensors, read in boxes of `rows`
+// slots (a divisor of the page and of a tile; 0: no maps) by 64 columns.
+struct PpMaps {
+    alignas(64) CUtensorMap k;
+    alignas(64) CUtensorMap v;
+    uint32_t rows;
+};
+LT_DEVINL void tma_load_4d(uint32_t dst, const CUtensorMap *map, uint32_t x, uint32_t slot, uint32_t head, uint32_t page,
+                           uint64_t *bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
+        "[%6];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(slot), "r"(head), "r"(page), "r"(smem_u32(bar))
+        : "memory");
+}
+
+// Two weights as packed f16 high and low terms: low = x - high by one
+// f16 x f16 + f32 product-sum per element.
+LT_DEVINL void split_weights(float x, float y, uint32_t &hi, uint32_t &lo) {
+    const __half2 h = __floats2half2_rn(x, y);
+    hi = *reinterpret_cast<const uint32_t *>(&h);
+    float dx, dy;
+    asm("{\n .reg .b16 a, b, m;\n mov.b32 {a, b}, %2;\n mov.b16 m, 0xBC00;\n"
+        " fma.rn.f32.f16 %0, a, m, %3;\n fma.rn.f32.f16 %1, b, m, %4;\n}\n"
+        : "=f"(dx), "=f"(dy)
+        : "r"(hi), "f"(x), "f"(y));
+    const __half2 l = __floats2half2_rn(dx, dy);
+    lo = *reinterpret_cast<const uint32_t *>(&l);
+}
+
+template <int N>
+struct IntC {
+    static constexpr int value = N;
+};
 
 // What one row sees and how it scores.
 struct PpRow {
@@ -145,7 +222,8 @@ __noinline__ __device__ void pp_slow_row(const PagedAttnArgs &a, const PpRow &r,
 }
 
 template <int HD, bool EXTRA>
-__global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(PagedAttnArgs a) {
+__global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(PagedAttnArgs a,
+                                                                const __grid_constant__ PpMaps maps) {
     using S = PpShape<HD>;
     constexpr int KT = S::KT, NS = S::STAGES;
     extern __shared__ __align__(1024) uint8_t smem[];
@@ -153,10 +231,14 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(PagedAttnArgs a)
     uint32_t *docs_s = reinterpret_cast<uint32_t *>(smem + S::OFF_DOCS);
     uint32_t *skip = reinterpret_cast<uint32_t *>(smem + S::OFF_SKIP);  // bit set: some row may see the tile
     uint64_t *full = reinterpret_cast<uint64_t *>(smem + S::OFF_BARS), *empty = full + NS;
-    uint64_t *s_full = empty + NS, *p_full = s_full + 2, *o_full = p_full + 2;
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(o_full + 2);
+    uint64_t *s_full = empty + NS, *p_full = s_full + 2, *o_full = p_full + 2, *p_half = o_full + 2;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(p_half + 2);
     volatile uint32_t *dead = tmem_slot + 1;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    // warp-uniform values go through a shuffle where the compiler cannot see that
+    // they are: the MMA operands then stay in uniform registers (65 instead of 90
+    // to 150 clocks per 128 x 128 x 16 product)
+    auto uniform = [](uint32_t v) { return __shfl_sync(0xffffffffu, v, 0); };
+    const int tid = threadIdx.x, warp = (int)uniform(tid >> 5), lane = tid & 31;
     pdl_launch_dependents();
     pdl_wait();
 
@@ -177,8 +259,9 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(PagedAttnArgs a)
     int64_t hi64 = len, lo64 = 0;
     if (a.causal) hi64 = min(hi64, max(i1 + 1, (int64_t)prefix));
     if (a.window) lo64 = max((int64_t)0, i0 - (int64_t)a.window + 1);
-    const uint32_t hi = (uint32_t)max((int64_t)0, hi64), lo = (uint32_t)min(lo64, (int64_t)hi);
-    const uint32_t tiles = (hi - lo + KT - 1) / KT;
+    const uint32_t hi = (uint32_t)max((int64_t)0, hi64), first = (uint32_t)min(lo64, (int64_t)hi);
+    const uint32_t lo = maps.rows ? first - first % maps.rows : first;  // tiles start on a box
+    const uint32_t tiles = uniform((hi - lo + KT - 1) / KT);
     const uint32_t *table = a.table + (uint64_t)s * a.kv.max_pages;
     const uint32_t *docs = a.docs ? a.docs + (uint64_t)s * a.doc_stride : nullptr;
     const bool skipping = docs && tiles <= kPpSkipTiles;
@@ -192,6 +275,7 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(PagedAttnArgs a)
             mbar_init(s_full + i, 1);
             mbar_init(p_full + i, HD == 256 ? 256 : 128);
             mbar_init(o_full + i, 1);
+            mbar_init(p_half + i, 128);
         }
         *dead = 0;
         fence_barrier_init();
@@ -229,7 +313,7 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(PagedAttnArgs a)
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = *tmem_slot;
+    const uint32_t tmem = uniform(*tmem_slot);
 
     auto wait = [&](uint64_t *bar, uint32_t phase) {
         if (*dead) return;
@@ -241,7 +325,7 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(PagedAttnArgs a)
     // the first tile at or after t that is worked on
     auto next_tile = [&](uint32_t t) {
         if (skipping)
-            while (t < tiles && !(skip[t / 32] >> (t % 32) & 1u)) t++;
+            while (t < tiles && !(uniform(skip[t / 32]) >> (t % 32) & 1u)) t++;
         return t;
     };
 
@@ -252,14 +336,14 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(PagedAttnArgs a)
             const int pt = tid - 288, pw = warp - 9;
             constexpr int CH = HD / 8, RPI = 32 / CH;  // 16-byte chunks per row, rows per warp and step
             const int col = lane % CH;
-            uint32_t n = 0, jj = 0;
-            for (uint32_t t = next_tile(0); t < tiles; t = next_tile(t + 1), jj++) {
-                uint64_t mine[(KT + kPpProducers - 1) / kPpProducers];
+            constexpr int PER = (KT + kPpProducers - 1) / kPpProducers;
+            uint64_t mine[PER];  // pool offsets of this thread's rows, looked up one tile ahead
+            auto look = [&](uint32_t t) {
 #pragma unroll
-                for (int u = 0; u < (KT + kPpProducers - 1) / kPpProducers; u++) {
+                for (int u = 0; u < PER; u++) {
                     const uint32_t r = pt + u * kPpProducers, j = lo + t * KT + r;
                     mine[u] = ~0ull;
-                    if (r < KT && j < hi) {
+                    if (r < KT && j >= first && j < hi) {
                         const uint32_t page = table[j / a.kv.page_size];
                         if (page < a.kv.n_pages)
                             mine[u] = paged_offset(a.kv, page, j, kh);
@@ -267,62 +351,168 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(PagedAttnArgs a)
                             atomicExch(a.err, DEV_ERR_BAD_INDEX);
                     }
                 }
-                named_sync<1, kPpProducers>();  // the last tile's offsets are read
-#pragma unroll
-                for (int u = 0; u < (KT + kPpProducers - 1) / kPpProducers; u++)
-                    if (pt + u * kPpProducers < KT) offs[pt + u * kPpProducers] = mine[u];
-                named_sync<1, kPpProducers>();
-                for (int kv = 0; kv < 2; kv++, n++) {
-                    const uint32_t st = n % NS;
-                    wait(empty + st, ((n / NS) & 1) ^ 1);
-                    if (docs && kv == 0)
-                        for (int r = pt; r < KT; r += kPpProducers)
-                            docs_s[(jj % S::DOCS) * KT + r] = lo + t * KT + r < hi ? docs[lo + t * KT + r] : 0;
-                    const uint8_t *src = kv ? a.kv.v : a.kv.k;
-                    const uint32_t dst = smem_u32(smem) + S::OFF_RING + st * S::STAGE + (col / 8) * (KT * 128);
-#pragma unroll 4
-                    for (int r = pw * RPI + lane / CH; r < KT; r += 3 * RPI) {
-                        const uint64_t o = offs[r];
-                        const bool take = o != ~0ull;
-                        cp_async16(dst + r * 128 + (((col & 7) ^ (r & 7)) << 4), src + (take ? o : 0) + col * 16, take);
-                    }
-                    cp_async_commit();
-                    if (n) {  // the copies before these have landed: hand their stage to the tensor cores
-                        cp_async_wait<1>();
-                        fence_async_smem();
-                        mbar_arrive(full + (n - 1) % NS);
-                    }
-                }
-            }
-            if (n) {
-                cp_async_wait<0>();
+            };
+            auto landed = [&](uint32_t stage) {  // this thread's copies are in place: hand the stage on
                 fence_async_smem();
-                mbar_arrive(full + (n - 1) % NS);
+                mbar_arrive(full + stage);
+            };
+            uint32_t jj = 0, st = 0, turn = 0;  // tile count; ring stage and how often it went round
+            uint32_t t = next_tile(0);
+            bool owed = false;                // the stage before st is copied but not handed on
+            // tiles of whole boxes: every slot holds a cached position
+            auto boxed = [&](uint32_t tt) {
+                const uint32_t k0 = lo + tt * KT;
+                return maps.rows && k0 >= first && (uint64_t)k0 + KT <= len;
+            };
+            const uint32_t boxes = maps.rows ? KT / maps.rows : 0;  // per 64 columns
+            uint32_t box_page = 0;
+            auto look_boxed = [&](uint32_t tt) {  // lane l of warp 9: box l % boxes of column block l / boxes
+                if (pw == 0 && (uint32_t)lane < boxes * S::NBLK) {
+                    box_page = table[(lo + tt * KT + lane % boxes * maps.rows) / a.kv.page_size];
+                    if (box_page >= a.kv.n_pages) atomicExch(a.err, DEV_ERR_BAD_INDEX);
+                }
+            };
+            auto ahead = [&](uint32_t tt) {
+                if (tt >= tiles) return;
+                if (boxed(tt))
+                    look_boxed(tt);
+                else
+                    look(tt);
+            };
+            ahead(t);
+            while (t < tiles) {
+                const bool by_box = boxed(t);
+                if (!by_box) {
+                    named_sync<1, kPpProducers>();  // the last such tile's offsets are read
+#pragma unroll
+                    for (int u = 0; u < PER; u++)
+                        if (pt + u * kPpProducers < KT) offs[pt + u * kPpProducers] = mine[u];
+                    named_sync<1, kPpProducers>();
+                }
+                const uint32_t tn = next_tile(t + 1), page = box_page;
+#pragma unroll 1
+                for (int kv = 0; kv < 2; kv++) {
+                    if (owed && (by_box || !mbar_try_wait(empty + st, (turn & 1) ^ 1))) {
+                        cp_async_wait<0>();
+                        landed(st ? st - 1 : NS - 1);
+                        owed = false;
+                    }
+                    wait(empty + st, (turn & 1) ^ 1);
+                    __syncwarp();
+                    if (docs && kv == 0)
+                        for (int r = pt; r < KT; r += kPpProducers) {
+                            const uint32_t j = lo + t * KT + r;
+                            docs_s[(jj % S::DOCS) * KT + r] = j < hi ? docs[j] : 0;
+                        }
+                    const uint32_t stage = smem_u32(smem) + S::OFF_RING + st * S::STAGE;
+                    if (by_box) {
+                        if (pw == 0) {
+                            if (lane == 0) mbar_arrive_expect_tx(full + st, S::STAGE);
+                            __syncwarp();
+                            if ((uint32_t)lane < boxes * S::NBLK) {
+                                const uint32_t r = lane % boxes * maps.rows, blk = lane / boxes;
+                                tma_load_4d(stage + blk * (KT * 128) + r * 128, kv ? &maps.v : &maps.k, blk * 64,
+                                            (lo + t * KT + r) % a.kv.page_size, kh, page, full + st);
+                            }
+                            if (lane) mbar_arrive(full + st);
+                        } else {
+                            mbar_arrive(full + st);
+                        }
+                        if (kv == 0) ahead(tn);
+                    } else {
+                        const uint8_t *src = (kv ? a.kv.v : a.kv.k) + col * 16;
+                        const uint32_t dst = stage + (col / 8) * (KT * 128);
+#pragma unroll 4
+                        for (int r = pw * RPI + lane / CH; r < KT; r += 3 * RPI) {
+                            const uint64_t o = offs[r];
+                            const bool take = o != ~0ull;
+                            cp_async16(dst + r * 128 + (((col & 7) ^ (r & 7)) << 4), src + (take ? o : 0), take);
+                        }
+                        cp_async_commit();
+                        if (kv == 0) ahead(tn);
+                        if (owed) {
+                            cp_async_wait<1>();
+                            landed(st ? st - 1 : NS - 1);
+                        }
+                        owed = true;
+                    }
+                    if (++st == NS) st = 0, turn++;
+                }
+                t = tn;
+                jj++;
             }
-        } else if (lane == 0) {
+            if (owed) {
+                cp_async_wait<0>();
+                landed(st ? st - 1 : NS - 1);
+            }
+        } else {
             // ── MMAs ──
             constexpr uint32_t IQK = umma_idesc_f16_f32(128, KT);
             constexpr uint32_t IPV = umma_idesc_f16_f32(128, HD) | kUmmaBTransposed;
             const uint32_t q_u = smem_u32(smem), ring = q_u + S::OFF_RING;
-            auto qk = [&](int tile, uint32_t stage, uint32_t d) {
-#pragma unroll 1
-                for (int pl = 1; pl >= 0; pl--) {  // low plane first: small terms while the sum is small
-                    const uint32_t qa = q_u + (tile * 2 + pl) * S::QPLANE;
+            // one lane issues; the loop around it stays uniform across the warp
+            auto qk = [&](int tile, uint32_t stage, uint32_t d, uint64_t *done, uint64_t *release) {
+                const uint32_t qa = umma_lo(q_u + tile * 2 * S::QPLANE), kb = umma_lo(ring + stage * S::STAGE);
+                if (elect_one()) {
+                    // low plane first: small terms while the sum is small
+#pragma unroll
+                    for (int i = 0; i < HD / 16; i++) {
+                        const uint32_t qi = qa + ((S::QPLANE + (i / 4) * 16384 + (i % 4) * 32) >> 4);
+                        const uint32_t ki = kb + (((i / 4) * (KT * 128) + (i % 4) * 32) >> 4);
+                        if (i == 0)
+                            umma_ss<false>(d, qi, ki, IQK);
+                        else
+                            umma_ss<true>(d, qi, ki, IQK);
+                    }
 #pragma unroll
                     for (int i = 0; i < HD / 16; i++)
-                        umma_f16(d, umma_desc_sw128(qa + (i / 4) * 16384 + (i % 4) * 32),
-                                 umma_desc_sw128(ring + stage * S::STAGE + (i / 4) * (KT * 128) + (i % 4) * 32), IQK,
-                                 pl == 0 || i > 0);
+                        umma_ss<true>(d, qa + (((i / 4) * 16384 + (i % 4) * 32) >> 4),
+                                      kb + (((i / 4) * (KT * 128) + (i % 4) * 32) >> 4), IQK);
+                    umma_commit(done);
+                    if (release) umma_commit(release);
                 }
+                __syncwarp();
             };
-            auto pv = [&](uint32_t p, uint32_t stage, uint32_t d) {
-#pragma unroll 1
-                for (int pl = 1; pl >= 0; pl--) {
+            // the products of `STEPS` 16-key steps from step FROM on
+            auto pv_steps = [&](auto from, auto steps, uint32_t p, uint32_t vb, uint32_t d) {
+                constexpr int FROM = decltype(from)::value, STEPS = decltype(steps)::value;
 #pragma unroll
-                    for (int i = 0; i < KT / 16; i++)
-                        umma_f16_ts(d, p + 32 * (i / 2) + 16 * pl + 8 * (i % 2),
-                                    umma_desc_sw128_mn(ring + stage * S::STAGE + i * 2048, KT * 128), IPV, pl == 0 || i > 0);
+                for (int i = FROM; i < FROM + STEPS; i++) {
+                    if (i == 0)
+                        umma_ts<false>(d, p + 8, vb, IPV);
+                    else
+                        umma_ts<true>(d, p + 16 * i + 8, vb + ((i * 2048) >> 4), IPV);
                 }
+#pragma unroll
+                for (int i = FROM; i < FROM + STEPS; i++) umma_ts<true>(d, p + 16 * i, vb + ((i * 2048) >> 4), IPV);
+            };
+            auto pv = [&](uint32_t p, uint32_t stage, uint32_t d, uint64_t *half, uint64_t *rest, uint32_t turn,
+                          uint64_t *done, uint64_t *release) {
+                const uint32_t vb = umma_lo_mn(ring + stage * S::STAGE, KT * 128);
+                constexpr int STEPS = KT / 16;
+                if constexpr (HD == 256) {
+                    wait(rest, turn ^ 1);
+                    tc_fence_after();
+                    if (elect_one()) {
+                        pv_steps(IntC<0>(), IntC<STEPS>(), p, vb, d);
+                        umma_commit(done);
+                        umma_commit(release);
+                    }
+                } else {
+                    // the first keys' weights while the softmax is still at the others
+                    wait(half, turn);
+                    tc_fence_after();
+                    if (elect_one()) pv_steps(IntC<0>(), IntC<STEPS / 2>(), p, vb, d);
+                    __syncwarp();
+                    wait(rest, turn ^ 1);
+                    tc_fence_after();
+                    if (elect_one()) {
+                        pv_steps(IntC<STEPS / 2>(), IntC<STEPS / 2>(), p, vb, d);
+                        umma_commit(done);
+                        if (release) umma_commit(release);
+                    }
+                }
+                __syncwarp();
             };
             uint32_t t = next_tile(0), jj = 0;
             if (t < tiles) {
@@ -332,15 +522,10 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(PagedAttnArgs a)
                 wait(full + 0, 0);
                 tc_fence_after();
                 if constexpr (HD == 256) {
-                    qk(0, 0, tmem + S::S_COL(0));
-                    umma_commit(s_full + 0);
-                    umma_commit(empty + 0);
+                    qk(0, 0, tmem + S::S_COL(0), s_full + 0, empty + 0);
                 } else {
-                    qk(0, 0, tmem + S::S_COL(0));
-                    umma_commit(s_full + 0);
-                    qk(1, 0, tmem + S::S_COL(1));
-                    umma_commit(s_full + 1);
-                    umma_commit(empty + 0);
+                    qk(0, 0, tmem + S::S_COL(0), s_full + 0, nullptr);
+                    qk(1, 0, tmem + S::S_COL(1), s_full + 1, empty + 0);
                 }
                 while (t < tiles) {
                     const uint32_t tn = next_tile(t + 1);
@@ -349,42 +534,28 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(PagedAttnArgs a)
                         if (tn < tiles) {
                             wait(full + nk % NS, (nk / NS) & 1);
                             tc_fence_after();
-                            qk(0, nk % NS, tmem + S::S_COL((jj + 1) & 1));
-                            umma_commit(s_full + ((jj + 1) & 1));
-                            umma_commit(empty + nk % NS);
+                            qk(0, nk % NS, tmem + S::S_COL((jj + 1) & 1), s_full + ((jj + 1) & 1), empty + nk % NS);
                         }
                         wait(full + nv % NS, (nv / NS) & 1);
-                        wait(p_full + 0, (jj + 1) & 1);
-                        tc_fence_after();
-                        pv(tmem + S::S_COL(jj & 1), nv % NS, tmem + S::O_COL(0));
-                        umma_commit(o_full + 0);
-                        umma_commit(empty + nv % NS);
+                        pv(tmem + S::S_COL(jj & 1), nv % NS, tmem + S::O_COL(0), nullptr, p_full + 0, jj & 1, o_full + 0,
+                           empty + nv % NS);
                     } else {
-#pragma unroll 1
-                        for (int w = 0; w < 2; w++) {
-                            if (w == 0) wait(full + nv % NS, (nv / NS) & 1);
-                            wait(p_full + w, (jj + 1) & 1);
+                        wait(full + nv % NS, (nv / NS) & 1);
+                        pv(tmem + S::S_COL(0), nv % NS, tmem + S::O_COL(0), p_half + 0, p_full + 0, jj & 1, o_full + 0, nullptr);
+                        if (tn < tiles) {
+                            wait(full + nk % NS, (nk / NS) & 1);
                             tc_fence_after();
-                            pv(tmem + S::S_COL(w), nv % NS, tmem + S::O_COL(w));
-                            umma_commit(o_full + w);
-                            if (w == 1) umma_commit(empty + nv % NS);
-                            if (tn < tiles) {
-                                if (w == 0) {
-                                    wait(full + nk % NS, (nk / NS) & 1);
-                                    tc_fence_after();
-                                }
-                                qk(w, nk % NS, tmem + S::S_COL(w));
-                                umma_commit(s_full + w);
-                                if (w == 1) umma_commit(empty + nk % NS);
-                            }
+                            qk(0, nk % NS, tmem + S::S_COL(0), s_full + 0, nullptr);
                         }
+                        pv(tmem + S::S_COL(1), nv % NS, tmem + S::O_COL(1), p_half + 1, p_full + 1, jj & 1, o_full + 1,
+                           empty + nv % NS);
+                        if (tn < tiles) qk(1, nk % NS, tmem + S::S_COL(1), s_full + 1, empty + nk % NS);
                     }
                     t = tn;
                     jj++;
                 }
             }
         }
-        __syncwarp();
     } else {
         // ── softmax: one row per thread ──
         regs_inc<224>();
@@ -413,41 +584,44 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(PagedAttnArgs a)
         // queries to two f16 planes: the warp takes its 32 rows one by one
         const float f0 = EXTRA && a.softcap != 0.0f ? a.scale / a.softcap : a.scale * 1.4426950408889634f;
         float rf = 0.0f;
+        const int n_rows = (int)min((int64_t)32, max((int64_t)0, (int64_t)rows - (R - lane)));  // of this warp's 32
         if (HD != 256 || wg == 0) {
-#pragma unroll 4
-            for (int x = 0; x < 32; x++) {
-                const uint32_t rr = (warp & 3) * 32 + x, RR = R0 + tile * 128 + rr;
-                constexpr int PER = HD / 32;
-                float v[PER];
+            constexpr int PER = HD / 32, BATCH = HD == 256 ? 16 : 32;
+#pragma unroll 1
+            for (int x0 = 0; x0 < 32; x0 += BATCH) {
+                float v[BATCH][PER];  // a batch of rows in flight
 #pragma unroll
-                for (int e = 0; e < PER; e++) v[e] = 0.0f;
-                if (RR < rows) {
-                    const float *src = a.q + (uint64_t)(c0 + RR / a.group) * a.q_stride + (uint64_t)(kh * a.group + RR % a.group) * HD;
+                for (int y = 0; y < BATCH; y++) {
+                    const float *src = reinterpret_cast<const float *>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(row.q), x0 + y));
 #pragma unroll
                     for (int e = 0; e < PER; e += 2) {
-                        const float2 y = *reinterpret_cast<const float2 *>(src + 64 * (e / 2) + 2 * lane);
-                        v[e] = y.x;
-                        v[e + 1] = y.y;
+                        const float2 z = x0 + y < n_rows ? *reinterpret_cast<const float2 *>(src + 32 * e + 2 * lane) : make_float2(0.0f, 0.0f);
+                        v[y][e] = z.x;
+                        v[y][e + 1] = z.y;
                     }
                 }
-                float top = 0.0f;
 #pragma unroll
-                for (int e = 0; e < PER; e++) top = fmaxf(top, fabsf(v[e]));
-                top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
-                float up = 1.0f;
-                if (top > 0.0f && top < INFINITY) {
-                    const int ex = min(max(8 - (int)(__float_as_uint(top) >> 23) + 127, -126), 126);
-                    up = __uint_as_float((uint32_t)(ex + 127) << 23);
-                }
-                if (lane == x) rf = f0 / up;
-                const float sg = f0 < 0.0f ? -up : up;  // the factor on the scores stays positive
+                for (int y = 0; y < BATCH; y++) {
+                    const uint32_t rr = (warp & 3) * 32 + x0 + y;
+                    float top = 0.0f;
 #pragma unroll
-                for (int e = 0; e < PER; e += 2) {
-                    uint32_t h, l;
-                    split_f16x2(v[e] * sg, v[e + 1] * sg, h, l);
-                    const uint32_t at = tile * 2 * S::QPLANE + (e / 2) * 16384 + sw128_offset(rr, 2 * lane);
-                    *reinterpret_cast<uint32_t *>(smem + at) = h;
-                    *reinterpret_cast<uint32_t *>(smem + at + S::QPLANE) = l;
+                    for (int e = 0; e < PER; e++) top = fmaxf(top, fabsf(v[y][e]));
+                    top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
+                    float up = 1.0f;
+                    if (top > 0.0f && top < INFINITY) {
+                        const int ex = min(max(8 - (int)(__float_as_uint(top) >> 23) + 127, -126), 126);
+                        up = __uint_as_float((uint32_t)(ex + 127) << 23);
+                    }
+                    if (lane == x0 + y) rf = f0 / up;
+                    const float sg = f0 < 0.0f ? -up : up;  // the factor on the scores stays positive
+#pragma unroll
+                    for (int e = 0; e < PER; e += 2) {
+                        uint32_t h, l;
+                        split_f16x2(v[y][e] * sg, v[y][e + 1] * sg, h, l);
+                        const uint32_t at = tile * 2 * S::QPLANE + (e / 2) * 16384 + sw128_offset(rr, 2 * lane);
+                        *reinterpret_cast<uint32_t *>(smem + at) = h;
+                        *reinterpret_cast<uint32_t *>(smem + at + S::QPLANE) = l;
+                    }
                 }
             }
             fence_async_smem();
@@ -475,13 +649,21 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(PagedAttnArgs a)
         float m = -INFINITY, l = 0.0f, alpha = 1.0f;
         const uint32_t o_addr = tmem + lane_base + S::O_COL(tile) + half * 128;
         auto add_o = [&]() {  // o = o * alpha + this tile's product
+            uint32_t v[2][32];
+            const float2 al2 = make_float2(alpha, alpha);
+            tmem_ld32(o_addr, v[0]);
 #pragma unroll
             for (int c = 0; c < OW; c += 32) {
-                uint32_t v[32];
-                tmem_ld32(o_addr + c, v);
-                tmem_wait_ld();
+                uint32_t(&u)[32] = v[(c / 32) & 1];
+                tmem_wait_ld(u);
+                if (c + 32 < OW) tmem_ld32(o_addr + c + 32, v[(c / 32 + 1) & 1]);
 #pragma unroll
-                for (int e = 0; e < 32; e++) o[c + e] = fmaf(o[c + e], alpha, __uint_as_float(v[e]));
+                for (int e = 0; e < 32; e += 2) {
+                    const float2 x = ffma2(make_float2(o[c + e], o[c + e + 1]), al2,
+                                           make_float2(__uint_as_float(u[e]), __uint_as_float(u[e + 1])));
+                    o[c + e] = x.x;
+                    o[c + e + 1] = x.y;
+                }
             }
         };
         uint32_t jj = 0;
@@ -494,36 +676,50 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(PagedAttnArgs a)
             tc_fence_after();
             const bool whole = !docs && row.lo <= k0 && k0 + CW <= row.hi;
             const bool plain = __all_sync(0xffffffffu, whole || !real);
-            // pass 1: the row's maximum; capped, biased or masked scores go back to tensor memory
+            // pass 1: the row's maximum; capped, biased or masked scores go back to tensor
+            // memory.  Each load runs while the columns before it are worked on.
             float top = -INFINITY;
+            {
+                uint32_t v[2][32];
+                tmem_ld32(s_addr, v[0]);
+                const int from = (int)max((int64_t)0, min((int64_t)CW, row.lo - k0));
+                const int to = (int)max((int64_t)0, min((int64_t)CW, row.hi - k0));
+                const float dist = (float)(row.i - k0);
 #pragma unroll
-            for (int c = 0; c < CW; c += 32) {
-                uint32_t v[32];
-                tmem_ld32(s_addr + c, v);
-                tmem_wait_ld();
-                if (!EXTRA && plain) {
-                    float x0 = -INFINITY, x1 = -INFINITY;
+                for (int c = 0; c < CW; c += 32) {
+                    uint32_t(&u)[32] = v[(c / 32) & 1];
+                    tmem_wait_ld(u);
+                    if (c + 32 < CW) tmem_ld32(s_addr + c + 32, v[(c / 32 + 1) & 1]);
+                    if (!EXTRA && plain) {
+                        float x0 = -INFINITY, x1 = -INFINITY;
 #pragma unroll
-                    for (int e = 0; e < 32; e += 2) {
-                        x0 = fmaxf(x0, __uint_as_float(v[e]));
-                        x1 = fmaxf(x1, __uint_as_float(v[e + 1]));
+                        for (int e = 0; e < 32; e += 4) {
+                            x0 = fmaxf(fmaxf(x0, __uint_as_float(u[e])), __uint_as_float(u[e + 1]));
+                            x1 = fmaxf(fmaxf(x1, __uint_as_float(u[e + 2])), __uint_as_float(u[e + 3]));
+                        }
+                        top = fmaxf(top, fmaxf(x0, x1));
+                        continue;
                     }
-                    top = fmaxf(top, fmaxf(x0, x1));
-                } else {
+                    bool small = true;
+                    if (EXTRA && a.softcap != 0.0f) {
+                        float big = 0.0f;
+#pragma unroll
+                        for (int e = 0; e < 32; e++) big = fmaxf(big, fabsf(__uint_as_float(u[e])));
+                        small = __all_sync(0xffffffffu, big * rf <= kTanhSmall);
+                    }
 #pragma unroll
                     for (int e = 0; e < 32; e++) {
-                        const int64_t j = k0 + c + e;
-                        float x = __uint_as_float(v[e]);
-                        if (EXTRA) x = score_log2(x, rf, a.softcap, row.slope, fabsf((float)(row.i - j)));
-                        bool seen = plain || (j >= row.lo && j < row.hi);
+                        float x = __uint_as_float(u[e]);
+                        if (EXTRA) x = score_log2(x, rf, a.softcap, row.slope, fabsf(dist - (float)(c + e)), small);
+                        bool seen = c + e >= from && c + e < to;
                         if (docs) seen = seen && docs_s[(jj % S::DOCS) * KT + half * 32 + c + e] == row.doc;
                         x = seen ? x : -INFINITY;
                         top = fmaxf(top, x);
-                        v[e] = __float_as_uint(x);
+                        u[e] = __float_as_uint(x);
                     }
-                    tmem_st32(s_addr + c, v);
-                    tmem_wait_st();
+                    tmem_st32(s_addr + c, u);
                 }
+                if (EXTRA || !plain) tmem_wait_st();
             }
             const float fs = EXTRA ? 1.0f : rf;
             top = top == -INFINITY ? top : top * fs;
@@ -543,24 +739,35 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(PagedAttnArgs a)
             m = mn;
             // weights times 2^10: small ones keep their f16 bits, and the sum carries the same factor
             const float base = m == -INFINITY ? 0.0f : 10.0f - m;
-            float l0 = 0.0f, l1 = 0.0f;
+            float2 sum = make_float2(0.0f, 0.0f);
+            {
+                const float2 fs2 = make_float2(fs, fs), base2 = make_float2(base, base);
+                uint32_t v[2][16];
+                tmem_ld16(s_addr, v[0]);
 #pragma unroll
-            for (int c = 0; c < CW; c += 32) {
-                uint32_t v[32], p[32];
-                tmem_ld32(s_addr + c, v);
-                tmem_wait_ld();
+                for (int c = 0; c < CW; c += 16) {
+                    uint32_t(&u)[16] = v[(c / 16) & 1];
+                    uint32_t p[16];
+                    tmem_wait_ld(u);
+                    if (c + 16 < CW) tmem_ld16(s_addr + c + 16, v[(c / 16 + 1) & 1]);
 #pragma unroll
-                for (int e = 0; e < 32; e += 2) {
-                    const float x = ex2(fmaf(__uint_as_float(v[e]), fs, base));
-                    const float y = ex2(fmaf(__uint_as_float(v[e + 1]), fs, base));
-                    l0 += x;
-                    l1 += y;
-                    split_f16x2(x, y, p[e / 2], p[16 + e / 2]);
+                    for (int e = 0; e < 16; e += 2) {
+                        float2 x = ffma2(make_float2(__uint_as_float(u[e]), __uint_as_float(u[e + 1])), fs2, base2);
+                        x.x = ex2(x.x);
+                        x.y = ex2(x.y);
+                        sum = fadd2(sum, x);
+                        split_weights(x.x, x.y, p[e / 2], p[8 + e / 2]);
+                    }
+                    tmem_st16(s_addr + c, p);
+                    if (HD != 256 && c + 16 == CW / 2) {
+                        tmem_wait_st();
+                        tc_fence_before();
+                        mbar_arrive(p_half + tile);
+                    }
                 }
-                tmem_st32(s_addr + c, p);
             }
             tmem_wait_st();
-            l = fmaf(l, al, l0 + l1);
+            l = fmaf(l, al, sum.x + sum.y);
             if constexpr (HD == 256) {
                 // the last tile's product was computed while this softmax ran
                 if (jj) {
@@ -599,20 +806,37 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(PagedAttnArgs a)
             l += tmem_ld1(x_addr + (wg ^ 1));
             tmem_wait_ld();
         }
-        if (real) {
-            float *dst = a.out + (uint64_t)(c0 + token) * a.out_stride + (uint64_t)head * HD + half * 128;
-            const float inv = l > 0.0f ? __fdiv_rn(1.0f, l) : (l == 0.0f ? 0.0f : l);
-            float bad = 0.0f;
+        // rows to the output through shared memory (this row tile's query planes are
+        // no longer read), 32 columns at a time, so that stores fill whole lines
+        const float inv = l > 0.0f ? __fdiv_rn(1.0f, l) : (l == 0.0f ? 0.0f : l);
+        float off = l - l;
 #pragma unroll
-            for (int e = 0; e < OW; e++) bad += (o[e] - o[e]);
-            if (bad == 0.0f && l - l == 0.0f) {
+        for (int e = 0; e < OW; e++) off += o[e] - o[e];
+        const bool fine = off == 0.0f;
+        constexpr int PITCH = 36;
+        float *st = reinterpret_cast<float *>(smem + tile * 2 * S::QPLANE) + (HD == 256 ? warp : warp & 3) * 32 * PITCH;
+        const uint64_t dst = reinterpret_cast<uint64_t>(a.out + (uint64_t)(c0 + token) * a.out_stride + (uint64_t)head * HD + half * 128);
+        const uint32_t fine_rows = __ballot_sync(0xffffffffu, fine && real);
 #pragma unroll
-                for (int e = 0; e < OW; e += 4)
-                    *reinterpret_cast<float4 *>(dst + e) = make_float4(o[e] * inv, o[e + 1] * inv, o[e + 2] * inv, o[e + 3] * inv);
-            } else {
-                pp_slow_row(a, row, table, docs, kh, f0, half * 128, OW, dst - half * 128);
+        for (int c = 0; c < OW; c += 32) {
+            __syncwarp();
+#pragma unroll
+            for (int e = 0; e < 32; e += 4)
+                *reinterpret_cast<float4 *>(st + lane * PITCH + e) =
+                    make_float4(o[c + e] * inv, o[c + e + 1] * inv, o[c + e + 2] * inv, o[c + e + 3] * inv);
+            __syncwarp();
+#pragma unroll
+            for (int x = 0; x < 8; x++) {
+                const int rr = x * 4 + lane / 8;
+                float *to = reinterpret_cast<float *>(__shfl_sync(0xffffffffu, dst, rr));
+                if (fine_rows >> rr & 1u)
+                    *reinterpret_cast<float4 *>(to + c + lane % 8 * 4) =
+                        *reinterpret_cast<const float4 *>(st + rr * PITCH + lane % 8 * 4);
             }
         }
+        if (real && !fine)
+            pp_slow_row(a, row, table, docs, kh, f0, half * 128, OW,
+                        a.out + (uint64_t)(c0 + token) * a.out_stride + (uint64_t)head * HD);
         tc_fence_before();
     }
     __syncthreads();
@@ -624,12 +848,49 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(PagedAttnArgs a)
 
 namespace {
 
+using EncodeTiledFn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
+                                   const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
+                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiledFn encode_tiled() {
+    static EncodeTiledFn fn = [] {
+        void *p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        const bool ok = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+                        q == cudaDriverEntryPointSuccess;
+        return ok ? reinterpret_cast<EncodeTiledFn>(p) : nullptr;
+    }();
+    return fn;
+}
+
+// Maps of the pool, or rows = 0 where its pages or strides do not allow them.
+void pp_maps(const PagedKvDev &kv, uint32_t tile, PpMaps &m) {
+    m.rows = 0;
+    uint32_t rows = tile;
+    while (kv.page_size % rows) rows /= 2;  // tile is a power of two: the largest box in both
+    const uint64_t most = 1ull << 40;
+    if (rows < 8 || kv.slot_stride >= most || kv.head_stride >= most || kv.page_stride >= most) return;
+    EncodeTiledFn fn = encode_tiled();
+    if (!fn) return;
+    const cuuint64_t dims[4] = {kv.hd, kv.page_size, kv.n_kv, kv.n_pages};
+    const cuuint64_t strides[3] = {kv.slot_stride, kv.head_stride, kv.page_stride};
+    const cuuint32_t box[4] = {64, rows, 1, 1}, step[4] = {1, 1, 1, 1};
+    for (int i = 0; i < 2; i++)
+        if (fn(i ? &m.v : &m.k, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, i ? kv.v : kv.k, dims, strides, box, step,
+               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+            return;
+    m.rows = rows;
+}
+
 template <int HD, bool EXTRA>
 cudaError_t pp_launch(const LaunchCfg &c, const PagedAttnArgs &a) {
     using S = PpShape<HD>;
     const uint64_t rows = (uint64_t)a.max_q * a.group;
+    PpMaps maps;
+    pp_maps(a.kv, S::KT, maps);
     return launch_k(c, "paged_prompt", k_paged_prompt<HD, EXTRA>,
-                    dim3((uint32_t)((rows + S::ROWS - 1) / S::ROWS), a.kv.n_kv, a.n_seq), dim3(kPpThreads), S::SMEM, a);
+                    dim3((uint32_t)((rows + S::ROWS - 1) / S::ROWS), a.kv.n_kv, a.n_seq), dim3(kPpThreads), S::SMEM, a, maps);
 }
 
 // The register split needs the registers that 168 per thread give a block.
