@@ -105,14 +105,27 @@ LT_DEVINL float tanh_small(float x) {
     return fmaf(r * y, x, x);
 }
 
+// tanh over the whole range: 1 - 2 / (1 + e^(2|x|)) with one Newton step on the
+// reciprocal past kTanhSmall (absolute error about 1e-7 there).  No branch and no
+// call: it stands in unrolled loops.
+LT_DEVINL float tanh_any(float x) {
+    const float a = fabsf(x), d = 1.0f + ex2(a * 2.885390081777927f);
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d));
+    r = d < 1e30f ? fmaf(r, fmaf(-d, r, 1.0f), r) : 0.0f;
+    const float t = copysignf(fmaf(-2.0f, r, 1.0f), x);
+    return a <= kTanhSmall ? tanh_small(x) : (x != x ? x : t);
+}
+
 // Score of one (query, key) pair in units of log2: the scaled product, capped
 // by cap * tanh(s / cap), minus slope * |distance|.  f is the row's factor on
 // the raw product: scale * log2(e) without a cap, scale / cap with one.
-// small: |dot * f| is known not to pass kTanhSmall.
-LT_DEVINL float score_log2(float dot, float f, float cap, float slope, float dist, bool small = false) {
+// SMALL: |dot * f| is known not to pass kTanhSmall.
+template <bool SMALL = false>
+LT_DEVINL float score_log2(float dot, float f, float cap, float slope, float dist) {
     constexpr float kLog2e = 1.4426950408889634f;
     float s = dot * f;
-    if (cap != 0.0f) s = (small || fabsf(s) <= kTanhSmall ? tanh_small(s) : tanhf(s)) * (cap * kLog2e);
+    if (cap != 0.0f) s = (SMALL ? tanh_small(s) : tanh_any(s)) * (cap * kLog2e);
     return fmaf(-slope * kLog2e, dist, s);
 }
 

@@ -41,6 +41,9 @@ struct PpShape {
     static constexpr int STAGE = KT * HD * 2;
     static constexpr int STAGES = HD == 64 ? 6 : 3;
     static constexpr int DOCS = HD == 64 ? 4 : 2;         // document-number buffers
+    // registers per thread after the split: 256 softmax threads and 128 others share the 384 x 168 of the launch
+    static constexpr int REGS_SOFTMAX = HD == 64 ? 200 : 208, REGS_REST = HD == 64 ? 104 : 88;
+    static_assert(256 * REGS_SOFTMAX + 128 * REGS_REST <= kPpThreads * 168, "more registers than the launch holds");
     static constexpr int QPLANE = 128 * HD * 2;
     static constexpr int Q_BYTES = TILES * 2 * QPLANE;
     static constexpr int OFF_RING = Q_BYTES;
@@ -54,17 +57,7 @@ struct PpShape {
     static constexpr uint32_t X_COL = 128;                // head_dim 256: the halves' row maxima and sums
 };
 
-// 32 consecutive TMEM columns of this thread's lane.
-LT_DEVINL void tmem_st32(uint32_t taddr, const uint32_t (&v)[32]) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
-        "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
-        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
-        "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]),
-        "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]),
-        "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
-        : "memory");
-}
+// 16 consecutive TMEM columns of this thread's lane.
 LT_DEVINL void tmem_ld16(uint32_t taddr, uint32_t (&v)[16]) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
@@ -191,7 +184,7 @@ LT_DEVINL float pp_kv(const uint8_t *p, uint32_t d) { return __half2float(reinte
 
 // The row by itself, key by key, masked keys never touched: for rows whose tile
 // result is not finite, which a value outside the row's own keys may have caused.
-__noinline__ __device__ void pp_slow_row(const PagedAttnArgs &a, const PpRow &r, const uint32_t *table,
+__noinline__ __device__ void pp_slow_row(const PagedAttnArgs &a, PpRow r, const uint32_t *table,
                                          const uint32_t *docs, uint32_t kh, float rf, uint32_t d0, uint32_t nd,
                                          float *out) {
     const uint32_t hd = a.kv.hd;
@@ -330,7 +323,7 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(PagedAttnArgs a,
     };
 
     if (warp >= 8) {
-        regs_dec<56>();
+        regs_dec<S::REGS_REST>();
         if (warp > 8) {
             // ── K and V tiles into the ring ──
             const int pt = tid - 288, pw = warp - 9;
@@ -558,7 +551,7 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(PagedAttnArgs a,
         }
     } else {
         // ── softmax: one row per thread ──
-        regs_inc<224>();
+        regs_inc<S::REGS_SOFTMAX>();
         const int wg = warp >> 2, r = tid & 127, tile = HD == 256 ? 0 : wg;
         constexpr int CW = HD == 256 ? 32 : KT;          // score columns of this thread
         constexpr int OW = HD == 256 ? 128 : HD;         // output columns
@@ -566,46 +559,53 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(PagedAttnArgs a,
         const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t R = R0 + tile * 128 + r;
         const bool real = R < rows;
-        PpRow row;
-        const uint32_t token = real ? R / a.group : 0, head = kh * a.group + (real ? R % a.group : 0);
-        row.q = a.q + (uint64_t)(c0 + token) * a.q_stride + (uint64_t)head * HD;
-        row.i = (int64_t)len - nq + token;
-        row.lo = a.window ? row.i - (int64_t)a.window + 1 : 0;
-        row.hi = a.causal ? min((int64_t)len, max(row.i + 1, (int64_t)prefix)) : (int64_t)len;
-        row.doc = 0;
-        row.slope = EXTRA && a.slopes ? a.slopes[head] : 0.0f;
+        // Registers are what this part is short of (o alone takes OW): positions are 32 bits
+        // wide here (a length is at most 2^30), and the row's addresses are computed again at the end.
+        auto token_of = [&]() { return real ? R / a.group : 0; };
+        auto head_of = [&]() { return kh * a.group + (real ? R % a.group : 0); };
+        auto q_of = [&]() { return a.q + (uint64_t)(c0 + token_of()) * a.q_stride + (uint64_t)head_of() * HD; };
+        const int row_i = (int)((int64_t)len - nq + token_of());
+        const int row_lo = a.window ? (int)max((int64_t)0, (int64_t)row_i - a.window + 1) : 0;
+        int row_hi = a.causal ? (int)min((int64_t)len, max((int64_t)row_i + 1, (int64_t)prefix)) : (int)len;
+        uint32_t row_doc = 0;
+        const float row_slope = EXTRA && a.slopes ? a.slopes[head_of()] : 0.0f;
         if (docs) {
-            if (row.i >= 0)
-                row.doc = docs[row.i];
+            if (row_i >= 0)
+                row_doc = docs[row_i];
             else
-                row.hi = 0;
+                row_hi = 0;
         }
-        if (!real) row.hi = 0;
-        // queries to two f16 planes: the warp takes its 32 rows one by one
+        if (!real) row_hi = 0;
+        // Queries to two f16 planes: a warp takes its 32 rows (head_dim 256: each group half of
+        // them) eight at a time, the next eight on their way.  A rolled loop: unrolled over
+        // the rows, fetching its instructions took longer than its loads.
         const float f0 = EXTRA && a.softcap != 0.0f ? a.scale / a.softcap : a.scale * 1.4426950408889634f;
         float rf = 0.0f;
-        const int n_rows = (int)min((int64_t)32, max((int64_t)0, (int64_t)rows - (R - lane)));  // of this warp's 32
-        if (HD != 256 || wg == 0) {
-            constexpr int PER = HD / 32, BATCH = HD == 256 ? 16 : 32;
-#pragma unroll 1
-            for (int x0 = 0; x0 < 32; x0 += BATCH) {
-                float v[BATCH][PER];  // a batch of rows in flight
+        {
+            constexpr int PER = HD / 32, B = 8, MINE = HD == 256 ? 16 : 32;
+            const int x_first = HD == 256 ? 16 * wg : 0;
+            const int n_rows = (int)min((int64_t)32, max((int64_t)0, (int64_t)rows - (R - lane)));  // of this warp's 32
+            const uint64_t row_q = reinterpret_cast<uint64_t>(q_of());
+            float v[2][B][PER];
+            auto load = [&](int x0, float(&w)[B][PER]) {
 #pragma unroll
-                for (int y = 0; y < BATCH; y++) {
-                    const float *src = reinterpret_cast<const float *>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(row.q), x0 + y));
+                for (int y = 0; y < B; y++) {
+                    const float *src = reinterpret_cast<const float *>(__shfl_sync(0xffffffffu, row_q, (x0 + y) & 31));
 #pragma unroll
                     for (int e = 0; e < PER; e += 2) {
                         const float2 z = x0 + y < n_rows ? *reinterpret_cast<const float2 *>(src + 32 * e + 2 * lane) : make_float2(0.0f, 0.0f);
-                        v[y][e] = z.x;
-                        v[y][e + 1] = z.y;
+                        w[y][e] = z.x;
+                        w[y][e + 1] = z.y;
                     }
                 }
+            };
+            auto convert = [&](int x0, const float(&w)[B][PER]) {
 #pragma unroll
-                for (int y = 0; y < BATCH; y++) {
+                for (int y = 0; y < B; y++) {
                     const uint32_t rr = (warp & 3) * 32 + x0 + y;
                     float top = 0.0f;
 #pragma unroll
-                    for (int e = 0; e < PER; e++) top = fmaxf(top, fabsf(v[y][e]));
+                    for (int e = 0; e < PER; e++) top = fmaxf(top, fabsf(w[y][e]));
                     top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
                     float up = 1.0f;
                     if (top > 0.0f && top < INFINITY) {
@@ -617,25 +617,32 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(PagedAttnArgs a,
 #pragma unroll
                     for (int e = 0; e < PER; e += 2) {
                         uint32_t h, l;
-                        split_f16x2(v[y][e] * sg, v[y][e + 1] * sg, h, l);
+                        split_f16x2(w[y][e] * sg, w[y][e + 1] * sg, h, l);
                         const uint32_t at = tile * 2 * S::QPLANE + (e / 2) * 16384 + sw128_offset(rr, 2 * lane);
                         *reinterpret_cast<uint32_t *>(smem + at) = h;
                         *reinterpret_cast<uint32_t *>(smem + at + S::QPLANE) = l;
                     }
                 }
+            };
+            load(x_first, v[0]);
+#pragma unroll 1
+            for (int x0 = x_first; x0 < x_first + MINE; x0 += 2 * B) {
+                load(x0 + B, v[1]);
+                convert(x0, v[0]);
+                if (x0 + 2 * B < x_first + MINE) load(x0 + 2 * B, v[0]);
+                convert(x0 + B, v[1]);
             }
             fence_async_smem();
         }
-        if constexpr (HD == 256) {  // the second group works on the same rows
-            if (wg == 0) {
-                tmem_st1(tmem + lane_base + S::X_COL, rf);
-                tmem_wait_st();
-            }
+        if constexpr (HD == 256) {  // the two groups have each other's rows' factors
+            tmem_st1(tmem + lane_base + S::X_COL + wg, rf);
+            tmem_wait_st();
             tc_fence_before();
             named_sync<2, 256>();
             tc_fence_after();
-            rf = tmem_ld1(tmem + lane_base + S::X_COL);
+            const float r0 = tmem_ld1(tmem + lane_base + S::X_COL), r1 = tmem_ld1(tmem + lane_base + S::X_COL + 1);
             tmem_wait_ld();
+            rf = lane < 16 ? r0 : r1;
             tc_fence_before();
             named_sync<2, 256>();
             tc_fence_after();
@@ -649,16 +656,16 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(PagedAttnArgs a,
         float m = -INFINITY, l = 0.0f, alpha = 1.0f;
         const uint32_t o_addr = tmem + lane_base + S::O_COL(tile) + half * 128;
         auto add_o = [&]() {  // o = o * alpha + this tile's product
-            uint32_t v[2][32];
+            uint32_t v[2][16];
             const float2 al2 = make_float2(alpha, alpha);
-            tmem_ld32(o_addr, v[0]);
+            tmem_ld16(o_addr, v[0]);
 #pragma unroll
-            for (int c = 0; c < OW; c += 32) {
-                uint32_t(&u)[32] = v[(c / 32) & 1];
+            for (int c = 0; c < OW; c += 16) {
+                uint32_t(&u)[16] = v[(c / 16) & 1];
                 tmem_wait_ld(u);
-                if (c + 32 < OW) tmem_ld32(o_addr + c + 32, v[(c / 32 + 1) & 1]);
+                if (c + 16 < OW) tmem_ld16(o_addr + c + 16, v[(c / 16 + 1) & 1]);
 #pragma unroll
-                for (int e = 0; e < 32; e += 2) {
+                for (int e = 0; e < 16; e += 2) {
                     const float2 x = ffma2(make_float2(o[c + e], o[c + e + 1]), al2,
                                            make_float2(__uint_as_float(u[e]), __uint_as_float(u[e + 1])));
                     o[c + e] = x.x;
@@ -670,54 +677,74 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(PagedAttnArgs a,
         for (uint32_t t = next_tile(0); t < tiles; t = next_tile(t + 1), jj++) {
             const int sb = HD == 256 ? (jj & 1) : tile;
             const uint32_t s_addr = tmem + lane_base + S::S_COL(sb) + half * 32;
-            const int64_t k0 = (int64_t)lo + t * KT + half * 32;
+            const int k0 = (int)(lo + t * KT) + half * 32;
             wait(s_full + sb, HD == 256 ? (jj / 2) & 1 : jj & 1);
             __syncwarp();
             tc_fence_after();
-            const bool whole = !docs && row.lo <= k0 && k0 + CW <= row.hi;
+            const bool whole = !docs && row_lo <= k0 && k0 + CW <= row_hi;
             const bool plain = __all_sync(0xffffffffu, whole || !real);
             // pass 1: the row's maximum; capped, biased or masked scores go back to tensor
             // memory.  Each load runs while the columns before it are worked on.
             float top = -INFINITY;
             {
-                uint32_t v[2][32];
-                tmem_ld32(s_addr, v[0]);
-                const int from = (int)max((int64_t)0, min((int64_t)CW, row.lo - k0));
-                const int to = (int)max((int64_t)0, min((int64_t)CW, row.hi - k0));
-                const float dist = (float)(row.i - k0);
-#pragma unroll
-                for (int c = 0; c < CW; c += 32) {
-                    uint32_t(&u)[32] = v[(c / 32) & 1];
+                uint32_t v[2][16];
+                tmem_ld16(s_addr, v[0]);
+                const int from = max(0, min(CW, row_lo - k0));
+                const int to = max(0, min(CW, row_hi - k0));
+                const float dist = (float)(row_i - k0);
+                constexpr int UNROLL = EXTRA ? 2 : CW / 16;  // the capped path is long: keep it in the instruction cache
+#pragma unroll UNROLL
+                for (int c = 0; c < CW; c += 16) {
+                    uint32_t(&u)[16] = v[(c / 16) & 1];
                     tmem_wait_ld(u);
-                    if (c + 32 < CW) tmem_ld32(s_addr + c + 32, v[(c / 32 + 1) & 1]);
+                    if (c + 16 < CW) tmem_ld16(s_addr + c + 16, v[(c / 16 + 1) & 1]);
                     if (!EXTRA && plain) {
                         float x0 = -INFINITY, x1 = -INFINITY;
 #pragma unroll
-                        for (int e = 0; e < 32; e += 4) {
+                        for (int e = 0; e < 16; e += 4) {
                             x0 = fmaxf(fmaxf(x0, __uint_as_float(u[e])), __uint_as_float(u[e + 1]));
                             x1 = fmaxf(fmaxf(x1, __uint_as_float(u[e + 2])), __uint_as_float(u[e + 3]));
                         }
                         top = fmaxf(top, fmaxf(x0, x1));
                         continue;
                     }
-                    bool small = true;
-                    if (EXTRA && a.softcap != 0.0f) {
+                    auto score = [&](auto small) {
+                        constexpr bool SMALL = decltype(small)::value;
+#pragma unroll
+                        for (int e = 0; e < 16; e++) {
+                            const float x = score_log2<SMALL>(__uint_as_float(u[e]), rf, a.softcap, row_slope,
+                                                              fabsf(dist - (float)(c + e)));
+                            u[e] = __float_as_uint(x);
+                        }
+                    };
+                    if (EXTRA) {
                         float big = 0.0f;
 #pragma unroll
-                        for (int e = 0; e < 32; e++) big = fmaxf(big, fabsf(__uint_as_float(u[e])));
-                        small = __all_sync(0xffffffffu, big * rf <= kTanhSmall);
+                        for (int e = 0; e < 16; e++) big = fmaxf(big, fabsf(__uint_as_float(u[e])));
+                        if (__all_sync(0xffffffffu, big * rf <= kTanhSmall))
+                            score(IntC<1>());
+                        else
+                            score(IntC<0>());
+                    }
+                    if (!plain) {
+                        uint32_t seen = to > c ? (to - c >= 16 ? 0xffffu : (1u << (to - c)) - 1u) : 0u;
+                        if (from > c) seen = from - c >= 16 ? 0u : seen & ~((1u << (from - c)) - 1u);
+                        if (docs) {
+                            const uint4 *dn = reinterpret_cast<const uint4 *>(docs_s + (jj % S::DOCS) * KT + half * 32 + c);
+#pragma unroll
+                            for (int e = 0; e < 4; e++) {
+                                const uint4 d = dn[e];
+                                seen &= ~((uint32_t)(d.x != row_doc) << (4 * e) | (uint32_t)(d.y != row_doc) << (4 * e + 1) |
+                                          (uint32_t)(d.z != row_doc) << (4 * e + 2) | (uint32_t)(d.w != row_doc) << (4 * e + 3));
+                            }
+                        }
+#pragma unroll
+                        for (int e = 0; e < 16; e++)
+                            if (!(seen >> e & 1u)) u[e] = 0xff800000u;  // -infinity
                     }
 #pragma unroll
-                    for (int e = 0; e < 32; e++) {
-                        float x = __uint_as_float(u[e]);
-                        if (EXTRA) x = score_log2(x, rf, a.softcap, row.slope, fabsf(dist - (float)(c + e)), small);
-                        bool seen = c + e >= from && c + e < to;
-                        if (docs) seen = seen && docs_s[(jj % S::DOCS) * KT + half * 32 + c + e] == row.doc;
-                        x = seen ? x : -INFINITY;
-                        top = fmaxf(top, x);
-                        u[e] = __float_as_uint(x);
-                    }
-                    tmem_st32(s_addr + c, u);
+                    for (int e = 0; e < 16; e++) top = fmaxf(top, __uint_as_float(u[e]));
+                    tmem_st16(s_addr + c, u);
                 }
                 if (EXTRA || !plain) tmem_wait_st();
             }
@@ -815,7 +842,7 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(PagedAttnArgs a,
         const bool fine = off == 0.0f;
         constexpr int PITCH = 36;
         float *st = reinterpret_cast<float *>(smem + tile * 2 * S::QPLANE) + (HD == 256 ? warp : warp & 3) * 32 * PITCH;
-        const uint64_t dst = reinterpret_cast<uint64_t>(a.out + (uint64_t)(c0 + token) * a.out_stride + (uint64_t)head * HD + half * 128);
+        const uint64_t dst = reinterpret_cast<uint64_t>(a.out + (uint64_t)(c0 + token_of()) * a.out_stride + (uint64_t)head_of() * HD + half * 128);
         const uint32_t fine_rows = __ballot_sync(0xffffffffu, fine && real);
 #pragma unroll
         for (int c = 0; c < OW; c += 32) {
@@ -835,8 +862,8 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(PagedAttnArgs a,
             }
         }
         if (real && !fine)
-            pp_slow_row(a, row, table, docs, kh, f0, half * 128, OW,
-                        a.out + (uint64_t)(c0 + token) * a.out_stride + (uint64_t)head * HD);
+            pp_slow_row(a, PpRow{q_of(), row_i, row_lo, row_hi, row_doc, row_slope}, table, docs, kh, f0, half * 128, OW,
+                        a.out + (uint64_t)(c0 + token_of()) * a.out_stride + (uint64_t)head_of() * HD);
         tc_fence_before();
     }
     __syncthreads();
