@@ -176,14 +176,16 @@ struct PagedAttnArgs {
     // scratch, set by the launcher
     float *part_o, *part_ml, *unit_ml, *scores;
     uint32_t *unit_info;
-    uint32_t row_blocks;            // 8-row blocks per (sequence, KV head) at most
+    uint32_t row_blocks;            // row blocks per (sequence, KV head) at most
+    uint32_t nsplit;                // lt_paged_prompt.cu: CTAs that share a row block's keys
     int *err;
 };
 size_t paged_attn_scratch(const PagedAttnArgs &a, int num_sms);
 cudaError_t launch_paged_attn(const LaunchCfg &c, PagedAttnArgs a, uint8_t *scratch);
-// Prompts over f16 caches on the tensor cores (lt_paged_prompt.cu); no scratch.
+// Prompts over f16 caches on the tensor cores (lt_paged_prompt.cu).
 bool paged_prompt_supported(const PagedAttnArgs &a);
-cudaError_t launch_paged_prompt(const LaunchCfg &c, PagedAttnArgs a);
+size_t paged_prompt_scratch(PagedAttnArgs a, int num_sms);
+cudaError_t launch_paged_prompt(const LaunchCfg &c, PagedAttnArgs a, uint8_t *scratch);
 
 // Eviction from a paged cache (lt_evict.cu).
 struct EvictArgs {

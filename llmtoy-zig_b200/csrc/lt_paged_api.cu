@@ -174,9 +174,11 @@ lt_status lt_paged_attn_prompt(lt_ctx *ctx, const lt_paged_attn_cfg *cfg, const 
     a.docs = dev_docs;
     a.doc_stride = (uint32_t)doc_stride;
     const lt::LaunchCfg c = lt::ctx_cfg(ctx);
-    if (lt::paged_prompt_supported(a))
-        return st_of(lt::ctx_launched(ctx, lt::launch_paged_prompt(c, a), "paged prompt attention"));
     uint8_t *scratch = nullptr;
+    if (lt::paged_prompt_supported(a)) {
+        if ((st = st_of(lt::ctx_scratch(ctx, lt::paged_prompt_scratch(a, c.num_sms), &scratch))) != LT_OK) return st;
+        return st_of(lt::ctx_launched(ctx, lt::launch_paged_prompt(c, a, scratch), "paged prompt attention"));
+    }
     if ((st = st_of(lt::ctx_scratch(ctx, lt::paged_attn_scratch(a, c.num_sms), &scratch))) != LT_OK) return st;
     return st_of(lt::ctx_launched(ctx, lt::launch_paged_attn(c, a, scratch), "paged prompt attention"));
 }

@@ -171,38 +171,42 @@ struct IntC {
     static constexpr int value = N;
 };
 
-// What one row sees and how it scores.
-struct PpRow {
-    const float *q;      // nullptr: no such row
-    int64_t i;           // position
-    int64_t lo, hi;      // keys [lo, hi), document aside
-    uint32_t doc;
-    float slope;
-};
-
 LT_DEVINL float pp_kv(const uint8_t *p, uint32_t d) { return __half2float(reinterpret_cast<const __half *>(p)[d]); }
 
-// The row by itself, key by key, masked keys never touched: for rows whose tile
-// result is not finite, which a value outside the row's own keys may have caused.
-__noinline__ __device__ void pp_slow_row(const PagedAttnArgs &a, PpRow r, const uint32_t *table,
-                                         const uint32_t *docs, uint32_t kh, float rf, uint32_t d0, uint32_t nd,
-                                         float *out) {
-    const uint32_t hd = a.kv.hd;
+// Row R of (sequence s, KV head kh) by itself, key by key, masked keys never
+// touched: for rows whose tile result is not finite, which a value outside the
+// row's own keys may have caused.  Output dims [d0, d0 + nd), nd a multiple of 16.
+__noinline__ __device__ void pp_slow_row(const PagedAttnArgs &a, uint32_t s, uint32_t kh, uint32_t R, uint32_t d0,
+                                         uint32_t nd) {
+    const uint32_t hd = a.kv.hd, cap = (uint32_t)min((uint64_t)a.kv.max_pages * a.kv.page_size, (uint64_t)a.max_len);
+    const uint32_t len = min(a.lens[s], cap), nq = a.cu[s + 1] - a.cu[s], q_row = a.cu[s] + R / a.group;
+    const uint32_t head = kh * a.group + R % a.group;
+    const float *q = a.q + (uint64_t)q_row * a.q_stride + (uint64_t)head * hd;
+    float *out = a.out + (uint64_t)q_row * a.out_stride + (uint64_t)head * hd;
+    const uint32_t *table = a.table + (uint64_t)s * a.kv.max_pages;
+    const uint32_t *docs = a.docs ? a.docs + (uint64_t)s * a.doc_stride : nullptr;
+    const int64_t i = (int64_t)len - nq + R / a.group;
+    int64_t lo = 0, hi = len;
+    if (a.window) lo = max((int64_t)0, i - (int64_t)a.window + 1);
+    if (a.causal) hi = min(hi, max(i + 1, a.prefix ? (int64_t)a.prefix[s] : (int64_t)0));
+    if (docs && i < 0) hi = 0;
+    const float slope = a.slopes ? a.slopes[head] : 0.0f;
+    const float f = a.softcap != 0.0f ? a.scale / a.softcap : a.scale * 1.4426950408889634f;
     float m = -INFINITY;
     for (uint32_t d = d0; d < d0 + nd; d += 16) {
         float o[16], l = 0.0f;
         for (int e = 0; e < 16; e++) o[e] = 0.0f;
         for (int pass = d == d0 ? 0 : 1; pass < 2; pass++) {
-            for (int64_t j = r.lo < 0 ? 0 : r.lo; j < r.hi; j++) {
-                if (docs && docs[j] != r.doc) continue;
+            for (int64_t j = lo; j < hi; j++) {
+                if (docs && docs[j] != docs[i]) continue;
                 const uint32_t page = table[j / a.kv.page_size];
                 if (page >= a.kv.n_pages) continue;
                 const uint64_t off = paged_offset(a.kv, page, (uint32_t)j, kh);
                 float dot = 0.0f;
-                for (uint32_t e = 0; e < hd; e++) dot = fmaf(r.q[e], pp_kv(a.kv.k + off, e), dot);
-                const float t = score_log2(dot, rf, a.softcap, r.slope, fabsf((float)(r.i - j)));
+                for (uint32_t e = 0; e < hd; e++) dot = fmaf(q[e], pp_kv(a.kv.k + off, e), dot);
+                const float t = score_log2(dot, f, a.softcap, slope, fabsf((float)(i - j)));
                 if (pass == 0) {
-                    m = t != t ? t : fmaxf(m, t);
+                    m = t != t || m != m ? NAN : fmaxf(m, t);
                 } else {
                     const float p = ex2(t - m);
                     l += p;
@@ -236,7 +240,9 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(PagedAttnArgs a,
     pdl_wait();
 
     // this CTA's rows; the longest (last) row blocks of a causal prompt come first
-    const uint32_t s = blockIdx.z, kh = blockIdx.y, rb = gridDim.x - 1 - blockIdx.x;
+    // (a row block may be shared by nsplit CTAs, each with its part of the keys)
+    const uint32_t s = blockIdx.z, kh = blockIdx.y, split = blockIdx.x % a.nsplit;
+    const uint32_t rb = gridDim.x / a.nsplit - 1 - blockIdx.x / a.nsplit;
     const uint32_t cap = (uint32_t)min((uint64_t)a.kv.max_pages * a.kv.page_size, (uint64_t)a.max_len);
     uint32_t len = a.lens[s];
     const uint32_t c0 = a.cu[s], c1 = a.cu[s + 1];
@@ -254,10 +260,11 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(PagedAttnArgs a,
     if (a.window) lo64 = max((int64_t)0, i0 - (int64_t)a.window + 1);
     const uint32_t hi = (uint32_t)max((int64_t)0, hi64), first = (uint32_t)min(lo64, (int64_t)hi);
     const uint32_t lo = maps.rows ? first - first % maps.rows : first;  // tiles start on a box
-    const uint32_t tiles = uniform((hi - lo + KT - 1) / KT);
+    const uint32_t all_tiles = (hi - lo + KT - 1) / KT, share = (all_tiles + a.nsplit - 1) / a.nsplit;
+    const uint32_t begin = uniform(min(all_tiles, split * share)), tiles = uniform(min(all_tiles, begin + share));
     const uint32_t *table = a.table + (uint64_t)s * a.kv.max_pages;
     const uint32_t *docs = a.docs ? a.docs + (uint64_t)s * a.doc_stride : nullptr;
-    const bool skipping = docs && tiles <= kPpSkipTiles;
+    const bool skipping = docs && all_tiles <= kPpSkipTiles;
 
     if (tid == 0) {
         for (int i = 0; i < NS; i++) {
@@ -288,7 +295,7 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(PagedAttnArgs a,
         dmin = __reduce_min_sync(0xffffffffu, dmin);
         dmax = __reduce_max_sync(0xffffffffu, dmax);
         __syncthreads();
-        for (uint32_t t = warp; t < tiles; t += kPpThreads / 32) {
+        for (uint32_t t = begin + warp; t < tiles; t += kPpThreads / 32) {
             uint32_t kmin = 0xffffffffu, kmax = 0;
 #pragma unroll
             for (int e = 0; e < KT / 32; e++) {
@@ -350,7 +357,7 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(PagedAttnArgs a,
                 mbar_arrive(full + stage);
             };
             uint32_t jj = 0, st = 0, turn = 0;  // tile count; ring stage and how often it went round
-            uint32_t t = next_tile(0);
+            uint32_t t = next_tile(begin);
             bool owed = false;                // the stage before st is copied but not handed on
             // tiles of whole boxes: every slot holds a cached position
             auto boxed = [&](uint32_t tt) {
@@ -507,7 +514,7 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(PagedAttnArgs a,
                 }
                 __syncwarp();
             };
-            uint32_t t = next_tile(0), jj = 0;
+            uint32_t t = next_tile(begin), jj = 0;
             if (t < tiles) {
                 // the queries are in place once both softmax groups have arrived on p_full the first time
                 wait(p_full + 0, 0);
@@ -674,7 +681,7 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(PagedAttnArgs a,
             }
         };
         uint32_t jj = 0;
-        for (uint32_t t = next_tile(0); t < tiles; t = next_tile(t + 1), jj++) {
+        for (uint32_t t = next_tile(begin); t < tiles; t = next_tile(t + 1), jj++) {
             const int sb = HD == 256 ? (jj & 1) : tile;
             const uint32_t s_addr = tmem + lane_base + S::S_COL(sb) + half * 32;
             const int k0 = (int)(lo + t * KT) + half * 32;
@@ -835,14 +842,22 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(PagedAttnArgs a,
         }
         // rows to the output through shared memory (this row tile's query planes are
         // no longer read), 32 columns at a time, so that stores fill whole lines
-        const float inv = l > 0.0f ? __fdiv_rn(1.0f, l) : (l == 0.0f ? 0.0f : l);
+        float inv = l > 0.0f ? __fdiv_rn(1.0f, l) : (l == 0.0f ? 0.0f : l);
         float off = l - l;
 #pragma unroll
         for (int e = 0; e < OW; e++) off += o[e] - o[e];
-        const bool fine = off == 0.0f;
+        bool fine = off == 0.0f;
         constexpr int PITCH = 36;
         float *st = reinterpret_cast<float *>(smem + tile * 2 * S::QPLANE) + (HD == 256 ? warp : warp & 3) * 32 * PITCH;
-        const uint64_t dst = reinterpret_cast<uint64_t>(a.out + (uint64_t)(c0 + token_of()) * a.out_stride + (uint64_t)head_of() * HD + half * 128);
+        uint64_t dst = reinterpret_cast<uint64_t>(a.out + (uint64_t)(c0 + token_of()) * a.out_stride + (uint64_t)head_of() * HD + half * 128);
+        if (a.nsplit > 1) {  // a record for k_paged_prompt_join: sums as they are, maximum and weight sum
+            const uint64_t rec = (((uint64_t)s * a.kv.n_kv + kh) * a.row_blocks + rb) * a.nsplit + split;
+            const uint64_t row = rec * S::ROWS + tile * 128 + r;
+            dst = reinterpret_cast<uint64_t>(a.part_o + row * HD + half * 128);
+            if (real && half == 0) *reinterpret_cast<float2 *>(a.part_ml + 2 * row) = make_float2(m, l);
+            inv = 1.0f;
+            fine = true;
+        }
         const uint32_t fine_rows = __ballot_sync(0xffffffffu, fine && real);
 #pragma unroll
         for (int c = 0; c < OW; c += 32) {
@@ -861,15 +876,67 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(PagedAttnArgs a,
                         *reinterpret_cast<const float4 *>(st + rr * PITCH + lane % 8 * 4);
             }
         }
-        if (real && !fine)
-            pp_slow_row(a, PpRow{q_of(), row_i, row_lo, row_hi, row_doc, row_slope}, table, docs, kh, f0, half * 128, OW,
-                        a.out + (uint64_t)(c0 + token_of()) * a.out_stride + (uint64_t)head_of() * HD);
+        if (real && !fine) pp_slow_row(a, s, kh, R, half * 128, OW);
         tc_fence_before();
     }
     __syncthreads();
     if (warp == 8) {
         tc_fence_after();
         tmem_dealloc(tmem, 512);
+    }
+}
+
+// Rows whose keys several CTAs share: one warp per row, the records in order.
+// Grid (row steps, n_kv, n_seq).
+constexpr int kPpJoinRows = 8;
+
+template <int HD>
+__global__ void __launch_bounds__(kPpJoinRows * 32) k_paged_prompt_join(PagedAttnArgs a) {
+    using S = PpShape<HD>;
+    constexpr int PER = HD / 64;  // float2 per lane
+    pdl_launch_dependents();
+    pdl_wait();
+    const uint32_t s = blockIdx.z, kh = blockIdx.y, R = blockIdx.x * kPpJoinRows + threadIdx.x / 32;
+    const int lane = threadIdx.x & 31;
+    const uint32_t c0 = a.cu[s], c1 = a.cu[s + 1];
+    if (!(c0 <= c1 && c1 <= a.total_q && c1 - c0 <= a.max_q) || R >= (c1 - c0) * a.group) return;
+    const uint64_t rec = (((uint64_t)s * a.kv.n_kv + kh) * a.row_blocks + R / S::ROWS) * a.nsplit;
+    const uint64_t row = rec * S::ROWS + R % S::ROWS;  // of split 0; a split's is S::ROWS further
+    float m = -INFINITY, l = 0.0f;
+    if ((uint32_t)lane < a.nsplit) {  // nsplit <= 32
+        const float2 ml = *reinterpret_cast<const float2 *>(a.part_ml + 2 * (row + (uint64_t)lane * S::ROWS));
+        m = ml.x;
+        l = ml.y;
+    }
+    float top = m;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const float w = m == -INFINITY ? 0.0f : ex2(m - top);
+    l = warp_sum(l * w);
+    float2 acc[PER];
+#pragma unroll
+    for (int e = 0; e < PER; e++) acc[e] = make_float2(0.0f, 0.0f);
+#pragma unroll 4
+    for (uint32_t i = 0; i < a.nsplit; i++) {
+        const float wi = __shfl_sync(0xffffffffu, w, i);
+        const float *src = a.part_o + (row + (uint64_t)i * S::ROWS) * HD + 2 * lane;
+#pragma unroll
+        for (int e = 0; e < PER; e++) {
+            const float2 v = *reinterpret_cast<const float2 *>(src + 64 * e);
+            acc[e].x = fmaf(v.x, wi, acc[e].x);
+            acc[e].y = fmaf(v.y, wi, acc[e].y);
+        }
+    }
+    const float inv = l > 0.0f ? __fdiv_rn(1.0f, l) : (l == 0.0f ? 0.0f : l);
+    float off = l - l;
+#pragma unroll
+    for (int e = 0; e < PER; e++) off += (acc[e].x - acc[e].x) + (acc[e].y - acc[e].y);
+    if (__all_sync(0xffffffffu, off == 0.0f)) {
+        float *dst = a.out + (uint64_t)(c0 + R / a.group) * a.out_stride + (uint64_t)(kh * a.group + R % a.group) * HD + 2 * lane;
+#pragma unroll
+        for (int e = 0; e < PER; e++) *reinterpret_cast<float2 *>(dst + 64 * e) = make_float2(acc[e].x * inv, acc[e].y * inv);
+    } else if (lane < HD / 16) {
+        pp_slow_row(a, s, kh, R, lane * 16, 16);
     }
 }
 
@@ -910,14 +977,35 @@ void pp_maps(const PagedKvDev &kv, uint32_t tile, PpMaps &m) {
     m.rows = rows;
 }
 
+// Row blocks that leave SMs without work share their keys among several CTAs:
+// as many as fill the SMs, each with at least two tiles of the longest row.
+template <int HD>
+void pp_split(PagedAttnArgs &a, int num_sms) {
+    using S = PpShape<HD>;
+    a.row_blocks = (uint32_t)(((uint64_t)a.max_q * a.group + S::ROWS - 1) / S::ROWS);
+    const uint64_t ctas = (uint64_t)a.row_blocks * a.kv.n_kv * a.n_seq, tiles = (a.max_len + S::KT - 1) / S::KT;
+    a.nsplit = (uint32_t)max((uint64_t)1, min(min((uint64_t)num_sms / ctas, tiles / 2), (uint64_t)32));
+}
+
+void pp_split(PagedAttnArgs &a, int num_sms) {
+    a.kv.hd == 64 ? pp_split<64>(a, num_sms) : a.kv.hd == 128 ? pp_split<128>(a, num_sms) : pp_split<256>(a, num_sms);
+}
+
+uint64_t pp_records(const PagedAttnArgs &a) {  // rows of all records
+    return (uint64_t)a.n_seq * a.kv.n_kv * a.row_blocks * a.nsplit * (a.kv.hd == 256 ? 128 : 256);
+}
+
 template <int HD, bool EXTRA>
 cudaError_t pp_launch(const LaunchCfg &c, const PagedAttnArgs &a) {
     using S = PpShape<HD>;
-    const uint64_t rows = (uint64_t)a.max_q * a.group;
     PpMaps maps;
     pp_maps(a.kv, S::KT, maps);
-    return launch_k(c, "paged_prompt", k_paged_prompt<HD, EXTRA>,
-                    dim3((uint32_t)((rows + S::ROWS - 1) / S::ROWS), a.kv.n_kv, a.n_seq), dim3(kPpThreads), S::SMEM, a, maps);
+    cudaError_t e = launch_k(c, "paged_prompt", k_paged_prompt<HD, EXTRA>, dim3(a.row_blocks * a.nsplit, a.kv.n_kv, a.n_seq),
+                             dim3(kPpThreads), S::SMEM, a, maps);
+    if (e != cudaSuccess || a.nsplit == 1) return e;
+    const uint32_t rows = a.max_q * a.group;
+    return launch_k(c, "paged_prompt_join", k_paged_prompt_join<HD>,
+                    dim3((rows + kPpJoinRows - 1) / kPpJoinRows, a.kv.n_kv, a.n_seq), dim3(kPpJoinRows * 32), 0, a);
 }
 
 // The register split needs the registers that 168 per thread give a block.
@@ -935,8 +1023,16 @@ bool paged_prompt_supported(const PagedAttnArgs &a) {
     return regs && a.kv.f16 && (uint64_t)a.max_q * a.group >= 64;
 }
 
-cudaError_t launch_paged_prompt(const LaunchCfg &c, PagedAttnArgs a) {
+size_t paged_prompt_scratch(PagedAttnArgs a, int num_sms) {
+    pp_split(a, num_sms);
+    return a.nsplit == 1 ? 0 : pp_records(a) * (a.kv.hd + 2) * 4;
+}
+
+cudaError_t launch_paged_prompt(const LaunchCfg &c, PagedAttnArgs a, uint8_t *scratch) {
     a.err = c.dev_err;
+    pp_split(a, c.num_sms);
+    a.part_o = (float *)scratch;
+    a.part_ml = a.part_o + (a.nsplit == 1 ? 0 : pp_records(a) * a.kv.hd);
     const bool extra = a.softcap != 0.0f || a.slopes;
     switch (a.kv.hd) {
     case 64: return extra ? pp_launch<64, true>(c, a) : pp_launch<64, false>(c, a);
