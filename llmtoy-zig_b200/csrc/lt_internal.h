@@ -144,7 +144,9 @@ struct PagedKvDev {
     uint64_t page_stride, slot_stride, head_stride;
     uint32_t n_kv, hd, f16;
     uint32_t page_size, n_pages, max_pages;
+    uint32_t page_shift;  // log2 of page_size, or kNoShift
 };
+constexpr uint32_t kNoShift = 0xffffffffu;
 
 // Rotated keys, values and queries of ntok tokens into / for a paged cache
 // (lt_paged_append.cu): launch_attn_prep's arithmetic per token.

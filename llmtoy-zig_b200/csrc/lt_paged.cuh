@@ -12,10 +12,18 @@
 
 namespace lt {
 
+// Page of a position and its slot there; a shift for the usual page sizes.
+LT_DEVINL uint32_t page_of(const PagedKvDev &kv, uint32_t j) {
+    return kv.page_shift != kNoShift ? j >> kv.page_shift : j / kv.page_size;
+}
+LT_DEVINL uint32_t slot_of(const PagedKvDev &kv, uint32_t j) {
+    return kv.page_shift != kNoShift ? j & (kv.page_size - 1) : j % kv.page_size;
+}
+
 // Byte offset of position j of a sequence (its page-table row `row`) for head
 // h, or ~0 when the page id lies outside the pool (the caller reports it).
 LT_DEVINL uint64_t paged_offset(const PagedKvDev &kv, uint32_t page, uint32_t j, uint32_t h) {
-    return (uint64_t)page * kv.page_stride + (uint64_t)(j % kv.page_size) * kv.slot_stride +
+    return (uint64_t)page * kv.page_stride + (uint64_t)slot_of(kv, j) * kv.slot_stride +
            (uint64_t)h * kv.head_stride;
 }
 

@@ -40,6 +40,9 @@ lt_status paged_kv(lt_ctx *ctx, const lt_paged_kv *kv, const char *who, lt::Page
     d.page_size = kv->page_size;
     d.n_pages = kv->n_pages;
     d.max_pages = kv->max_pages;
+    d.page_shift = lt::kNoShift;
+    for (uint32_t i = 0; i < 32; i++)
+        if (kv->page_size == 1u << i) d.page_shift = i;
     return LT_OK;
 }
 

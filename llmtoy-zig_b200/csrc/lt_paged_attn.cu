@@ -27,7 +27,7 @@
 
 namespace lt {
 
-constexpr int kPaWarps = 4, kPaThreads = kPaWarps * 32, kPaStages = 3, kPaRows = 8;
+constexpr int kPaWarps = 4, kPaThreads = kPaWarps * 32, kPaRows = 8;
 constexpr int kMassThreads = 256, kMassKeys = 1024;
 
 template <int HD, bool F16>
@@ -37,10 +37,11 @@ struct PaShape {
     static constexpr int ROW = HD * (F16 ? 2 : 4);          // bytes
     static constexpr int KP = ROW + (F16 ? 16 : 64), VP = ROW + 16;
     static constexpr int BLOCK = KB * (KP + VP);
+    static constexpr int STAGES = 3;
     static constexpr int QSTEPS = F16 ? HD / 16 : HD / 8;   // k-steps of 512-byte operand fragments
-    static constexpr int RING = BLOCK * kPaStages * kPaWarps;
+    static constexpr int RING = BLOCK * STAGES * kPaWarps;
     static constexpr int QBYTES = QSTEPS * 512;
-    static constexpr int MERGE = 2 * kPaRows * (HD + 2) * 4;
+    static constexpr int MERGE = kPaRows * (HD + 2) * 4;
     static constexpr int UNION = QBYTES > MERGE ? QBYTES : MERGE;
     static constexpr int SMEM = RING + UNION + 16 * 8 * kPaWarps + 64;
     static constexpr int CTAS = HD == 256 ? 1 : HD == 128 ? 2 : 3;
@@ -50,6 +51,7 @@ struct PaShape {
 struct PaSeq {
     uint32_t len, nq, q0;   // cached positions, query tokens, first query row
     uint32_t lo;            // first position any query sees
+    uint32_t base;          // where its tiles start: lo, or the block of 16 it lies in
     uint32_t blocks, tiles; // 8-row blocks per KV head, tiles per unit
 };
 
@@ -76,7 +78,8 @@ LT_DEVINL PaSeq pa_seq(const PagedAttnArgs &a, uint32_t s, uint32_t tile, bool r
         q.lo = a.window && n > a.window ? n - a.window : 0;
         q.blocks = (a.group + kPaRows - 1) / kPaRows;
     }
-    q.tiles = max(1u, (n - q.lo + tile - 1) / tile);
+    q.base = q.lo & ~15u;  // blocks then lie within pages whose size is a multiple of theirs
+    q.tiles = max(1u, (n - q.base + tile - 1) / tile);
     if (bad && report) atomicExch(a.err, DEV_ERR_BAD_INDEX);
     return q;
 }
@@ -88,12 +91,14 @@ struct PaWalk {
     PaSeq q;
     uint32_t kh, rb;
     uint32_t lo, hi;         // positions that this unit's rows can see
+    uint32_t base;
 
     LT_DEVINL void set_unit(const PagedAttnArgs &a) {
         kh = q.blocks ? unit / q.blocks : 0;
         rb = q.blocks ? unit % q.blocks : 0;
         lo = q.lo;
         hi = q.len;
+        base = q.base;
         if (PROMPT) {
             const uint32_t rows = q.nq * a.group;  // nq <= max_q: checked on the host not to overflow
             const uint32_t t0 = rb * kPaRows / a.group, t1 = (min(rows, rb * kPaRows + kPaRows) - 1) / a.group;
@@ -135,7 +140,8 @@ LT_DEVINL uint64_t pa_unit(const PagedAttnArgs &a, uint32_t s, uint32_t kh, uint
     return ((uint64_t)s * a.kv.n_kv + kh) * a.row_blocks + rb;
 }
 
-template <int HD, bool F16, bool PROMPT>
+// PLAIN: neither cap nor distance bias.
+template <int HD, bool F16, bool PROMPT, bool PLAIN>
 __global__ void __launch_bounds__(kPaThreads, PaShape<HD, F16>::CTAS) k_paged_attn(PagedAttnArgs a) {
     using S = PaShape<HD, F16>;
     constexpr int KB = S::KB, TILE = S::TILE, NB = HD / 8;
@@ -144,7 +150,7 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<HD, F16>::CTAS) k_paged_at
     __shared__ uint64_t s_rem;
     __shared__ uint32_t s_seq;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, j4 = lane & 3;
-    uint8_t *ring = smem + warp * (S::BLOCK * kPaStages);
+    uint8_t *ring = smem + warp * (S::BLOCK * S::STAGES);
     uint8_t *qm = smem + S::RING;  // query fragments, then the merge records
     uint64_t *offs = reinterpret_cast<uint64_t *>(smem + S::RING + S::UNION) + warp * 16;
     float *rowf = reinterpret_cast<float *>(smem + S::RING + S::UNION + 16 * 8 * kPaWarps);
@@ -202,35 +208,68 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<HD, F16>::CTAS) k_paged_at
     cw.set_unit(a);
     lw = cw;
 
-    // lane r < KB looks up row r of the block to copy next
+    // The block to copy next: where whole blocks lie within pages, its page is looked up
+    // once and its rows are a stride apart; else lane r < KB looks up row r.
+    constexpr int CH = S::ROW / 16, STEP = 32 / (CH < 32 ? CH : 32);
+    const bool in_page = a.kv.page_size % KB == 0;
+    const int row0 = CH < 32 ? lane / CH : 0, col0 = CH < 32 ? lane % CH : lane;
+    const uint64_t lane_off = (uint64_t)row0 * a.kv.slot_stride + col0 * 16, step_off = STEP * a.kv.slot_stride;
     uint32_t page = 0, key = 0;
-    bool take = false;
     auto look = [&]() {
-        key = lw.q.lo + lw.tile * TILE + warp * KB + lane;
-        take = lane < KB && key < lw.hi && key >= lw.lo;
-        if (take) {
-            page = a.table[(uint64_t)lw.s * a.kv.max_pages + key / a.kv.page_size];
-        }
+        key = lw.base + lw.tile * TILE + warp * KB + (in_page ? 0 : lane);
+        page = a.kv.n_pages;
+        if (in_page ? key < lw.hi && key + KB > lw.lo : lane < KB && key < lw.hi && key >= lw.lo)
+            page = a.table[(uint64_t)lw.s * a.kv.max_pages + page_of(a.kv, key)];
+        else
+            key = 0xffffffffu;
     };
     auto copy = [&](int stage) {
+        bool take = key != 0xffffffffu;
         if (take && page >= a.kv.n_pages) {
             take = false;
             atomicExch(a.err, DEV_ERR_BAD_INDEX);
         }
+        const uint32_t kdst = ring_u + stage * S::BLOCK + row0 * S::KP + col0 * 16;
+        const uint32_t vdst = ring_u + stage * S::BLOCK + KB * S::KP + row0 * S::VP + col0 * 16;
+        if (in_page) {
+            const uint64_t o = take ? paged_offset(a.kv, page, key, lw.kh) + lane_off : 0;
+            const uint8_t *pk = a.kv.k + o, *pv = a.kv.v + o;
+            if (take && key >= lw.lo && key + KB <= lw.hi) {
+#pragma unroll
+                for (int r = 0; r < KB; r += STEP) {
+#pragma unroll
+                    for (int x = 0; x < CH; x += 32) {
+                        cp_async16(kdst + r * S::KP + x * 16, pk + x * 16, true);
+                        cp_async16(vdst + r * S::VP + x * 16, pv + x * 16, true);
+                    }
+                    pk += step_off;
+                    pv += step_off;
+                }
+            } else {
+#pragma unroll
+                for (int r = 0; r < KB; r += STEP) {
+                    const bool t = take && key + r + row0 >= lw.lo && key + r + row0 < lw.hi;
+#pragma unroll
+                    for (int x = 0; x < CH; x += 32) {
+                        cp_async16(kdst + r * S::KP + x * 16, t ? pk + x * 16 : a.kv.k, t);
+                        cp_async16(vdst + r * S::VP + x * 16, t ? pv + x * 16 : a.kv.v, t);
+                    }
+                    pk += step_off;
+                    pv += step_off;
+                }
+            }
+            return;
+        }
         __syncwarp();
         if (lane < KB) offs[lane] = take ? paged_offset(a.kv, page, key, lw.kh) : ~0ull;
         __syncwarp();
-        constexpr int CH = S::ROW / 16, STEP = 32 / (CH < 32 ? CH : 32);
-        const uint32_t kdst = ring_u + stage * S::BLOCK, vdst = kdst + KB * S::KP;
 #pragma unroll
-        for (int r0 = 0; r0 < KB; r0 += STEP) {
-            const int r = r0 + (CH < 32 ? lane / CH : 0);
-            const uint64_t o = offs[r];
+        for (int r = 0; r < KB; r += STEP) {
+            const uint64_t o = offs[r + row0];
             const bool t = o != ~0ull;
 #pragma unroll
-            for (int x0 = 0; x0 < CH; x0 += 32) {
-                const int x = x0 + (CH < 32 ? lane % CH : lane);
-                const uint64_t src = t ? o + x * 16 : 0;
+            for (int x = 0; x < CH; x += 32) {
+                const uint64_t src = t ? o + (x + col0) * 16 : 0;
                 cp_async16(kdst + r * S::KP + x * 16, a.kv.k + src, t);
                 cp_async16(vdst + r * S::VP + x * 16, a.kv.v + src, t);
             }
@@ -240,7 +279,7 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<HD, F16>::CTAS) k_paged_at
     uint64_t ahead = 0;
     look();
 #pragma unroll
-    for (int st = 0; st < kPaStages - 1; st++) {
+    for (int st = 0; st < S::STAGES - 1; st++) {
         if (ahead < nf) {
             copy(st);
             ahead++;
@@ -321,17 +360,18 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<HD, F16>::CTAS) k_paged_at
         const float rf = rowf[g];
         const uint32_t head = cw.kh * a.group + R % a.group;
         const float slope = a.slopes && (uint32_t)g < rows ? a.slopes[head] : 0.0f;
-        int64_t row_i = (int64_t)cw.q.len - cw.q.nq + R / a.group;
-        int64_t row_lo = cw.q.lo, row_hi = cw.q.len;
+        // positions are 32 bits wide here: a length is at most 2^30, and a query before position 0 below -2^31 is clamped
+        const int row_i = (int)max((int64_t)cw.q.len - cw.q.nq + R / a.group, (int64_t)-0x7fffffff);
+        int row_lo = cw.q.lo, row_hi = cw.q.len;
         uint32_t my_doc = 0;
         const uint32_t *docs = nullptr;
         if (PROMPT) {
             if (a.causal) {
                 row_hi = row_i + 1;
-                if (a.prefix) row_hi = max(row_hi, (int64_t)a.prefix[cw.s]);
-                row_hi = min(row_hi, (int64_t)cw.q.len);
+                if (a.prefix) row_hi = (int)max((int64_t)row_hi, (int64_t)a.prefix[cw.s]);
+                row_hi = min(row_hi, (int)cw.q.len);
             }
-            row_lo = a.window ? row_i - (int64_t)a.window + 1 : 0;
+            row_lo = a.window ? (int)max((int64_t)0, (int64_t)row_i - a.window + 1) : 0;
             if (a.docs) {
                 docs = a.docs + (uint64_t)cw.s * a.doc_stride;
                 if ((uint32_t)g < rows && row_i >= 0)
@@ -340,21 +380,24 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<HD, F16>::CTAS) k_paged_at
                     row_hi = 0;
             }
         }
-        float o[NB][4];
+        // Sums in registers; each block's product is computed from zero and added here: the tensor
+        // core truncates where it accumulates, and so do long chains of products (hence C chains below).
+        float o[NB][2];
 #pragma unroll
-        for (int n = 0; n < NB; n++) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
+        for (int n = 0; n < NB; n++) o[n][0] = o[n][1] = 0.0f;
         float m = -INFINITY, l = 0.0f;
 
         for (uint32_t it = 0; it < seg; it++) {
-            cp_async_wait<kPaStages - 2>();
+            cp_async_wait<S::STAGES - 2>();
             __syncwarp();
-            const uint32_t k0 = cw.q.lo + cw.tile * TILE + warp * KB;  // the block's first position
+            const uint32_t k0 = cw.base + cw.tile * TILE + warp * KB;  // the block's first position
             if (k0 < cw.hi && k0 + KB > cw.lo) {
                 const uint32_t kb = ring_u + stage * S::BLOCK, vb = kb + KB * S::KP;
                 constexpr int NS = KB / 4;  // scores per thread: keys k0 + 8 (n / 2) + 2 j4 + n % 2
                 float sc[NS];
                 if constexpr (F16) {
-                    float s0[4] = {}, s1[4] = {};
+                    constexpr int C = HD == 256 ? 4 : 2;
+                    float s0[C][4] = {}, s1[C][4] = {};
                     const uint32_t ka = kb + ((lane >> 4) * 8 + (lane & 7)) * S::KP + ((lane >> 3) & 1) * 16;
 #pragma unroll
                     for (int i = 0; i < S::QSTEPS; i++) {
@@ -368,17 +411,25 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<HD, F16>::CTAS) k_paged_at
                             qa[0] = __float_as_uint(t.x), qa[1] = __float_as_uint(t.y);
                             qa[2] = __float_as_uint(t.z), qa[3] = __float_as_uint(t.w);
                         }
-                        mma_f16(s0, qa, b[0], b[1]);
-                        mma_f16(s1, qa, b[2], b[3]);
+                        mma_f16(s0[i % C], qa, b[0], b[1]);
+                        mma_f16(s1[i % C], qa, b[2], b[3]);
                     }
-                    sc[0] = s0[0] + s0[2];
-                    sc[1] = s0[1] + s0[3];
-                    sc[2] = s1[0] + s1[2];
-                    sc[3] = s1[1] + s1[3];
+#pragma unroll
+                    for (int n = 0; n < NS; n++) {
+                        const float(&x)[C][4] = n < 2 ? s0 : s1;
+                        sc[n] = x[0][n & 1] + x[1][n & 1];
+                        float lo = x[0][2 + (n & 1)] + x[1][2 + (n & 1)];
+                        if (C == 4) {
+                            sc[n] += x[C - 2][n & 1] + x[C - 1][n & 1];
+                            lo += x[C - 2][2 + (n & 1)] + x[C - 1][2 + (n & 1)];
+                        }
+                        sc[n] += lo;
+                    }
                 } else {
-                    float s0[4] = {}, s1[4] = {};
+                    constexpr int C = HD / 64;  // chains of 4 (high terms of K) and 8 products
+                    float s0[2 * C][4] = {}, s1[C][4] = {};
                     const uint32_t ka = kb + g * S::KP + j4 * 16;
-#pragma unroll 4
+#pragma unroll
                     for (int i = 0; i < HD / 16; i++) {
                         const float4 t = lds128(ka + i * 64);
                         const float kv4[4] = {t.x, t.y, t.z, t.w};
@@ -390,45 +441,44 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<HD, F16>::CTAS) k_paged_at
                             const float4 u = lds128(qm_u + (2 * i + e) * 512 + lane * 16);
                             const uint32_t qa[4] = {__float_as_uint(u.x), __float_as_uint(u.y), __float_as_uint(u.z),
                                                     __float_as_uint(u.w)};
-                            mma_tf32(s0, qa, bh[2 * e], bh[2 * e + 1]);
-                            mma_tf32(s1, qa, bl[2 * e], bl[2 * e + 1]);
+                            mma_tf32(s0[i % (2 * C)], qa, bh[2 * e], bh[2 * e + 1]);
+                            mma_tf32(s1[i % C], qa, bl[2 * e], bl[2 * e + 1]);
                         }
                     }
-                    sc[0] = (s0[0] + s1[0]) + (s0[2] + s1[2]);
-                    sc[1] = (s0[1] + s1[1]) + (s0[3] + s1[3]);
+#pragma unroll
+                    for (int n = 0; n < 2; n++) {
+                        float hi = 0.0f, lo = 0.0f;
+#pragma unroll
+                        for (int c = 0; c < 2 * C; c++) hi += s0[c][n], lo += s0[c][2 + n];
+#pragma unroll
+                        for (int c = 0; c < C; c++) lo += s1[c][n] + s1[c][2 + n];
+                        sc[n] = hi + lo;
+                    }
                 }
                 float top = -INFINITY;
+                const bool whole = !PROMPT && k0 >= cw.lo && k0 + KB <= cw.hi;
 #pragma unroll
                 for (int n = 0; n < NS; n++) {
-                    const uint32_t j = k0 + 8 * (n / 2) + 2 * j4 + (n & 1);
-                    sc[n] = score_log2(sc[n], rf, a.softcap, slope, fabsf((float)(row_i - (int64_t)j)));
-                    bool seen;
+                    const int j = (int)k0 + 8 * (n / 2) + 2 * j4 + (n & 1);
+                    sc[n] = PLAIN ? sc[n] * rf : score_log2(sc[n], rf, a.softcap, slope, fabsf((float)row_i - (float)j));
                     if (PROMPT) {
-                        seen = (int64_t)j >= row_lo && (int64_t)j < row_hi;
+                        bool seen = j >= row_lo && j < row_hi;
                         if (docs && seen) seen = docs[j] == my_doc;
+                        if (!seen) sc[n] = -INFINITY;
                     } else {
-                        seen = j < cw.q.len;
+                        const bool seen = whole || (j >= row_lo && j < row_hi);
                         if (a.mass && seen && (uint32_t)g < rows)
                             a.scores[((uint64_t)cw.s * a.n_heads + head) * a.max_len + j] = sc[n];
+                        if (!seen) sc[n] = -INFINITY;
                     }
-                    if (!seen) sc[n] = -INFINITY;
                     top = fmaxf(top, sc[n]);
                 }
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
                 const float mn = fmaxf(m, top);
-                if (__any_sync(0xffffffffu, mn > m)) {
-                    const float al = mn > m ? ex2(m - mn) : 1.0f;  // m = -inf: 0
-                    l *= al;
-#pragma unroll
-                    for (int n = 0; n < NB; n++) {
-                        o[n][0] *= al;
-                        o[n][1] *= al;
-                        o[n][2] *= al;
-                        o[n][3] *= al;
-                    }
-                    m = mn;
-                }
+                const float al = mn > m ? ex2(m - mn) : 1.0f;  // m = -inf: 0
+                l *= al;
+                m = mn;
                 // weights scaled by 2^10 so that small ones keep their f16 bits; l carries the same factor
                 const float base = m == -INFINITY ? 0.0f : m - (F16 ? 10.0f : 0.0f);
 #pragma unroll
@@ -445,8 +495,13 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<HD, F16>::CTAS) k_paged_at
                     for (int n = 0; n < NB; n += 2) {
                         uint32_t b[4];
                         ldsm4_t(b, va + n * 16);
-                        mma_f16(o[n], pa, b[0], b[1]);
-                        mma_f16(o[n + 1], pa, b[2], b[3]);
+                        float c0[4] = {}, c1[4] = {};
+                        mma_f16(c0, pa, b[0], b[1]);
+                        mma_f16(c1, pa, b[2], b[3]);
+                        o[n][0] = fmaf(o[n][0], al, c0[0] + c0[2]);
+                        o[n][1] = fmaf(o[n][1], al, c0[1] + c0[3]);
+                        o[n + 1][0] = fmaf(o[n + 1][0], al, c1[0] + c1[2]);
+                        o[n + 1][1] = fmaf(o[n + 1][1], al, c1[1] + c1[3]);
                     }
                 } else {
                     // operand index j4 is key 2 j4, index j4 + 4 key 2 j4 + 1; column g of product c is dim 32 i + 4 g + c
@@ -463,15 +518,18 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<HD, F16>::CTAS) k_paged_at
                             uint32_t h0, l0, h1, l1;
                             split_tf32(x0[e], h0, l0);
                             split_tf32(x1[e], h1, l1);
-                            mma_tf32(o[4 * i + e], pa, h0, h1);
-                            mma_tf32(o[4 * i + e], pa, l0, l1);
+                            float c0[4] = {};
+                            mma_tf32(c0, pa, l0, l1);
+                            mma_tf32(c0, pa, h0, h1);
+                            o[4 * i + e][0] = fmaf(o[4 * i + e][0], al, c0[0] + c0[2]);
+                            o[4 * i + e][1] = fmaf(o[4 * i + e][1], al, c0[1] + c0[3]);
                         }
                     }
                 }
             }
             __syncwarp();
-            int fill = stage + kPaStages - 1;
-            if (fill >= kPaStages) fill -= kPaStages;
+            int fill = stage + S::STAGES - 1;
+            if (fill >= S::STAGES) fill -= S::STAGES;
             if (ahead < nf) {
                 copy(fill);
                 ahead++;
@@ -481,24 +539,19 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<HD, F16>::CTAS) k_paged_at
                 }
             }
             cp_async_commit();
-            if (++stage == kPaStages) stage = 0;
+            if (++stage == S::STAGES) stage = 0;
             if (it + 1 < seg) cw.tile++;
         }
 
-        // ── merge the warps: 2 and 3 into 0 and 1, then 1 into 0 ──
+        // ── merge the warps into warp 0, in their order ──
         l += __shfl_xor_sync(0xffffffffu, l, 1);
         l += __shfl_xor_sync(0xffffffffu, l, 2);
-#pragma unroll
-        for (int n = 0; n < NB; n++) {
-            o[n][0] += o[n][2];
-            o[n][1] += o[n][3];
-        }
         auto dim = [&](int n, int e) { return F16 ? 8 * n + 2 * j4 + e : 32 * (n / 4) + 8 * j4 + 4 * e + n % 4; };
         __syncthreads();  // every warp is done with the query fragments
-#pragma unroll
-        for (int half = kPaWarps / 2; half >= 1; half /= 2) {
-            float *rec = reinterpret_cast<float *>(qm) + (warp % half) * kPaRows * (HD + 2) + g * (HD + 2);
-            if (warp >= half && warp < 2 * half) {
+#pragma unroll 1
+        for (int from = 1; from < kPaWarps; from++) {
+            float *rec = reinterpret_cast<float *>(qm) + g * (HD + 2);
+            if (warp == from) {
 #pragma unroll
                 for (int n = 0; n < NB; n++) {
                     rec[dim(n, 0)] = o[n][0];
@@ -510,7 +563,7 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<HD, F16>::CTAS) k_paged_at
                 }
             }
             __syncthreads();
-            if (warp < half) {
+            if (warp == 0) {
                 const float m2 = rec[HD], mn = fmaxf(m, m2);
                 const float w1 = m == -INFINITY ? 0.0f : ex2(m - mn), w2 = m2 == -INFINITY ? 0.0f : ex2(m2 - mn);
                 l = l * w1 + rec[HD + 1] * w2;
@@ -714,8 +767,13 @@ uint32_t pa_grid(uint32_t hd, int num_sms) { return (uint32_t)num_sms * (hd == 2
 
 template <int HD, bool F16, bool PROMPT>
 cudaError_t pa_launch(const LaunchCfg &c, const PagedAttnArgs &a, uint64_t units) {
-    cudaError_t e = launch_k(c, PROMPT ? "paged_attn_rows" : "paged_attn", k_paged_attn<HD, F16, PROMPT>,
-                             dim3(pa_grid(HD, c.num_sms)), dim3(kPaThreads), PaShape<HD, F16>::SMEM, a);
+    const char *label = PROMPT ? "paged_attn_rows" : "paged_attn";
+    const dim3 grid(pa_grid(HD, c.num_sms));
+    cudaError_t e;
+    if (a.softcap == 0.0f && !a.slopes)
+        e = launch_k(c, label, k_paged_attn<HD, F16, PROMPT, true>, grid, dim3(kPaThreads), PaShape<HD, F16>::SMEM, a);
+    else
+        e = launch_k(c, label, k_paged_attn<HD, F16, PROMPT, false>, grid, dim3(kPaThreads), PaShape<HD, F16>::SMEM, a);
     if (e != cudaSuccess) return e;
     e = launch_k(c, "paged_join", k_paged_join<HD, PROMPT>, dim3((uint32_t)units, kPaRows), dim3(128), 0, a);
     if (e != cudaSuccess || PROMPT || !a.mass) return e;
