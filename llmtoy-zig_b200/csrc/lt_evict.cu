@@ -5,7 +5,7 @@
 // accumulated weight (the lowest position first among equals).  What stays keeps
 // its order; its K and V rows and its weights move to slots 0 .. budget - 1.
 //
-// k_evict_select: one CTA per (sequence, KV head).  The weights become
+// k_evict_select: one CTA per (sequence, KV head), or a cluster of four.  The weights become
 // order-preserving 32-bit keys; three passes of 11, 11 and 10 bits narrow the
 // budget-th largest key down (histograms in shared memory), and one ordered
 // pass writes what stays: a kept position's slot is the number of larger keys
@@ -15,13 +15,18 @@
 // position >= i, so a CTA that goes up in steps, reading a step before it writes
 // it, never overwrites what a later step reads; 32-byte columns of the rows are
 // independent of each other and give the parallelism.
+#include <cooperative_groups.h>
+
 #include "lt_paged.cuh"
 
 namespace lt {
 
+namespace cg = cooperative_groups;
+
 constexpr int kSelThreads = 1024;
 constexpr int kSelPer = 4;
 constexpr int kSelBins = 2048;
+constexpr uint32_t kSelCluster = 8192;  // rows longer than this take a cluster
 constexpr int kMoveThreads = 256;
 constexpr int kMoveRows = 64;
 
@@ -58,13 +63,23 @@ LT_DEVINL uint64_t block_excl(uint64_t v, uint64_t *s_warp, uint64_t *total) {
     return x - v + (warp ? s_warp[warp - 1] : 0);
 }
 
+// CL CTAs (a cluster) per (sequence, KV head), each with a contiguous part of the positions.
+template <int CL>
 __global__ void __launch_bounds__(kSelThreads) k_evict_select(EvictArgs a) {
     __shared__ uint32_t s_hist[kSelBins];
-    __shared__ uint64_t s_warp[32];
+    __shared__ uint64_t s_warp[32], s_mine;
     __shared__ uint32_t s_bin, s_left;
     pdl_launch_dependents();
     pdl_wait();
-    const uint32_t h = blockIdx.x, s = blockIdx.y, tid = threadIdx.x;
+    const cg::cluster_group cluster = cg::this_cluster();
+    const uint32_t rank = CL > 1 ? cluster.block_rank() : 0, tid = threadIdx.x;
+    auto sync_all = [&]() {
+        if constexpr (CL > 1)
+            cluster.sync();
+        else
+            __syncthreads();
+    };
+    const uint32_t h = blockIdx.x / CL, s = blockIdx.y;
     const uint64_t pair = (uint64_t)s * a.kv.n_kv + h;
     uint32_t n = a.lens[s];
     if (n > a.max_len || (n + a.kv.page_size - 1) / a.kv.page_size > a.kv.max_pages) {
@@ -75,9 +90,27 @@ __global__ void __launch_bounds__(kSelThreads) k_evict_select(EvictArgs a) {
     const float *mass = a.mass + pair * a.mass_stride;
     float *mass_out = a.mass_out + pair * a.mass_out_stride;
     uint32_t *kept = a.kept + pair * a.budget;
-    if (h == 0 && tid == 0) a.new_len[s] = keep;
+    if (h == 0 && rank == 0 && tid == 0) a.new_len[s] = keep;
     const uint32_t old = n > a.budget ? n - a.recent : 0;  // positions that compete
     uint32_t want = n > a.budget ? a.budget - a.recent : 0;
+    constexpr uint32_t CHUNK = kSelThreads * kSelPer;
+    const uint32_t part = ((n + CL - 1) / CL + CHUNK - 1) / CHUNK * CHUNK;
+    const uint32_t from = min(n, rank * part), to = min(n, from + part);  // this CTA's positions
+    const bool wide = (reinterpret_cast<uintptr_t>(mass) & 15) == 0;
+
+    // four weights in a row per thread and chunk; a part of one chunk is loaded once
+    float m[kSelPer];
+    auto load = [&](uint32_t j, float(&w)[kSelPer]) {
+        if (wide && j + kSelPer <= to) {
+            const float4 v = *reinterpret_cast<const float4 *>(mass + j);
+            w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+        } else {
+#pragma unroll
+            for (int u = 0; u < kSelPer; u++) w[u] = j + u < to ? mass[j + u] : 0.0f;
+        }
+    };
+    const bool once = to - from <= CHUNK;
+    if (once) load(from + tid * kSelPer, m);
 
     // the want-th largest key among the first `old`, bits from the top
     uint32_t prefix = 0, done = 0;
@@ -85,24 +118,37 @@ __global__ void __launch_bounds__(kSelThreads) k_evict_select(EvictArgs a) {
         const int bits = pass == 2 ? 10 : 11, shift = 32 - (int)done - bits, bins = 1 << bits;
         for (int i = tid; i < kSelBins; i += kSelThreads) s_hist[i] = 0;
         __syncthreads();
-        for (uint32_t j0 = 0; j0 < old; j0 += kSelThreads * 8) {
-            float m[8];
+        auto count = [&](uint32_t j, const float(&w)[kSelPer]) {
 #pragma unroll
-            for (int u = 0; u < 8; u++) {
-                const uint32_t j = j0 + u * kSelThreads + tid;
-                m[u] = j < old ? mass[j] : 0.0f;
-            }
-#pragma unroll
-            for (int u = 0; u < 8; u++) {
-                const uint32_t k = mass_key(m[u]);
-                if (j0 + u * kSelThreads + tid < old && (done == 0 || k >> (32 - done) == prefix))
+            for (int u = 0; u < kSelPer; u++) {
+                const uint32_t k = mass_key(w[u]);
+                if (j + u < old && j + u < to && (done == 0 || k >> (32 - done) == prefix))
                     atomicAdd(&s_hist[(k >> shift) & (bins - 1)], 1u);
             }
+        };
+        if (once) {
+            count(from + tid * kSelPer, m);
+        } else {
+            for (uint32_t j = from + tid * kSelPer; j < min(to, old); j += 2 * CHUNK) {
+                float w0[kSelPer], w1[kSelPer];
+                load(j, w0);
+                load(j + CHUNK, w1);
+                count(j, w0);
+                count(j + CHUNK, w1);
+            }
         }
-        __syncthreads();
-        // bins from the top: thread t takes bins - 1 - 2 t and the one below
+        sync_all();
+        // bins from the top: thread t takes bins - 1 - 2 t and the one below, of all parts
         const int b0 = bins - 1 - 2 * (int)tid, b1 = b0 - 1;
-        const uint32_t c0 = b0 >= 0 ? s_hist[b0] : 0, c1 = b1 >= 0 ? s_hist[b1] : 0;
+        uint32_t c0 = 0, c1 = 0;
+        if (b1 >= 0) {
+#pragma unroll
+            for (int r = 0; r < CL; r++) {
+                const uint32_t *hist = CL > 1 ? cluster.map_shared_rank(s_hist, r) : s_hist;
+                c0 += hist[b0];
+                c1 += hist[b1];
+            }
+        }
         uint64_t total;
         const uint32_t before = (uint32_t)block_excl((uint64_t)c0 + c1, s_warp, &total);
         if (before < want && want <= before + c0) {
@@ -112,32 +158,50 @@ __global__ void __launch_bounds__(kSelThreads) k_evict_select(EvictArgs a) {
             s_bin = b1;
             s_left = want - before - c0;
         }
-        __syncthreads();
+        sync_all();  // and nobody reads this part's bins any more
         prefix = (prefix << bits) | s_bin;
         want = s_left;
         done += bits;
-        __syncthreads();
     }
     // want now counts the keys equal to prefix that stay
     const bool any = n > a.budget && a.budget > a.recent;
-    uint32_t greater = 0, equal = 0;  // so far
-    for (uint32_t j0 = 0; j0 < n; j0 += kSelThreads * kSelPer) {
-        const uint32_t j = j0 + tid * kSelPer;
-        float m[kSelPer];
-        uint32_t gt = 0, eq = 0;  // bit u: element j + u
+    auto sides = [&](uint32_t j, const float(&w)[kSelPer], uint32_t &gt, uint32_t &eq) {  // bit u: element j + u
+        gt = eq = 0;
 #pragma unroll
         for (int u = 0; u < kSelPer; u++) {
-            m[u] = j + u < n ? mass[j + u] : 0.0f;
-            const uint32_t k = mass_key(m[u]);
-            if (j + u < n) {
-                if (j + u >= old)
-                    gt |= 1u << u;  // newest, or nothing is evicted
-                else if (any && k > prefix)
-                    gt |= 1u << u;
-                else if (any && k == prefix)
-                    eq |= 1u << u;
-            }
+            if (j + u >= to) continue;
+            const uint32_t k = mass_key(w[u]);
+            if (j + u >= old || (any && k > prefix))
+                gt |= 1u << u;  // newest, or nothing is evicted, or heavier
+            else if (any && k == prefix)
+                eq |= 1u << u;
         }
+    };
+    uint32_t greater = 0, equal = 0;  // so far, the parts before this one included
+    if constexpr (CL > 1) {
+        uint64_t mine = 0;
+        for (uint32_t j = from + tid * kSelPer; j < to; j += CHUNK) {
+            if (!once) load(j, m);
+            uint32_t gt, eq;
+            sides(j, m, gt, eq);
+            mine += ((uint64_t)__popc(gt) << 32) | __popc(eq);
+        }
+        uint64_t total;
+        block_excl(mine, s_warp, &total);
+        if (tid == 0) s_mine = total;
+        cluster.sync();
+        for (uint32_t r = 0; r < rank; r++) {
+            const uint64_t t = *cluster.map_shared_rank(&s_mine, r);
+            greater += (uint32_t)(t >> 32);
+            equal += (uint32_t)t;
+        }
+        cluster.sync();  // nobody leaves before its count is read
+    }
+    for (uint32_t j0 = from; j0 < to; j0 += CHUNK) {
+        const uint32_t j = j0 + tid * kSelPer;
+        if (!once) load(j, m);
+        uint32_t gt, eq;
+        sides(j, m, gt, eq);
         uint64_t total;
         const uint64_t before = block_excl(((uint64_t)__popc(gt) << 32) | __popc(eq), s_warp, &total);
         uint32_t g = greater + (uint32_t)(before >> 32), e = equal + (uint32_t)before;
@@ -145,9 +209,9 @@ __global__ void __launch_bounds__(kSelThreads) k_evict_select(EvictArgs a) {
         for (int u = 0; u < kSelPer; u++) {
             const bool is_eq = eq >> u & 1u;
             if ((gt >> u & 1u) || (is_eq && e < want)) {
-                const uint32_t to = g + min(e, want);
-                kept[to] = j + u;
-                mass_out[to] = m[u];
+                const uint32_t at = g + min(e, want);
+                kept[at] = j + u;
+                mass_out[at] = m[u];
             }
             g += gt >> u & 1u;
             e += is_eq;
@@ -246,6 +310,36 @@ __global__ void __launch_bounds__(kMoveThreads) k_evict_move_in_place(EvictArgs 
     }
 }
 
+namespace {
+
+// launch_k with a cluster along x.
+template <typename Kern, typename... Args>
+cudaError_t launch_cluster(const LaunchCfg &c, const char *label, Kern kern, dim3 grid, dim3 block, uint32_t size, Args... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.stream = c.stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = size;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    const bool timed = c.prof && c.prof->on;
+    if (c.pdl && !timed) {
+        attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[1].val.programmaticStreamSerializationAllowed = 1;
+        cfg.numAttrs = 2;
+    }
+    Profiler::Rec rec;
+    if (timed) c.prof->begin(label, c.stream, rec);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, args...);
+    if (timed) c.prof->end(rec, c.stream);
+    return e;
+}
+
+}  // namespace
+
 size_t evict_scratch(const EvictArgs &a, bool have_kept) {
     const size_t lens = ((size_t)a.n_seq * 4 + 255) & ~(size_t)255;
     return lens + (have_kept ? 0 : (size_t)a.n_seq * a.kv.n_kv * a.budget * 4);
@@ -255,7 +349,13 @@ cudaError_t launch_evict(const LaunchCfg &c, EvictArgs a, uint8_t *scratch) {
     a.new_len = (uint32_t *)scratch;
     if (!a.kept) a.kept = (uint32_t *)(scratch + (((size_t)a.n_seq * 4 + 255) & ~(size_t)255));
     a.err = c.dev_err;
-    cudaError_t e = launch_k(c, "evict_select", k_evict_select, dim3(a.kv.n_kv, a.n_seq), dim3(kSelThreads), 0, a);
+    // Long rows by clusters of four.  Not where the weights are compacted in place: a CTA writes where
+    // those before it read, which only one CTA's own order makes safe.
+    cudaError_t e;
+    if (a.max_len > kSelCluster && a.mass_out != a.mass)
+        e = launch_cluster(c, "evict_select", k_evict_select<4>, dim3(4 * a.kv.n_kv, a.n_seq), dim3(kSelThreads), 4, a);
+    else
+        e = launch_k(c, "evict_select", k_evict_select<1>, dim3(a.kv.n_kv, a.n_seq), dim3(kSelThreads), 0, a);
     if (e != cudaSuccess) return e;
     if (a.in_place) {
         const uint32_t cols = a.kv.hd * (a.kv.f16 ? 2 : 4) / 32;

@@ -65,8 +65,10 @@ LT_DEVINL void store_kv(uint8_t *p, uint32_t i, const float (&v)[N], uint32_t f1
     }
 }
 
-// Lane l holds N = HD / 64 rotation pairs.  Halves (NeoX): elements l N .. and
-// HD / 2 + l N ..; consecutive pairs: elements 2 l N .. 2 l N + 2 N - 1.
+// Lane l holds N = HD / 64 rotation pairs, as elements l N .. and HD / 2 + l N ..,
+// so that a warp's accesses are contiguous: pair by pair across the two (NeoX), or
+// each half of them consecutive pairs.  Consecutive pairs of head_dim 64 (N = 1)
+// would straddle lanes: there elements 2 l and 2 l + 1.
 // Grid (ntok, ceil(vectors / heads_per_cta)).
 template <int HD>
 __global__ void __launch_bounds__(kAppThreads) k_paged_append(PagedAppendArgs a) {
@@ -96,7 +98,8 @@ __global__ void __launch_bounds__(kAppThreads) k_paged_append(PagedAppendArgs a)
     __syncthreads();
 
     const bool neox = a.rope_neox;
-    const uint32_t e0 = neox ? lane * N : 2 * lane * N, e1 = neox ? HALF + lane * N : 2 * lane * N + N;
+    const bool split = neox || N > 1;
+    const uint32_t e0 = split ? lane * N : 2 * lane, e1 = split ? HALF + lane * N : 2 * lane + 1;
     for (uint32_t h = first + warp; h < last; h += kAppThreads / 32) {
         const float *src = a.qkv + ((uint64_t)t * vecs + h) * HD;
         float x[N], y[N];
@@ -129,19 +132,21 @@ __global__ void __launch_bounds__(kAppThreads) k_paged_append(PagedAppendArgs a)
                     x[e] = __fsub_rn(__fmul_rn(p, cs.x), __fmul_rn(q, cs.y));
                     y[e] = __fadd_rn(__fmul_rn(p, cs.y), __fmul_rn(q, cs.x));
                 }
-            } else {  // the 2 N consecutive elements x, y hold N pairs
-                float z[2 * N];
+            } else if constexpr (N > 1) {  // x and y hold N / 2 consecutive pairs each
 #pragma unroll
-                for (int e = 0; e < N; e++) z[e] = x[e], z[N + e] = y[e];
-#pragma unroll
-                for (int e = 0; e < N; e++) {
-                    const float2 cs = s_cs[lane * N + e];
-                    const float p = z[2 * e], q = z[2 * e + 1];
-                    z[2 * e] = __fsub_rn(__fmul_rn(p, cs.x), __fmul_rn(q, cs.y));
-                    z[2 * e + 1] = __fadd_rn(__fmul_rn(p, cs.y), __fmul_rn(q, cs.x));
+                for (int e = 0; e < N; e += 2) {
+                    const float2 cx = s_cs[(lane * N + e) / 2], cy = s_cs[(HALF + lane * N + e) / 2];
+                    const float p = x[e], q = x[e + 1], t = y[e], u = y[e + 1];
+                    x[e] = __fsub_rn(__fmul_rn(p, cx.x), __fmul_rn(q, cx.y));
+                    x[e + 1] = __fadd_rn(__fmul_rn(p, cx.y), __fmul_rn(q, cx.x));
+                    y[e] = __fsub_rn(__fmul_rn(t, cy.x), __fmul_rn(u, cy.y));
+                    y[e + 1] = __fadd_rn(__fmul_rn(t, cy.y), __fmul_rn(u, cy.x));
                 }
-#pragma unroll
-                for (int e = 0; e < N; e++) x[e] = z[e], y[e] = z[N + e];
+            } else {
+                const float2 cs = s_cs[lane];
+                const float p = x[0], q = y[0];
+                x[0] = __fsub_rn(__fmul_rn(p, cs.x), __fmul_rn(q, cs.y));
+                y[0] = __fadd_rn(__fmul_rn(p, cs.y), __fmul_rn(q, cs.x));
             }
         }
         if (is_q) {
