@@ -177,6 +177,7 @@ struct PagedAttnArgs {
     float *out;
     // scratch, set by the launcher
     float *part_o, *part_ml, *unit_ml, *scores;
+    uint64_t score_stride;          // floats between the score rows of two heads
     uint32_t *unit_info;
     uint32_t row_blocks;            // row blocks per (sequence, KV head) at most
     uint32_t nsplit;                // lt_paged_prompt.cu: CTAs that share a row block's keys

@@ -13,7 +13,7 @@
 //   through one after the other; every CTA takes an equal share of the tiles,
 //   wherever it begins and ends, so lengths may differ as they like.  A unit
 //   that several CTAs share leaves partial (m, l, sum) records, which
-//   k_paged_join adds up in CTA order: the result does not depend on timing.
+//   k_paged_finish adds up in CTA order: the result does not depend on timing.
 // - Each warp owns 16 keys of a tile (8 for f32 caches) and a ring of kStages
 //   such blocks in shared memory, filled by 16-byte asynchronous copies; rows sit
 //   at padded pitches so that matrix loads meet no bank conflict.
@@ -28,7 +28,7 @@
 namespace lt {
 
 constexpr int kPaWarps = 4, kPaThreads = kPaWarps * 32, kPaRows = 8;
-constexpr int kMassThreads = 256, kMassKeys = 1024;
+constexpr uint32_t kMassKeys = 512;
 
 template <int HD, bool F16>
 struct PaShape {
@@ -41,7 +41,7 @@ struct PaShape {
     static constexpr int QSTEPS = F16 ? HD / 16 : HD / 8;   // k-steps of 512-byte operand fragments
     static constexpr int RING = BLOCK * STAGES * kPaWarps;
     static constexpr int QBYTES = QSTEPS * 512;
-    static constexpr int MERGE = kPaRows * (HD + 2) * 4;
+    static constexpr int MERGE = 2 * kPaRows * (HD + 2) * 4;
     static constexpr int UNION = QBYTES > MERGE ? QBYTES : MERGE;
     static constexpr int SMEM = RING + UNION + 16 * 8 * kPaWarps + 64;
     static constexpr int CTAS = HD == 256 ? 1 : HD == 128 ? 2 : 3;
@@ -131,9 +131,20 @@ struct PaWalk {
     }
 };
 
-// First tile of CTA c of G among T tiles, and the CTA that holds tile f.
-LT_DEVINL uint64_t pa_start(uint64_t T, uint32_t c, uint32_t G) { return T * c / G; }
-LT_DEVINL uint32_t pa_owner(uint64_t T, uint64_t f, uint32_t G) { return (uint32_t)(((f + 1) * G - 1) / T); }
+LT_DEVINL uint64_t div_small(uint64_t a, uint64_t b) {  // 32-bit division where it will do
+    return (a | b) >> 32 ? a / b : (uint32_t)a / (uint32_t)b;
+}
+
+// T tiles over G <= T CTAs: the first `more` get each + 1, the others each.
+struct PaShare {
+    uint64_t each, more;
+    LT_DEVINL PaShare(uint64_t T, uint32_t G) : each(div_small(T, G)), more(T - each * G) {}
+    LT_DEVINL uint64_t start(uint32_t c) const { return each * c + min((uint64_t)c, more); }
+    LT_DEVINL uint32_t owner(uint64_t f) const {
+        const uint64_t big = more * (each + 1);
+        return (uint32_t)(f < big ? div_small(f, each + 1) : more + div_small(f - big, each));
+    }
+};
 
 // A unit's place in the records: its first CTA and how many CTAs share it.
 LT_DEVINL uint64_t pa_unit(const PagedAttnArgs &a, uint32_t s, uint32_t kh, uint32_t rb) {
@@ -149,6 +160,7 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<HD, F16>::CTAS) k_paged_at
     __shared__ uint64_t s_scan[kPaWarps];
     __shared__ uint64_t s_rem;
     __shared__ uint32_t s_seq;
+    __shared__ PaSeq s_q;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, j4 = lane & 3;
     uint8_t *ring = smem + warp * (S::BLOCK * S::STAGES);
     uint8_t *qm = smem + S::RING;  // query fragments, then the merge records
@@ -185,7 +197,8 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<HD, F16>::CTAS) k_paged_at
     // no more CTAs than tiles, so that every CTA of a unit leaves a record
     const uint32_t G = (uint32_t)min((uint64_t)gridDim.x, T);
     if (c >= G) return;
-    const uint64_t f0 = pa_start(T, c, G), f1 = pa_start(T, c + 1, G);
+    const PaShare share(T, G);
+    const uint64_t f0 = share.start(c), f1 = share.start(c + 1);
     if (f0 >= before && f0 < before + mine) {
         uint64_t rem = f0 - before;
         for (uint32_t s = sa; s < sb; s++) {
@@ -194,6 +207,7 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<HD, F16>::CTAS) k_paged_at
             if (rem < w) {
                 s_seq = s;
                 s_rem = rem;
+                s_q = q;
                 break;
             }
             rem -= w;
@@ -202,11 +216,29 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<HD, F16>::CTAS) k_paged_at
     __syncthreads();
     PaWalk<PROMPT> cw, lw;  // the compute walk and the copies ahead of it
     cw.s = s_seq;
-    cw.q = pa_seq<PROMPT>(a, cw.s, TILE, false);
-    cw.unit = (uint32_t)(s_rem / cw.q.tiles);
-    cw.tile = (uint32_t)(s_rem % cw.q.tiles);
+    cw.q = s_q;
+    cw.unit = (uint32_t)div_small(s_rem, cw.q.tiles);
+    cw.tile = (uint32_t)(s_rem - (uint64_t)cw.unit * cw.q.tiles);
     cw.set_unit(a);
     lw = cw;
+
+    // a unit's queries: warp w takes rows 2 w and 2 w + 1; the first unit's come while K and V are looked up
+    float qv[2][HD / 32];
+    auto load_q = [&]() {
+        const uint32_t rows = min((uint32_t)kPaRows, cw.q.nq * a.group - cw.rb * kPaRows);
+#pragma unroll
+        for (int rr = 0; rr < 2; rr++) {
+            const uint32_t r = warp * 2 + rr, R = cw.rb * kPaRows + r;
+            const float *src = a.q + (uint64_t)(cw.q.q0 + R / a.group) * a.q_stride + (uint64_t)(cw.kh * a.group + R % a.group) * HD;
+#pragma unroll
+            for (int e = 0; e < HD / 64; e++) {
+                const float2 t = r < rows ? *reinterpret_cast<const float2 *>(src + 64 * e + 2 * lane) : make_float2(0.0f, 0.0f);
+                qv[rr][2 * e] = t.x;
+                qv[rr][2 * e + 1] = t.y;
+            }
+        }
+    };
+    load_q();
 
     // The block to copy next: where whole blocks lie within pages, its page is looked up
     // once and its rows are a stride apart; else lane r < KB looks up row r.
@@ -214,56 +246,48 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<HD, F16>::CTAS) k_paged_at
     const bool in_page = a.kv.page_size % KB == 0;
     const int row0 = CH < 32 ? lane / CH : 0, col0 = CH < 32 ? lane % CH : lane;
     const uint64_t lane_off = (uint64_t)row0 * a.kv.slot_stride + col0 * 16, step_off = STEP * a.kv.slot_stride;
-    uint32_t page = 0, key = 0;
-    auto look = [&]() {
-        key = lw.base + lw.tile * TILE + warp * KB + (in_page ? 0 : lane);
-        page = a.kv.n_pages;
-        if (in_page ? key < lw.hi && key + KB > lw.lo : lane < KB && key < lw.hi && key >= lw.lo)
-            page = a.table[(uint64_t)lw.s * a.kv.max_pages + page_of(a.kv, key)];
-        else
-            key = 0xffffffffu;
+    struct Job {
+        uint32_t page, key, kh, lo, hi;  // key 0xffffffff: nothing to copy
     };
-    auto copy = [&](int stage) {
+    auto look = [&]() {
+        Job j = {a.kv.n_pages, lw.base + lw.tile * TILE + warp * KB + (in_page ? 0 : lane), lw.kh, lw.lo, lw.hi};
+        if (in_page ? j.key < j.hi && j.key + KB > j.lo : lane < KB && j.key < j.hi && j.key >= j.lo)
+            j.page = a.table[(uint64_t)lw.s * a.kv.max_pages + page_of(a.kv, j.key)];
+        else
+            j.key = 0xffffffffu;
+        return j;
+    };
+    auto copy = [&](const Job &j, int stage) {
+        const uint32_t key = j.key;
         bool take = key != 0xffffffffu;
-        if (take && page >= a.kv.n_pages) {
+        if (take && j.page >= a.kv.n_pages) {
             take = false;
             atomicExch(a.err, DEV_ERR_BAD_INDEX);
         }
         const uint32_t kdst = ring_u + stage * S::BLOCK + row0 * S::KP + col0 * 16;
         const uint32_t vdst = ring_u + stage * S::BLOCK + KB * S::KP + row0 * S::VP + col0 * 16;
+        // (one short body for whole and partial blocks: this code runs few times, and its fetching shows)
         if (in_page) {
-            const uint64_t o = take ? paged_offset(a.kv, page, key, lw.kh) + lane_off : 0;
+            const uint64_t o = take ? paged_offset(a.kv, j.page, key, j.kh) + lane_off : 0;
             const uint8_t *pk = a.kv.k + o, *pv = a.kv.v + o;
-            if (take && key >= lw.lo && key + KB <= lw.hi) {
+            const uint32_t from = take ? max(j.lo, key) - key : 0, to = take ? min(j.hi - key, (uint32_t)KB) : 0;
 #pragma unroll
-                for (int r = 0; r < KB; r += STEP) {
+            for (int r = 0; r < KB; r += STEP) {
+                const bool t = r + row0 >= from && r + row0 < to;
 #pragma unroll
-                    for (int x = 0; x < CH; x += 32) {
-                        cp_async16(kdst + r * S::KP + x * 16, pk + x * 16, true);
-                        cp_async16(vdst + r * S::VP + x * 16, pv + x * 16, true);
-                    }
-                    pk += step_off;
-                    pv += step_off;
+                for (int x = 0; x < CH; x += 32) {
+                    cp_async16(kdst + r * S::KP + x * 16, pk + x * 16, t);
+                    cp_async16(vdst + r * S::VP + x * 16, pv + x * 16, t);
                 }
-            } else {
-#pragma unroll
-                for (int r = 0; r < KB; r += STEP) {
-                    const bool t = take && key + r + row0 >= lw.lo && key + r + row0 < lw.hi;
-#pragma unroll
-                    for (int x = 0; x < CH; x += 32) {
-                        cp_async16(kdst + r * S::KP + x * 16, t ? pk + x * 16 : a.kv.k, t);
-                        cp_async16(vdst + r * S::VP + x * 16, t ? pv + x * 16 : a.kv.v, t);
-                    }
-                    pk += step_off;
-                    pv += step_off;
-                }
+                pk += step_off;
+                pv += step_off;
             }
             return;
         }
         __syncwarp();
-        if (lane < KB) offs[lane] = take ? paged_offset(a.kv, page, key, lw.kh) : ~0ull;
+        if (lane < KB) offs[lane] = take ? paged_offset(a.kv, j.page, key, j.kh) : ~0ull;
         __syncwarp();
-#pragma unroll
+#pragma unroll 1
         for (int r = 0; r < KB; r += STEP) {
             const uint64_t o = offs[r + row0];
             const bool t = o != ~0ull;
@@ -275,21 +299,26 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<HD, F16>::CTAS) k_paged_at
             }
         }
     };
+    // all pages of the first blocks are looked up before the first copy waits for its own
     const uint64_t nf = f1 - f0;
-    uint64_t ahead = 0;
-    look();
+    uint64_t looked = 0, copied = 0;
+    Job jobs[S::STAGES];
+    auto look_next = [&](Job &j) {
+        if (looked >= nf) return;
+        j = look();
+        if (++looked < nf) lw.template next<TILE>(a);
+    };
+#pragma unroll
+    for (int st = 0; st < S::STAGES; st++) look_next(jobs[st]);
 #pragma unroll
     for (int st = 0; st < S::STAGES - 1; st++) {
-        if (ahead < nf) {
-            copy(st);
-            ahead++;
-            if (ahead < nf) {
-                lw.template next<TILE>(a);
-                look();
-            }
+        if (copied < nf) {
+            copy(jobs[st], st);
+            copied++;
         }
         cp_async_commit();
     }
+    Job job = jobs[S::STAGES - 1];
 
     uint64_t f = f0;
     int stage = 0;
@@ -299,21 +328,14 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<HD, F16>::CTAS) k_paged_at
         const uint32_t seg = (uint32_t)min(left, f1 - f);
         const uint64_t unit_f0 = f - cw.tile;
         const uint32_t rows = min((uint32_t)kPaRows, cw.q.nq * a.group - cw.rb * kPaRows);
-        // queries to operand fragments: warp w takes rows 2 w and 2 w + 1
+        // queries to operand fragments
 #pragma unroll
         for (int rr = 0; rr < 2; rr++) {
             const uint32_t r = warp * 2 + rr;
-            float v[HD / 32];
-            const uint32_t R = cw.rb * kPaRows + r;
-            const float *src = a.q + (uint64_t)(cw.q.q0 + R / a.group) * a.q_stride + (uint64_t)(cw.kh * a.group + R % a.group) * HD;
+            float(&v)[HD / 32] = qv[rr];
             float top = 0.0f;
 #pragma unroll
-            for (int e = 0; e < HD / 64; e++) {
-                const float2 t = r < rows ? *reinterpret_cast<const float2 *>(src + 64 * e + 2 * lane) : make_float2(0.0f, 0.0f);
-                v[2 * e] = t.x;
-                v[2 * e + 1] = t.y;
-                top = fmaxf(top, fmaxf(fabsf(t.x), fabsf(t.y)));
-            }
+            for (int e = 0; e < HD / 32; e++) top = fmaxf(top, fabsf(v[e]));
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
             // the largest element lands in [2^8, 2^9)
@@ -468,7 +490,7 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<HD, F16>::CTAS) k_paged_at
                     } else {
                         const bool seen = whole || (j >= row_lo && j < row_hi);
                         if (a.mass && seen && (uint32_t)g < rows)
-                            a.scores[((uint64_t)cw.s * a.n_heads + head) * a.max_len + j] = sc[n];
+                            a.scores[((uint64_t)cw.s * a.n_heads + head) * a.score_stride + j] = sc[n];
                         if (!seen) sc[n] = -INFINITY;
                     }
                     top = fmaxf(top, sc[n]);
@@ -530,28 +552,25 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<HD, F16>::CTAS) k_paged_at
             __syncwarp();
             int fill = stage + S::STAGES - 1;
             if (fill >= S::STAGES) fill -= S::STAGES;
-            if (ahead < nf) {
-                copy(fill);
-                ahead++;
-                if (ahead < nf) {
-                    lw.template next<TILE>(a);
-                    look();
-                }
+            if (copied < nf) {
+                copy(job, fill);
+                copied++;
+                look_next(job);
             }
             cp_async_commit();
             if (++stage == S::STAGES) stage = 0;
             if (it + 1 < seg) cw.tile++;
         }
 
-        // ── merge the warps into warp 0, in their order ──
+        // ── merge the warps: 2 and 3 into 0 and 1, then 1 into 0 ──
         l += __shfl_xor_sync(0xffffffffu, l, 1);
         l += __shfl_xor_sync(0xffffffffu, l, 2);
         auto dim = [&](int n, int e) { return F16 ? 8 * n + 2 * j4 + e : 32 * (n / 4) + 8 * j4 + 4 * e + n % 4; };
         __syncthreads();  // every warp is done with the query fragments
-#pragma unroll 1
-        for (int from = 1; from < kPaWarps; from++) {
-            float *rec = reinterpret_cast<float *>(qm) + g * (HD + 2);
-            if (warp == from) {
+#pragma unroll
+        for (int half = kPaWarps / 2; half >= 1; half /= 2) {
+            float *rec = reinterpret_cast<float *>(qm) + (warp % half) * kPaRows * (HD + 2) + g * (HD + 2);
+            if (warp >= half && warp < 2 * half) {
 #pragma unroll
                 for (int n = 0; n < NB; n++) {
                     rec[dim(n, 0)] = o[n][0];
@@ -563,7 +582,7 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<HD, F16>::CTAS) k_paged_at
                 }
             }
             __syncthreads();
-            if (warp == 0) {
+            if (warp < half) {
                 const float m2 = rec[HD], mn = fmaxf(m, m2);
                 const float w1 = m == -INFINITY ? 0.0f : ex2(m - mn), w2 = m2 == -INFINITY ? 0.0f : ex2(m2 - mn);
                 l = l * w1 + rec[HD + 1] * w2;
@@ -577,7 +596,7 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<HD, F16>::CTAS) k_paged_at
             __syncthreads();
         }
         if (warp == 0) {
-            const uint32_t first = pa_owner(T, unit_f0, G), last = pa_owner(T, unit_f0 + cw.q.tiles - 1, G);
+            const uint32_t first = share.owner(unit_f0), last = share.owner(unit_f0 + cw.q.tiles - 1);
             const uint64_t u = pa_unit(a, cw.s, cw.kh, cw.rb);
             if (unit_f0 == f && lane == 0) {
                 a.unit_info[2 * u] = first;
@@ -613,7 +632,10 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<HD, F16>::CTAS) k_paged_at
         }
         __syncthreads();  // the merge records are read before the next queries overwrite them
         f += seg;
-        if (f < f1) cw.template next<TILE>(a);
+        if (f < f1) {
+            cw.template next<TILE>(a);
+            load_q();
+        }
     }
     cp_async_wait<0>();
 }
@@ -622,16 +644,13 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<HD, F16>::CTAS) k_paged_at
 // the later ones' first.
 LT_DEVINL uint64_t pa_part(uint32_t first, uint32_t p) { return 2 * (uint64_t)(first + p) + (p == 0 ? 1 : 0); }
 
-// Units that several CTAs share: grid (units, rows), one row per CTA.
+// Units that several CTAs share: one row per CTA.
 template <int HD, bool PROMPT>
-__global__ void __launch_bounds__(128) k_paged_join(PagedAttnArgs a) {
+LT_DEVINL void pa_join_row(const PagedAttnArgs &a, uint64_t u, uint32_t r) {
     constexpr int LANES = HD / 4, GROUPS = 128 / LANES;
     __shared__ float s_red[4], s_red2[4];
     __shared__ float4 s_o[128];
-    pdl_launch_dependents();
-    pdl_wait();
-    const uint64_t u = blockIdx.x;
-    const uint32_t r = blockIdx.y, rb = (uint32_t)(u % a.row_blocks);
+    const uint32_t rb = (uint32_t)(u % a.row_blocks);
     const uint32_t kh = (uint32_t)(u / a.row_blocks % a.kv.n_kv), s = (uint32_t)(u / a.row_blocks / a.kv.n_kv);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     uint32_t nq = 1, q0 = s;
@@ -692,17 +711,25 @@ __global__ void __launch_bounds__(128) k_paged_join(PagedAttnArgs a) {
     dst[3] = acc.w * inv;
 }
 
-// mass[s][kv head][j] += sum over the KV head's query heads of 2^(score - m) / l.
-// Grid (key steps, n_kv, n_seq); one thread per key, so each cell has one writer.
-__global__ void __launch_bounds__(kMassThreads) k_paged_mass(PagedAttnArgs a) {
+// mass[s][kv head][j] += sum over the KV head's query heads of 2^(score - m) / l, for
+// kMassKeys positions from j0 on; a thread's cells are its own.  The scores are on
+// their way while the heads' m and l are put together.
+LT_DEVINL void pa_mass(const PagedAttnArgs &a, uint32_t s, uint32_t kh, uint32_t j0) {
     extern __shared__ float s_ml[];  // [group] maxima, [group] 1 / sum
-    pdl_launch_dependents();
-    pdl_wait();
-    const uint32_t kh = blockIdx.y, s = blockIdx.z, j0 = blockIdx.x * kMassKeys;
     const PaSeq q = pa_seq<false>(a, s, 1, false);
     if (j0 >= q.len || j0 + kMassKeys <= q.lo) return;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    for (uint32_t h = warp; h < a.group; h += kMassThreads / 32) {
+    constexpr int H = 8;
+    const uint32_t j = j0 + 4 * tid;
+    const float *sc = a.scores + ((uint64_t)s * a.n_heads + kh * a.group) * a.score_stride + j;
+    float4 v[H];
+    auto load = [&](uint32_t h0) {
+#pragma unroll
+        for (int h = 0; h < H; h++)
+            if (j < q.len && h0 + h < a.group) v[h] = *reinterpret_cast<const float4 *>(sc + (h0 + h) * a.score_stride);
+    };
+    load(0);
+    for (uint32_t h = warp; h < a.group; h += 4) {
         const uint64_t u = pa_unit(a, s, kh, h / kPaRows);
         const uint32_t r = h % kPaRows, first = a.unit_info[2 * u], n = a.unit_info[2 * u + 1];
         float m = -INFINITY, l = 0.0f;
@@ -726,14 +753,36 @@ __global__ void __launch_bounds__(kMassThreads) k_paged_mass(PagedAttnArgs a) {
         }
     }
     __syncthreads();
-    float *mass = a.mass + ((uint64_t)s * a.kv.n_kv + kh) * a.mass_stride;
-    const float *sc = a.scores + ((uint64_t)s * a.n_heads + kh * a.group) * a.max_len;
-    const uint32_t end = min(q.len, j0 + kMassKeys);
-    for (uint32_t j = max(q.lo, j0) + tid; j < end; j += kMassThreads) {
-        float w = 0.0f;
-#pragma unroll 8
-        for (uint32_t h = 0; h < a.group; h++) w = fmaf(ex2(sc[(uint64_t)h * a.max_len + j] - s_ml[h]), s_ml[a.group + h], w);
-        mass[j] += w;
+    if (j >= q.len) return;
+    float w[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (uint32_t h0 = 0; h0 < a.group; h0 += H) {
+        if (h0) load(h0);
+#pragma unroll
+        for (int h = 0; h < H; h++) {
+            if (h0 + h >= a.group) break;
+            const float m = s_ml[h0 + h], f = s_ml[a.group + h0 + h];
+            w[0] = fmaf(ex2(v[h].x - m), f, w[0]);
+            w[1] = fmaf(ex2(v[h].y - m), f, w[1]);
+            w[2] = fmaf(ex2(v[h].z - m), f, w[2]);
+            w[3] = fmaf(ex2(v[h].w - m), f, w[3]);
+        }
+    }
+    float *mass = a.mass + ((uint64_t)s * a.kv.n_kv + kh) * a.mass_stride + j;
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+        if (j + e >= q.lo && j + e < q.len) mass[e] += w[e];
+}
+
+// What is left when the tiles are done: rows to join, then weights to add up.
+template <int HD, bool PROMPT>
+__global__ void __launch_bounds__(128) k_paged_finish(PagedAttnArgs a, uint32_t n_join) {
+    pdl_launch_dependents();
+    pdl_wait();
+    if (blockIdx.x < n_join) {
+        pa_join_row<HD, PROMPT>(a, blockIdx.x / kPaRows, blockIdx.x % kPaRows);
+    } else if (!PROMPT) {
+        const uint32_t b = blockIdx.x - n_join, steps = (a.max_len + kMassKeys - 1) / kMassKeys;
+        pa_mass(a, b / steps / a.kv.n_kv, b / steps % a.kv.n_kv, b % steps * kMassKeys);
     }
 }
 
@@ -758,7 +807,7 @@ PaScratch pa_layout(const PagedAttnArgs &a, uint32_t G) {
     s.part_ml = take((size_t)2 * G * 16 * 4);
     s.unit_info = take(units * 8);
     s.unit_ml = take(a.mass ? units * 64 : 0);
-    s.scores = take(a.mass ? (size_t)a.n_seq * a.n_heads * a.max_len * 4 : 0);
+    s.scores = take(a.mass ? (size_t)a.n_seq * a.n_heads * ((a.max_len + 3) & ~3u) * 4 : 0);
     s.total = off;
     return s;
 }
@@ -775,10 +824,12 @@ cudaError_t pa_launch(const LaunchCfg &c, const PagedAttnArgs &a, uint64_t units
     else
         e = launch_k(c, label, k_paged_attn<HD, F16, PROMPT, false>, grid, dim3(kPaThreads), PaShape<HD, F16>::SMEM, a);
     if (e != cudaSuccess) return e;
-    e = launch_k(c, "paged_join", k_paged_join<HD, PROMPT>, dim3((uint32_t)units, kPaRows), dim3(128), 0, a);
-    if (e != cudaSuccess || PROMPT || !a.mass) return e;
-    return launch_k(c, "paged_mass", k_paged_mass, dim3((a.max_len + kMassKeys - 1) / kMassKeys, a.kv.n_kv, a.n_seq),
-                    dim3(kMassThreads), 2 * a.group * sizeof(float), a);
+    if (e != cudaSuccess) return e;
+    const uint64_t join = units * kPaRows;
+    const uint64_t mass = a.mass ? (uint64_t)((a.max_len + kMassKeys - 1) / kMassKeys) * a.kv.n_kv * a.n_seq : 0;
+    if (join + mass > 0x7fffffffull) return cudaErrorInvalidValue;
+    return launch_k(c, "paged_finish", k_paged_finish<HD, PROMPT>, dim3((uint32_t)(join + mass)), dim3(128),
+                    a.mass ? 2 * a.group * sizeof(float) : 0, a, (uint32_t)join);
 }
 
 template <bool F16, bool PROMPT>
@@ -802,6 +853,7 @@ cudaError_t launch_paged_attn(const LaunchCfg &c, PagedAttnArgs a, uint8_t *scra
     a.unit_info = (uint32_t *)(scratch + s.unit_info);
     a.unit_ml = (float *)(scratch + s.unit_ml);
     a.scores = (float *)(scratch + s.scores);
+    a.score_stride = (a.max_len + 3) & ~3u;
     a.err = c.dev_err;
     const uint64_t rows = (uint64_t)(a.cu ? a.max_q : 1) * a.group;
     a.row_blocks = (uint32_t)((rows + kPaRows - 1) / kPaRows);
