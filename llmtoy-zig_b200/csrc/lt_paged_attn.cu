@@ -604,7 +604,14 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<HD, F16>::CTAS) k_paged_at
             }
             if (first == last) {
                 const float inv = l > 0.0f ? __fdiv_rn(1.0f, l) : (l == 0.0f ? 0.0f : l);
-                if ((uint32_t)g < rows) {
+                float off = l - l;  // not 0 where the row is not finite
+#pragma unroll
+                for (int n = 0; n < NB; n++) off += (o[n][0] - o[n][0]) + (o[n][1] - o[n][1]);
+                off += __shfl_xor_sync(0xffffffffu, off, 1);
+                off += __shfl_xor_sync(0xffffffffu, off, 2);
+                if (PROMPT && off != 0.0f) {
+                    if ((uint32_t)g < rows) slow_row(a, cw.s, cw.kh, R, j4 * (HD / 4), HD / 4);
+                } else if ((uint32_t)g < rows) {
                     float *dst = a.out + (uint64_t)(cw.q.q0 + R / a.group) * a.out_stride + (uint64_t)head * HD;
 #pragma unroll
                     for (int n = 0; n < NB; n++) {
@@ -650,6 +657,7 @@ LT_DEVINL void pa_join_row(const PagedAttnArgs &a, uint64_t u, uint32_t r) {
     constexpr int LANES = HD / 4, GROUPS = 128 / LANES;
     __shared__ float s_red[4], s_red2[4];
     __shared__ float4 s_o[128];
+    __shared__ uint32_t s_off;
     const uint32_t rb = (uint32_t)(u % a.row_blocks);
     const uint32_t kh = (uint32_t)(u / a.row_blocks % a.kv.n_kv), s = (uint32_t)(u / a.row_blocks / a.kv.n_kv);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -692,23 +700,30 @@ LT_DEVINL void pa_join_row(const PagedAttnArgs &a, uint64_t u, uint32_t r) {
         acc.w = fmaf(v.w, w, acc.w);
     }
     s_o[tid] = acc;
+    if (tid == 0) s_off = 0;
     __syncthreads();
-    if (grp) return;
-    l = (s_red2[0] + s_red2[1]) + (s_red2[2] + s_red2[3]);
+    if (grp == 0) {
+        l = (s_red2[0] + s_red2[1]) + (s_red2[2] + s_red2[3]);
 #pragma unroll
-    for (int i = 1; i < GROUPS; i++) {
-        const float4 v = s_o[i * LANES + x];
-        acc.x += v.x;
-        acc.y += v.y;
-        acc.z += v.z;
-        acc.w += v.w;
+        for (int i = 1; i < GROUPS; i++) {
+            const float4 v = s_o[i * LANES + x];
+            acc.x += v.x;
+            acc.y += v.y;
+            acc.z += v.z;
+            acc.w += v.w;
+        }
+        const float inv = l > 0.0f ? __fdiv_rn(1.0f, l) : (l == 0.0f ? 0.0f : l);
+        float *dst = a.out + (uint64_t)(q0 + R / a.group) * a.out_stride + (uint64_t)(kh * a.group + R % a.group) * HD + 4 * x;
+        dst[0] = acc.x * inv;
+        dst[1] = acc.y * inv;
+        dst[2] = acc.z * inv;
+        dst[3] = acc.w * inv;
+        if (PROMPT && (acc.x - acc.x) + (acc.y - acc.y) + (acc.z - acc.z) + (acc.w - acc.w) + (l - l) != 0.0f) s_off = 1;
     }
-    const float inv = l > 0.0f ? __fdiv_rn(1.0f, l) : (l == 0.0f ? 0.0f : l);
-    float *dst = a.out + (uint64_t)(q0 + R / a.group) * a.out_stride + (uint64_t)(kh * a.group + R % a.group) * HD + 4 * x;
-    dst[0] = acc.x * inv;
-    dst[1] = acc.y * inv;
-    dst[2] = acc.z * inv;
-    dst[3] = acc.w * inv;
+    if (PROMPT) {
+        __syncthreads();
+        if (s_off && tid < HD / 16) slow_row(a, s, kh, R, tid * 16, 16);
+    }
 }
 
 // mass[s][kv head][j] += sum over the KV head's query heads of 2^(score - m) / l, for

@@ -171,53 +171,6 @@ struct IntC {
     static constexpr int value = N;
 };
 
-LT_DEVINL float pp_kv(const uint8_t *p, uint32_t d) { return __half2float(reinterpret_cast<const __half *>(p)[d]); }
-
-// Row R of (sequence s, KV head kh) by itself, key by key, masked keys never
-// touched: for rows whose tile result is not finite, which a value outside the
-// row's own keys may have caused.  Output dims [d0, d0 + nd), nd a multiple of 16.
-__noinline__ __device__ void pp_slow_row(const PagedAttnArgs &a, uint32_t s, uint32_t kh, uint32_t R, uint32_t d0,
-                                         uint32_t nd) {
-    const uint32_t hd = a.kv.hd, cap = (uint32_t)min((uint64_t)a.kv.max_pages * a.kv.page_size, (uint64_t)a.max_len);
-    const uint32_t len = min(a.lens[s], cap), nq = a.cu[s + 1] - a.cu[s], q_row = a.cu[s] + R / a.group;
-    const uint32_t head = kh * a.group + R % a.group;
-    const float *q = a.q + (uint64_t)q_row * a.q_stride + (uint64_t)head * hd;
-    float *out = a.out + (uint64_t)q_row * a.out_stride + (uint64_t)head * hd;
-    const uint32_t *table = a.table + (uint64_t)s * a.kv.max_pages;
-    const uint32_t *docs = a.docs ? a.docs + (uint64_t)s * a.doc_stride : nullptr;
-    const int64_t i = (int64_t)len - nq + R / a.group;
-    int64_t lo = 0, hi = len;
-    if (a.window) lo = max((int64_t)0, i - (int64_t)a.window + 1);
-    if (a.causal) hi = min(hi, max(i + 1, a.prefix ? (int64_t)a.prefix[s] : (int64_t)0));
-    if (docs && i < 0) hi = 0;
-    const float slope = a.slopes ? a.slopes[head] : 0.0f;
-    const float f = a.softcap != 0.0f ? a.scale / a.softcap : a.scale * 1.4426950408889634f;
-    float m = -INFINITY;
-    for (uint32_t d = d0; d < d0 + nd; d += 16) {
-        float o[16], l = 0.0f;
-        for (int e = 0; e < 16; e++) o[e] = 0.0f;
-        for (int pass = d == d0 ? 0 : 1; pass < 2; pass++) {
-            for (int64_t j = lo; j < hi; j++) {
-                if (docs && docs[j] != docs[i]) continue;
-                const uint32_t page = table[j / a.kv.page_size];
-                if (page >= a.kv.n_pages) continue;
-                const uint64_t off = paged_offset(a.kv, page, (uint32_t)j, kh);
-                float dot = 0.0f;
-                for (uint32_t e = 0; e < hd; e++) dot = fmaf(q[e], pp_kv(a.kv.k + off, e), dot);
-                const float t = score_log2(dot, f, a.softcap, slope, fabsf((float)(i - j)));
-                if (pass == 0) {
-                    m = t != t || m != m ? NAN : fmaxf(m, t);
-                } else {
-                    const float p = ex2(t - m);
-                    l += p;
-                    for (int e = 0; e < 16; e++) o[e] = fmaf(p, pp_kv(a.kv.v + off, d + e), o[e]);
-                }
-            }
-        }
-        for (int e = 0; e < 16; e++) out[d + e] = l == 0.0f ? 0.0f : o[e] / l;
-    }
-}
-
 template <int HD, bool EXTRA>
 __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(PagedAttnArgs a,
                                                                 const __grid_constant__ PpMaps maps) {
@@ -876,7 +829,7 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(PagedAttnArgs a,
                         *reinterpret_cast<const float4 *>(st + rr * PITCH + lane % 8 * 4);
             }
         }
-        if (real && !fine) pp_slow_row(a, s, kh, R, half * 128, OW);
+        if (real && !fine) slow_row(a, s, kh, R, half * 128, OW);
         tc_fence_before();
     }
     __syncthreads();
@@ -936,7 +889,7 @@ __global__ void __launch_bounds__(kPpJoinRows * 32) k_paged_prompt_join(PagedAtt
 #pragma unroll
         for (int e = 0; e < PER; e++) *reinterpret_cast<float2 *>(dst + 64 * e) = make_float2(acc[e].x * inv, acc[e].y * inv);
     } else if (lane < HD / 16) {
-        pp_slow_row(a, s, kh, R, lane * 16, 16);
+        slow_row(a, s, kh, R, lane * 16, 16);
     }
 }
 

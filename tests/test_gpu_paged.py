@@ -521,6 +521,44 @@ def test_prompt_few_tokens_long_cache(pkg, ctx):
         check_prompt(pkg, ctx, 32, 4, 128, f16, 16, [4, 5, 1], [3000, 777, 1200], seed=7)
 
 
+@pytest.mark.parametrize("heads,kv,hd", [(14, 2, 64), (32, 4, 128), (16, 8, 256)])
+@pytest.mark.parametrize("f16", [True, False])
+@pytest.mark.parametrize("mask", ["causal", "window", "docs", "split"])
+def test_prompt_masked_values_may_be_anything(pkg, ctx, heads, kv, hd, f16, mask):
+    """Infinities and NaN in K and V of positions that a query does not see do not reach it."""
+    rng = np.random.default_rng(21)
+    n, m = (1300, 40) if mask == "split" else (230, 230)
+    c = Cache(pkg, rng, [n], kv, hd, f16, 16)
+    bad = n - 7 if mask in ("causal", "split") else 100
+    for j, x in ((bad, np.nan), (bad + 1, np.inf)):
+        c.hk[c.table[0, j // 16], j % 16] = x
+        c.hv[c.table[0, j // 16], j % 16] = -x
+    c.upload(pkg)
+    q = rng.normal(0, 1.5, (m, heads, hd)).astype(np.float32)
+    docs = np.zeros((1, n), np.int64)
+    docs[0, 90:110] = 1
+    window = 50 if mask == "window" else 0
+    cfg = pkg.PagedAttnCfg(n_heads=heads, window=window, causal=1, scale=1 / math.sqrt(hd))
+    qd, out = torch.from_numpy(q.reshape(m, -1)).cuda(), torch.zeros(m, heads * hd, device="cuda")
+    cu, ln, dd = i32([0, m]), i32([n]), i32(docs)
+    ctx.paged_attn_prompt(cfg, c.desc, qd, 1, cu, m, m, c.dtable, ln, n, out, None, dd if mask == "docs" else None, n)
+    ctx.sync()
+    got = out.cpu().numpy().reshape(m, heads, hd)
+    i, j = np.arange(n - m, n)[:, None], np.arange(n)[None]
+    seen = j <= i
+    if window:
+        seen = seen & (i - j < window)
+    if mask == "docs":
+        seen = seen & (docs[0][i] == docs[0][j])
+    clean = ~seen[:, bad:bad + 2].any(1)
+    assert clean.any() and not clean.all()
+    K, V = c.seq(0)
+    K, V = np.nan_to_num(K, nan=0, posinf=0, neginf=0), np.nan_to_num(V, nan=0, posinf=0, neginf=0)
+    want, _ = attend(q[clean], K, V, i[clean, 0], seen[clean], 1 / math.sqrt(hd))
+    assert rel(got[clean], want) < ATTN_BAR
+    assert np.isnan(got[~clean]).any(axis=(1, 2)).all()
+
+
 def test_prompt_bad_ranges_reported(pkg, ctx):
     rng = np.random.default_rng(14)
     c = Cache(pkg, rng, [40, 40], 2, 64, True, 16)
