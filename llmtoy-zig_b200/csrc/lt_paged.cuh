@@ -27,6 +27,8 @@ LT_DEVINL uint64_t paged_offset(const PagedKvDev &kv, uint32_t page, uint32_t j,
            (uint64_t)h * kv.head_stride;
 }
 
+LT_DEVINL void prefetch_l2(const void *p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
+
 LT_DEVINL float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

@@ -169,6 +169,17 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<HD, F16>::CTAS) k_paged_at
     const uint32_t ring_u = smem_u32(ring), qm_u = smem_u32(qm);
     const uint32_t c = blockIdx.x;
     pdl_launch_dependents();
+    // Lengths, page table and queries towards L2, and their translations towards this SM, while the
+    // kernel before still runs (only hints: the values are read after the wait).
+    {
+        const uint64_t line = ((uint64_t)c * kPaThreads + tid) * 32, entries = (uint64_t)a.n_seq * a.kv.max_pages;
+        if (line < entries) prefetch_l2(a.table + line);
+        if (tid == 0) prefetch_l2(a.table + (c < entries ? c : 0));
+        if (tid < 32 && tid * 32 < a.n_seq) prefetch_l2(a.lens + tid * 32);
+        if (tid == 32) prefetch_l2(a.q);
+        if (tid == 64) prefetch_l2(a.kv.k);
+        if (tid == 96) prefetch_l2(a.kv.v);
+    }
     pdl_wait();
 
     // the tiles of all sequences, and where this CTA's share begins
@@ -448,10 +459,10 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<HD, F16>::CTAS) k_paged_at
                         sc[n] += lo;
                     }
                 } else {
-                    constexpr int C = HD / 64;  // chains of 4 (high terms of K) and 8 products
+                    constexpr int C = 2;  // chains: 4 of the high terms of K, 2 of the low ones
                     float s0[2 * C][4] = {}, s1[C][4] = {};
                     const uint32_t ka = kb + g * S::KP + j4 * 16;
-#pragma unroll
+#pragma unroll 4
                     for (int i = 0; i < HD / 16; i++) {
                         const float4 t = lds128(ka + i * 64);
                         const float kv4[4] = {t.x, t.y, t.z, t.w};
@@ -651,11 +662,14 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<HD, F16>::CTAS) k_paged_at
 // the later ones' first.
 LT_DEVINL uint64_t pa_part(uint32_t first, uint32_t p) { return 2 * (uint64_t)(first + p) + (p == 0 ? 1 : 0); }
 
-// Units that several CTAs share: one row per CTA.
+constexpr uint32_t kPaMaxParts = 512;  // CTAs of a launch at most (pa_grid), and so records of a unit
+
+// Row r of a unit that several CTAs share: out = sum_p 2^(m_p - m) o_p / sum_p 2^(m_p - m) l_p over
+// its records in CTA order.  The first records' sums are on their way while the weights are found.
 template <int HD, bool PROMPT>
 LT_DEVINL void pa_join_row(const PagedAttnArgs &a, uint64_t u, uint32_t r) {
-    constexpr int LANES = HD / 4, GROUPS = 128 / LANES;
-    __shared__ float s_red[4], s_red2[4];
+    constexpr int LANES = HD / 4, GROUPS = 128 / LANES, EARLY = 8;
+    __shared__ float s_w[kPaMaxParts], s_red[4], s_red2[4];
     __shared__ float4 s_o[128];
     __shared__ uint32_t s_off;
     const uint32_t rb = (uint32_t)(u % a.row_blocks);
@@ -671,53 +685,67 @@ LT_DEVINL void pa_join_row(const PagedAttnArgs &a, uint64_t u, uint32_t r) {
     const uint32_t R = rb * kPaRows + r;
     if (R >= nq * a.group) return;
     const uint32_t first = a.unit_info[2 * u], n = a.unit_info[2 * u + 1];
-    if (n < 2) return;
-    float m = -INFINITY;
-    for (uint32_t p = tid; p < n; p += 128) m = fmaxf(m, a.part_ml[pa_part(first, p) * 16 + r]);
+    if (n < 2 || n > kPaMaxParts) return;
+    const int grp = tid / LANES, x = tid % LANES;
+    const auto sums = [&](uint32_t p) {
+        return *reinterpret_cast<const float4 *>(a.part_o + (pa_part(first, p) * kPaRows + r) * HD + 4 * x);
+    };
+    float4 v[EARLY];
+#pragma unroll
+    for (int i = 0; i < EARLY; i++)
+        if (grp + i * GROUPS < n) v[i] = sums(grp + i * GROUPS);
+    constexpr int PER = kPaMaxParts / 128;
+    float pm[PER], pl[PER], m = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+        pm[i] = -INFINITY;
+        pl[i] = 0.0f;
+        if (tid + 128 * i < n) {
+            const float *ml = a.part_ml + pa_part(first, tid + 128 * i) * 16 + r;
+            pm[i] = ml[0];
+            pl[i] = ml[8];
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < PER; i++) m = fmaxf(m, pm[i]);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     if (lane == 0) s_red[warp] = m;
+    if (tid == 0) s_off = 0;
     __syncthreads();
     m = fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3]));
     const float ms = m == -INFINITY ? 0.0f : m;
     float l = 0.0f;
-    for (uint32_t p = tid; p < n; p += 128) {
-        const float *ml = a.part_ml + pa_part(first, p) * 16 + r;
-        l += ml[8] * ex2(ml[0] - ms);
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+        const float w = ex2(pm[i] - ms);
+        if (tid + 128 * i < n) s_w[tid + 128 * i] = w;
+        l = fmaf(pl[i], w, l);
     }
     l = warp_sum(l);
     if (lane == 0) s_red2[warp] = l;
-    const int grp = tid / LANES, x = tid % LANES;
+    __syncthreads();
     float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    auto add = [&](const float4 &t, float w) {
+        acc.x = fmaf(t.x, w, acc.x);
+        acc.y = fmaf(t.y, w, acc.y);
+        acc.z = fmaf(t.z, w, acc.z);
+        acc.w = fmaf(t.w, w, acc.w);
+    };
+#pragma unroll
+    for (int i = 0; i < EARLY; i++)
+        if (grp + i * GROUPS < n) add(v[i], s_w[grp + i * GROUPS]);
 #pragma unroll 8
-    for (uint32_t p = grp; p < n; p += GROUPS) {
-        const uint64_t k = pa_part(first, p);
-        const float w = ex2(a.part_ml[k * 16 + r] - ms);
-        const float4 v = *reinterpret_cast<const float4 *>(a.part_o + (k * kPaRows + r) * HD + 4 * x);
-        acc.x = fmaf(v.x, w, acc.x);
-        acc.y = fmaf(v.y, w, acc.y);
-        acc.z = fmaf(v.z, w, acc.z);
-        acc.w = fmaf(v.w, w, acc.w);
-    }
+    for (uint32_t p = grp + EARLY * GROUPS; p < n; p += GROUPS) add(sums(p), s_w[p]);
     s_o[tid] = acc;
-    if (tid == 0) s_off = 0;
     __syncthreads();
     if (grp == 0) {
         l = (s_red2[0] + s_red2[1]) + (s_red2[2] + s_red2[3]);
 #pragma unroll
-        for (int i = 1; i < GROUPS; i++) {
-            const float4 v = s_o[i * LANES + x];
-            acc.x += v.x;
-            acc.y += v.y;
-            acc.z += v.z;
-            acc.w += v.w;
-        }
+        for (int i = 1; i < GROUPS; i++) add(s_o[i * LANES + x], 1.0f);
         const float inv = l > 0.0f ? __fdiv_rn(1.0f, l) : (l == 0.0f ? 0.0f : l);
         float *dst = a.out + (uint64_t)(q0 + R / a.group) * a.out_stride + (uint64_t)(kh * a.group + R % a.group) * HD + 4 * x;
-        dst[0] = acc.x * inv;
-        dst[1] = acc.y * inv;
-        dst[2] = acc.z * inv;
-        dst[3] = acc.w * inv;
+        *reinterpret_cast<float4 *>(dst) = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
         if (PROMPT && (acc.x - acc.x) + (acc.y - acc.y) + (acc.z - acc.z) + (acc.w - acc.w) + (l - l) != 0.0f) s_off = 1;
     }
     if (PROMPT) {
@@ -728,12 +756,12 @@ LT_DEVINL void pa_join_row(const PagedAttnArgs &a, uint64_t u, uint32_t r) {
 
 // mass[s][kv head][j] += sum over the KV head's query heads of 2^(score - m) / l, for
 // kMassKeys positions from j0 on; a thread's cells are its own.  The scores are on
-// their way while the heads' m and l are put together.
+// their way while the heads' m and l are put together, 16 threads to a head.
 LT_DEVINL void pa_mass(const PagedAttnArgs &a, uint32_t s, uint32_t kh, uint32_t j0) {
     extern __shared__ float s_ml[];  // [group] maxima, [group] 1 / sum
     const PaSeq q = pa_seq<false>(a, s, 1, false);
     if (j0 >= q.len || j0 + kMassKeys <= q.lo) return;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x;
     constexpr int H = 8;
     const uint32_t j = j0 + 4 * tid;
     const float *sc = a.scores + ((uint64_t)s * a.n_heads + kh * a.group) * a.score_stride + j;
@@ -744,24 +772,51 @@ LT_DEVINL void pa_mass(const PagedAttnArgs &a, uint32_t s, uint32_t kh, uint32_t
             if (j < q.len && h0 + h < a.group) v[h] = *reinterpret_cast<const float4 *>(sc + (h0 + h) * a.score_stride);
     };
     load(0);
-    for (uint32_t h = warp; h < a.group; h += 4) {
-        const uint64_t u = pa_unit(a, s, kh, h / kPaRows);
-        const uint32_t r = h % kPaRows, first = a.unit_info[2 * u], n = a.unit_info[2 * u + 1];
-        float m = -INFINITY, l = 0.0f;
-        if (n < 2) {
-            m = a.unit_ml[u * 16 + r];
-            l = a.unit_ml[u * 16 + 8 + r];
-        } else {
-            for (uint32_t p = lane; p < n; p += 32) m = fmaxf(m, a.part_ml[pa_part(first, p) * 16 + r]);
+    float *mass = a.mass + ((uint64_t)s * a.kv.n_kv + kh) * a.mass_stride + j;
+    float old[4];
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-            for (uint32_t p = lane; p < n; p += 32) {
-                const float *ml = a.part_ml + pa_part(first, p) * 16 + r;
-                l += ml[8] * ex2(ml[0] - (m == -INFINITY ? 0.0f : m));
+    for (int e = 0; e < 4; e++) old[e] = j + e >= q.lo && j + e < q.len ? mass[e] : 0.0f;
+    for (uint32_t h0 = 0; h0 < a.group; h0 += 8) {  // 8 heads at once: the rows of one unit
+        const uint32_t h = h0 + tid / 16, t = tid % 16;
+        const uint64_t u = pa_unit(a, s, kh, h0 / kPaRows);
+        const uint32_t r = tid / 16, first = a.unit_info[2 * u], n = a.unit_info[2 * u + 1];
+        float m = -INFINITY, l = 0.0f;
+        if (h < a.group) {
+            if (n < 2) {
+                if (t == 0) {
+                    m = a.unit_ml[u * 16 + r];
+                    l = a.unit_ml[u * 16 + 8 + r];
+                }
+            } else {
+                for (uint32_t p0 = t; p0 < n; p0 += 16 * 8) {
+                    float pm[8], pl[8];
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const bool there = p0 + 16 * i < n;
+                        const float *ml = a.part_ml + pa_part(first, there ? p0 + 16 * i : 0) * 16 + r;
+                        pm[i] = there ? ml[0] : -INFINITY;
+                        pl[i] = there ? ml[8] : 0.0f;
+                    }
+                    float mn = m;
+#pragma unroll
+                    for (int i = 0; i < 8; i++) mn = fmaxf(mn, pm[i]);
+                    const float ms = mn == -INFINITY ? 0.0f : mn;
+                    l *= ex2(m - ms);
+#pragma unroll
+                    for (int i = 0; i < 8; i++) l = fmaf(pl[i], ex2(pm[i] - ms), l);
+                    m = mn;
+                }
             }
-            l = warp_sum(l);
         }
-        if (lane == 0) {
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) {
+            const float m2 = __shfl_xor_sync(0xffffffffu, m, o), l2 = __shfl_xor_sync(0xffffffffu, l, o);
+            const float mn = fmaxf(m, m2), ms = mn == -INFINITY ? 0.0f : mn;
+            const float x = l * ex2(m - ms), y = l2 * ex2(m2 - ms);
+            l = x + y;
+            m = mn;
+        }
+        if (t == 0 && h < a.group) {
             // the sums carry the weights' factor 2^10 on f16 caches
             s_ml[h] = m == -INFINITY ? 0.0f : m - (a.kv.f16 ? 10.0f : 0.0f);
             s_ml[a.group + h] = l > 0.0f ? 1.0f / l : 0.0f;
@@ -782,10 +837,9 @@ LT_DEVINL void pa_mass(const PagedAttnArgs &a, uint32_t s, uint32_t kh, uint32_t
             w[3] = fmaf(ex2(v[h].w - m), f, w[3]);
         }
     }
-    float *mass = a.mass + ((uint64_t)s * a.kv.n_kv + kh) * a.mass_stride + j;
 #pragma unroll
     for (int e = 0; e < 4; e++)
-        if (j + e >= q.lo && j + e < q.len) mass[e] += w[e];
+        if (j + e >= q.lo && j + e < q.len) mass[e] = old[e] + w[e];
 }
 
 // What is left when the tiles are done: rows to join, then weights to add up.
@@ -827,7 +881,9 @@ PaScratch pa_layout(const PagedAttnArgs &a, uint32_t G) {
     return s;
 }
 
-uint32_t pa_grid(uint32_t hd, int num_sms) { return (uint32_t)num_sms * (hd == 256 ? 1 : hd == 128 ? 2 : 3); }
+uint32_t pa_grid(uint32_t hd, int num_sms) {
+    return min((uint32_t)num_sms * (hd == 256 ? 1 : hd == 128 ? 2 : 3), kPaMaxParts);
+}
 
 template <int HD, bool F16, bool PROMPT>
 cudaError_t pa_launch(const LaunchCfg &c, const PagedAttnArgs &a, uint64_t units) {
