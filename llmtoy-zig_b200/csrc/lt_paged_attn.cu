@@ -10,7 +10,8 @@
 //
 // Bound: memory (K and V are read once per 8 query heads of a KV head).
 // - Work is (sequence, KV head, 8 rows) x tiles of the sequence's keys, counted
-//   through one after the other; every CTA takes an equal share of the tiles,
+//   through one after the other (a unit's start counts as kUnitCost tiles more:
+//   its queries, its merge, its output); every CTA takes an equal share of the count,
 //   wherever it begins and ends, so lengths may differ as they like.  A unit
 //   that several CTAs share leaves partial (m, l, sum) records, which
 //   k_paged_finish adds up in CTA order: the result does not depend on timing.
@@ -47,12 +48,17 @@ struct PaShape {
     static constexpr int CTAS = HD == 256 ? 1 : HD == 128 ? 2 : 3;
 };
 
+// What a unit costs beyond its tiles, in tiles.  64 sequences of 200 to 8192: 66 us without, 62 with 1,
+// 58 with 2 to 4 (a CTA of many short units was the last to end).
+constexpr uint32_t kUnitCost = 3;
+
 // A sequence's share of the work.
 struct PaSeq {
     uint32_t len, nq, q0;   // cached positions, query tokens, first query row
     uint32_t lo;            // first position any query sees
     uint32_t base;          // where its tiles start: lo, or the block of 16 it lies in
     uint32_t blocks, tiles; // 8-row blocks per KV head, tiles per unit
+    LT_DEVINL uint32_t cost() const { return tiles + kUnitCost; }
 };
 
 template <bool PROMPT>
@@ -111,19 +117,14 @@ struct PaWalk {
             if (a.window) lo = (uint32_t)max((int64_t)q.lo, i0 - (int64_t)a.window + 1);
         }
     }
-    LT_DEVINL uint32_t units(const PagedAttnArgs &a) const { return q.blocks * a.kv.n_kv; }
-    // The next tile; the caller stops at the end of its share, which is never past the last sequence.
+    // The next unit's first tile; past the last sequence s == n_seq.
     template <int TILE>
-    LT_DEVINL void next(const PagedAttnArgs &a) {
-        if (++tile < q.tiles) return;
+    LT_DEVINL void next_unit(const PagedAttnArgs &a) {
         tile = 0;
-        if (++unit >= units(a)) {
+        if (++unit >= q.blocks * a.kv.n_kv) {
             unit = 0;
             do {
-                if (++s >= a.n_seq) {
-                    q.tiles = 0xffffffffu;
-                    return;
-                }
+                if (++s >= a.n_seq) return;
                 q = pa_seq<PROMPT>(a, s, TILE, false);
             } while (q.blocks == 0);
         }
@@ -189,7 +190,7 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<HD, F16>::CTAS) k_paged_at
 #pragma unroll 4
     for (uint32_t s = sa; s < sb; s++) {
         const PaSeq q = pa_seq<PROMPT>(a, s, TILE, c == 0);
-        mine += (uint64_t)q.blocks * a.kv.n_kv * q.tiles;
+        mine += (uint64_t)q.blocks * a.kv.n_kv * q.cost();
     }
     uint64_t incl = mine;
 #pragma unroll
@@ -209,12 +210,13 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<HD, F16>::CTAS) k_paged_at
     const uint32_t G = (uint32_t)min((uint64_t)gridDim.x, T);
     if (c >= G) return;
     const PaShare share(T, G);
-    const uint64_t f0 = share.start(c), f1 = share.start(c + 1);
+    uint64_t f0 = share.start(c);
+    const uint64_t f1 = share.start(c + 1);
     if (f0 >= before && f0 < before + mine) {
         uint64_t rem = f0 - before;
         for (uint32_t s = sa; s < sb; s++) {
             const PaSeq q = pa_seq<PROMPT>(a, s, TILE, false);
-            const uint64_t w = (uint64_t)q.blocks * a.kv.n_kv * q.tiles;
+            const uint64_t w = (uint64_t)q.blocks * a.kv.n_kv * q.cost();
             if (rem < w) {
                 s_seq = s;
                 s_rem = rem;
@@ -228,10 +230,17 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<HD, F16>::CTAS) k_paged_at
     PaWalk<PROMPT> cw, lw;  // the compute walk and the copies ahead of it
     cw.s = s_seq;
     cw.q = s_q;
-    cw.unit = (uint32_t)div_small(s_rem, cw.q.tiles);
-    cw.tile = (uint32_t)(s_rem - (uint64_t)cw.unit * cw.q.tiles);
-    cw.set_unit(a);
+    cw.unit = (uint32_t)div_small(s_rem, cw.q.cost());
+    cw.tile = (uint32_t)(s_rem - (uint64_t)cw.unit * cw.q.cost());
+    if (cw.tile >= cw.q.tiles) {  // in what the unit before costs beyond its tiles
+        f0 += cw.q.cost() - cw.tile;
+        if (f0 >= f1) return;
+        cw.template next_unit<TILE>(a);
+    } else {
+        cw.set_unit(a);
+    }
     lw = cw;
+    uint64_t lf = f0;  // lw's place in the count
 
     // a unit's queries: warp w takes rows 2 w and 2 w + 1; the first unit's come while K and V are looked up
     float qv[2][HD / 32];
@@ -258,10 +267,11 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<HD, F16>::CTAS) k_paged_at
     const int row0 = CH < 32 ? lane / CH : 0, col0 = CH < 32 ? lane % CH : lane;
     const uint64_t lane_off = (uint64_t)row0 * a.kv.slot_stride + col0 * 16, step_off = STEP * a.kv.slot_stride;
     struct Job {
-        uint32_t page, key, kh, lo, hi;  // key 0xffffffff: nothing to copy
+        uint32_t page, key, kh, lo, hi;  // key 0xffffffff: only zeros
+        bool there;
     };
     auto look = [&]() {
-        Job j = {a.kv.n_pages, lw.base + lw.tile * TILE + warp * KB + (in_page ? 0 : lane), lw.kh, lw.lo, lw.hi};
+        Job j = {a.kv.n_pages, lw.base + lw.tile * TILE + warp * KB + (in_page ? 0 : lane), lw.kh, lw.lo, lw.hi, true};
         if (in_page ? j.key < j.hi && j.key + KB > j.lo : lane < KB && j.key < j.hi && j.key >= j.lo)
             j.page = a.table[(uint64_t)lw.s * a.kv.max_pages + page_of(a.kv, j.key)];
         else
@@ -311,22 +321,23 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<HD, F16>::CTAS) k_paged_at
         }
     };
     // all pages of the first blocks are looked up before the first copy waits for its own
-    const uint64_t nf = f1 - f0;
-    uint64_t looked = 0, copied = 0;
     Job jobs[S::STAGES];
     auto look_next = [&](Job &j) {
-        if (looked >= nf) return;
+        j.there = lf < f1;
+        if (!j.there) return;
         j = look();
-        if (++looked < nf) lw.template next<TILE>(a);
+        if (++lw.tile < lw.q.tiles) {
+            lf++;
+        } else {
+            lf += 1 + kUnitCost;
+            if (lf < f1) lw.template next_unit<TILE>(a);
+        }
     };
 #pragma unroll
     for (int st = 0; st < S::STAGES; st++) look_next(jobs[st]);
 #pragma unroll
     for (int st = 0; st < S::STAGES - 1; st++) {
-        if (copied < nf) {
-            copy(jobs[st], st);
-            copied++;
-        }
+        if (jobs[st].there) copy(jobs[st], st);
         cp_async_commit();
     }
     Job job = jobs[S::STAGES - 1];
@@ -335,8 +346,7 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<HD, F16>::CTAS) k_paged_at
     int stage = 0;
     while (f < f1) {
         // ── one segment: this CTA's tiles of one unit ──
-        const uint64_t left = cw.q.tiles - cw.tile;
-        const uint32_t seg = (uint32_t)min(left, f1 - f);
+        const uint32_t seg = (uint32_t)min((uint64_t)(cw.q.tiles - cw.tile), f1 - f);
         const uint64_t unit_f0 = f - cw.tile;
         const uint32_t rows = min((uint32_t)kPaRows, cw.q.nq * a.group - cw.rb * kPaRows);
         // queries to operand fragments
@@ -563,9 +573,8 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<HD, F16>::CTAS) k_paged_at
             __syncwarp();
             int fill = stage + S::STAGES - 1;
             if (fill >= S::STAGES) fill -= S::STAGES;
-            if (copied < nf) {
+            if (job.there) {
                 copy(job, fill);
-                copied++;
                 look_next(job);
             }
             cp_async_commit();
@@ -649,9 +658,9 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<HD, F16>::CTAS) k_paged_at
             }
         }
         __syncthreads();  // the merge records are read before the next queries overwrite them
-        f += seg;
+        f = unit_f0 + cw.q.cost();  // the next unit, unless this one goes on elsewhere
         if (f < f1) {
-            cw.template next<TILE>(a);
+            cw.template next_unit<TILE>(a);
             load_q();
         }
     }
