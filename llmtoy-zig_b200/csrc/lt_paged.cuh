@@ -115,6 +115,26 @@ LT_DEVINL float tanh_small(float x) {
     return fmaf(r * y, x, x);
 }
 
+LT_DEVINL float2 fmul2(float2 a, float2 b) {
+    f2u A, B, D;
+    A.f = a;
+    B.f = b;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(D.u) : "l"(A.u), "l"(B.u));
+    return D.f;
+}
+// tanh_small of two values.
+LT_DEVINL float2 tanh_small2(float2 x) {
+    const float2 y = fmul2(x, x);
+    auto both = [](float c) { return make_float2(c, c); };
+    float2 r = both(0.0022146995179355145f);
+    r = ffma2(r, y, both(-0.008248303085565567f));
+    r = ffma2(r, y, both(0.021726185455918312f));
+    r = ffma2(r, y, both(-0.05395074933767319f));
+    r = ffma2(r, y, both(0.133332297205925f));
+    r = ffma2(r, y, both(-0.3333333134651184f));
+    return ffma2(fmul2(r, y), x, x);
+}
+
 // tanh over the whole range: 1 - 2 / (1 + e^(2|x|)) with one Newton step on the
 // reciprocal past kTanhSmall (absolute error about 1e-7 there).  No branch and no
 // call: it stands in unrolled loops.
@@ -130,12 +150,10 @@ LT_DEVINL float tanh_any(float x) {
 // Score of one (query, key) pair in units of log2: the scaled product, capped
 // by cap * tanh(s / cap), minus slope * |distance|.  f is the row's factor on
 // the raw product: scale * log2(e) without a cap, scale / cap with one.
-// SMALL: |dot * f| is known not to pass kTanhSmall.
-template <bool SMALL = false>
 LT_DEVINL float score_log2(float dot, float f, float cap, float slope, float dist) {
     constexpr float kLog2e = 1.4426950408889634f;
     float s = dot * f;
-    if (cap != 0.0f) s = (SMALL ? tanh_small(s) : tanh_any(s)) * (cap * kLog2e);
+    if (cap != 0.0f) s = tanh_any(s) * (cap * kLog2e);
     return fmaf(-slope * kLog2e, dist, s);
 }
 

@@ -856,9 +856,15 @@ template <int HD, bool PROMPT>
 __global__ void __launch_bounds__(128) k_paged_finish(PagedAttnArgs a, uint32_t n_join) {
     pdl_launch_dependents();
     pdl_wait();
-    if (blockIdx.x < n_join) {
+    if constexpr (PROMPT) {  // many units, few of them shared: a CTA looks at one unit
+        if (a.unit_info[2 * (uint64_t)blockIdx.x + 1] < 2) return;
+        for (uint32_t r = 0; r < kPaRows; r++) {
+            pa_join_row<HD, PROMPT>(a, blockIdx.x, r);
+            __syncthreads();
+        }
+    } else if (blockIdx.x < n_join) {  // few units: a CTA does one row
         pa_join_row<HD, PROMPT>(a, blockIdx.x / kPaRows, blockIdx.x % kPaRows);
-    } else if (!PROMPT) {
+    } else {
         const uint32_t b = blockIdx.x - n_join, steps = (a.max_len + kMassKeys - 1) / kMassKeys;
         pa_mass(a, b / steps / a.kv.n_kv, b / steps % a.kv.n_kv, b % steps * kMassKeys);
     }
@@ -905,7 +911,7 @@ cudaError_t pa_launch(const LaunchCfg &c, const PagedAttnArgs &a, uint64_t units
         e = launch_k(c, label, k_paged_attn<HD, F16, PROMPT, false>, grid, dim3(kPaThreads), PaShape<HD, F16>::SMEM, a);
     if (e != cudaSuccess) return e;
     if (e != cudaSuccess) return e;
-    const uint64_t join = units * kPaRows;
+    const uint64_t join = PROMPT ? units : units * kPaRows;
     const uint64_t mass = a.mass ? (uint64_t)((a.max_len + kMassKeys - 1) / kMassKeys) * a.kv.n_kv * a.n_seq : 0;
     if (join + mass > 0x7fffffffull) return cudaErrorInvalidValue;
     return launch_k(c, "paged_finish", k_paged_finish<HD, PROMPT>, dim3((uint32_t)(join + mass)), dim3(128),

@@ -237,32 +237,6 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(PagedAttnArgs a,
         tmem_alloc(tmem_slot, 512);
         tmem_relinquish();
     }
-    if (skipping) {
-        // a tile is left out when the ranges of document numbers do not meet
-        for (int i = tid; i < kPpSkipTiles / 32; i += kPpThreads) skip[i] = 0;
-        uint32_t dmin = 0xffffffffu, dmax = 0;
-        for (int64_t i = max((int64_t)0, i0) + lane; i <= i1; i += 32) {
-            dmin = min(dmin, docs[i]);
-            dmax = max(dmax, docs[i]);
-        }
-        dmin = __reduce_min_sync(0xffffffffu, dmin);
-        dmax = __reduce_max_sync(0xffffffffu, dmax);
-        __syncthreads();
-        for (uint32_t t = begin + warp; t < tiles; t += kPpThreads / 32) {
-            uint32_t kmin = 0xffffffffu, kmax = 0;
-#pragma unroll
-            for (int e = 0; e < KT / 32; e++) {
-                const uint32_t j = lo + t * KT + e * 32 + lane;
-                if (j < hi) {
-                    kmin = min(kmin, docs[j]);
-                    kmax = max(kmax, docs[j]);
-                }
-            }
-            kmin = __reduce_min_sync(0xffffffffu, kmin);
-            kmax = __reduce_max_sync(0xffffffffu, kmax);
-            if (lane == 0 && kmin <= dmax && dmin <= kmax) atomicOr(skip + t / 32, 1u << (t % 32));
-        }
-    }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -284,6 +258,33 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(PagedAttnArgs a,
 
     if (warp >= 8) {
         regs_dec<S::REGS_REST>();
+        if (skipping) {
+            // a tile is left out when the ranges of document numbers do not meet
+            for (int i = tid - 256; i < kPpSkipTiles / 32; i += 128) skip[i] = 0;
+            uint32_t dmin = 0xffffffffu, dmax = 0;
+            for (int64_t i = max((int64_t)0, i0) + lane; i <= i1; i += 32) {
+                dmin = min(dmin, docs[i]);
+                dmax = max(dmax, docs[i]);
+            }
+            dmin = __reduce_min_sync(0xffffffffu, dmin);
+            dmax = __reduce_max_sync(0xffffffffu, dmax);
+            named_sync<4, 128>();
+            for (uint32_t t = begin + warp - 8; t < tiles; t += 4) {
+                uint32_t kmin = 0xffffffffu, kmax = 0;
+    #pragma unroll
+                for (int e = 0; e < KT / 32; e++) {
+                    const uint32_t j = lo + t * KT + e * 32 + lane;
+                    if (j < hi) {
+                        kmin = min(kmin, docs[j]);
+                        kmax = max(kmax, docs[j]);
+                    }
+                }
+                kmin = __reduce_min_sync(0xffffffffu, kmin);
+                kmax = __reduce_max_sync(0xffffffffu, kmax);
+                if (lane == 0 && kmin <= dmax && dmin <= kmax) atomicOr(skip + t / 32, 1u << (t % 32));
+            }
+            named_sync<3, kPpThreads>();
+        }
         if (warp > 8) {
             // ── K and V tiles into the ring ──
             const int pt = tid - 288, pw = warp - 9;
@@ -608,6 +609,7 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(PagedAttnArgs a,
             tc_fence_after();
         }
         rf = fabsf(rf);
+        if (skipping) named_sync<3, kPpThreads>();
         mbar_arrive(p_full + tile);
 
         float o[OW];
@@ -668,23 +670,32 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(PagedAttnArgs a,
                         top = fmaxf(top, fmaxf(x0, x1));
                         continue;
                     }
-                    auto score = [&](auto small) {
-                        constexpr bool SMALL = decltype(small)::value;
-#pragma unroll
-                        for (int e = 0; e < 16; e++) {
-                            const float x = score_log2<SMALL>(__uint_as_float(u[e]), rf, a.softcap, row_slope,
-                                                              fabsf(dist - (float)(c + e)));
-                            u[e] = __float_as_uint(x);
-                        }
-                    };
-                    if (EXTRA) {
+                    if (EXTRA) {  // score_log2, the usual case two at a time
+                        constexpr float kLog2e = 1.4426950408889634f;
                         float big = 0.0f;
 #pragma unroll
                         for (int e = 0; e < 16; e++) big = fmaxf(big, fabsf(__uint_as_float(u[e])));
-                        if (__all_sync(0xffffffffu, big * rf <= kTanhSmall))
-                            score(IntC<1>());
-                        else
-                            score(IntC<0>());
+                        if (a.softcap == 0.0f || __all_sync(0xffffffffu, big * rf <= kTanhSmall)) {
+                            const float2 f2 = make_float2(rf, rf);
+                            const float cl = a.softcap * kLog2e;
+#pragma unroll
+                            for (int e = 0; e < 16; e += 2) {
+                                float2 x = fmul2(make_float2(__uint_as_float(u[e]), __uint_as_float(u[e + 1])), f2);
+                                if (a.softcap != 0.0f) x = fmul2(tanh_small2(x), make_float2(cl, cl));
+                                u[e] = __float_as_uint(x.x);
+                                u[e + 1] = __float_as_uint(x.y);
+                            }
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 16; e++)
+                                u[e] = __float_as_uint(tanh_any(__uint_as_float(u[e]) * rf) * (a.softcap * kLog2e));
+                        }
+                        if (a.slopes) {
+                            const float sl = -row_slope * kLog2e;
+#pragma unroll
+                            for (int e = 0; e < 16; e++)
+                                u[e] = __float_as_uint(fmaf(sl, fabsf(dist - (float)(c + e)), __uint_as_float(u[e])));
+                        }
                     }
                     if (!plain) {
                         uint32_t seen = to > c ? (to - c >= 16 ? 0xffffu : (1u << (to - c)) - 1u) : 0u;
@@ -973,7 +984,12 @@ bool pp_regs() {
 bool paged_prompt_supported(const PagedAttnArgs &a) {
     static const bool regs = pp_regs<64, false>() && pp_regs<64, true>() && pp_regs<128, false>() &&
                              pp_regs<128, true>() && pp_regs<256, false>() && pp_regs<256, true>();
-    return regs && a.kv.f16 && (uint64_t)a.max_q * a.group >= 64;
+    // Few rows: the kernel for single tokens reads the cache once per 8 rows.  Measured at 1 and 8
+    // sequences of 60 to 8000 cached tokens: 8 rows 31 to 110 us there and 38 to 213 here, 16 rows
+    // about alike (60 and 70 us at most), 28 rows of 60 tokens 7.9 and 10.0 us, 32 rows of 8000
+    // tokens 100 and 72 us, 56 rows of 60 tokens 16 and 10 us.
+    const uint64_t rows = (uint64_t)a.max_q * a.group;
+    return regs && a.kv.f16 && rows > (a.max_len > 256 ? 16 : 32);
 }
 
 size_t paged_prompt_scratch(PagedAttnArgs a, int num_sms) {
