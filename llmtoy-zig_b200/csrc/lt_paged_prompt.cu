@@ -25,11 +25,15 @@
 // of high terms, then 8 of low ones, over the 16 columns of S they come from.
 //
 // Bound: the tensor cores, from a few hundred rows on.  One B200, 8192 tokens,
-// 32/4 heads of 128, causal (550 GFLOP, 1.1 TFLOP as done): 0.98 ms, that is
-// 1.12 PFLOP/s of products against 1.38 sustained by a cuBLAS bf16 GEMM on this
+// 32/4 heads of 128, causal (550 GFLOP, 1.1 TFLOP as done): 0.97 ms, that is
+// 1.13 PFLOP/s of products against 1.38 sustained by a cuBLAS bf16 GEMM on this
 // part (1.65 in a burst); a pass over one tile of 256 x 128 takes 5350 clocks, its
 // products alone 4160.  With few rows, latency: a 257-token follow-up on 1243 cached
 // ones (14/2 heads of 64) takes 21 us with its keys shared by 6 CTAs, 37 us without.
+// head_dim 256 (6320 tokens of packed documents, 246 us) waits for K: the queries
+// leave room for three stages only, and a K tile's copy starts when the product
+// before the last is done.  Prefetching tiles into L2 made every case slower (8192
+// tokens 1.15 ms), as did one KV head after the other (1.01 ms).
 #include <cuda.h>  // CUtensorMap (encoded through the runtime's driver entry point)
 
 #include "lt_paged.cuh"
@@ -200,10 +204,11 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(PagedAttnArgs a,
     pdl_launch_dependents();
     pdl_wait();
 
-    // this CTA's rows; the longest (last) row blocks of a causal prompt come first
+    // this CTA's rows; the last row blocks of all prompts, the longest of causal ones, come first
     // (a row block may be shared by nsplit CTAs, each with its part of the keys)
-    const uint32_t s = blockIdx.z, kh = blockIdx.y, split = blockIdx.x % a.nsplit;
-    const uint32_t rb = gridDim.x / a.nsplit - 1 - blockIdx.x / a.nsplit;
+    uint32_t at = blockIdx.x;
+    const uint32_t split = at % a.nsplit, kh = (at /= a.nsplit) % a.kv.n_kv, s = (at /= a.kv.n_kv) % a.n_seq;
+    const uint32_t rb = a.row_blocks - 1 - at / a.n_seq;
     const uint32_t cap = (uint32_t)min((uint64_t)a.kv.max_pages * a.kv.page_size, (uint64_t)a.max_len);
     uint32_t len = a.lens[s];
     const uint32_t c0 = a.cu[s], c1 = a.cu[s + 1];
@@ -651,8 +656,9 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(PagedAttnArgs a,
             wait(s_full + sb, HD == 256 ? (jj / 2) & 1 : jj & 1);
             __syncwarp();
             tc_fence_after();
-            const bool whole = !docs && row_lo <= k0 && k0 + CW <= row_hi;
-            const bool plain = __all_sync(0xffffffffu, whole || !real);
+            // whether every row of the warp sees all of its columns, documents aside and altogether
+            const bool in_range = __all_sync(0xffffffffu, (row_lo <= k0 && k0 + CW <= row_hi) || !real);
+            const bool plain = in_range && !docs;
             // pass 1: the row's maximum; capped, biased or masked scores go back to tensor
             // memory.  Each load runs while the columns before it are worked on.
             float top = -INFINITY;
@@ -683,13 +689,20 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(PagedAttnArgs a,
                         float big = 0.0f;
 #pragma unroll
                         for (int e = 0; e < 16; e++) big = fmaxf(big, fabsf(__uint_as_float(u[e])));
-                        if (a.softcap == 0.0f || __all_sync(0xffffffffu, big * rf <= kTanhSmall)) {
-                            const float2 f2 = make_float2(rf, rf);
-                            const float cl = a.softcap * kLog2e;
+                        const float2 f2 = make_float2(rf, rf);
+                        if (a.softcap == 0.0f) {
+#pragma unroll
+                            for (int e = 0; e < 16; e += 2) {
+                                const float2 x = fmul2(make_float2(__uint_as_float(u[e]), __uint_as_float(u[e + 1])), f2);
+                                u[e] = __float_as_uint(x.x);
+                                u[e + 1] = __float_as_uint(x.y);
+                            }
+                        } else if (__all_sync(0xffffffffu, big * rf <= kTanhSmall)) {
+                            const float2 cl = make_float2(a.softcap * kLog2e, a.softcap * kLog2e);
 #pragma unroll
                             for (int e = 0; e < 16; e += 2) {
                                 float2 x = fmul2(make_float2(__uint_as_float(u[e]), __uint_as_float(u[e + 1])), f2);
-                                if (a.softcap != 0.0f) x = fmul2(tanh_small2(x), make_float2(cl, cl));
+                                x = fmul2(tanh_small2(x), cl);
                                 u[e] = __float_as_uint(x.x);
                                 u[e + 1] = __float_as_uint(x.y);
                             }
@@ -705,21 +718,21 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(PagedAttnArgs a,
                                 u[e] = __float_as_uint(fmaf(sl, fabsf(dist - (float)(c + e)), __uint_as_float(u[e])));
                         }
                     }
-                    if (!plain) {
-                        uint32_t seen = to > c ? (to - c >= 16 ? 0xffffu : (1u << (to - c)) - 1u) : 0u;
-                        if (from > c) seen = from - c >= 16 ? 0u : seen & ~((1u << (from - c)) - 1u);
-                        if (docs) {
-                            const uint4 *dn = reinterpret_cast<const uint4 *>(docs_s + (jj % S::DOCS) * KT + half * 32 + c);
+                    constexpr uint32_t kMinusInf = 0xff800000u;
+                    if (!in_range) {
 #pragma unroll
-                            for (int e = 0; e < 4; e++) {
-                                const uint4 d = dn[e];
-                                seen &= ~((uint32_t)(d.x != row_doc) << (4 * e) | (uint32_t)(d.y != row_doc) << (4 * e + 1) |
-                                          (uint32_t)(d.z != row_doc) << (4 * e + 2) | (uint32_t)(d.w != row_doc) << (4 * e + 3));
-                            }
+                        for (int e = 0; e < 16; e++) u[e] = c + e >= from && c + e < to ? u[e] : kMinusInf;
+                    }
+                    if (docs) {
+                        const uint4 *dn = reinterpret_cast<const uint4 *>(docs_s + (jj % S::DOCS) * KT + half * 32 + c);
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            const uint4 d = dn[e];
+                            u[4 * e] = d.x == row_doc ? u[4 * e] : kMinusInf;
+                            u[4 * e + 1] = d.y == row_doc ? u[4 * e + 1] : kMinusInf;
+                            u[4 * e + 2] = d.z == row_doc ? u[4 * e + 2] : kMinusInf;
+                            u[4 * e + 3] = d.w == row_doc ? u[4 * e + 3] : kMinusInf;
                         }
-#pragma unroll
-                        for (int e = 0; e < 16; e++)
-                            if (!(seen >> e & 1u)) u[e] = 0xff800000u;  // -infinity
                     }
 #pragma unroll
                     for (int e = 0; e < 16; e++) top = fmaxf(top, __uint_as_float(u[e]));
@@ -973,8 +986,10 @@ cudaError_t pp_launch(const LaunchCfg &c, const PagedAttnArgs &a) {
     using S = PpShape<HD>;
     PpMaps maps;
     pp_maps(a.kv, S::KT, maps);
-    cudaError_t e = launch_k(c, "paged_prompt", k_paged_prompt<HD, EXTRA>, dim3(a.row_blocks * a.nsplit, a.kv.n_kv, a.n_seq),
-                             dim3(kPpThreads), S::SMEM, a, maps);
+    const uint64_t ctas = (uint64_t)a.row_blocks * a.nsplit * a.kv.n_kv * a.n_seq;
+    if (ctas > 0x7fffffffull) return cudaErrorInvalidValue;
+    cudaError_t e = launch_k(c, "paged_prompt", k_paged_prompt<HD, EXTRA>, dim3((uint32_t)ctas), dim3(kPpThreads), S::SMEM, a,
+                             maps);
     if (e != cudaSuccess || a.nsplit == 1) return e;
     const uint32_t rows = a.max_q * a.group;
     return launch_k(c, "paged_prompt_join", k_paged_prompt_join<HD>,
