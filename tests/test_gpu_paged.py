@@ -515,6 +515,99 @@ def test_prompt_longer(pkg, ctx, heads, kv, hd):
     check_prompt(pkg, ctx, heads, kv, hd, True, 16, [300, 700], [900, 700], seed=6, layout="hnd", q_pad=8)
 
 
+@pytest.mark.parametrize("heads,kv,hd", [(14, 2, 64), (32, 4, 128), (16, 8, 256)])
+@pytest.mark.parametrize("page,layout", [(1, "nhd"), (8, "hnd"), (20, "nhd"), (64, "hnd"), (128, "nhd"), (200, "hnd")])
+def test_prompt_pages(pkg, ctx, heads, kv, hd, page, layout):
+    """Pages smaller and larger than a tile of keys, a multiple of 8 slots or not, in both layouts."""
+    check_prompt(pkg, ctx, heads, kv, hd, True, page, [70, 150], [333, 150], seed=page, layout=layout)
+    check_prompt(pkg, ctx, heads, kv, hd, True, page, [90], [421], seed=page, layout=layout, window=130)
+
+
+def test_prompt_offsets_past_32_bits(pkg, ctx):
+    """Pages more than 4 GiB apart, on the way that copies them by tensor maps and on the other."""
+    rng = np.random.default_rng(19)
+    heads, kv, hd = 8, 1, 64
+    for page in (32, 9):
+        stride = 1 << 30  # elements: 2 GiB in f16
+        n = 4 * page - 3
+        c = Cache(pkg, rng, [n], kv, hd, True, page, extra_pages=0)
+        pools = []
+        for src in (c._k, c._v):
+            t = torch.empty(3 * stride + page * hd, dtype=torch.float16, device="cuda")
+            for p in range(4):
+                t[p * stride:p * stride + page * hd] = torch.from_numpy(np.nan_to_num(src[p])).cuda().reshape(-1)
+            pools.append(t)
+        desc = pkg.PagedKV(n_kv_heads=kv, head_dim=hd, kv_f16=1, page_size=page, n_pages=4, max_pages=c.width,
+                           page_stride=stride, slot_stride=hd, head_stride=hd, k=pools[0].data_ptr(), v=pools[1].data_ptr())
+        q = rng.normal(0, 1.5, (n, heads, hd)).astype(np.float32)
+        qd, out = torch.from_numpy(q.reshape(n, -1)).cuda(), torch.zeros(n, heads * hd, device="cuda")
+        cu, ln = i32([0, n]), i32([n])
+        cfg = pkg.PagedAttnCfg(n_heads=heads, causal=1, scale=1 / math.sqrt(hd))
+        ctx.paged_attn_prompt(cfg, desc, qd, 1, cu, n, n, c.dtable, ln, n, out)
+        ctx.sync()
+        K, V = c.seq(0)
+        i = np.arange(n)
+        want, _ = attend(q, K, V, i, i[None] <= i[:, None], 1 / math.sqrt(hd))
+        assert rel(out.cpu().numpy().reshape(want.shape), want) < ATTN_BAR
+        del pools, t
+
+
+@pytest.mark.parametrize("f16", [True, False])
+def test_serving_step_in_a_graph(pkg, ctx, f16):
+    """Append, prompt attention, decode with weights and eviction, recorded once and replayed on other contents."""
+    rng = np.random.default_rng(20)
+    heads, kv, hd, page, m = 14, 2, 64, 16, 40
+    lens = [60, 120]
+    c = Cache(pkg, rng, [n + 1 for n in lens], kv, hd, f16, page, extra_pages=12)
+    acfg = pkg.AttnCfg(n_heads=heads, n_kv_heads=kv, head_dim=hd, rope_neox=1, rope_theta=1e4, eps=1e-6, scale=1.0, kv_cap=1,
+                       kv_f16=int(f16))
+    cfg = pkg.PagedAttnCfg(n_heads=heads, causal=1, scale=1 / math.sqrt(hd))
+    qkv = torch.zeros(2, (heads + 2 * kv) * hd, device="cuda")
+    q, out = torch.zeros(2, heads * hd, device="cuda"), torch.zeros(2, heads * hd, device="cuda")
+    pq, pout = torch.zeros(2 * m, heads * hd, device="cuda"), torch.zeros(2 * m, heads * hd, device="cuda")
+    cu, seq, pos, ln = i32([0, m, 2 * m]), i32([0, 1]), i32(lens), i32([n + 1 for n in lens])
+    mass, mass2 = torch.zeros(2, kv, 128, device="cuda"), torch.zeros(2, kv, 50, device="cuda")
+    kept, ln2 = torch.zeros(2, kv, 50, dtype=torch.int32, device="cuda"), i32([0, 0])
+    dst = np.full_like(c.table, 0xFFFFFFFF)
+    dst[0, :4], dst[1, :4] = c.free[:4], c.free[4:8]
+    dd = i32(dst)
+    torch.cuda.synchronize()
+
+    def step():
+        ctx.paged_append(acfg, c.desc, qkv, 2, None, None, seq, pos, None, c.dtable, 2, q)
+        ctx.paged_attn_prompt(cfg, c.desc, pq, 2, cu, 2 * m, m, c.dtable, ln, 121, pout)
+        ctx.paged_attn_decode(cfg, c.desc, q, 2, c.dtable, ln, 121, out, mass, 128)
+        ctx.kv_evict(c.desc, 2, c.dtable, ln, 121, mass, 128, 50, 10, dd, ln2, mass2, 50, kept)
+
+    def fill(seed):
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        for t in (qkv, pq):
+            t.copy_(torch.randn(t.shape, generator=g, device="cuda"))
+        mass.zero_()
+        torch.cuda.synchronize()
+
+    fill(1)
+    step()  # the arena grows here
+    ctx.sync()
+    ctx.capture_begin()
+    step()
+    graph = ctx.capture_end()
+    for seed in (2, 3):
+        fill(seed)
+        step()
+        ctx.sync()
+        want = [t.clone() for t in (out, pout, mass, mass2, kept, ln2, c.dk, c.dv)]
+        for t in (out, pout, mass2, kept, ln2):
+            t.zero_()
+        fill(seed)
+        graph.launch()
+        ctx.sync()
+        got = (out, pout, mass, mass2, kept, ln2, c.dk, c.dv)
+        assert all(torch.equal(a.nan_to_num(), b.nan_to_num()) for a, b in zip(got, want))
+        assert ln2.tolist() == [50, 50] and float(mass.sum()) == pytest.approx(2 * heads, rel=1e-5)
+    graph.free()
+
+
 def test_prompt_few_tokens_long_cache(pkg, ctx):
     """A handful of queries per sequence over long caches, as in checking drafted tokens."""
     for f16 in (True, False):
