@@ -619,7 +619,7 @@ __global__ void __launch_bounds__(kGThreadsV2, 1) k_moe_gemm(const __grid_consta
                 tmem_ld32(lane_addr + c0, vh);
                 tmem_ld32(lane_addr + c0 + NP, vl);
             }
-            tmem_wait_ld();
+            tmem_wait_ld(vh, vl);
         };
         // superblock accumulator n (global count) of superblock sb; stacked
         // planes pass their own factor fs = 2^E

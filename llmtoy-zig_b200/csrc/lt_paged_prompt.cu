@@ -85,19 +85,16 @@ LT_DEVINL void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
         "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
         : "memory");
 }
-// Wait for this thread's TMEM loads; naming the loaded registers keeps their uses behind the wait.
-template <int N>
-LT_DEVINL void tmem_wait_ld(uint32_t (&v)[N]) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-    for (int i = 0; i < N; i++) asm volatile("" : "+r"(v[i]));
-}
 LT_DEVINL void tmem_st1(uint32_t taddr, float v) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(taddr), "r"(__float_as_uint(v)) : "memory");
 }
+// One column, there when the call returns.
 LT_DEVINL float tmem_ld1(uint32_t taddr) {
     uint32_t v;
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(v) : "r"(taddr));
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];\n tcgen05.wait::ld.sync.aligned;"
+                 : "=r"(v)
+                 : "r"(taddr)
+                 : "memory");
     return __uint_as_float(v);
 }
 LT_DEVINL void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -615,7 +612,6 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(PagedAttnArgs a,
             named_sync<2, 256>();
             tc_fence_after();
             const float r0 = tmem_ld1(tmem + lane_base + S::X_COL), r1 = tmem_ld1(tmem + lane_base + S::X_COL + 1);
-            tmem_wait_ld();
             rf = lane < 16 ? r0 : r1;
             tc_fence_before();
             named_sync<2, 256>();
@@ -750,7 +746,6 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(PagedAttnArgs a,
                 named_sync<2, 256>();
                 tc_fence_after();
                 const float other = tmem_ld1(x_addr + (wg ^ 1));
-                tmem_wait_ld();
                 top = fmaxf(top, other);
             }
             const float mn = fmaxf(m, top);
@@ -823,7 +818,6 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(PagedAttnArgs a,
             named_sync<2, 256>();
             tc_fence_after();
             l += tmem_ld1(x_addr + (wg ^ 1));
-            tmem_wait_ld();
         }
         // rows to the output through shared memory (this row tile's query planes are
         // no longer read), 32 columns at a time, so that stores fill whole lines

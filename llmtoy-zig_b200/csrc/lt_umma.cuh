@@ -76,6 +76,19 @@ LT_DEVINL void tmem_ld32(uint32_t taddr, uint32_t (&v)[32]) {
           "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
         : "r"(taddr));
 }
-LT_DEVINL void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// Wait for this thread's TMEM loads.  A load's registers are undefined until then, and only naming them
+// here keeps their uses behind the wait, so there is no form that names none.
+template <int N>
+LT_DEVINL void tmem_wait_ld(uint32_t (&v)[N]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < N; i++) asm volatile("" : "+r"(v[i]));
+}
+template <int N>
+LT_DEVINL void tmem_wait_ld(uint32_t (&v)[N], uint32_t (&w)[N]) {
+    tmem_wait_ld(v);
+#pragma unroll
+    for (int i = 0; i < N; i++) asm volatile("" : "+r"(w[i]));
+}
 
 }  // namespace lt
