@@ -243,7 +243,11 @@ lt_status lt_profile_reset(lt_ctx *ctx);
  * Records the device ops issued between begin and end on the context stream
  * into a graph that lt_graph_launch replays (one launch per decode token
  * instead of one per kernel).  The stream must not be the legacy default
- * stream; call lt_reserve first so no op allocates while capturing. */
+ * stream; call lt_reserve, or each op once at its largest sizes, first so no op
+ * allocates while capturing.  An op that needs a larger arena later gets a new
+ * one: what graphs were recorded with stays allocated until lt_free, and they
+ * may be launched as before.  The same holds where the owner of the stream
+ * records it. */
 typedef struct lt_graph lt_graph;
 lt_status lt_capture_begin(lt_ctx *ctx);
 lt_status lt_capture_end(lt_ctx *ctx, lt_graph **out);

@@ -46,6 +46,10 @@ struct lt_ctx {
     uint8_t *pinned = nullptr;       // pinned staging for the host-buffer entry points
     size_t pinned_bytes = 0;
     bool capturing = false;          // between lt_capture_begin and lt_capture_end
+    // Whether a graph may hold the address of the arena, the counters, the constants; such a buffer is
+    // replaced by a larger one without being freed, and lt_free frees it.
+    bool scratch_recorded = false, counters_recorded = false, consts_recorded = false;
+    std::vector<void *> kept;
     cudaStream_t cap_user = nullptr; // the caller's stream while a capture runs on `own`
     cudaEvent_t cap_ev = nullptr;    // joins `own` to the caller's stream for such a capture
     lt::Profiler prof;
@@ -105,11 +109,24 @@ lt::LaunchCfg cfg_of(lt_ctx *ctx) {
     return c;
 }
 
+// Whether ops are recorded into a graph now: by lt_capture_begin, or by the owner of the stream.
+bool recording(const lt_ctx *ctx) {
+    if (ctx->capturing) return true;
+    if (ctx->stream == nullptr || ctx->stream == cudaStreamLegacy) return false;  // cannot be captured
+    cudaStreamCaptureStatus s = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(ctx->stream, &s) != cudaSuccess) {
+        cudaGetLastError();
+        return false;
+    }
+    return s != cudaStreamCaptureStatusNone;
+}
+
 lt_status enter(lt_ctx *ctx) {
     if (!ctx) return LT_EINVAL;
     ctx->err.clear();
     cudaError_t e = cudaSetDevice(ctx->device);
     if (e != cudaSuccess) return cuda_fail(ctx, e, "cudaSetDevice");
+    if (recording(ctx)) ctx->scratch_recorded = ctx->counters_recorded = ctx->consts_recorded = true;
     return LT_OK;
 }
 
@@ -120,16 +137,31 @@ lt_status enter_uncaptured(lt_ctx *ctx, const char *what) {
     return st;
 }
 
+// A buffer that makes way for a larger one (nothing in flight uses it): freed, unless a graph that may be
+// launched again was recorded with it.
+void retire(lt_ctx *ctx, void *p, bool recorded) {
+    if (!p) return;
+    if (!recorded) {
+        cudaFree(p);
+        return;
+    }
+    try {
+        ctx->kept.push_back(p);
+    } catch (...) {  // no memory for the list: the buffer stays until the process ends
+    }
+}
+
 // Grow the scratch arena; waits for the stream first so nothing in flight
 // still uses the old buffer.
 lt_status ensure_scratch(lt_ctx *ctx, size_t bytes) {
     if (bytes <= ctx->scratch_bytes) return LT_OK;
-    if (ctx->capturing)
+    if (recording(ctx))
         return fail(ctx, LT_EINVAL, "op needs %zu scratch bytes while capturing: call lt_reserve first", bytes);
     LT_CUDA(ctx, cudaStreamSynchronize(ctx->stream), "cudaStreamSynchronize");
-    if (ctx->scratch) cudaFree(ctx->scratch);
+    retire(ctx, ctx->scratch, ctx->scratch_recorded);
     ctx->scratch = nullptr;
     ctx->scratch_bytes = 0;
+    ctx->scratch_recorded = false;
     bytes = (bytes + (1u << 20) - 1) & ~((size_t)(1u << 20) - 1);
     LT_CUDA(ctx, cudaMalloc(&ctx->scratch, bytes), "cudaMalloc(scratch)");
     ctx->scratch_bytes = bytes;
@@ -138,11 +170,12 @@ lt_status ensure_scratch(lt_ctx *ctx, size_t bytes) {
 
 lt_status ensure_counters(lt_ctx *ctx, size_t n) {
     if (n <= ctx->n_counters) return LT_OK;
-    if (ctx->capturing) return fail(ctx, LT_EINVAL, "op needs more counters while capturing: call lt_reserve first");
+    if (recording(ctx)) return fail(ctx, LT_EINVAL, "op needs more counters while capturing: call lt_reserve first");
     LT_CUDA(ctx, cudaStreamSynchronize(ctx->stream), "cudaStreamSynchronize");
-    if (ctx->counters) cudaFree(ctx->counters);
+    retire(ctx, ctx->counters, ctx->counters_recorded);
     ctx->counters = nullptr;
     ctx->n_counters = 0;
+    ctx->counters_recorded = false;
     n = (n + 4095) & ~(size_t)4095;
     LT_CUDA(ctx, cudaMalloc(&ctx->counters, n * 4), "cudaMalloc(counters)");
     LT_CUDA(ctx, cudaMemset(ctx->counters, 0, n * 4), "cudaMemset(counters)");
@@ -158,13 +191,14 @@ void clear_prefetch(lt_ctx *ctx) {
 // Constant slot weights (1) and expert ids (0) for n tokens.
 lt_status ensure_consts(lt_ctx *ctx, size_t n) {
     if (n <= ctx->n_const) return LT_OK;
-    if (ctx->capturing) return fail(ctx, LT_EINVAL, "dense FFN for %zu tokens while capturing: run it once first", n);
+    if (recording(ctx)) return fail(ctx, LT_EINVAL, "dense FFN for %zu tokens while capturing: run it once first", n);
     LT_CUDA(ctx, cudaStreamSynchronize(ctx->stream), "cudaStreamSynchronize");
-    if (ctx->ones) cudaFree(ctx->ones);
-    if (ctx->zeros) cudaFree(ctx->zeros);
+    retire(ctx, ctx->ones, ctx->consts_recorded);
+    retire(ctx, ctx->zeros, ctx->consts_recorded);
     ctx->ones = nullptr;
     ctx->zeros = nullptr;
     ctx->n_const = 0;
+    ctx->consts_recorded = false;
     n = (n + 1023) & ~(size_t)1023;
     LT_CUDA(ctx, cudaMalloc(&ctx->ones, n * 4), "cudaMalloc(ones)");
     LT_CUDA(ctx, cudaMalloc(&ctx->zeros, n * 4), "cudaMalloc(zeros)");
@@ -357,6 +391,7 @@ void lt_free(lt_ctx *ctx) {
     }
     if (ctx->stream) cudaStreamSynchronize(ctx->stream);
     ctx->prof.destroy();
+    for (void *p : ctx->kept) cudaFree(p);
     if (ctx->scratch) cudaFree(ctx->scratch);
     if (ctx->counters) cudaFree(ctx->counters);
     if (ctx->dev_err) cudaFree(ctx->dev_err);
