@@ -191,7 +191,8 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(PagedAttnArgs a,
     uint32_t *skip = reinterpret_cast<uint32_t *>(smem + S::OFF_SKIP);  // bit set: some row may see the tile
     uint64_t *full = reinterpret_cast<uint64_t *>(smem + S::OFF_BARS), *empty = full + NS;
     uint64_t *s_full = empty + NS, *p_full = s_full + 2, *o_full = p_full + 2, *p_half = o_full + 2;
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(p_half + 2);
+    uint64_t *mma_end = p_half + 2;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(mma_end + 1);
     volatile uint32_t *dead = tmem_slot + 1;
     // warp-uniform values go through a shuffle where the compiler cannot see that
     // they are: the MMA operands then stay in uniform registers (65 instead of 90
@@ -240,6 +241,7 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(PagedAttnArgs a,
             mbar_init(o_full + i, 1);
             mbar_init(p_half + i, 128);
         }
+        mbar_init(mma_end, 1);
         *dead = 0;
         fence_barrier_init();
     }
@@ -252,13 +254,15 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(PagedAttnArgs a,
     tc_fence_after();
     const uint32_t tmem = uniform(*tmem_slot);
 
-    auto wait = [&](uint64_t *bar, uint32_t phase) {
-        if (*dead) return;
-        if (!mbar_wait_bounded(bar, phase, kWaitLimitNs)) {
-            *dead = 1;
-            atomicExch(a.err, DEV_ERR_TMA_TIMEOUT);
-        }
+    // A wait that runs out lets all others pass (*dead): no copy is issued after that, and the CTA ends
+    // when what is in flight has ended, or has had as long again.
+    auto wait_always = [&](uint64_t *bar, uint32_t phase) {
+        if (mbar_wait_bounded(bar, phase, kWaitLimitNs)) return true;
+        *dead = 1;
+        atomicExch(a.err, DEV_ERR_TMA_TIMEOUT);
+        return false;
     };
+    auto wait = [&](uint64_t *bar, uint32_t phase) { return !*dead && wait_always(bar, phase); };
     // the first tile at or after t that is worked on
     auto next_tile = [&](uint32_t t) {
         if (skipping)
@@ -321,6 +325,7 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(PagedAttnArgs a,
                 mbar_arrive(full + stage);
             };
             uint32_t jj = 0, st = 0, turn = 0;  // tile count; ring stage and how often it went round
+            uint32_t boxes_in = 0, boxes_phase = 0;  // bit per stage: last filled by TMA, and in which phase
             uint32_t t = next_tile(begin);
             bool owed = false;                // the stage before st is copied but not handed on
             // tiles of whole boxes: every slot holds a cached position
@@ -361,8 +366,10 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(PagedAttnArgs a,
                         landed(st ? st - 1 : NS - 1);
                         owed = false;
                     }
-                    wait(empty + st, (turn & 1) ^ 1);
-                    __syncwarp();
+                    if (!__all_sync(0xffffffffu, wait(empty + st, (turn & 1) ^ 1))) continue;
+                    const uint32_t bit = 1u << st;
+                    boxes_in = by_box ? boxes_in | bit : boxes_in & ~bit;
+                    boxes_phase = turn & 1 ? boxes_phase | bit : boxes_phase & ~bit;
                     if (docs && kv == 0)
                         for (int r = pt; r < KT; r += kPpProducers) {
                             const uint32_t j = lo + t * KT + r;
@@ -409,6 +416,9 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(PagedAttnArgs a,
                 cp_async_wait<0>();
                 landed(st ? st - 1 : NS - 1);
             }
+            if (pw == 0)  // no copy of this CTA is under way when it ends
+                for (int i = 0; i < NS; i++)
+                    if ((boxes_in >> i & 1u) && !wait_always(full + i, boxes_phase >> i & 1u)) break;
         } else {
             // ── MMAs ──
             constexpr uint32_t IQK = umma_idesc_f16_f32(128, KT);
@@ -518,6 +528,10 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(PagedAttnArgs a,
                     t = tn;
                     jj++;
                 }
+                // no product either, nor its arrival
+                if (elect_one()) umma_commit(mma_end);
+                __syncwarp();
+                wait_always(mma_end, 0);
             }
         }
     } else {
@@ -855,7 +869,7 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(PagedAttnArgs a,
                         *reinterpret_cast<const float4 *>(st + rr * PITCH + lane % 8 * 4);
             }
         }
-        if (real && !fine) slow_row(a, s, kh, R, half * 128, OW);
+        if (real && !fine && !*dead) slow_row(a, s, kh, R, half * 128, OW);
         tc_fence_before();
     }
     __syncthreads();

@@ -32,3 +32,23 @@ def test_scalar_loads_carry_their_wait():
             found += 1
             assert "tcgen05.wait::ld" in m.group(0), name
     assert found
+
+
+def test_prompt_kernel_ends_after_its_copies_and_products():
+    """A CTA that gave up on a wait, too, stays until its TMA copies and tensor-core products have ended: they write to
+    its shared and tensor memory and arrive on its barriers.  A wait cannot be made to run out here without leaving
+    copies behind, so the order is read from the source."""
+    text = dict(sources())["lt_paged_prompt.cu"]
+    kernel = text[text.index("void __launch_bounds__(kPpThreads, 1) k_paged_prompt("):text.index("kPpJoinRows")]
+    end = kernel.rindex("tmem_dealloc(")
+    # the copies: none after a wait ran out, and a bounded wait for the last of every stage behind the loop
+    last = kernel.rindex("tma_load_4d(")
+    assert "if (!__all_sync(0xffffffffu, wait(empty + st, (turn & 1) ^ 1))) continue;" in kernel[:last]
+    assert re.search(r"for \(int i = 0; i < NS; i\+\+\)\s+if \(\(boxes_in >> i & 1u\) && !wait_always\(full \+ i,", kernel[last:end])
+    # the products: one commit behind all of them, and a bounded wait for it
+    last = max(kernel.rindex("umma_ts<"), kernel.rindex("qk(1,"), kernel.rindex("pv(tmem"))
+    drain = re.search(r"umma_commit\(mma_end\);\s+__syncwarp\(\);\s+wait_always\(mma_end, 0\);", kernel[last:end])
+    assert drain
+    # both regardless of *dead
+    always = kernel[kernel.index("auto wait_always"):kernel.index("auto wait =")]
+    assert "mbar_wait_bounded(" in always and "if (!*dead)" not in always
