@@ -137,7 +137,7 @@ class BatchDecoder:
             if q.allowed is not None:
                 mask = len(masks)
                 words = np.zeros((self.spec.vocab + 31) // 32, np.uint32)
-                a = np.asarray(q.allowed, np.int64)
+                a = np.asarray([t for t in q.allowed if t < self.spec.vocab], np.int64)
                 np.bitwise_or.at(words, a // 32, (np.uint32(1) << (a % 32).astype(np.uint32)))
                 masks.append(words)
             rules[r] = LogitRule(q.repetition, q.frequency, q.presence, len(history), len(self.tokens[r]), len(ids),
@@ -148,14 +148,29 @@ class BatchDecoder:
         return (self._dev(np.frombuffer(rules, np.uint32)), self._dev(history), self._dev(ids), self._dev(values, "float32"),
                 self._dev(np.concatenate(masks)) if masks else None)
 
+    def _checked(self, requests: list) -> list:
+        """The requests, or ValueError.  Prompt ids index the embedding on the device, which takes them as they are.
+        Ids past the vocabulary in bias and allowed name no token and are skipped."""
+        requests = [q if isinstance(q, Request) else Request(list(q)) for q in requests]
+        new = [len(q.prompt) for q in requests]
+        if not 0 < len(new) <= self.max_seqs or not 0 < min(new) <= max(new) < self.max_len:
+            raise ValueError("1 .. max_seqs prompts of 1 .. max_len - 1 tokens")
+        vocab = self.spec.vocab
+        for r, q in enumerate(requests):
+            bad = [t for t in q.prompt if not 0 <= t < vocab]
+            if bad:
+                raise ValueError(f"request {r}: prompt token {bad[0]} of a vocabulary of {vocab}")
+            if q.allowed is not None and (any(t < 0 for t in q.allowed) or not any(t < vocab for t in q.allowed)):
+                raise ValueError(f"request {r}: allowed tokens are negative or leave nothing of the vocabulary")
+        return requests
+
     def start(self, requests: list) -> list[int]:
         """Run the prompts; the first token of each sequence."""
         import torch
-        self.requests = [q if isinstance(q, Request) else Request(list(q)) for q in requests]
+        requests = self._checked(requests)
+        self.requests = requests
         self.n_seq, self.tokens = len(requests), [list(q.prompt) for q in self.requests]
         new = [len(t) for t in self.tokens]
-        if not 0 < self.n_seq <= self.max_seqs or not 0 < min(new) <= max(new) < self.max_len:
-            raise ValueError("1 .. max_seqs prompts of 1 .. max_len - 1 tokens")
         for m in self.mass:
             if m is not None:
                 m.zero_()
