@@ -14,6 +14,7 @@ the single-sequence decoder uses, on several rows.
 """
 from __future__ import annotations
 
+from contextlib import contextmanager
 from dataclasses import dataclass, field
 
 from . import AttnCfg, Context, LogitRule, NO_MASK, PagedAttnCfg, PagedKV
@@ -65,6 +66,7 @@ class BatchDecoder:
         self.pool = PagePool(self.n_pages)
         kind = torch.float16 if s.kv_f16 else torch.float32
         shape = (self.n_pages, page_size, s.n_kv_heads, s.head_dim)
+        torch.cuda.synchronize()
         self.emb = torch.empty(s.vocab, s.d_model, device="cuda")
         ctx.dequant(s.token_emb, 0, s.vocab, self.emb)
         self.cfg = AttnCfg(s.n_heads, s.n_kv_heads, s.head_dim, int(s.rope_neox), s.rope_theta, s.eps, s.head_dim ** -0.5, 1)
@@ -77,6 +79,18 @@ class BatchDecoder:
             self.caches.append((kv, k, v))
             self.mass.append(torch.zeros(max_seqs, s.n_kv_heads, max_len, device="cuda") if budget else None)
         torch.cuda.synchronize()
+
+    @contextmanager
+    def _between(self):
+        """What runs in here allocates with torch and launches on the context's stream only.  torch hands a block out
+        again in the order of its own stream, so all work, whosever, ends before and after; in between no torch kernel
+        runs, and blocks change hands in the order of the context's stream."""
+        import torch
+        torch.cuda.synchronize()
+        try:
+            yield
+        finally:
+            torch.cuda.synchronize()
 
     def _dev(self, values, dtype="uint32"):
         """A host list as a device array (torch tensor of its bits)."""
@@ -95,13 +109,15 @@ class BatchDecoder:
         nq, nkv = s.n_heads * s.head_dim, s.n_kv_heads * s.head_dim
         xn, qkv = torch.empty_like(x), torch.empty(ntok, nq + 2 * nkv, device="cuda")
         q, att = torch.empty(ntok, nq, device="cuda"), torch.empty(ntok, nq, device="cuda")
+        bias = zeros = None
         for i, L in enumerate(s.layers):
             ctx.rmsnorm(x, L.attn_norm, s.eps, s.d_model, ntok, xn)
             if L.qkv_bias is None:
                 ctx.qmatvec(L.wqkv, xn, qkv, ntok)
             else:
-                bias = L.qkv_bias.repeat(ntok, 1)
-                torch.cuda.synchronize()
+                if bias is None:
+                    bias, zeros = torch.empty_like(qkv), self._dev([0] * ntok)
+                ctx.gather_rows(L.qkv_bias, nq + 2 * nkv, zeros, ntok, bias)  # its one row for every token
                 ctx.qmatvec_add(L.wqkv, xn, bias, qkv, ntok)
             ctx.paged_append(self.cfg, self.caches[i][0], qkv, ntok, L.q_norm, L.k_norm, seq, pos, slot, self.table,
                              self.n_seq, q)
@@ -112,8 +128,6 @@ class BatchDecoder:
             else:
                 ctx.moe_block(L.router, L.exp_gate, L.exp_up, L.exp_down, s.act, s.norm_topk, None, L.ffn_norm, s.eps, x,
                               ntok, s.n_used, x)
-            if L.qkv_bias is not None:
-                ctx.sync()  # the repeated bias is freed
 
     def _choose(self, x, rows) -> list[int]:
         """The next token of every sequence from rows `rows` of x."""
@@ -166,7 +180,6 @@ class BatchDecoder:
 
     def start(self, requests: list) -> list[int]:
         """Run the prompts; the first token of each sequence."""
-        import torch
         requests = self._checked(requests)
         self.requests = requests
         self.n_seq, self.tokens = len(requests), [list(q.prompt) for q in self.requests]
@@ -176,49 +189,55 @@ class BatchDecoder:
                 m.zero_()
         self.pages = [self.pool.take(-(-n // self.page)) for n in new]
         self.lens, self.pos = list(new), list(new)  # cached positions; the next token's place in the text
+        with self._between():
+            return self._take(self._prompts(new))
+
+    def _prompts(self, new: list[int]) -> list[int]:
+        import torch
         self._tables()
         cu = [sum(new[:i]) for i in range(self.n_seq + 1)]
         seq = self._dev([r for r, n in enumerate(new) for _ in range(n)])
         pos = self._dev([j for n in new for j in range(n)])
         dcu, total, most = self._dev(cu), cu[-1], max(new)
         x = torch.empty(total, self.spec.d_model, device="cuda")
-        torch.cuda.synchronize()
         self.ctx.gather_rows(self.emb, self.spec.d_model, self._dev([t for s in self.tokens for t in s]), total, x)
         self._layers(x, total, seq, pos, None, lambda i, q, out: self.ctx.paged_attn_prompt(
             self.attn, self.caches[i][0], q, self.n_seq, dcu, total, most, self.table, self.dlens, most, out))
-        return self._take(self._choose(x, [c - 1 for c in cu[1:]]))
+        return self._choose(x, [c - 1 for c in cu[1:]])
 
     def step(self) -> list[int]:
         """One more token of every sequence."""
-        import torch
-        n = self.n_seq
-        for r in range(n):
+        for r in range(self.n_seq):
             if self.lens[r] >= self.max_len:
                 raise ValueError(f"sequence {r} is at max_len")
             if self.lens[r] % self.page == 0 and self.lens[r] // self.page == len(self.pages[r]):
                 self.pages[r] += self.pool.take(1)
+        with self._between():
+            ids = self._next()
+            if self.budget and max(self.lens) > self.budget:
+                self._evict()
+        return self._take(ids)
+
+    def _next(self) -> list[int]:
+        import torch
+        n = self.n_seq
         seq, pos, slot = self._dev(range(n)), self._dev(self.pos), self._dev(self.lens)
         self.lens = [v + 1 for v in self.lens]
         self.pos = [v + 1 for v in self.pos]
         self._tables()
         x = torch.empty(n, self.spec.d_model, device="cuda")
-        torch.cuda.synchronize()
         self.ctx.gather_rows(self.emb, self.spec.d_model, self._dev([t[-1] for t in self.tokens]), n, x)
         self._layers(x, n, seq, pos, slot, lambda i, q, out: self.ctx.paged_attn_decode(
             self.attn, self.caches[i][0], q, n, self.table, self.dlens, max(self.lens), out, self.mass[i], self.max_len))
-        ids = self._choose(x, range(n))
-        if self.budget and max(self.lens) > self.budget:
-            self._evict()
-        return self._take(ids)
+        return self._choose(x, range(n))
 
     def _evict(self) -> None:
         import torch
         out = torch.empty(self.n_seq, dtype=torch.int32, device="cuda")
-        torch.cuda.synchronize()
         for (kv, _, _), m in zip(self.caches, self.mass):
             self.ctx.kv_evict(kv, self.n_seq, self.table, self.dlens, max(self.lens), m, self.max_len, self.budget, self.recent,
                               None, out, m, self.max_len)
-        self.ctx.sync()
+        self.ctx.sync()  # nothing is under way on the context's stream while torch clears these
         for m in self.mass:  # slots that the coming tokens take start from nothing
             m[:, :, self.budget:] = 0
         torch.cuda.synchronize()
