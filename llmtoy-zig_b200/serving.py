@@ -64,6 +64,7 @@ class BatchDecoder:
         self.width = -(-max_len // page_size)
         self.n_pages = n_pages or max_seqs * self.width
         self.pool = PagePool(self.n_pages)
+        self.pages = []  # of each sequence
         kind = torch.float16 if s.kv_f16 else torch.float32
         shape = (self.n_pages, page_size, s.n_kv_heads, s.head_dim)
         torch.cuda.synchronize()
@@ -179,15 +180,21 @@ class BatchDecoder:
         return requests
 
     def start(self, requests: list) -> list[int]:
-        """Run the prompts; the first token of each sequence."""
+        """Run the prompts; the first token of each sequence.  The batch before gives its pages back; a batch that is
+        refused (ValueError, MemoryError) leaves it as it was."""
         requests = self._checked(requests)
+        new = [len(q.prompt) for q in requests]
+        need = [-(-n // self.page) for n in new]
+        there = len(self.pool.free) + sum(len(p) for p in self.pages)
+        if sum(need) > there:
+            raise MemoryError(f"{sum(need)} cache pages wanted, {there} free")
+        self.close()
         self.requests = requests
         self.n_seq, self.tokens = len(requests), [list(q.prompt) for q in self.requests]
-        new = [len(t) for t in self.tokens]
         for m in self.mass:
             if m is not None:
                 m.zero_()
-        self.pages = [self.pool.take(-(-n // self.page)) for n in new]
+        self.pages = [self.pool.take(n) for n in need]
         self.lens, self.pos = list(new), list(new)  # cached positions; the next token's place in the text
         with self._between():
             return self._take(self._prompts(new))
@@ -258,16 +265,17 @@ class BatchDecoder:
 
     def close(self) -> None:
         """Give the batch's pages back."""
-        for pages in getattr(self, "pages", []):
+        for pages in self.pages:
             self.pool.give(pages)
         self.pages = []
 
     def generate(self, requests: list, n_gen: int) -> list[list[int]]:
         """n_gen new token ids per request."""
-        first = self.start(requests)
-        out = [[t] for t in first]
-        for _ in range(n_gen - 1):
-            for o, t in zip(out, self.step()):
-                o.append(t)
-        self.close()
+        try:
+            out = [[t] for t in self.start(requests)]
+            for _ in range(n_gen - 1):
+                for o, t in zip(out, self.step()):
+                    o.append(t)
+        finally:
+            self.close()
         return out
