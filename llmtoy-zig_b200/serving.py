@@ -214,6 +214,8 @@ class BatchDecoder:
 
     def step(self) -> list[int]:
         """One more token of every sequence."""
+        if not self.pages:
+            raise ValueError("no batch is running: start one first")
         for r in range(self.n_seq):
             if self.lens[r] >= self.max_len:
                 raise ValueError(f"sequence {r} is at max_len")

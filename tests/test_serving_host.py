@@ -112,3 +112,15 @@ def test_generate_gives_the_pages_back_when_it_fails(what):
         d.generate([[1] * 7, [1] * 7] if what == "pool" else [[1] * 14], 8)
     assert held(d) == 0
     assert len(d.generate([[1] * 7], 1)[0]) == 1 and held(d) == 0
+
+
+def test_step_without_a_batch_is_refused():
+    """Its page table would be empty."""
+    d = decoder()
+    with pytest.raises(ValueError):
+        d.step()
+    d.start([[1, 2]])
+    d.step()
+    d.close()
+    with pytest.raises(ValueError):
+        d.step()
