@@ -273,6 +273,8 @@ class BatchDecoder:
 
     def generate(self, requests: list, n_gen: int) -> list[list[int]]:
         """n_gen new token ids per request."""
+        if n_gen < 1:
+            raise ValueError("n_gen: at least one token")
         try:
             out = [[t] for t in self.start(requests)]
             for _ in range(n_gen - 1):

@@ -124,3 +124,12 @@ def test_step_without_a_batch_is_refused():
     d.close()
     with pytest.raises(ValueError):
         d.step()
+
+
+def test_number_of_generated_tokens():
+    d = decoder(max_len=32, n_pages=8)
+    for n in (1, 2, 7):
+        assert [len(t) for t in d.generate([[1], [2, 3]], n)] == [n, n]
+    for n in (0, -1):
+        with pytest.raises(ValueError):
+            d.generate([[1]], n)
