@@ -85,6 +85,7 @@ lt_status fail(lt_ctx *ctx, lt_status st, const char *fmt, ...) {
 }
 
 lt_status cuda_fail(lt_ctx *ctx, cudaError_t e, const char *what) {
+    cudaGetLastError();  // this call reports it; the next one, which reads the last error after a launch, must not
     if (e == cudaErrorMemoryAllocation)
         return fail(ctx, LT_ENOMEM, "%s: %s", what, cudaGetErrorString(e));
     return fail(ctx, LT_ECUDA, "%s: %s", what, cudaGetErrorString(e));

@@ -104,3 +104,25 @@ def test_graph_recorded_by_the_streams_owner(pkg):
         assert all(torch.equal(a, b) for a, b in zip(step.result(), want))
         del graph
         ctx.set_stream(None)
+
+
+def test_a_failed_allocation_fails_its_own_call_only(pkg):
+    """64 heads' scores at 2^30 positions are more than the device has; the next op is none the worse."""
+    rng = np.random.default_rng(9)
+    c = Cache(pkg, rng, [40], 2, 64, True, 16)
+    q, out, ln = torch.randn(1, 64 * 64, device="cuda"), torch.zeros(1, 64 * 64, device="cuda"), i32([40])
+    cfg, mass = pkg.PagedAttnCfg(n_heads=64, scale=0.125), torch.zeros(2 * 40, device="cuda")
+    torch.cuda.synchronize()
+    with pkg.Context(0) as ctx:
+        ctx.paged_attn_decode(cfg, c.desc, q, 1, c.dtable, ln, 40, out)
+        ctx.sync()
+        want = out.clone()
+        for _ in range(2):
+            with pytest.raises(pkg.LtError) as e:
+                ctx.paged_attn_decode(cfg, c.desc, q, 1, c.dtable, ln, 1 << 30, out, mass, 1 << 30)
+            assert e.value.status == 3  # LT_ENOMEM
+            out.zero_()
+            torch.cuda.synchronize()
+            ctx.paged_attn_decode(cfg, c.desc, q, 1, c.dtable, ln, 40, out)
+            ctx.sync()
+            assert torch.equal(out, want)
