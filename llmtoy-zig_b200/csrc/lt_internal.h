@@ -187,7 +187,7 @@ size_t paged_attn_scratch(const PagedAttnArgs &a, int num_sms);
 cudaError_t launch_paged_attn(const LaunchCfg &c, PagedAttnArgs a, uint8_t *scratch);
 // Prompts over f16 caches on the tensor cores (lt_paged_prompt.cu).
 bool paged_prompt_supported(const PagedAttnArgs &a);
-size_t paged_prompt_scratch(PagedAttnArgs a, int num_sms);
+size_t paged_prompt_scratch(const PagedAttnArgs &a, int num_sms);
 cudaError_t launch_paged_prompt(const LaunchCfg &c, PagedAttnArgs a, uint8_t *scratch);
 
 // Eviction from a paged cache (lt_evict.cu).

@@ -985,9 +985,15 @@ void pp_split(PagedAttnArgs &a, int num_sms) {
     a.kv.hd == 64 ? pp_split<64>(a, num_sms) : a.kv.hd == 128 ? pp_split<128>(a, num_sms) : pp_split<256>(a, num_sms);
 }
 
+uint32_t pp_rows(const PagedAttnArgs &a) { return a.kv.hd == 256 ? PpShape<256>::ROWS : PpShape<128>::ROWS; }
+static_assert(PpShape<64>::ROWS == PpShape<128>::ROWS, "one branch for both");
+
 uint64_t pp_records(const PagedAttnArgs &a) {  // rows of all records
-    return (uint64_t)a.n_seq * a.kv.n_kv * a.row_blocks * a.nsplit * (a.kv.hd == 256 ? 128 : 256);
+    return (uint64_t)a.n_seq * a.kv.n_kv * a.row_blocks * a.nsplit * pp_rows(a);
 }
+
+// Fewest rows for this kernel (see paged_prompt_supported).
+constexpr uint32_t kPpMinRows = 16, kPpMinRowsShort = 32;
 
 template <int HD, bool EXTRA>
 cudaError_t pp_launch(const LaunchCfg &c, const PagedAttnArgs &a) {
@@ -1023,12 +1029,17 @@ bool paged_prompt_supported(const PagedAttnArgs &a) {
     // about alike (60 and 70 us at most), 28 rows of 60 tokens 7.9 and 10.0 us, 32 rows of 8000
     // tokens 100 and 72 us, 56 rows of 60 tokens 16 and 10 us.
     const uint64_t rows = (uint64_t)a.max_q * a.group;
-    return regs && a.kv.f16 && rows > (a.max_len > 256 ? 16 : 32);
+    return regs && a.kv.f16 && rows > (a.max_len > 256 ? kPpMinRows : kPpMinRowsShort);
 }
 
-size_t paged_prompt_scratch(PagedAttnArgs a, int num_sms) {
-    pp_split(a, num_sms);
-    return a.nsplit == 1 ? 0 : pp_records(a) * (a.kv.hd + 2) * 4;
+// Enough for this call and for every smaller one, so that an op run once at its largest sizes has its scratch when a
+// smaller call is recorded.  Only smaller calls may share their keys, and there are records only where a launch has no
+// more CTAs than SMs; the fewest rows take the other kernel with its own scratch.
+size_t paged_prompt_scratch(const PagedAttnArgs &a, int num_sms) {
+    const size_t records = (size_t)num_sms * pp_rows(a) * (a.kv.hd + 2) * 4;
+    PagedAttnArgs few = a;
+    few.max_q = min(a.max_q, kPpMinRowsShort / a.group);
+    return few.max_q ? max(records, paged_attn_scratch(few, num_sms)) : records;
 }
 
 cudaError_t launch_paged_prompt(const LaunchCfg &c, PagedAttnArgs a, uint8_t *scratch) {

@@ -126,3 +126,57 @@ def test_a_failed_allocation_fails_its_own_call_only(pkg):
             ctx.paged_attn_decode(cfg, c.desc, q, 1, c.dtable, ln, 40, out)
             ctx.sync()
             assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("heads,kv,hd", [(14, 2, 64), (32, 4, 128), (16, 8, 256)])
+@pytest.mark.parametrize("f16", [True, False])
+def test_smaller_calls_need_no_more_scratch(pkg, heads, kv, hd, f16):
+    """Each op run once with its largest sizes, then recorded with smaller ones: fewer rows are shared among more CTAs,
+    the fewest go to another kernel, and the arena has to hold what either needs."""
+    rng = np.random.default_rng(1)
+    n, most = 600, 8192
+    c = Cache(pkg, rng, [n] * 3, kv, hd, f16, 16, spare=most // 16)
+    cfg = pkg.PagedAttnCfg(n_heads=heads, causal=1, scale=1 / math.sqrt(hd))
+    q, out = torch.randn(2048, heads * hd, device="cuda"), torch.zeros(2048, heads * hd, device="cuda")
+    mass, ln = torch.zeros(3 * kv * most, device="cuda"), i32([n] * 3)
+    kept, lens_out = torch.zeros(3 * kv * 512, dtype=torch.int32, device="cuda"), i32([0] * 3)
+    cus = {(s, m): i32(np.arange(s + 1) * m) for s in (1, 2, 3) for m in (600, 300, 64, 9, 3, 1)}
+    small = torch.zeros(3 * kv * 512, device="cuda")
+    torch.cuda.synchronize()
+
+    def prompt(ctx, s, m, max_q, max_len):
+        ctx.paged_attn_prompt(cfg, c.desc, q, s, cus[s, m], s * m, max_q, c.dtable, ln, max_len, out)
+
+    with pkg.Context(0) as ctx:
+        prompt(ctx, 3, 600, most, most)
+        ctx.sync()
+        want = []
+        calls = [(s, m, k, l) for s in (3, 1) for m in (600, 300, 64, 9, 3, 1) for k in {m, most} for l in (n, 1024, most)]
+        for a in calls:
+            ctx.capture_begin()
+            prompt(ctx, *a)
+            graph = ctx.capture_end()
+            out.zero_()
+            torch.cuda.synchronize()
+            graph.launch()
+            ctx.sync()
+            want.append(out.clone())
+            graph.free()
+    with pkg.Context(0) as ctx:  # and they compute what they do without a graph
+        for a, w in zip(calls, want):
+            out.zero_()
+            torch.cuda.synchronize()
+            prompt(ctx, *a)
+            ctx.sync()
+            assert torch.equal(out, w), a
+    with pkg.Context(0) as ctx:
+        ctx.paged_attn_decode(cfg, c.desc, q, 3, c.dtable, ln, most, out, mass, most)
+        ctx.kv_evict(c.desc, 3, c.dtable, ln, most, mass, most, 512, 8, None, lens_out, small, 512)
+        ctx.sync()
+        ctx.capture_begin()
+        for s, l in ((3, n), (1, most), (2, 1000)):
+            ctx.paged_attn_decode(cfg, c.desc, q, s, c.dtable, ln, l, out, mass, most)
+            ctx.paged_attn_decode(cfg, c.desc, q, s, c.dtable, ln, l, out)
+            ctx.kv_evict(c.desc, s, c.dtable, ln, l, mass, most, 512, 8, None, lens_out, small, 512)
+            ctx.kv_evict(c.desc, s, c.dtable, ln, l, mass, most, 64, 8, None, lens_out, small, 64, kept)
+        ctx.capture_end().free()
