@@ -417,9 +417,8 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<HD, F16>::CTAS) k_paged_at
         const uint32_t *docs = nullptr;
         if (PROMPT) {
             if (a.causal) {
-                row_hi = row_i + 1;
-                if (a.prefix) row_hi = (int)max((int64_t)row_hi, (int64_t)a.prefix[cw.s]);
-                row_hi = min(row_hi, (int)cw.q.len);
+                row_hi = min(row_i + 1, (int)cw.q.len);
+                if (a.prefix) row_hi = max(row_hi, (int)min(a.prefix[cw.s], cw.q.len));  // any prefix up to 2^32 - 1
             }
             row_lo = a.window ? (int)max((int64_t)0, (int64_t)row_i - a.window + 1) : 0;
             if (a.docs) {
