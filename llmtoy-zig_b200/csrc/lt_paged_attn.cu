@@ -410,8 +410,9 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<HD, F16>::CTAS) k_paged_at
         const float rf = rowf[g];
         const uint32_t head = cw.kh * a.group + R % a.group;
         const float slope = a.slopes && (uint32_t)g < rows ? a.slopes[head] : 0.0f;
-        // positions are 32 bits wide here: a length is at most 2^30, and a query before position 0 below -2^31 is clamped
-        const int row_i = (int)max((int64_t)cw.q.len - cw.q.nq + R / a.group, (int64_t)-0x7fffffff);
+        // positions are 32 bits wide here, and so are their differences: a length is at most 2^30, and a query that
+        // far before position 0 is clamped
+        const int row_i = (int)max((int64_t)cw.q.len - cw.q.nq + R / a.group, -((int64_t)1 << 30));
         int row_lo = cw.q.lo, row_hi = cw.q.len;
         uint32_t my_doc = 0;
         const uint32_t *docs = nullptr;
@@ -506,10 +507,12 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<HD, F16>::CTAS) k_paged_at
                 }
                 float top = -INFINITY;
                 const bool whole = !PROMPT && k0 >= cw.lo && k0 + KB <= cw.hi;
+                // distance to this thread's first key; the positions alone may need more than a float's 24 bits
+                const float dist = (float)(row_i - (int)(k0 + 2 * j4));
 #pragma unroll
                 for (int n = 0; n < NS; n++) {
                     const int j = (int)k0 + 8 * (n / 2) + 2 * j4 + (n & 1);
-                    sc[n] = PLAIN ? sc[n] * rf : score_log2(sc[n], rf, a.softcap, slope, fabsf((float)row_i - (float)j));
+                    sc[n] = PLAIN ? sc[n] * rf : score_log2(sc[n], rf, a.softcap, slope, fabsf(dist - (float)(8 * (n / 2) + (n & 1))));
                     if (PROMPT) {
                         bool seen = j >= row_lo && j < row_hi;
                         if (docs && seen) seen = docs[j] == my_doc;

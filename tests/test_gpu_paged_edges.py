@@ -28,3 +28,41 @@ def test_prefix_past_31_bits(pkg, ctx, f16, new, window):
     """A prefix longer than any sequence: everything cached is seen in both directions."""
     for prefix in ([0xFFFFFFFF, 1 << 31], [(1 << 31) - 1, (1 << 31) + 50]):
         check_prompt(pkg, ctx, 8, 2, 64, f16, 16, new, [100, 90], prefix=prefix, window=window, seed=1)
+
+
+@pytest.mark.parametrize("f16", [True, False])
+@pytest.mark.parametrize("m", [0, 1, 5, 40])
+def test_distances_past_24_bits(pkg, ctx, f16, m):
+    """The distance bias of a window near position 2^25 (m = 0: decode, else m rows of a prompt): differences of
+    positions are exact, whatever the positions."""
+    rng = np.random.default_rng(2)
+    heads, kv, hd, page, window = 8, 2, 64, 1 << 12, 24
+    n = (1 << 25) + 5
+    width = -(-n // page)
+    near = window + max(m, 1)  # positions that any query sees, and one
+    K, V = (rng.normal(0, 1, (near, kv, hd)).astype(np.float16) for _ in range(2))
+    pools = [torch.zeros(2, page, kv, hd, dtype=torch.float16 if f16 else torch.float32, device="cuda") for _ in range(2)]
+    table = np.full((1, width), 0xFFFFFFFF, np.int64)  # the pages before the window are gone
+    table[0, -2:] = [1, 0]
+    j = np.arange(n - near, n)
+    for pool, x in zip(pools, (K, V)):
+        pool[table[0, j // page], j % page] = torch.from_numpy(x).cuda().to(pool.dtype)
+    desc = pkg.PagedKV(n_kv_heads=kv, head_dim=hd, kv_f16=int(f16), page_size=page, n_pages=2, max_pages=width,
+                       k=pools[0].data_ptr(), v=pools[1].data_ptr())
+    slopes = (2.0 ** -np.arange(heads)).astype(np.float32)
+    sl = dev(slopes)
+    cfg = pkg.PagedAttnCfg(n_heads=heads, window=window, causal=1, scale=1 / math.sqrt(hd), slopes=sl.data_ptr())
+    rows = max(m, 1)
+    q = rng.normal(0, 1.5, (rows, heads, hd)).astype(np.float32)
+    qd, out, dt, ln = dev(q), torch.zeros(rows, heads * hd, device="cuda"), i32(table), i32([n])
+    cu = i32([0, rows])
+    torch.cuda.synchronize()
+    if m == 0:
+        ctx.paged_attn_decode(cfg, desc, qd, 1, dt, ln, n, out)
+    else:
+        ctx.paged_attn_prompt(cfg, desc, qd, 1, cu, m, m, dt, ln, n, out)
+    ctx.sync()
+    i = np.arange(n - rows, n)
+    seen = (j[None] <= i[:, None]) & (i[:, None] - j[None] < window)
+    want, _ = attend(q, K.astype(np.float64), V.astype(np.float64), i - (n - near), seen, 1 / math.sqrt(hd), slopes=slopes)
+    assert rel(out.cpu().numpy().reshape(want.shape), want) < ATTN_BAR
