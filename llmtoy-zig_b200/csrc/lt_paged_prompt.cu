@@ -631,7 +631,9 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(PagedAttnArgs a,
             named_sync<2, 256>();
             tc_fence_after();
         }
-        rf = fabsf(rf);
+        // never 0, by which a masked score's -inf would become NaN: products are below 1e10, so the least
+        // normal number makes nothing of them either
+        rf = fmaxf(fabsf(rf), 1.17549435e-38f);
         if (skipping) named_sync<3, kPpThreads>();
         mbar_arrive(p_full + tile);
 

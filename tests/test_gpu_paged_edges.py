@@ -66,3 +66,68 @@ def test_distances_past_24_bits(pkg, ctx, f16, m):
     seen = (j[None] <= i[:, None]) & (i[:, None] - j[None] < window)
     want, _ = attend(q, K.astype(np.float64), V.astype(np.float64), i - (n - near), seen, 1 / math.sqrt(hd), slopes=slopes)
     assert rel(out.cpu().numpy().reshape(want.shape), want) < ATTN_BAR
+
+
+# ── scores ───────────────────────────────────────────────────────────────────
+
+def run_scaled(pkg, ctx, heads, kv, hd, f16, n, m, scale, q, cap=0.0, seed=0, layout_page=16):
+    """Decode (m = 0) or a causal prompt of m rows over n positions; got, want."""
+    rng = np.random.default_rng(seed)
+    c = Cache(pkg, rng, [n], kv, hd, f16, layout_page)
+    rows = max(m, 1)
+    q = np.asarray(q(rng, (rows, heads, hd)), np.float32)
+    cfg = pkg.PagedAttnCfg(n_heads=heads, causal=1, scale=scale, softcap=cap)
+    qd, out, ln, cu = dev(q), torch.zeros(rows, heads * hd, device="cuda"), i32([n]), i32([0, rows])
+    torch.cuda.synchronize()
+    if m == 0:
+        ctx.paged_attn_decode(cfg, c.desc, qd, 1, c.dtable, ln, n, out)
+    else:
+        ctx.paged_attn_prompt(cfg, c.desc, qd, 1, cu, m, m, c.dtable, ln, n, out)
+    ctx.sync()
+    K, V = c.seq(0)
+    i = np.arange(n - rows, n)
+    # the scale as the call takes it, in 32 bits
+    want, _ = attend(q, K, V, i, np.arange(n)[None] <= i[:, None], float(np.float32(scale)), cap)
+    return out.cpu().numpy().reshape(want.shape), want
+
+
+SHAPES = [(14, 2, 64), (32, 4, 128), (16, 8, 256)]
+
+
+@pytest.mark.parametrize("heads,kv,hd", SHAPES)
+@pytest.mark.parametrize("f16", [True, False])
+@pytest.mark.parametrize("m", [0, 2, 150])
+@pytest.mark.parametrize("scale,size,cap", [(0.0, 1.5, 0.0), (-0.125, 1.5, 0.0), (-0.125, 1.5, 2.0), (0.0, 1.5, 2.0),
+                                            (1e-30, 1e-20, 0.0), (1e-38, 1e-38, 0.0), (1e20, 1e-20, 0.0)])
+def test_scales(pkg, ctx, heads, kv, hd, f16, m, scale, size, cap):
+    got, want = run_scaled(pkg, ctx, heads, kv, hd, f16, 200, m, scale, lambda r, sh: r.normal(0, size, sh), cap, seed=hd)
+    assert np.isfinite(got).all()
+    assert rel(got, want) < ATTN_BAR
+
+
+def prompt_ms(pkg, ctx, hd, scale, size):
+    """Shortest of three causal prompts of 1024 tokens over an f16 cache, in ms."""
+    heads, kv, n = 8, 2, 1024
+    c = Cache(pkg, np.random.default_rng(3), [n], kv, hd, True, 128)
+    cfg = pkg.PagedAttnCfg(n_heads=heads, causal=1, scale=scale)
+    q, out = torch.randn(n, heads * hd, device="cuda") * size, torch.zeros(n, heads * hd, device="cuda")
+    ln, cu = i32([n]), i32([0, n])
+    torch.cuda.synchronize()
+    ctx.profile(True)
+    best = []
+    for _ in range(3):
+        ctx.profile_reset()
+        ctx.paged_attn_prompt(cfg, c.desc, q, 1, cu, n, n, c.dtable, ln, n, out)
+        ctx.sync()
+        best.append(sum(r["total_ms"] for r in ctx.profile_read().values()))
+    ctx.profile(False)
+    ctx.profile_reset()
+    return min(best)
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_scores_of_zero_take_no_longer(pkg, ctx, hd):
+    """Rows without finite results are done again one by one, hundreds of times slower; scores of zero are finite."""
+    usual = prompt_ms(pkg, ctx, hd, 0.125, 1.0)
+    for scale, size in ((0.0, 1.0), (1e-38, 1e-38), (0.125, 0.0)):
+        assert prompt_ms(pkg, ctx, hd, scale, size) < 5 * usual
