@@ -837,7 +837,7 @@ LT_DEVINL void pa_mass(const PagedAttnArgs &a, uint32_t s, uint32_t kh, uint32_t
         if (t == 0 && h < a.group) {
             // the sums carry the weights' factor 2^10 on f16 caches
             s_ml[h] = m == -INFINITY ? 0.0f : m - (a.kv.f16 ? 10.0f : 0.0f);
-            s_ml[a.group + h] = l > 0.0f ? 1.0f / l : 0.0f;
+            s_ml[a.group + h] = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);  // NaN stays, as in the output
         }
     }
     __syncthreads();

@@ -131,3 +131,26 @@ def test_scores_of_zero_take_no_longer(pkg, ctx, hd):
     usual = prompt_ms(pkg, ctx, hd, 0.125, 1.0)
     for scale, size in ((0.0, 1.0), (1e-38, 1e-38), (0.125, 0.0)):
         assert prompt_ms(pkg, ctx, hd, scale, size) < 5 * usual
+
+
+def test_weights_of_a_row_that_is_not_finite(pkg, ctx):
+    """A score that overflows makes the row's output NaN, and NaN is what it adds to every position that it sees."""
+    heads, kv, hd, n = 4, 2, 64, 90
+    rng = np.random.default_rng(5)
+    c = Cache(pkg, rng, [n, n], kv, hd, False, 16)
+    c.hk[c.table[0, 1], 4, 0, 7] = 1e30  # position 20 of the first sequence, KV head 0
+    c.upload(pkg)
+    q = rng.normal(0, 1, (2, heads, hd)).astype(np.float32)
+    q[0, 1, 7] = 1e30
+    cfg = pkg.PagedAttnCfg(n_heads=heads, window=80, scale=0.125)
+    qd, out, ln = dev(q), torch.zeros(2, heads * hd, device="cuda"), i32([n, n])
+    mass = torch.zeros(2, kv, n, device="cuda")
+    torch.cuda.synchronize()
+    ctx.paged_attn_decode(cfg, c.desc, qd, 2, c.dtable, ln, n, out, mass, n)
+    ctx.sync()
+    got, m = out.cpu().numpy().reshape(2, heads, hd), mass.cpu().numpy()
+    assert np.isnan(got[0, 1]).any()
+    assert np.isnan(m[0, 0, n - 80:]).all() and not m[0, 0, :n - 80].any()
+    for s, h in ((0, 1), (1, 0), (1, 1)):  # the others are as they would be
+        assert np.isfinite(got[s, 2 * h:2 * h + 2]).all()
+        assert m[s, h].sum() == pytest.approx(2.0, rel=1e-5)
