@@ -93,7 +93,7 @@ __global__ void __launch_bounds__(kSelThreads) k_evict_select(EvictArgs a) {
     const uint32_t keep = min(n, a.budget);
     const float *mass = a.mass + pair * a.mass_stride;
     float *mass_out = a.mass_out + pair * a.mass_out_stride;
-    uint32_t *kept = a.kept + pair * a.budget;
+    uint32_t *kept = a.kept + pair * a.kept_stride;
     if (h == 0 && rank == 0 && tid == 0) a.new_len[s] = keep;
     const uint32_t old = n > a.budget ? n - a.recent : 0;  // positions that compete
     uint32_t want = n > a.budget ? a.budget - a.recent : 0;
@@ -250,7 +250,7 @@ __global__ void __launch_bounds__(kMoveThreads) k_evict_move(EvictArgs a) {
     const uint64_t pair = (uint64_t)s * a.kv.n_kv + h;
     if (tid < rows) {
         uint64_t f = ~0ull, t = ~0ull;
-        const bool ok = evict_offset(a, a.table, s, a.kept[pair * a.budget + i0 + tid], h, f) &&
+        const bool ok = evict_offset(a, a.table, s, a.kept[pair * a.kept_stride + i0 + tid], h, f) &&
                         evict_offset(a, a.dst_table, s, i0 + tid, h, t);
         s_from[tid] = ok ? f : ~0ull;
         s_to[tid] = t;
@@ -289,7 +289,7 @@ __global__ void __launch_bounds__(kMoveThreads) k_evict_move_in_place(EvictArgs 
     const uint32_t byte = blockIdx.x % cols * 32 + (tid & 1) * 16;
     const uint32_t keep = a.new_len[s];
     if (h == 0 && blockIdx.x == 0 && tid == 0) a.lens_out[s] = keep;
-    const uint32_t *kept = a.kept + ((uint64_t)s * a.kv.n_kv + h) * a.budget;
+    const uint32_t *kept = a.kept + ((uint64_t)s * a.kv.n_kv + h) * a.kept_stride;
     constexpr int U = 4, R = kMoveThreads / 2;
     for (uint32_t i0 = 0; i0 < keep; i0 += R * U) {
         uint4 x[U];
@@ -344,13 +344,17 @@ cudaError_t launch_cluster(const LaunchCfg &c, const char *label, Kern kern, dim
 
 }  // namespace
 
+// Positions a row can keep: a budget may say "no limit".
+static uint32_t evict_most(const EvictArgs &a) { return min(a.budget, a.max_len); }
+
 size_t evict_scratch(const EvictArgs &a, bool have_kept) {
     const size_t lens = ((size_t)a.n_seq * 4 + 255) & ~(size_t)255;
-    return lens + (have_kept ? 0 : (size_t)a.n_seq * a.kv.n_kv * a.budget * 4);
+    return lens + (have_kept ? 0 : (size_t)a.n_seq * a.kv.n_kv * evict_most(a) * 4);
 }
 
 cudaError_t launch_evict(const LaunchCfg &c, EvictArgs a, uint8_t *scratch) {
     a.new_len = (uint32_t *)scratch;
+    a.kept_stride = a.kept ? a.budget : evict_most(a);
     if (!a.kept) a.kept = (uint32_t *)(scratch + (((size_t)a.n_seq * 4 + 255) & ~(size_t)255));
     a.err = c.dev_err;
     // Long rows by clusters of four.  Not where the weights are compacted in place: a CTA writes where
@@ -366,8 +370,7 @@ cudaError_t launch_evict(const LaunchCfg &c, EvictArgs a, uint8_t *scratch) {
         return launch_k(c, "evict_move", k_evict_move_in_place, dim3(2 * cols, a.kv.n_kv, a.n_seq), dim3(kMoveThreads),
                         0, a);
     }
-    const uint32_t most = min(a.budget, a.max_len);
-    return launch_k(c, "evict_move", k_evict_move, dim3((most + kMoveRows - 1) / kMoveRows, a.kv.n_kv, a.n_seq),
+    return launch_k(c, "evict_move", k_evict_move, dim3((evict_most(a) + kMoveRows - 1) / kMoveRows, a.kv.n_kv, a.n_seq),
                     dim3(kMoveThreads), 0, a);
 }
 

@@ -200,6 +200,7 @@ struct EvictArgs {
     uint32_t *lens_out, *kept;
     float *mass_out;
     uint32_t *new_len;              // [n_seq] scratch
+    uint32_t kept_stride;           // entries between the rows of kept, set by the launcher
     int in_place;
     int *err;
 };

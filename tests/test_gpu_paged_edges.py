@@ -154,3 +154,29 @@ def test_weights_of_a_row_that_is_not_finite(pkg, ctx):
     for s, h in ((0, 1), (1, 0), (1, 1)):  # the others are as they would be
         assert np.isfinite(got[s, 2 * h:2 * h + 2]).all()
         assert m[s, h].sum() == pytest.approx(2.0, rel=1e-5)
+
+
+# ── eviction ─────────────────────────────────────────────────────────────────
+
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("budget", [0xFFFFFFFF, 1 << 31, 41])
+def test_evict_without_a_limit(pkg, ctx, in_place, budget):
+    """A budget past every length keeps everything, and needs no room for more."""
+    rng = np.random.default_rng(7)
+    kv, hd, lens = 16, 64, [40, 0, 17]
+    c = Cache(pkg, rng, lens, kv, hd, True, 16, extra_pages=6)
+    mass = rng.uniform(0, 1, (3, kv, 40)).astype(np.float32)
+    dm, ln, out, lens_out = dev(mass), i32(lens), torch.zeros(3, kv, 40, device="cuda"), i32([9, 9, 9])
+    dst = np.full_like(c.table, 0xFFFFFFFF)
+    dst[0, :3], dst[2, :2] = c.free[:3], c.free[3:5]
+    dd = i32(dst)
+    torch.cuda.synchronize()
+    ctx.kv_evict(c.desc, 3, c.dtable, ln, 40, dm, 40, budget, 5, None if in_place else dd, lens_out, out, 40)
+    ctx.sync()
+    assert lens_out.tolist() == lens
+    gk = c.dk.cpu().numpy()
+    for s, n in enumerate(lens):
+        assert np.array_equal(out[s, :, :n].cpu().numpy(), mass[s, :, :n])
+        j = np.arange(n)
+        t = c.table if in_place else dst
+        assert np.array_equal(gk[t[s, j // 16], j % 16], c.hk[c.table[s, j // 16], j % 16])
