@@ -180,3 +180,96 @@ def test_evict_without_a_limit(pkg, ctx, in_place, budget):
         j = np.arange(n)
         t = c.table if in_place else dst
         assert np.array_equal(gk[t[s, j // 16], j % 16], c.hk[c.table[s, j // 16], j % 16])
+
+
+def test_evict_bad_page_keeps_to_its_own(pkg, ctx):
+    """A bad page id of one sequence: reported, the others' slots and the free pages are as they should be."""
+    rng = np.random.default_rng(8)
+    kv, hd, lens, budget, recent = 2, 64, [90, 90], 40, 8
+    c = Cache(pkg, rng, lens, kv, hd, True, 16, extra_pages=3)
+    mass = rng.uniform(0, 1, (2, kv, 90)).astype(np.float32)
+    good = c.table.copy()
+    c.table[0, 1] = 1 << 20
+    dm, ln, dt = dev(mass), i32(lens), i32(c.table)
+    torch.cuda.synchronize()
+    ctx.kv_evict(c.desc, 2, dt, ln, 90, dm, 90, budget, recent, None, ln, dm, 90)
+    with pytest.raises(pkg.LtError) as e:
+        ctx.sync()
+    assert e.value.status == 1
+    for got, host in ((c.dk.cpu().numpy(), c.hk), (c.dv.cpu().numpy(), c.hv)):
+        for p in [*c.free, good[0, 1]]:
+            assert np.array_equal(got[p], host[p], equal_nan=True)
+        for h in range(kv):
+            keep, i = evict_ref(mass[1, h], 90, budget, recent), np.arange(budget)
+            assert np.array_equal(got[good[1, i // 16], i % 16, h], host[good[1, keep // 16], keep % 16, h])
+        # beyond the budget nothing of either sequence moved
+        for s in (0, 1):
+            i = np.arange(48, 90)
+            assert np.array_equal(got[good[s, i // 16], i % 16], host[good[s, i // 16], i % 16])
+    ctx.sync()
+
+
+# ── what was not reached before ──────────────────────────────────────────────
+
+@pytest.mark.parametrize("heads,kv,hd", SHAPES)
+@pytest.mark.parametrize("f16", [True, False])
+@pytest.mark.parametrize("new", [[90, 151], [2, 1]])
+@pytest.mark.parametrize("cap", [0.05, 1.0, 4.0])
+def test_prompt_caps_that_bite(pkg, ctx, heads, kv, hd, f16, new, cap):
+    """Scores of standard deviation 1.5 under caps of that size and below: both ranges of the tanh."""
+    check_prompt(pkg, ctx, heads, kv, hd, f16, 16, new, [140, 151], cap=cap, alibi=True, seed=4)
+
+
+@pytest.mark.parametrize("op", ["decode", "prompt"])
+@pytest.mark.parametrize("f16", [True, False])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_capped_score_by_itself(pkg, ctx, op, f16, hd):
+    """4096 heads with scores c tanh(x), x from -4 to 4, against a score of 0: the two weights' quotient is e^score.
+
+    Error of log(p0 / p1) at a cap c of 10: the tanh 6.1e-8 (relative, below ln(3)/2 where it is at most 1/2) or
+    1.5e-7, times c; the score in log2 units and its difference from the maximum, half an ulp of up to 14.4 each, 4.8e-7
+    (below: of up to 7.3, 2.4e-7) times ln 2; two exponentials of 2^-22; two weights of 2^-22; x itself to 2^-23 times
+    c x (1 - tanh^2) <= 0.45 c; two quotients of 2^-24.  In all 4.4e-6 and 2.6e-6."""
+    heads, cap = 4096, 10.0
+    x = np.linspace(-4, 4, heads).astype(np.float32)
+    pools = [torch.zeros(1, 16, 1, hd, dtype=torch.float16 if f16 else torch.float32, device="cuda") for _ in range(2)]
+    pools[0][0, 0, 0, 0] = 1.0          # the first key's score is the query's first element
+    pools[1][0, 0, 0, 0] = pools[1][0, 1, 0, 1] = 1.0
+    desc = pkg.PagedKV(n_kv_heads=1, head_dim=hd, kv_f16=int(f16), page_size=16, n_pages=1, max_pages=1,
+                       k=pools[0].data_ptr(), v=pools[1].data_ptr())
+    q = np.zeros((1, heads, hd), np.float32)
+    q[0, :, 0] = x * np.float32(cap)
+    cfg = pkg.PagedAttnCfg(n_heads=heads, causal=1, scale=1.0, softcap=cap)
+    qd, out, dt, ln, cu = dev(q), torch.zeros(1, heads * hd, device="cuda"), i32([[0]]), i32([2]), i32([0, 1])
+    torch.cuda.synchronize()
+    if op == "decode":
+        ctx.paged_attn_decode(cfg, desc, qd, 1, dt, ln, 2, out)
+    else:
+        ctx.paged_attn_prompt(cfg, desc, qd, 1, cu, 1, 1, dt, ln, 2, out)
+    ctx.sync()
+    p = out.cpu().numpy().reshape(heads, hd).astype(np.float64)
+    want = cap * np.tanh(q[0, :, 0].astype(np.float64) / cap)
+    off = np.abs(np.log(p[:, 0] / p[:, 1]) - want)
+    low = np.abs(x) < 0.549
+    assert off[low].max() < 2.6e-6
+    assert off.max() < 4.4e-6
+    assert not p[:, 2:].any()
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("extra", [False, True])
+def test_prompts_over_f16_run_on_the_tensor_cores(pkg, ctx, hd, extra):
+    """The other kernel gives the same results, many times slower, so a call that went there would not show."""
+    heads, kv, n = 8, 2, 300
+    c = Cache(pkg, np.random.default_rng(6), [n], kv, hd, True, 16)
+    cfg = pkg.PagedAttnCfg(n_heads=heads, causal=1, scale=0.125, softcap=30.0 if extra else 0.0)
+    q, out, ln, cu = torch.randn(n, heads * hd, device="cuda"), torch.zeros(n, heads * hd, device="cuda"), i32([n]), i32([0, n])
+    torch.cuda.synchronize()
+    ctx.profile(True)
+    ctx.profile_reset()
+    ctx.paged_attn_prompt(cfg, c.desc, q, 1, cu, n, n, c.dtable, ln, n, out)
+    ctx.sync()
+    labels = set(ctx.profile_read())
+    ctx.profile(False)
+    ctx.profile_reset()
+    assert "paged_prompt" in labels and "paged_attn_rows" not in labels
