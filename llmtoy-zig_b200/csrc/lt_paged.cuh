@@ -155,16 +155,48 @@ LT_DEVINL float score_log2(float dot, float f, float cap, float slope, float dis
     return fmaf(-slope * kLog2e, dist, s);
 }
 
-// Row R of (sequence s, KV head kh) by itself, key by key, masked keys never
-// touched: for rows whose tile result is not finite, which a value outside the
-// row's own keys may have caused.  Output dims [d0, d0 + nd), nd a multiple of 16.
+// N consecutive cache elements from element i, a multiple of N: 4 bytes or a multiple of 8.
+template <int N>
+LT_DEVINL void kv_ld_row(const uint8_t *p, uint32_t i, uint32_t f16, float (&v)[N]) {
+    if (f16) {
+        uint32_t w[N / 2];
+        const uint8_t *at = p + 2 * i;
+        if constexpr (N == 2) {
+            w[0] = *reinterpret_cast<const uint32_t *>(at);
+        } else {
+#pragma unroll
+            for (int e = 0; e < N / 2; e += 2) {
+                const uint2 t = *reinterpret_cast<const uint2 *>(at + 4 * e);
+                w[e] = t.x, w[e + 1] = t.y;
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < N; e += 2) {
+            const float2 t = __half22float2(*reinterpret_cast<const __half2 *>(&w[e / 2]));
+            v[e] = t.x, v[e + 1] = t.y;
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < N; e += 2) {
+            const float2 t = *reinterpret_cast<const float2 *>(p + 4 * (i + e));
+            v[e] = t.x, v[e + 1] = t.y;
+        }
+    }
+}
+
+// Row R of (sequence s, KV head kh) by itself, by one warp, key by key, masked keys never touched: for rows
+// whose tile result is not finite, which a value outside the row's own keys may have caused.  Lane l holds
+// elements l HD / 32 on; output dims [d0, d0 + nd).  A sum that is NaN makes every dim NaN: the rest of the
+// keys is then left alone.  Several keys at a time, so that their loads and sums overlap.
+template <int HD>
 static __noinline__ __device__ void slow_row(const PagedAttnArgs &a, uint32_t s, uint32_t kh, uint32_t R, uint32_t d0,
-                                         uint32_t nd) {
-    const uint32_t hd = a.kv.hd, cap = (uint32_t)min((uint64_t)a.kv.max_pages * a.kv.page_size, (uint64_t)a.max_len);
+                                             uint32_t nd) {
+    constexpr int N = HD / 32, U = 4;
+    const uint32_t e0 = (threadIdx.x & 31) * N;
+    const uint32_t cap = (uint32_t)min((uint64_t)a.kv.max_pages * a.kv.page_size, (uint64_t)a.max_len);
     const uint32_t len = min(a.lens[s], cap), nq = a.cu[s + 1] - a.cu[s], q_row = a.cu[s] + R / a.group;
     const uint32_t head = kh * a.group + R % a.group;
-    const float *q = a.q + (uint64_t)q_row * a.q_stride + (uint64_t)head * hd;
-    float *out = a.out + (uint64_t)q_row * a.out_stride + (uint64_t)head * hd;
+    const float *q = a.q + (uint64_t)q_row * a.q_stride + (uint64_t)head * HD;
     const uint32_t *table = a.table + (uint64_t)s * a.kv.max_pages;
     const uint32_t *docs = a.docs ? a.docs + (uint64_t)s * a.doc_stride : nullptr;
     const int64_t i = (int64_t)len - nq + R / a.group;
@@ -174,30 +206,54 @@ static __noinline__ __device__ void slow_row(const PagedAttnArgs &a, uint32_t s,
     if (docs && i < 0) hi = 0;
     const float slope = a.slopes ? a.slopes[head] : 0.0f;
     const float f = a.softcap != 0.0f ? a.scale / a.softcap : a.scale * 1.4426950408889634f;
-    float m = -INFINITY;
-    for (uint32_t d = d0; d < d0 + nd; d += 16) {
-        float o[16], l = 0.0f;
-        for (int e = 0; e < 16; e++) o[e] = 0.0f;
-        for (int pass = d == d0 ? 0 : 1; pass < 2; pass++) {
-            for (int64_t j = lo; j < hi; j++) {
-                if (docs && docs[j] != docs[i]) continue;
-                const uint32_t page = table[j / a.kv.page_size];
-                if (page >= a.kv.n_pages) continue;
-                const uint64_t off = paged_offset(a.kv, page, (uint32_t)j, kh);
-                float dot = 0.0f;
-                for (uint32_t e = 0; e < hd; e++) dot = fmaf(q[e], kv_ld(a.kv.k + off, e, a.kv.f16), dot);
-                const float t = score_log2(dot, f, a.softcap, slope, fabsf((float)(i - j)));
-                if (pass == 0) {
-                    m = t != t || m != m ? NAN : fmaxf(m, t);
-                } else {
-                    const float p = ex2(t - m);
-                    l += p;
-                    for (int e = 0; e < 16; e++) o[e] = fmaf(p, kv_ld(a.kv.v + off, d + e, a.kv.f16), o[e]);
-                }
+    float x[N], o[N], m = -INFINITY, l = 0.0f;
+#pragma unroll
+    for (int e = 0; e < N; e++) {
+        x[e] = q[e0 + e];
+        o[e] = 0.0f;
+    }
+    for (int64_t j0 = lo; j0 < hi && l == l; j0 += U) {
+        uint64_t off[U];
+        bool seen[U];
+        float dot[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) {  // alike in all lanes
+            const int64_t j = j0 + u;
+            seen[u] = j < hi && (!docs || docs[j] == docs[i]);
+            const uint32_t page = seen[u] ? table[page_of(a.kv, (uint32_t)j)] : 0;
+            seen[u] = seen[u] && page < a.kv.n_pages;
+            off[u] = seen[u] ? paged_offset(a.kv, page, (uint32_t)j, kh) : 0;
+            dot[u] = 0.0f;
+            if (seen[u]) {
+                float k[N];
+                kv_ld_row(a.kv.k + off[u], e0, a.kv.f16, k);
+#pragma unroll
+                for (int e = 0; e < N; e++) dot[u] = fmaf(x[e], k[e], dot[u]);
             }
         }
-        for (int e = 0; e < 16; e++) out[d + e] = l == 0.0f ? 0.0f : o[e] / l;
+#pragma unroll
+        for (int w = 16; w > 0; w >>= 1) {
+#pragma unroll
+            for (int u = 0; u < U; u++) dot[u] += __shfl_xor_sync(0xffffffffu, dot[u], w);
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            if (!seen[u]) continue;
+            float v[N];
+            kv_ld_row(a.kv.v + off[u], e0, a.kv.f16, v);
+            const float t = score_log2(dot[u], f, a.softcap, slope, fabsf((float)(i - j0 - u)));
+            const float mn = t == t ? fmaxf(m, t) : t, base = mn == -INFINITY ? 0.0f : mn;
+            const float al = ex2(m - base), p = ex2(t - base);
+            m = mn;
+            l = fmaf(l, al, p);
+#pragma unroll
+            for (int e = 0; e < N; e++) o[e] = fmaf(o[e], al, p * v[e]);
+        }
     }
+    if (e0 < d0 || e0 >= d0 + nd) return;
+    float *out = a.out + (uint64_t)q_row * a.out_stride + (uint64_t)head * HD;
+#pragma unroll
+    for (int e = 0; e < N; e++) out[e0 + e] = l == 0.0f ? 0.0f : (l == l ? o[e] / l : l);
 }
 
 }  // namespace lt

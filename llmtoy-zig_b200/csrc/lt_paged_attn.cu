@@ -161,7 +161,7 @@ LT_DEVINL uint64_t pa_unit(const PagedAttnArgs &a, uint32_t s, uint32_t kh, uint
 
 // PLAIN: neither cap nor distance bias.
 template <int HD, bool F16, bool PROMPT, bool PLAIN>
-__global__ void __launch_bounds__(kPaThreads, PaShape<HD, F16>::CTAS) k_paged_attn(PagedAttnArgs a) {
+__global__ void __launch_bounds__(kPaThreads, PaShape<HD, F16>::CTAS) k_paged_attn(const __grid_constant__ PagedAttnArgs a) {
     using S = PaShape<HD, F16>;
     constexpr int KB = S::KB, TILE = S::TILE, NB = HD / 8;
     extern __shared__ __align__(128) uint8_t smem[];
@@ -638,15 +638,18 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<HD, F16>::CTAS) k_paged_at
                 for (int n = 0; n < NB; n++) off += (o[n][0] - o[n][0]) + (o[n][1] - o[n][1]);
                 off += __shfl_xor_sync(0xffffffffu, off, 1);
                 off += __shfl_xor_sync(0xffffffffu, off, 2);
-                if (PROMPT && off != 0.0f) {
-                    if ((uint32_t)g < rows) slow_row(a, cw.s, cw.kh, R, j4 * (HD / 4), HD / 4);
-                } else if ((uint32_t)g < rows) {
+                if ((uint32_t)g < rows && (!PROMPT || off == 0.0f)) {
                     float *dst = a.out + (uint64_t)(cw.q.q0 + R / a.group) * a.out_stride + (uint64_t)head * HD;
 #pragma unroll
                     for (int n = 0; n < NB; n++) {
                         dst[dim(n, 0)] = o[n][0] * inv;
                         dst[dim(n, 1)] = o[n][1] * inv;
                     }
+                }
+                if (PROMPT) {
+                    uint32_t again = __ballot_sync(0xffffffffu, (uint32_t)g < rows && off != 0.0f) & 0x11111111u;
+                    for (; again; again &= again - 1)
+                        slow_row<HD>(a, cw.s, cw.kh, cw.rb * kPaRows + (__ffs(again) - 1) / 4, 0, HD);
                 }
                 if (!PROMPT && a.mass && j4 == 0) {
                     a.unit_ml[u * 16 + g] = m;
@@ -768,7 +771,7 @@ LT_DEVINL void pa_join_row(const PagedAttnArgs &a, uint64_t u, uint32_t r) {
     }
     if (PROMPT) {
         __syncthreads();
-        if (s_off && tid < HD / 16) slow_row(a, s, kh, R, tid * 16, 16);
+        if (s_off && warp == 0) slow_row<HD>(a, s, kh, R, 0, HD);
     }
 }
 
@@ -862,7 +865,7 @@ LT_DEVINL void pa_mass(const PagedAttnArgs &a, uint32_t s, uint32_t kh, uint32_t
 
 // What is left when the tiles are done: rows to join, then weights to add up.
 template <int HD, bool PROMPT>
-__global__ void __launch_bounds__(128) k_paged_finish(PagedAttnArgs a, uint32_t n_join) {
+__global__ void __launch_bounds__(128) k_paged_finish(const __grid_constant__ PagedAttnArgs a, uint32_t n_join) {
     pdl_launch_dependents();
     pdl_wait();
     if constexpr (PROMPT) {  // many units, few of them shared: a CTA looks at one unit

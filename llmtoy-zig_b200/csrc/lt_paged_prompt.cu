@@ -181,7 +181,7 @@ struct IntC {
 };
 
 template <int HD, bool EXTRA>
-__global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(PagedAttnArgs a,
+__global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_constant__ PagedAttnArgs a,
                                                                 const __grid_constant__ PpMaps maps) {
     using S = PpShape<HD>;
     constexpr int KT = S::KT, NS = S::STAGES;
@@ -871,7 +871,8 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(PagedAttnArgs a,
                         *reinterpret_cast<const float4 *>(st + rr * PITCH + lane % 8 * 4);
             }
         }
-        if (real && !fine && !*dead) slow_row(a, s, kh, R, half * 128, OW);
+        uint32_t again = __ballot_sync(0xffffffffu, real && !fine && !*dead);
+        for (; again; again &= again - 1) slow_row<HD>(a, s, kh, R - lane + __ffs(again) - 1, half * 128, OW);
         tc_fence_before();
     }
     __syncthreads();
@@ -886,7 +887,7 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(PagedAttnArgs a,
 constexpr int kPpJoinRows = 8;
 
 template <int HD>
-__global__ void __launch_bounds__(kPpJoinRows * 32) k_paged_prompt_join(PagedAttnArgs a) {
+__global__ void __launch_bounds__(kPpJoinRows * 32) k_paged_prompt_join(const __grid_constant__ PagedAttnArgs a) {
     using S = PpShape<HD>;
     constexpr int PER = HD / 64;  // float2 per lane
     pdl_launch_dependents();
@@ -930,8 +931,8 @@ __global__ void __launch_bounds__(kPpJoinRows * 32) k_paged_prompt_join(PagedAtt
         float *dst = a.out + (uint64_t)(c0 + R / a.group) * a.out_stride + (uint64_t)(kh * a.group + R % a.group) * HD + 2 * lane;
 #pragma unroll
         for (int e = 0; e < PER; e++) *reinterpret_cast<float2 *>(dst + 64 * e) = make_float2(acc[e].x * inv, acc[e].y * inv);
-    } else if (lane < HD / 16) {
-        slow_row(a, s, kh, R, lane * 16, 16);
+    } else {
+        slow_row<HD>(a, s, kh, R, 0, HD);
     }
 }
 
