@@ -97,19 +97,6 @@ lt_status cuda_fail(lt_ctx *ctx, cudaError_t e, const char *what) {
         if (e_ != cudaSuccess) return cuda_fail(ctx, e_, what); \
     } while (0)
 
-lt::LaunchCfg cfg_of(lt_ctx *ctx) {
-    lt::LaunchCfg c;
-    c.stream = ctx->stream;
-    // No programmatic dependent launch on the default streams (legacy or
-    // per-thread): only on explicit streams.
-    c.pdl = ctx->pdl && ctx->stream != cudaStreamLegacy && ctx->stream != cudaStreamPerThread &&
-            ctx->stream != nullptr;
-    c.dev_err = ctx->dev_err;
-    c.num_sms = ctx->num_sms;
-    c.prof = &ctx->prof;
-    return c;
-}
-
 // Whether ops are recorded into a graph now: by lt_capture_begin, or by the owner of the stream.
 bool recording(const lt_ctx *ctx) {
     if (ctx->capturing) return true;
@@ -122,12 +109,25 @@ bool recording(const lt_ctx *ctx) {
     return s != cudaStreamCaptureStatusNone;
 }
 
+lt::LaunchCfg cfg_of(lt_ctx *ctx) {
+    if (recording(ctx)) ctx->scratch_recorded = ctx->counters_recorded = ctx->consts_recorded = true;
+    lt::LaunchCfg c;
+    c.stream = ctx->stream;
+    // No programmatic dependent launch on the default streams (legacy or
+    // per-thread): only on explicit streams.
+    c.pdl = ctx->pdl && ctx->stream != cudaStreamLegacy && ctx->stream != cudaStreamPerThread &&
+            ctx->stream != nullptr;
+    c.dev_err = ctx->dev_err;
+    c.num_sms = ctx->num_sms;
+    c.prof = &ctx->prof;
+    return c;
+}
+
 lt_status enter(lt_ctx *ctx) {
     if (!ctx) return LT_EINVAL;
     ctx->err.clear();
     cudaError_t e = cudaSetDevice(ctx->device);
     if (e != cudaSuccess) return cuda_fail(ctx, e, "cudaSetDevice");
-    if (recording(ctx)) ctx->scratch_recorded = ctx->counters_recorded = ctx->consts_recorded = true;
     return LT_OK;
 }
 

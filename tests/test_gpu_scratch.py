@@ -180,3 +180,27 @@ def test_smaller_calls_need_no_more_scratch(pkg, heads, kv, hd, f16):
             ctx.kv_evict(c.desc, s, c.dtable, ln, l, mass, most, 512, 8, None, lens_out, small, 512)
             ctx.kv_evict(c.desc, s, c.dtable, ln, l, mass, most, 64, 8, None, lens_out, small, 64, kept)
         ctx.capture_end().free()
+
+
+def test_leaving_a_stream_that_is_gone(pkg):
+    """A caller may destroy its stream and then give the context another: the old one is not looked at again."""
+    import ctypes
+    rt = torch.cuda.cudart()
+    step = Step(pkg)
+    with pkg.Context(0) as ctx:
+        step(ctx, 1 << 10)
+        ctx.sync()
+        want = step.result()
+        handle = ctypes.c_void_p()
+        assert int(rt.cudaStreamCreate(ctypes.addressof(handle))) == 0
+        ctx.set_stream(handle.value)
+        step.clear()
+        step(ctx, 1 << 10)
+        ctx.sync()
+        assert all(torch.equal(a, b) for a, b in zip(step.result(), want))
+        assert int(rt.cudaStreamDestroy(handle.value)) == 0
+        ctx.set_stream(None)
+        step.clear()
+        step(ctx, 1 << 10)
+        ctx.sync()
+        assert all(torch.equal(a, b) for a, b in zip(step.result(), want))
