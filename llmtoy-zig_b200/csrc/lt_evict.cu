@@ -17,8 +17,8 @@
 // independent of each other and give the parallelism.
 //
 // One B200, 16 sequences of 20000 to 32768 with 4 KV heads of 128 in f16, budget
-// 8192: 120 us, the moves 82 us of it (6.5 TB/s); the selection by one CTA per row
-// instead of four took 18 us more.  8 sequences of about 1100: 11 us, two launches.
+// 8192: 116 us, the moves 82 us of it (6.5 TB/s).  8 sequences of about 1100: 11 us,
+// two launches.
 #include <cooperative_groups.h>
 
 #include "lt_paged.cuh"
@@ -30,7 +30,10 @@ namespace cg = cooperative_groups;
 constexpr int kSelThreads = 1024;
 constexpr int kSelPer = 4;
 constexpr int kSelBins = 2048;
-constexpr uint32_t kSelCluster = 8192;  // rows longer than this take a cluster
+// Rows longer than this take a cluster where all clusters run at once.  The selection by one CTA and by four,
+// 4 or 16 rows: 9000 positions 17.8 and 18.5 us, 12000 18.6 and 18.6, 16000 20.6 and 18.7, 32768 32.9 and 24.
+// 64 rows, whose 256 CTAs take turns: 22.4 and 28.7 us at 16000, 34.9 and 37.0 at 32768.
+constexpr uint32_t kSelCluster = 12288;
 constexpr int kMoveThreads = 256;
 constexpr int kMoveRows = 64;
 
@@ -357,10 +360,10 @@ cudaError_t launch_evict(const LaunchCfg &c, EvictArgs a, uint8_t *scratch) {
     a.kept_stride = a.kept ? a.budget : evict_most(a);
     if (!a.kept) a.kept = (uint32_t *)(scratch + (((size_t)a.n_seq * 4 + 255) & ~(size_t)255));
     a.err = c.dev_err;
-    // Long rows by clusters of four.  Not where the weights are compacted in place: a CTA writes where
+    // Long rows by clusters of four (kSelCluster).  Not where the weights are compacted in place: a CTA writes where
     // those before it read, which only one CTA's own order makes safe.
     cudaError_t e;
-    if (a.max_len > kSelCluster && a.mass_out != a.mass)
+    if (a.max_len > kSelCluster && 4 * a.kv.n_kv * a.n_seq <= (uint32_t)c.num_sms && a.mass_out != a.mass)
         e = launch_cluster(c, "evict_select", k_evict_select<4>, dim3(4 * a.kv.n_kv, a.n_seq), dim3(kSelThreads), 4, a);
     else
         e = launch_k(c, "evict_select", k_evict_select<1>, dim3(a.kv.n_kv, a.n_seq), dim3(kSelThreads), 0, a);
