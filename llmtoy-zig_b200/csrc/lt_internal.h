@@ -211,7 +211,6 @@ cudaError_t launch_evict(const LaunchCfg &c, EvictArgs a, uint8_t *scratch);
 struct LogitArgs {
     const float *logits;
     uint32_t n, n_rows;
-    uint64_t in_stride, out_stride;
     const void *rules;
     const uint32_t *history, *bias_ids;
     const float *bias_values;

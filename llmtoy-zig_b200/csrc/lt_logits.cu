@@ -15,7 +15,7 @@
 // biases, the table holding the largest list index, so that of a token listed
 // twice the last entry counts.
 //
-// One B200, 64 rows of 262144: 20.8 us without lists (6.6 TB/s), 40 us with
+// One B200, 64 rows of 262144: 20.8 us without lists (6.6 TB/s), 42 us with
 // histories of up to 8192 and 300 biases, which every chunk of a row scans.  Counts
 // and biases applied to every token instead of a work list: 95 us; one scan per
 // cluster of eight chunks, counting into each other's shared memory: 41 to 52 us
@@ -58,8 +58,8 @@ __global__ void __launch_bounds__(kLgThreads) k_logits(LogitArgs a) {
     const uint32_t tid = threadIdx.x, row = blockIdx.y, t0 = blockIdx.x * kLgChunk, nt = min((uint32_t)kLgChunk, a.n - t0);
     const lt_logit_rule r = static_cast<const lt_logit_rule *>(a.rules)[row];
     const uint32_t hist_len = a.history ? r.history_len : 0, bias_len = a.bias_ids ? r.bias_len : 0;
-    const float *x = a.logits + row * a.in_stride + t0;
-    float *y = a.out + row * a.out_stride + t0;
+    const float *x = a.logits + (uint64_t)row * a.n + t0;
+    float *y = a.out + (uint64_t)row * a.n + t0;
     const uint32_t *mask = r.mask_row == LT_NO_MASK || !a.masks ? nullptr : a.masks + (uint64_t)r.mask_row * ((a.n + 31) / 32);
     const bool wide = ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(y)) & 15) == 0;
 

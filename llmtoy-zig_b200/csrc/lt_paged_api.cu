@@ -237,7 +237,7 @@ lt_status lt_logits_process(lt_ctx *ctx, const float *dev_logits, uint32_t n, ui
     if ((dev_bias_ids == nullptr) != (dev_bias_values == nullptr))
         return st_of(ctx_fail(ctx, LT_EINVAL, "lt_logits_process: bias ids and values go together"));
     if (n == 0 || n_rows == 0) return LT_OK;
-    lt::LogitArgs a = {dev_logits, n, n_rows, n, n, dev_rules, dev_history, dev_bias_ids, dev_bias_values, dev_masks, dev_out};
+    lt::LogitArgs a = {dev_logits, n, n_rows, dev_rules, dev_history, dev_bias_ids, dev_bias_values, dev_masks, dev_out};
     return st_of(lt::ctx_launched(ctx, lt::launch_logits(lt::ctx_cfg(ctx), a), "logits"));
 }
 
