@@ -560,15 +560,17 @@ void lt_rng_seed(uint64_t seed, uint64_t state_out[4]);
  * common prefix) as long as nobody appends to or evicts from them.  The
  * tables, lengths and positions are device arrays, so one captured graph
  * serves every step; max_len / max_q are host bounds on them (they size scratch
- * and grids).  Scratch comes from the context arena: run an op once with the
- * largest sizes before capturing it.
+ * and grids).  Scratch comes from the context arena (lt_reserve does not count
+ * it): run an op once with the largest sizes before capturing it, smaller calls
+ * need no more.
  *
  * A page id >= n_pages, a length past max_len or past the table, a query range
  * outside total_q / max_q is reported by lt_sync as LT_EINVAL; nothing outside
  * the given buffers is read or written, the results concerned are unspecified.
  * Page-table entries past a sequence's length are never read; cache slots past
  * it, or outside every query's window, may hold anything, infinities and NaN
- * included.  K and V of visible positions must be finite. */
+ * included.  K and V of visible positions must be finite (an f16 cache holds
+ * magnitudes up to 65504). */
 typedef struct lt_paged_kv {
     uint32_t n_kv_heads, head_dim;  /* head_dim 64, 128 or 256 */
     uint32_t kv_f16;                /* 1: IEEE f16 elements, 0: f32 */
@@ -616,7 +618,7 @@ typedef struct lt_paged_attn_cfg {
 /* One query per sequence: dev_out[s] over the dev_lens[s] cached positions.
  * dev_mass (nullable) [n_seq][n_kv_heads][mass_stride]: += the sum of the
  * normalised weights of the KV head's query heads, for every position seen (what
- * lt_kv_evict ranks by). */
+ * lt_kv_evict ranks by; clear a position's cells when a new token takes it). */
 lt_status lt_paged_attn_decode(lt_ctx *ctx, const lt_paged_attn_cfg *cfg, const lt_paged_kv *kv, const float *dev_q,
                                uint32_t n_seq, const uint32_t *dev_page_table, const uint32_t *dev_lens,
                                uint32_t max_len, float *dev_mass, uint64_t mass_stride, float *dev_out);

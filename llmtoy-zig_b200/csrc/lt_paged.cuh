@@ -20,8 +20,8 @@ LT_DEVINL uint32_t slot_of(const PagedKvDev &kv, uint32_t j) {
     return kv.page_shift != kNoShift ? j & (kv.page_size - 1) : j % kv.page_size;
 }
 
-// Byte offset of position j of a sequence (its page-table row `row`) for head
-// h, or ~0 when the page id lies outside the pool (the caller reports it).
+// Byte offset in a pool of position j of a sequence, on page `page` of it (which
+// the caller has looked up and checked), for head h.
 LT_DEVINL uint64_t paged_offset(const PagedKvDev &kv, uint32_t page, uint32_t j, uint32_t h) {
     return (uint64_t)page * kv.page_stride + (uint64_t)slot_of(kv, j) * kv.slot_stride +
            (uint64_t)h * kv.head_stride;

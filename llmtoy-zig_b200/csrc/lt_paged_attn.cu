@@ -27,10 +27,10 @@
 //
 // One B200: 64 sequences of 200 to 8192 positions, 32/4 heads of 128, f16 (289
 // MB): 58 us, 5.0 TB/s; one sequence of 130001 with weights accumulated (270 MB):
-// 66 us, the main kernel's tile loop at 6.9 TB/s, the rest its start, its end and the
-// second kernel (11 us); one window of 1024 over an f32 cache, 16/8 heads of 256:
-// 15 us, three dependent round trips to memory and two launches.  Two stages with
-// 12 warps per SM instead of three with 8: 89 us for the 64 sequences.
+// 67 us, the main kernel about 55 of it, the second about 11; one window of 1024
+// over an f32 cache, 16/8 heads of 256: 15 us, three dependent round trips to memory
+// and two launches.  Two stages with 12 warps per SM instead of three with 8: 89 us
+// for the 64 sequences.
 #include "lt_paged.cuh"
 
 namespace lt {
@@ -154,7 +154,7 @@ struct PaShare {
     }
 };
 
-// A unit's place in the records: its first CTA and how many CTAs share it.
+// The number of a unit: its place in unit_info and unit_ml.
 LT_DEVINL uint64_t pa_unit(const PagedAttnArgs &a, uint32_t s, uint32_t kh, uint32_t rb) {
     return ((uint64_t)s * a.kv.n_kv + kh) * a.row_blocks + rb;
 }
@@ -673,7 +673,7 @@ __global__ void __launch_bounds__(kPaThreads, PaShape<HD, F16>::CTAS) k_paged_at
         f = unit_f0 + cw.q.cost();  // the next unit, unless this one goes on elsewhere
         if (f < f1) {
             cw.template next_unit<TILE>(a);
-            load_q();
+            load_q();  // (fetched before the merge they cost registers: 59.5 us for the 64 sequences, 57.6 without)
         }
     }
     cp_async_wait<0>();
@@ -776,7 +776,9 @@ LT_DEVINL void pa_join_row(const PagedAttnArgs &a, uint64_t u, uint32_t r) {
 }
 
 // mass[s][kv head][j] += sum over the KV head's query heads of 2^(score - m) / l, for
-// kMassKeys positions from j0 on; a thread's cells are its own.  The scores are on
+// kMassKeys positions from j0 on; a thread's cells are its own.  m and l are those of the
+// whole row, which no CTA knows before all of the unit's are done: the scores wait in
+// scratch (33 MB next to 270 MB of K and V for the long sequence; K again would be 135).  The scores are on
 // their way while the heads' m and l are put together, 16 threads to a head.
 LT_DEVINL void pa_mass(const PagedAttnArgs &a, uint32_t s, uint32_t kh, uint32_t j0) {
     extern __shared__ float s_ml[];  // [group] maxima, [group] 1 / sum
@@ -921,7 +923,6 @@ cudaError_t pa_launch(const LaunchCfg &c, const PagedAttnArgs &a, uint64_t units
         e = launch_k(c, label, k_paged_attn<HD, F16, PROMPT, true>, grid, dim3(kPaThreads), PaShape<HD, F16>::SMEM, a);
     else
         e = launch_k(c, label, k_paged_attn<HD, F16, PROMPT, false>, grid, dim3(kPaThreads), PaShape<HD, F16>::SMEM, a);
-    if (e != cudaSuccess) return e;
     if (e != cudaSuccess) return e;
     const uint64_t join = PROMPT ? units : units * kPaRows;
     const uint64_t mass = a.mass ? (uint64_t)((a.max_len + kMassKeys - 1) / kMassKeys) * a.kv.n_kv * a.n_seq : 0;

@@ -25,15 +25,15 @@
 // of high terms, then 8 of low ones, over the 16 columns of S they come from.
 //
 // Bound: the tensor cores, from a few hundred rows on.  One B200, 8192 tokens,
-// 32/4 heads of 128, causal (550 GFLOP, 1.1 TFLOP as done): 0.97 ms, that is
-// 1.13 PFLOP/s of products against 1.38 sustained by a cuBLAS bf16 GEMM on this
-// part (1.65 in a burst); a pass over one tile of 256 x 128 takes 5350 clocks, its
-// products alone 4160.  With few rows, latency: a 257-token follow-up on 1243 cached
-// ones (14/2 heads of 64) takes 21 us with its keys shared by 6 CTAs, 37 us without.
-// head_dim 256 (6320 tokens of packed documents, 246 us) waits for K: the queries
-// leave room for three stages only, and a K tile's copy starts when the product
-// before the last is done.  Prefetching tiles into L2 made every case slower (8192
-// tokens 1.15 ms), as did one KV head after the other (1.01 ms).
+// 32/4 heads of 128, causal (550 GFLOP, 1.1 TFLOP as done): 0.91 to 0.94 ms in a row,
+// that is 1.17 to 1.21 PFLOP/s of products against 1.38 sustained by a cuBLAS bf16
+// GEMM on this part (1.65 in a burst); 0.78 ms when launches are far enough apart to
+// stay clear of the power cap.  With few rows, latency: a 257-token follow-up on 1243
+// cached ones (14/2 heads of 64) takes 19 us with its keys shared by 6 CTAs, 37 us
+// without.  head_dim 256 (6320 tokens of packed documents, 231 us) waits for K: the
+// queries leave room for three stages only, and a K tile's copy starts when the
+// product before the last is done.  Prefetching tiles into L2 made every case slower
+// (8192 tokens 1.15 ms, 1.00 without), as did one KV head after the other (1.01 ms).
 #include <cuda.h>  // CUtensorMap (encoded through the runtime's driver entry point)
 
 #include "lt_paged.cuh"
@@ -42,7 +42,9 @@
 namespace lt {
 
 constexpr int kPpThreads = 384, kPpProducers = 96;
-constexpr int kPpSkipTiles = 4096;  // tiles whose documents are looked at beforehand
+// Tiles whose documents are looked at beforehand: 512 bytes of bits, what shared memory leaves beside the queries and
+// the ring at head_dim 128.  Longer rows (512 K keys; 256 K at head_dim 256) go through every tile.
+constexpr int kPpSkipTiles = 4096;
 
 template <int HD>
 struct PpShape {
@@ -1027,10 +1029,11 @@ bool pp_regs() {
 bool paged_prompt_supported(const PagedAttnArgs &a) {
     static const bool regs = pp_regs<64, false>() && pp_regs<64, true>() && pp_regs<128, false>() &&
                              pp_regs<128, true>() && pp_regs<256, false>() && pp_regs<256, true>();
-    // Few rows: the kernel for single tokens reads the cache once per 8 rows.  Measured at 1 and 8
-    // sequences of 60 to 8000 cached tokens: 8 rows 31 to 110 us there and 38 to 213 here, 16 rows
-    // about alike (60 and 70 us at most), 28 rows of 60 tokens 7.9 and 10.0 us, 32 rows of 8000
-    // tokens 100 and 72 us, 56 rows of 60 tokens 16 and 10 us.
+    // Few rows: the kernel for single tokens reads the cache once per 8 rows.  Measured there and here,
+    // over head_dim 64, 128 and 256: 8 rows of 8 sequences of 8000 cached tokens 23, 41 and 114 us and
+    // 30, 65 and 206; 16 rows of them 33, 59 and 218 us and 30, 69 and 206; 32 rows 52, 99 and 424 us and
+    // 30, 68 and 207.  A cache of 60 tokens: 28 to 32 rows 7.3, 7.8 and 19.5 us and 10.2, 12.6 and 13.7,
+    // 56 rows 16, 18 and 20 us and 10, 13 and 14; of 200 tokens, 16 rows 16, 17 and 19 us and 13, 16 and 16.
     const uint64_t rows = (uint64_t)a.max_q * a.group;
     return regs && a.kv.f16 && rows > (a.max_len > 256 ? kPpMinRows : kPpMinRowsShort);
 }
