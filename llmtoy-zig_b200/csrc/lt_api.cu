@@ -157,7 +157,9 @@ void retire(lt_ctx *ctx, void *p, bool recorded) {
 lt_status ensure_scratch(lt_ctx *ctx, size_t bytes) {
     if (bytes <= ctx->scratch_bytes) return LT_OK;
     if (recording(ctx))
-        return fail(ctx, LT_EINVAL, "op needs %zu scratch bytes while capturing: call lt_reserve first", bytes);
+        return fail(ctx, LT_EINVAL,
+                    "op needs %zu scratch bytes while capturing: call lt_reserve, or run it once at its largest sizes, first",
+                    bytes);
     LT_CUDA(ctx, cudaStreamSynchronize(ctx->stream), "cudaStreamSynchronize");
     retire(ctx, ctx->scratch, ctx->scratch_recorded);
     ctx->scratch = nullptr;
@@ -310,8 +312,8 @@ int lt::ctx_fail(lt_ctx *ctx, int status, const char *fmt, ...) {
     return status;
 }
 
-int lt::ctx_scratch(lt_ctx *ctx, size_t bytes, uint8_t **out) {
-    const lt_status st = ensure_scratch(ctx, bytes);
+int lt::ctx_scratch(lt_ctx *ctx, size_t bytes, size_t need, uint8_t **out) {
+    const lt_status st = ensure_scratch(ctx, bytes > ctx->scratch_bytes && recording(ctx) ? need : bytes);
     *out = ctx->scratch;
     return st;
 }

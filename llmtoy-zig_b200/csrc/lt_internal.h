@@ -15,11 +15,12 @@ int ctx_device(const lt_ctx *ctx);
 cudaStream_t ctx_stream(const lt_ctx *ctx);
 
 // What entry points in other files need of the context: device selection and
-// a cleared error, a failure with its message, the arena and the counters
-// (grown outside capture only), launch settings, a launch's outcome.
+// a cleared error, a failure with its message, the arena (grown outside capture
+// only, and then to `bytes`; while ops are recorded it need only hold `need`),
+// launch settings, a launch's outcome.
 int ctx_enter(lt_ctx *ctx);
 int ctx_fail(lt_ctx *ctx, int status, const char *fmt, ...);
-int ctx_scratch(lt_ctx *ctx, size_t bytes, uint8_t **out);
+int ctx_scratch(lt_ctx *ctx, size_t bytes, size_t need, uint8_t **out);
 int ctx_launched(lt_ctx *ctx, cudaError_t e, const char *what);
 
 // A weight matrix as the kernels see it: GGUF rows at a 16-byte pitch.
@@ -187,7 +188,8 @@ size_t paged_attn_scratch(const PagedAttnArgs &a, int num_sms);
 cudaError_t launch_paged_attn(const LaunchCfg &c, PagedAttnArgs a, uint8_t *scratch);
 // Prompts over f16 caches on the tensor cores (lt_paged_prompt.cu).
 bool paged_prompt_supported(const PagedAttnArgs &a);
-size_t paged_prompt_scratch(const PagedAttnArgs &a, int num_sms);
+size_t paged_prompt_scratch(PagedAttnArgs a, int num_sms);            // of this call
+size_t paged_prompt_scratch_most(const PagedAttnArgs &a, int num_sms);  // and of every smaller one
 cudaError_t launch_paged_prompt(const LaunchCfg &c, PagedAttnArgs a, uint8_t *scratch);
 
 // Eviction from a paged cache (lt_evict.cu).

@@ -142,7 +142,8 @@ lt_status lt_paged_attn_decode(lt_ctx *ctx, const lt_paged_attn_cfg *cfg, const 
     a.mass_stride = mass_stride;
     const lt::LaunchCfg c = lt::ctx_cfg(ctx);
     uint8_t *scratch = nullptr;
-    if ((st = st_of(lt::ctx_scratch(ctx, lt::paged_attn_scratch(a, c.num_sms), &scratch))) != LT_OK) return st;
+    const size_t need = lt::paged_attn_scratch(a, c.num_sms);
+    if ((st = st_of(lt::ctx_scratch(ctx, need, need, &scratch))) != LT_OK) return st;
     return st_of(lt::ctx_launched(ctx, lt::launch_paged_attn(c, a, scratch), "paged attention"));
 }
 
@@ -179,10 +180,12 @@ lt_status lt_paged_attn_prompt(lt_ctx *ctx, const lt_paged_attn_cfg *cfg, const 
     const lt::LaunchCfg c = lt::ctx_cfg(ctx);
     uint8_t *scratch = nullptr;
     if (lt::paged_prompt_supported(a)) {
-        if ((st = st_of(lt::ctx_scratch(ctx, lt::paged_prompt_scratch(a, c.num_sms), &scratch))) != LT_OK) return st;
+        const size_t need = lt::paged_prompt_scratch(a, c.num_sms), most = lt::paged_prompt_scratch_most(a, c.num_sms);
+        if ((st = st_of(lt::ctx_scratch(ctx, most, need, &scratch))) != LT_OK) return st;
         return st_of(lt::ctx_launched(ctx, lt::launch_paged_prompt(c, a, scratch), "paged prompt attention"));
     }
-    if ((st = st_of(lt::ctx_scratch(ctx, lt::paged_attn_scratch(a, c.num_sms), &scratch))) != LT_OK) return st;
+    const size_t need = lt::paged_attn_scratch(a, c.num_sms);
+    if ((st = st_of(lt::ctx_scratch(ctx, need, need, &scratch))) != LT_OK) return st;
     return st_of(lt::ctx_launched(ctx, lt::launch_paged_attn(c, a, scratch), "paged prompt attention"));
 }
 
@@ -221,7 +224,8 @@ lt_status lt_kv_evict(lt_ctx *ctx, const lt_paged_kv *kv, uint32_t n_seq, const 
     a.kept = dev_kept;
     a.mass_out = dev_mass_out;
     uint8_t *scratch = nullptr;
-    if ((st = st_of(lt::ctx_scratch(ctx, lt::evict_scratch(a, dev_kept != nullptr), &scratch))) != LT_OK) return st;
+    const size_t need = lt::evict_scratch(a, dev_kept != nullptr);
+    if ((st = st_of(lt::ctx_scratch(ctx, need, need, &scratch))) != LT_OK) return st;
     return st_of(lt::ctx_launched(ctx, lt::launch_evict(lt::ctx_cfg(ctx), a, scratch), "evict"));
 }
 

@@ -1038,10 +1038,15 @@ bool paged_prompt_supported(const PagedAttnArgs &a) {
     return regs && a.kv.f16 && rows > (a.max_len > 256 ? kPpMinRows : kPpMinRowsShort);
 }
 
+size_t paged_prompt_scratch(PagedAttnArgs a, int num_sms) {
+    pp_split(a, num_sms);
+    return a.nsplit == 1 ? 0 : pp_records(a) * (a.kv.hd + 2) * 4;
+}
+
 // Enough for this call and for every smaller one, so that an op run once at its largest sizes has its scratch when a
 // smaller call is recorded.  Only smaller calls may share their keys, and there are records only where a launch has no
 // more CTAs than SMs; the fewest rows take the other kernel with its own scratch.
-size_t paged_prompt_scratch(const PagedAttnArgs &a, int num_sms) {
+size_t paged_prompt_scratch_most(const PagedAttnArgs &a, int num_sms) {
     const size_t records = (size_t)num_sms * pp_rows(a) * (a.kv.hd + 2) * 4;
     PagedAttnArgs few = a;
     few.max_q = min(a.max_q, kPpMinRowsShort / a.group);

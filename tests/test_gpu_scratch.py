@@ -204,3 +204,32 @@ def test_leaving_a_stream_that_is_gone(pkg):
         step(ctx, 1 << 10)
         ctx.sync()
         assert all(torch.equal(a, b) for a, b in zip(step.result(), want))
+
+
+def test_a_recording_asks_only_for_what_its_calls_need(pkg):
+    """A long prompt shares no keys and needs no scratch: it can be recorded on a context that has run nothing."""
+    rng = np.random.default_rng(3)
+    heads, kv, hd, n = 32, 4, 128, 1300
+    c = Cache(pkg, rng, [n] * 2, kv, hd, True, 16)
+    cfg = pkg.PagedAttnCfg(n_heads=heads, causal=1, scale=1 / math.sqrt(hd))
+    q, out = torch.randn(2 * n, heads * hd, device="cuda"), torch.zeros(2 * n, heads * hd, device="cuda")
+    cu, ln = i32([0, n, 2 * n]), i32([n, n])
+    torch.cuda.synchronize()
+    with pkg.Context(0) as ctx:
+        ctx.capture_begin()
+        ctx.paged_attn_prompt(cfg, c.desc, q, 2, cu, 2 * n, n, c.dtable, ln, n, out)
+        graph = ctx.capture_end()
+        graph.launch()
+        ctx.sync()
+        got = out.clone()
+        out.zero_()
+        torch.cuda.synchronize()
+        ctx.paged_attn_prompt(cfg, c.desc, q, 2, cu, 2 * n, n, c.dtable, ln, n, out)  # the arena comes now
+        ctx.sync()
+        assert torch.equal(out, got) and bool(out.any())
+        out.zero_()
+        torch.cuda.synchronize()
+        graph.launch()
+        ctx.sync()
+        assert torch.equal(out, got)
+        graph.free()
