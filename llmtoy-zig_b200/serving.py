@@ -72,20 +72,22 @@ class BatchDecoder:
         ctx.dequant(s.token_emb, 0, s.vocab, self.emb)
         self.cfg = AttnCfg(s.n_heads, s.n_kv_heads, s.head_dim, int(s.rope_neox), s.rope_theta, s.eps, s.head_dim ** -0.5, 1)
         self.attn = PagedAttnCfg(n_heads=s.n_heads, causal=1, scale=s.head_dim ** -0.5)
-        self.caches, self.mass = [], []
-        for _ in s.layers:
+        self.caches, self.mass, self.biases = [], [], []
+        for L in s.layers:
             k, v = torch.zeros(shape, dtype=kind, device="cuda"), torch.zeros(shape, dtype=kind, device="cuda")
             kv = PagedKV(n_kv_heads=s.n_kv_heads, head_dim=s.head_dim, kv_f16=int(s.kv_f16), page_size=page_size,
                          n_pages=self.n_pages, max_pages=self.width, k=k.data_ptr(), v=v.data_ptr())
             self.caches.append((kv, k, v))
             self.mass.append(torch.zeros(max_seqs, s.n_kv_heads, max_len, device="cuda") if budget else None)
+            b = None if L.qkv_bias is None else L.qkv_bias.contiguous()  # read 16 bytes at a time
+            self.biases.append(b if b is None or b.data_ptr() % 16 == 0 else b.clone())
         torch.cuda.synchronize()
 
     @contextmanager
     def _between(self):
         """What runs in here allocates with torch and launches on the context's stream only.  torch hands a block out
         again in the order of its own stream, so all work, whosever, ends before and after; in between no torch kernel
-        runs, and blocks change hands in the order of the context's stream."""
+        runs while the context's stream has work, and blocks change hands in the order of that stream."""
         import torch
         torch.cuda.synchronize()
         try:
@@ -113,12 +115,12 @@ class BatchDecoder:
         bias = zeros = None
         for i, L in enumerate(s.layers):
             ctx.rmsnorm(x, L.attn_norm, s.eps, s.d_model, ntok, xn)
-            if L.qkv_bias is None:
+            if self.biases[i] is None:
                 ctx.qmatvec(L.wqkv, xn, qkv, ntok)
             else:
                 if bias is None:
                     bias, zeros = torch.empty_like(qkv), self._dev([0] * ntok)
-                ctx.gather_rows(L.qkv_bias, nq + 2 * nkv, zeros, ntok, bias)  # its one row for every token
+                ctx.gather_rows(self.biases[i], nq + 2 * nkv, zeros, ntok, bias)  # its one row for every token
                 ctx.qmatvec_add(L.wqkv, xn, bias, qkv, ntok)
             ctx.paged_append(self.cfg, self.caches[i][0], qkv, ntok, L.q_norm, L.k_norm, seq, pos, slot, self.table,
                              self.n_seq, q)

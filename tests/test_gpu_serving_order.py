@@ -90,3 +90,20 @@ def test_biases_of_every_token(ctx, kv_f16):
     with decoder.Decoder(ctx, spec) as one:
         want = [one.generate(p, 10) for p in prompts]
     assert serving.BatchDecoder(ctx, spec, max_seqs=3, max_len=128).generate(prompts, 10) == want
+
+
+def test_biases_at_any_address(ctx):
+    """A bias that is a view into something larger, at an odd address or with a stride."""
+    serving = importlib.import_module("llmtoy-zig_b200.serving")
+    _, spec = upload(ctx, "biases")
+    prompts = [[5, 17, 2999], [1]]
+    want = serving.BatchDecoder(ctx, spec, max_seqs=2, max_len=32).generate(prompts, 6)
+    for i, L in enumerate(spec.layers):
+        n = L.qkv_bias.numel()
+        room = torch.zeros(2 * n + 1, device="cuda")
+        view = room[1:n + 1] if i % 2 == 0 else room[1::2]
+        view.copy_(L.qkv_bias)
+        assert view.data_ptr() % 16
+        L.qkv_bias = view
+    torch.cuda.synchronize()
+    assert serving.BatchDecoder(ctx, spec, max_seqs=2, max_len=32).generate(prompts, 6) == want
