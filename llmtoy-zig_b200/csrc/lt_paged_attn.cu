@@ -26,7 +26,7 @@
 //   that its f16 terms neither overflow nor vanish.
 //
 // One B200: 64 sequences of 200 to 8192 positions, 32/4 heads of 128, f16 (289
-// MB): 58 us, 5.0 TB/s; one sequence of 130001 with weights accumulated (270 MB):
+// MB): 57 to 61 us, 5.0 TB/s; one sequence of 130001 with weights accumulated (270 MB):
 // 67 us, the main kernel about 55 of it, the second about 11; one window of 1024
 // over an f32 cache, 16/8 heads of 256: 15 us, three dependent round trips to memory
 // and two launches.  Two stages with 12 warps per SM instead of three with 8: 89 us
