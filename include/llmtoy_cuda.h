@@ -651,6 +651,41 @@ lt_status lt_kv_evict(lt_ctx *ctx, const lt_paged_kv *kv, uint32_t n_seq, const 
                       uint32_t budget, uint32_t recent, const uint32_t *dev_dst_table, uint32_t *dev_lens_out,
                       float *dev_mass_out, uint64_t mass_out_stride, uint32_t *dev_kept);
 
+/* ── pages planned on the device ────────────────────────────────────────────
+ * What a batch keeps from step to step, all in device memory: the cached length
+ * of each sequence, its pages (a page belongs to one sequence), and the pages
+ * that none holds, a stack of *dev_n_free entries. */
+typedef struct lt_paged_state {
+    uint32_t n_seq;                 /* at most 65535 */
+    uint32_t page_size, n_pages;    /* fewer than 2^32 slots in all */
+    uint32_t max_pages;             /* entries per page-table row */
+    uint32_t *dev_lens;             /* [n_seq] */
+    uint32_t *dev_page_table;       /* [n_seq][max_pages] */
+    uint32_t *dev_free;             /* [n_pages] */
+    uint32_t *dev_n_free;           /* [1] */
+} lt_paged_state;
+
+/* Pages and places of the coming tokens.  Of sequence s the first dev_keep[s] <=
+ * dev_lens[s] positions stay (dev_keep NULL: all; 0 ends a sequence), and
+ * dev_new[s] tokens come behind them.  Pages that held only what goes are pushed
+ * on the stack, the last sequence's first and each sequence's last page first, and
+ * their table entries become 0xffffffff; then the pages still wanted are popped, the first
+ * sequence's first.  Updates the state (dev_lens[s] becomes keep + new) and writes
+ *   dev_cu_q[n_seq + 1]   the running sums of dev_new (lt_paged_attn_prompt's)
+ *   dev_seq, dev_pos      sequence and position of each new token (lt_paged_append's)
+ *   dev_pool_slot         page * page_size + slot of it in the pool
+ * the last three nullable, with room for total_q tokens; entries past the last
+ * token stay as they are.  The outputs must not overlap the inputs.
+ *
+ * All or nothing: a plan that wants more pages than there are is reported by
+ * lt_sync as LT_ENOMEM, one with keep > lens, more positions than a table row (or
+ * 2^30) holds, more tokens than total_q, or a page id or stack past n_pages, as
+ * LT_EINVAL; the state then stays as it was and dev_cu_q is all 0: the ops that
+ * follow find no new rows. */
+lt_status lt_paged_plan(lt_ctx *ctx, const lt_paged_state *state, const uint32_t *dev_keep, const uint32_t *dev_new,
+                        uint32_t total_q, uint32_t *dev_cu_q, uint32_t *dev_seq, uint32_t *dev_pos,
+                        uint32_t *dev_pool_slot);
+
 /* What a request asks of one row of logits (device array, one per row).
  * For a token that occurs c > 0 times in the row's history:
  *   x = (x > 0 ? x / repetition : x * repetition) - (c * frequency + presence)

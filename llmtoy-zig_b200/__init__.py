@@ -44,7 +44,7 @@ EXPORTS = [
     "lt_qmatvec_multi", "lt_noalloc_status", "lt_selftest_wait",
     "lt_stack_create", "lt_stack_run", "lt_stack_free", "lt_ep_unique_id", "lt_ep_init", "lt_ep_free",
     "lt_moe_ffn_ep", "lt_paged_append", "lt_paged_attn_decode", "lt_paged_attn_prompt", "lt_kv_evict",
-    "lt_logits_process",
+    "lt_logits_process", "lt_paged_plan",
 ]
 
 
@@ -87,6 +87,13 @@ class PagedAttnCfg(ctypes.Structure):
     _fields_ = [("n_heads", ctypes.c_uint32), ("window", ctypes.c_uint32), ("causal", ctypes.c_uint32),
                 ("scale", ctypes.c_float), ("softcap", ctypes.c_float), ("slopes", ctypes.c_void_p),
                 ("q_stride", ctypes.c_uint64), ("out_stride", ctypes.c_uint64)]
+
+
+class PagedState(ctypes.Structure):
+    """lt_paged_state: lengths, page tables and free pages of a batch, in device memory."""
+    _fields_ = [("n_seq", ctypes.c_uint32), ("page_size", ctypes.c_uint32), ("n_pages", ctypes.c_uint32),
+                ("max_pages", ctypes.c_uint32), ("lens", ctypes.c_void_p), ("page_table", ctypes.c_void_p),
+                ("free", ctypes.c_void_p), ("n_free", ctypes.c_void_p)]
 
 
 class LogitRule(ctypes.Structure):
@@ -199,6 +206,7 @@ def load_library() -> ctypes.CDLL:
                                      P]),
         "lt_paged_attn_prompt": (I, [P, ctypes.POINTER(PagedAttnCfg), ctypes.POINTER(PagedKV), P, U32, P, U32, U32, P, P,
                                      U32, P, P, U64, P]),
+        "lt_paged_plan": (I, [P, ctypes.POINTER(PagedState), P, P, U32, P, P, P, P]),
         "lt_kv_evict": (I, [P, ctypes.POINTER(PagedKV), U32, P, P, U32, P, U64, U32, U32, P, P, P, U64, P]),
         "lt_logits_process": (I, [P, P, U32, U32, P, P, P, P, P, P]),
         "lt_quant_matvec_host": (I, [P, P, P, U32, P, U64, U64]),
@@ -531,6 +539,12 @@ class Context:
         self._check(self.lib.lt_kv_evict(self.ptr, ctypes.byref(kv), n_seq, _ptr(page_table), _ptr(lens), max_len,
                                          _ptr(mass), mass_stride, budget, recent, _ptr(dst_table), _ptr(lens_out),
                                          _ptr(mass_out), mass_out_stride, _ptr(kept)))
+
+    def paged_plan(self, state: PagedState, keep, new, total_q: int, cu_q, seq=None, pos=None, pool_slot=None) -> None:
+        """Give back the pages behind keep[s] positions (None: all stay), take those that new[s] more need; cu_q[n_seq + 1]
+        and, for up to total_q tokens, the sequence, position and pool slot of each."""
+        self._check(self.lib.lt_paged_plan(self.ptr, ctypes.byref(state), _ptr(keep), _ptr(new), total_q, _ptr(cu_q),
+                                           _ptr(seq), _ptr(pos), _ptr(pool_slot)))
 
     def logits_process(self, logits, n: int, n_rows: int, rules, history, bias_ids, bias_values, masks, out) -> None:
         """Penalties, biases and grammar masks on n_rows rows of logits; rules: n_rows LogitRule on the device."""

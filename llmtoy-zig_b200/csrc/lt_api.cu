@@ -523,6 +523,7 @@ lt_status lt_sync(lt_ctx *ctx) {
     if (h != 0) {
         cudaMemset(ctx->dev_err, 0, 4);
         if (h == lt::DEV_ERR_BAD_INDEX) return fail(ctx, LT_EINVAL, "a device-side index was out of range");
+        if (h == lt::DEV_ERR_NO_PAGES) return fail(ctx, LT_ENOMEM, "too few free cache pages for the tokens to come");
         return fail(ctx, LT_ETIMEOUT, "a device-side wait gave up (code %d)", h);
     }
     return LT_OK;

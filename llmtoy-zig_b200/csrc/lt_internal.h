@@ -209,6 +209,18 @@ struct EvictArgs {
 size_t evict_scratch(const EvictArgs &a, bool have_kept);
 cudaError_t launch_evict(const LaunchCfg &c, EvictArgs a, uint8_t *scratch);
 
+// Pages and slots of the coming tokens (lt_paged_plan.cu).
+struct PagedPlanArgs {
+    uint32_t n_seq, page, n_pages, max_pages, total_q;
+    const uint32_t *keep, *add;     // keep: nullptr, all stay
+    uint32_t *lens, *table, *free, *n_free, *cu, *seq, *pos, *slot;
+    // scratch, set by the launcher: {stack top before taking, pages taken, tokens}; [n_seq] each
+    uint32_t *head, *take, *gone, *stay, *have;
+    int *err;
+};
+size_t paged_plan_scratch(const PagedPlanArgs &a);
+cudaError_t launch_paged_plan(const LaunchCfg &c, PagedPlanArgs a, uint8_t *scratch);
+
 // Rules on logits (lt_logits.cu).  The rule struct is lt_logit_rule.
 struct LogitArgs {
     const float *logits;

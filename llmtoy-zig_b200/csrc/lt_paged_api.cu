@@ -229,6 +229,45 @@ lt_status lt_kv_evict(lt_ctx *ctx, const lt_paged_kv *kv, uint32_t n_seq, const 
     return st_of(lt::ctx_launched(ctx, lt::launch_evict(lt::ctx_cfg(ctx), a, scratch), "evict"));
 }
 
+lt_status lt_paged_plan(lt_ctx *ctx, const lt_paged_state *state, const uint32_t *dev_keep, const uint32_t *dev_new,
+                        uint32_t total_q, uint32_t *dev_cu_q, uint32_t *dev_seq, uint32_t *dev_pos,
+                        uint32_t *dev_pool_slot) {
+    lt_status st = st_of(lt::ctx_enter(ctx));
+    if (st != LT_OK) return st;
+    if (!state || !state->dev_lens || !state->dev_page_table || !state->dev_free || !state->dev_n_free || !dev_new || !dev_cu_q)
+        return st_of(ctx_fail(ctx, LT_EINVAL, "lt_paged_plan: null argument"));
+    if (state->page_size == 0 || state->n_pages == 0 || state->max_pages == 0)
+        return st_of(ctx_fail(ctx, LT_EINVAL, "lt_paged_plan: page_size %u, n_pages %u, max_pages %u", state->page_size,
+                              state->n_pages, state->max_pages));
+    if ((uint64_t)state->n_pages * state->page_size > 0xffffffffull)
+        return st_of(ctx_fail(ctx, LT_EINVAL, "lt_paged_plan: %u pages of %u slots (fewer than 2^32 slots)", state->n_pages,
+                              state->page_size));
+    if (state->n_seq > 65535 || total_q > kMaxLen)
+        return st_of(ctx_fail(ctx, LT_EINVAL, "lt_paged_plan: %u sequences (at most 65535), %u tokens (at most %u)",
+                              state->n_seq, total_q, kMaxLen));
+    if (state->n_seq == 0) return LT_OK;
+    lt::PagedPlanArgs a = {};
+    a.n_seq = state->n_seq;
+    a.page = state->page_size;
+    a.n_pages = state->n_pages;
+    a.max_pages = state->max_pages;
+    a.total_q = total_q;
+    a.keep = dev_keep;
+    a.add = dev_new;
+    a.lens = state->dev_lens;
+    a.table = state->dev_page_table;
+    a.free = state->dev_free;
+    a.n_free = state->dev_n_free;
+    a.cu = dev_cu_q;
+    a.seq = dev_seq;
+    a.pos = dev_pos;
+    a.slot = dev_pool_slot;
+    uint8_t *scratch = nullptr;
+    const size_t need = lt::paged_plan_scratch(a);
+    if ((st = st_of(lt::ctx_scratch(ctx, need, need, &scratch))) != LT_OK) return st;
+    return st_of(lt::ctx_launched(ctx, lt::launch_paged_plan(lt::ctx_cfg(ctx), a, scratch), "page plan"));
+}
+
 lt_status lt_logits_process(lt_ctx *ctx, const float *dev_logits, uint32_t n, uint32_t n_rows,
                             const lt_logit_rule *dev_rules, const uint32_t *dev_history,
                             const uint32_t *dev_bias_ids, const float *dev_bias_values, const uint32_t *dev_masks,
