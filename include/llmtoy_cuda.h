@@ -634,6 +634,54 @@ lt_status lt_paged_attn_prompt(lt_ctx *ctx, const lt_paged_attn_cfg *cfg, const 
                                const uint32_t *dev_prefix, const uint32_t *dev_docs, uint64_t doc_stride,
                                float *dev_out);
 
+/* ── a paged cache in 8 bits ────────────────────────────────────────────────
+ * Half the bytes of an f16 cache.  `block` consecutive slots of a page share a
+ * scale per KV head, one for K and one for V: a value is its code, a signed byte,
+ * times its block's scale.  Tables, lengths and rules as for lt_paged_kv.  Codes may
+ * be anything anywhere; scales of blocks that hold visible positions must be finite
+ * and not negative, V's at most 2^60 (below 2^-60 they count as 2^-60), else the rows that
+ * see the block are NaN. */
+typedef struct lt_paged_q8 {
+    uint32_t n_kv_heads, head_dim;  /* head_dim 64, 128 or 256 */
+    uint32_t page_size;             /* slots per page, a multiple of block */
+    uint32_t block;                 /* slots that share a scale: 16, 32, 64 or 128 */
+    uint32_t n_pages, max_pages;
+    /* Bytes between pages, slots and KV heads of the codes; each row of head_dim
+     * bytes is contiguous.  All 0: [page][head][slot][head_dim], so that what an
+     * attention head reads of a page is contiguous.  Multiples of 16, as the addresses. */
+    uint64_t page_stride, slot_stride, head_stride;
+    void *dev_k, *dev_v;
+    float *dev_k_scale, *dev_v_scale;  /* [page][head][page_size / block] */
+} lt_paged_q8;
+
+/* lt_paged_append into an 8-bit cache, for whole sequences' ends: rows dev_cu_q[s]
+ * .. dev_cu_q[s + 1] - 1 of dev_qkv (and dev_q) are the last positions of sequence
+ * s, which holds dev_lens[s] with them; at most max_q rows per sequence, total_q in
+ * all (as lt_paged_attn_prompt).  The queries and keys are rotated to dev_pos[row]
+ * (NULL: the position in the sequence).  Angles keep their f32 precision at any position
+ * (lt_paged_append rounds them as the reference does).
+ *
+ * A block whose first slot is written starts afresh, on scale = max |x| / 127.  In
+ * others the codes before the new rows stay; where the new rows need a larger scale they
+ * are rounded to it again.  code = x / scale to nearest.  A value that is not finite or
+ * exceeds 2^60 makes its block's scale NaN, until the block starts afresh.
+ * Pages written to must not be shared.  Repeating a call changes nothing. */
+lt_status lt_paged_q8_append(lt_ctx *ctx, const lt_attn_cfg *cfg, const lt_paged_q8 *kv, const float *dev_qkv,
+                             uint32_t n_seq, const uint32_t *dev_cu_q, uint32_t total_q, uint32_t max_q,
+                             const float *dev_q_norm, const float *dev_k_norm, const uint32_t *dev_pos,
+                             const uint32_t *dev_page_table, const uint32_t *dev_lens, float *dev_q);
+
+/* lt_paged_attn_decode (without weights accumulated) and lt_paged_attn_prompt over
+ * an 8-bit cache. */
+lt_status lt_paged_q8_attn_decode(lt_ctx *ctx, const lt_paged_attn_cfg *cfg, const lt_paged_q8 *kv, const float *dev_q,
+                                  uint32_t n_seq, const uint32_t *dev_page_table, const uint32_t *dev_lens,
+                                  uint32_t max_len, float *dev_out);
+lt_status lt_paged_q8_attn_prompt(lt_ctx *ctx, const lt_paged_attn_cfg *cfg, const lt_paged_q8 *kv, const float *dev_q,
+                                  uint32_t n_seq, const uint32_t *dev_cu_q, uint32_t total_q, uint32_t max_q,
+                                  const uint32_t *dev_page_table, const uint32_t *dev_lens, uint32_t max_len,
+                                  const uint32_t *dev_prefix, const uint32_t *dev_docs, uint64_t doc_stride,
+                                  float *dev_out);
+
 /* Eviction by accumulated attention weight.  A sequence of more than budget
  * positions keeps, per KV head, its newest `recent` and of the others the
  * budget - recent with the largest dev_mass (the lowest position first among

@@ -44,7 +44,8 @@ EXPORTS = [
     "lt_qmatvec_multi", "lt_noalloc_status", "lt_selftest_wait",
     "lt_stack_create", "lt_stack_run", "lt_stack_free", "lt_ep_unique_id", "lt_ep_init", "lt_ep_free",
     "lt_moe_ffn_ep", "lt_paged_append", "lt_paged_attn_decode", "lt_paged_attn_prompt", "lt_kv_evict",
-    "lt_logits_process", "lt_paged_plan",
+    "lt_logits_process", "lt_paged_plan", "lt_paged_q8_append", "lt_paged_q8_attn_decode",
+    "lt_paged_q8_attn_prompt",
 ]
 
 
@@ -87,6 +88,15 @@ class PagedAttnCfg(ctypes.Structure):
     _fields_ = [("n_heads", ctypes.c_uint32), ("window", ctypes.c_uint32), ("causal", ctypes.c_uint32),
                 ("scale", ctypes.c_float), ("softcap", ctypes.c_float), ("slopes", ctypes.c_void_p),
                 ("q_stride", ctypes.c_uint64), ("out_stride", ctypes.c_uint64)]
+
+
+class PagedQ8(ctypes.Structure):
+    """lt_paged_q8: one layer's pool of cache pages in 8-bit codes with a scale for each block of slots and KV head
+    (strides in bytes, all 0: [page][head][slot][head_dim]; scales [page][head][page_size / block])."""
+    _fields_ = [("n_kv_heads", ctypes.c_uint32), ("head_dim", ctypes.c_uint32), ("page_size", ctypes.c_uint32),
+                ("block", ctypes.c_uint32), ("n_pages", ctypes.c_uint32), ("max_pages", ctypes.c_uint32),
+                ("page_stride", ctypes.c_uint64), ("slot_stride", ctypes.c_uint64), ("head_stride", ctypes.c_uint64),
+                ("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p)]
 
 
 class PagedState(ctypes.Structure):
@@ -206,6 +216,10 @@ def load_library() -> ctypes.CDLL:
                                      P]),
         "lt_paged_attn_prompt": (I, [P, ctypes.POINTER(PagedAttnCfg), ctypes.POINTER(PagedKV), P, U32, P, U32, U32, P, P,
                                      U32, P, P, U64, P]),
+        "lt_paged_q8_append": (I, [P, ctypes.POINTER(AttnCfg), ctypes.POINTER(PagedQ8), P, U32, P, U32, U32, P, P, P, P, P, P]),
+        "lt_paged_q8_attn_decode": (I, [P, ctypes.POINTER(PagedAttnCfg), ctypes.POINTER(PagedQ8), P, U32, P, P, U32, P]),
+        "lt_paged_q8_attn_prompt": (I, [P, ctypes.POINTER(PagedAttnCfg), ctypes.POINTER(PagedQ8), P, U32, P, U32, U32, P, P,
+                                        U32, P, P, U64, P]),
         "lt_paged_plan": (I, [P, ctypes.POINTER(PagedState), P, P, U32, P, P, P, P]),
         "lt_kv_evict": (I, [P, ctypes.POINTER(PagedKV), U32, P, P, U32, P, U64, U32, U32, P, P, P, U64, P]),
         "lt_logits_process": (I, [P, P, U32, U32, P, P, P, P, P, P]),
@@ -539,6 +553,26 @@ class Context:
         self._check(self.lib.lt_kv_evict(self.ptr, ctypes.byref(kv), n_seq, _ptr(page_table), _ptr(lens), max_len,
                                          _ptr(mass), mass_stride, budget, recent, _ptr(dst_table), _ptr(lens_out),
                                          _ptr(mass_out), mass_out_stride, _ptr(kept)))
+
+    def paged_q8_append(self, cfg: AttnCfg, kv: PagedQ8, qkv, n_seq: int, cu_q, total_q: int, max_q: int, q_norm, k_norm, pos,
+                        page_table, lens, q) -> None:
+        """Rows cu_q[s] .. cu_q[s + 1] - 1 of qkv are the last of the lens[s] positions of sequence s: rotated queries (to
+        pos, None: the position in the sequence) to q, K and V as codes into the cache."""
+        self._check(self.lib.lt_paged_q8_append(self.ptr, ctypes.byref(cfg), ctypes.byref(kv), _ptr(qkv), n_seq, _ptr(cu_q),
+                                                total_q, max_q, _ptr(q_norm), _ptr(k_norm), _ptr(pos), _ptr(page_table),
+                                                _ptr(lens), _ptr(q)))
+
+    def paged_q8_attn_decode(self, cfg: PagedAttnCfg, kv: PagedQ8, q, n_seq: int, page_table, lens, max_len: int, out) -> None:
+        """One query per sequence over an 8-bit cache."""
+        self._check(self.lib.lt_paged_q8_attn_decode(self.ptr, ctypes.byref(cfg), ctypes.byref(kv), _ptr(q), n_seq,
+                                                     _ptr(page_table), _ptr(lens), max_len, _ptr(out)))
+
+    def paged_q8_attn_prompt(self, cfg: PagedAttnCfg, kv: PagedQ8, q, n_seq: int, cu_q, total_q: int, max_q: int, page_table,
+                             lens, max_len: int, out, prefix=None, docs=None, doc_stride: int = 0) -> None:
+        """Rows cu_q[s] .. cu_q[s + 1] - 1 of q are the last positions of sequence s, over an 8-bit cache."""
+        self._check(self.lib.lt_paged_q8_attn_prompt(self.ptr, ctypes.byref(cfg), ctypes.byref(kv), _ptr(q), n_seq,
+                                                     _ptr(cu_q), total_q, max_q, _ptr(page_table), _ptr(lens), max_len,
+                                                     _ptr(prefix), _ptr(docs), doc_stride, _ptr(out)))
 
     def paged_plan(self, state: PagedState, keep, new, total_q: int, cu_q, seq=None, pos=None, pool_slot=None) -> None:
         """Give back the pages behind keep[s] positions (None: all stay), take those that new[s] more need; cu_q[n_seq + 1]

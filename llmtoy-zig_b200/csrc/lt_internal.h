@@ -146,6 +146,9 @@ struct PagedKvDev {
     uint32_t n_kv, hd, f16;
     uint32_t page_size, n_pages, max_pages;
     uint32_t page_shift;  // log2 of page_size, or kNoShift
+    // 8-bit codes (k_scale != nullptr): scales [page][KV head][blocks of the page], 2^block_shift slots to a block
+    float *k_scale, *v_scale;
+    uint32_t block_shift, page_blocks;
 };
 constexpr uint32_t kNoShift = 0xffffffffu;
 
@@ -208,6 +211,24 @@ struct EvictArgs {
 };
 size_t evict_scratch(const EvictArgs &a, bool have_kept);
 cudaError_t launch_evict(const LaunchCfg &c, EvictArgs a, uint8_t *scratch);
+
+// The same into a cache of 8-bit codes (lt_paged_q8_append.cu): rows cu[s] .. cu[s + 1] - 1 are the last of the
+// lens[s] positions of sequence s.
+struct PagedQ8AppendArgs {
+    PagedKvDev kv;
+    uint32_t n_heads, rope_neox, v_norm, n_seq, total_q, max_q;
+    double log2_theta;
+    float eps;
+    const float *qkv, *q_norm, *k_norm;
+    const uint32_t *cu, *pos, *table, *lens;
+    float *q;
+    uint32_t heads_per_cta;  // head vectors per CTA, set by the launcher
+    int *err;
+};
+cudaError_t launch_paged_q8_append(const LaunchCfg &c, PagedQ8AppendArgs a);
+// Attention over a cache of 8-bit codes (lt_paged_q8_attn.cu), queries as in launch_paged_attn.
+size_t paged_q8_attn_scratch(const PagedAttnArgs &a, int num_sms);
+cudaError_t launch_paged_q8_attn(const LaunchCfg &c, PagedAttnArgs a, uint8_t *scratch);
 
 // Pages and slots of the coming tokens (lt_paged_plan.cu).
 struct PagedPlanArgs {

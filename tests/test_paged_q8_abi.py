@@ -11,7 +11,8 @@ import pytest
 REPO = Path(__file__).resolve().parent.parent
 
 STRUCTS = {"PagedState": ("lt_paged_state", {"lens": "dev_lens", "page_table": "dev_page_table", "free": "dev_free",
-                                             "n_free": "dev_n_free"})}
+                                             "n_free": "dev_n_free"}),
+           "PagedQ8": ("lt_paged_q8", {"k": "dev_k", "v": "dev_v", "k_scale": "dev_k_scale", "v_scale": "dev_v_scale"})}
 
 
 def test_structures_match_the_header(pkg, tmp_path):
@@ -33,7 +34,8 @@ def test_structures_match_the_header(pkg, tmp_path):
             assert int(got[f"{py}.{f}"]) == getattr(t, f).offset, (py, f)
 
 
-@pytest.mark.parametrize("name", ["lt_paged_plan"])
+@pytest.mark.parametrize("name", ["lt_paged_plan", "lt_paged_q8_append", "lt_paged_q8_attn_decode",
+                                  "lt_paged_q8_attn_prompt"])
 def test_no_context_is_refused(pkg, name):
     fn = getattr(pkg.load_library(), name)
     args = [None if a is ctypes.c_void_p or hasattr(a, "contents") or issubclass(a, ctypes._Pointer) else 0 for a in fn.argtypes]
