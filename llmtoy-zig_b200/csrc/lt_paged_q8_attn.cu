@@ -1,118 +1,592 @@
-// lt_paged_q8_attn.cu — attention over a paged cache of 8-bit codes.
+// lt_paged_q8_attn.cu — attention over a paged cache of 8-bit codes: one new token
+// per sequence, and a few.
 //
 // The formulas are lt_paged_attn.cu's, with the blocks' scales as lt_paged_q8.cuh puts
-// them.  One warp per query row and head: it goes through the keys with the running
-// maximum m and sum l, lane i on dims i hd / 32 on.
+// them, in one pass over the keys with the running maximum m and sum l.
+//
+// Bound: memory (K and V are read once per 8 query heads of a KV head); the work is
+// shared as lt_paged_walk.cuh says.
+// - Each warp owns KB keys of a tile and a ring of kStages such pieces in shared memory,
+//   filled by 16-byte asynchronous copies, with the pieces' scales beside them.  Rows of
+//   codes lie one behind the other, their 16-byte columns permuted so that neither matrix
+//   load meets a bank conflict.
+// - Scores are exact: a query row becomes 32-bit integers (a power of two times the row,
+//   its largest element in [2^29, 2^30)), those four signed 8-bit digits, in rows r and r + 8 of two
+//   operands of the integer tensor-core product with K's codes as they lie in memory.
+// - Weights go in as two f16 terms (22 bits) in rows r and r + 8, against V's codes in
+//   f16, where they are exact: a transposing 8-bit matrix load gives 4 keys of a dimension,
+//   and a byte b next to 0x64 is the f16 number 1024 + b.
+// - Keys are dealt to the columns of the score product so that a thread's scores are
+//   those of 4 consecutive keys, as its weights have to be for the second product.
 #include "lt_paged_q8.cuh"
+#include "lt_paged_walk.cuh"
 
 namespace lt {
 
-constexpr int kQrWarps = 4;
+template <int HD>
+struct Q8Shape {
+    static constexpr int KB = HD == 256 ? 16 : 32;          // keys per warp and tile
+    static constexpr int NG = KB / 16;                      // groups of 16, each within a block and a page
+    static constexpr int TILE = KB * kPaWarps;
+    static constexpr int STAGES = 3;
+    static constexpr int HALF = KB * HD;                    // bytes of K's codes, and of V's
+    static constexpr int PIECE = 2 * HALF;
+    static constexpr int RING = PIECE * STAGES * kPaWarps;
+    static constexpr int SCALES = NG * 8;                   // bytes per piece: K and V scale of each group
+    static constexpr int QSTEPS = HD / 32;
+    static constexpr int QBYTES = QSTEPS * 1024;
+    static constexpr int RECS = HD == 256 ? 1 : 2;          // merge records at a time
+    static constexpr int MERGE = RECS * kPaRows * (HD + 2) * 4;
+    static constexpr int UNION = QBYTES > MERGE ? QBYTES : MERGE;
+    static constexpr int OFF_SCALES = RING + UNION;
+    static constexpr int OFF_ROWF = OFF_SCALES + SCALES * STAGES * kPaWarps;
+    static constexpr int SMEM = OFF_ROWF + kPaRows * 4;
+    static constexpr int CTAS = HD == 64 ? 4 : 2;
+};
 
-template <int N>
-LT_DEVINL void q8_ld_row(const uint8_t *p, float (&v)[N]) {
-#pragma unroll
-    for (int e = 0; e < N; e++) v[e] = (float)(int8_t)p[e];
+// Place of 16-byte column c of row r of a piece.  Eight rows of a matrix load are 0-7 or 8-15 (V), or the 8
+// of 16 whose second bit is alike (K, see key_of): the column's permutation differs among the rows of each.
+template <int HD>
+LT_DEVINL uint32_t q8_at(uint32_t r, uint32_t c) {
+    const uint32_t b = ((r >> 1) ^ (r >> 3)) & 1;
+    const uint32_t f = HD == 64 ? (r & 4) >> 1 | b : (r & 4) | (r & 1) << 1 | b;
+    return r * HD + ((c ^ f) << 4);
 }
 
-template <int HD>
-__global__ void __launch_bounds__(kQrWarps * 32) k_paged_q8_rows(const __grid_constant__ PagedAttnArgs a, uint64_t rows) {
-    constexpr int N = HD / 32, U = 4;
+// C[16x8] += A[16x32] B[32x8], signed bytes, exact.
+LT_DEVINL void mma_s8(int (&c)[4], const uint4 &a, uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+        : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+}
+// Two 16x16 matrices of bytes, transposed: lanes 0-15 give the first's rows, 16-31 the second's.
+// Register i: bytes 4 (lane % 4) .. + 3 of column lane / 4 + 8 (i % 2) of matrix i / 2.
+LT_DEVINL void ldsm_t8(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m16n16.x2.trans.shared.b8 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+// Four signed bytes as f16.
+LT_DEVINL void s8_to_f16(uint32_t w, uint32_t &b0, uint32_t &b1) {
+    const uint32_t x = w ^ 0x80808080u;
+    const uint32_t p = __byte_perm(x, 0x64646464u, 0x4140), q = __byte_perm(x, 0x64646464u, 0x4342);
+    const __half2 off = __float2half2_rn(1152.0f);
+    const __half2 u = __hsub2(*reinterpret_cast<const __half2 *>(&p), off), v = __hsub2(*reinterpret_cast<const __half2 *>(&q), off);
+    b0 = *reinterpret_cast<const uint32_t *>(&u);
+    b1 = *reinterpret_cast<const uint32_t *>(&v);
+}
+LT_DEVINL void cp_async4(uint32_t dst, const void *src, bool take) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(take ? 4 : 0) : "memory");
+}
+LT_DEVINL uint4 lds_u4(uint32_t addr) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+    return v;
+}
+
+// PLAIN: neither cap nor distance bias.
+template <int HD, bool PROMPT, bool PLAIN>
+__global__ void __launch_bounds__(kPaThreads, Q8Shape<HD>::CTAS) k_paged_q8(const __grid_constant__ PagedAttnArgs a) {
+    using S = Q8Shape<HD>;
+    constexpr int KB = S::KB, NG = S::NG, TILE = S::TILE, NB = HD / 8;
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ uint64_t s_scan[kPaWarps];
+    __shared__ uint64_t s_rem;
+    __shared__ uint32_t s_seq;
+    __shared__ PaSeq s_q;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, j4 = lane & 3;
+    uint8_t *qm = smem + S::RING;  // query fragments, then the merge records
+    float *rowf = reinterpret_cast<float *>(smem + S::OFF_ROWF);
+    const uint32_t ring_u = smem_u32(smem) + warp * (S::PIECE * S::STAGES), qm_u = smem_u32(qm);
+    const uint32_t scale_u = smem_u32(smem) + S::OFF_SCALES + warp * (S::SCALES * S::STAGES);
+    const uint32_t c = blockIdx.x;
     pdl_launch_dependents();
     pdl_wait();
-    const uint64_t r = (uint64_t)blockIdx.x * kQrWarps + threadIdx.x / 32;
-    if (r >= rows) return;
-    const uint32_t lane = threadIdx.x & 31, head = (uint32_t)(r % a.n_heads), kh = head / a.group;
-    const uint64_t rest = r / a.n_heads;
-    const uint32_t s = (uint32_t)(rest / a.max_q), t = (uint32_t)(rest % a.max_q);
-    const uint32_t cap = (uint32_t)min((uint64_t)a.kv.max_pages * a.kv.page_size, (uint64_t)a.max_len);
-    const uint32_t given = a.lens[s], len = min(given, cap);
-    uint32_t q0 = s, nq = 1;
-    bool bad = given > cap;
-    if (a.cu) {
-        const uint32_t c0 = a.cu[s], c1 = a.cu[s + 1];
-        const bool ok = c0 <= c1 && c1 <= a.total_q && c1 - c0 <= a.max_q;
-        bad |= !ok;
-        q0 = c0;
-        nq = ok ? c1 - c0 : 0;
+
+    // the tiles of all sequences, and where this CTA's share begins
+    const uint32_t per = (a.n_seq + kPaThreads - 1) / kPaThreads;
+    const uint32_t sa = min(a.n_seq, tid * per), sb = min(a.n_seq, sa + per);
+    uint64_t mine = 0;
+#pragma unroll 4
+    for (uint32_t s = sa; s < sb; s++) {
+        const PaSeq q = pa_seq<PROMPT>(a, s, TILE, c == 0);
+        mine += (uint64_t)q.blocks * a.kv.n_kv * q.cost();
     }
-    if (bad && lane == 0 && t == 0) atomicExch(a.err, DEV_ERR_BAD_INDEX);
-    if (t >= nq) return;
-    const uint32_t row = q0 + t, *table = a.table + (uint64_t)s * a.kv.max_pages;
-    const uint32_t *docs = a.docs ? a.docs + (uint64_t)s * a.doc_stride : nullptr;
-    const int64_t i = (int64_t)len - nq + t;
-    int64_t lo = 0, hi = len;
-    if (a.window) lo = max((int64_t)0, i - (int64_t)a.window + 1);
-    if (a.cu && a.causal) hi = min(hi, max(i + 1, a.prefix ? (int64_t)a.prefix[s] : (int64_t)0));
-    if (docs && i < 0) hi = 0;
-    const float slope = a.slopes ? a.slopes[head] : 0.0f;
-    const float f = a.softcap != 0.0f ? a.scale / a.softcap : a.scale * 1.4426950408889634f;
-    const float *q = a.q + (uint64_t)row * a.q_stride + (uint64_t)head * HD + lane * N;
-    float x[N], o[N], m = -INFINITY, l = 0.0f;
+    uint64_t incl = mine;
 #pragma unroll
-    for (int e = 0; e < N; e++) {
-        x[e] = q[e];
-        o[e] = 0.0f;
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint64_t y = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += y;
     }
-    for (int64_t j0 = lo; j0 < hi; j0 += U) {
-        uint32_t page[U];
-        bool seen[U];
-        float dot[U];
+    if (lane == 31) s_scan[warp] = incl;
+    __syncthreads();
+    uint64_t T = 0, before = incl - mine;
 #pragma unroll
-        for (int u = 0; u < U; u++) {  // alike in all lanes
-            const int64_t j = j0 + u;
-            seen[u] = j < hi && (!docs || docs[j] == docs[i]);
-            page[u] = seen[u] ? table[page_of(a.kv, (uint32_t)j)] : 0;
-            if (page[u] >= a.kv.n_pages) {
-                if (lane == 0) atomicExch(a.err, DEV_ERR_BAD_INDEX);
-                seen[u] = false;
+    for (int w = 0; w < kPaWarps; w++) {
+        if (w < warp) before += s_scan[w];
+        T += s_scan[w];
+    }
+    // no more CTAs than tiles, so that every CTA of a unit leaves a record
+    const uint32_t G = (uint32_t)min((uint64_t)gridDim.x, T);
+    if (c >= G) return;
+    const PaShare share(T, G);
+    uint64_t f0 = share.start(c);
+    const uint64_t f1 = share.start(c + 1);
+    if (f0 >= before && f0 < before + mine) {
+        uint64_t rem = f0 - before;
+        for (uint32_t s = sa; s < sb; s++) {
+            const PaSeq q = pa_seq<PROMPT>(a, s, TILE, false);
+            const uint64_t w = (uint64_t)q.blocks * a.kv.n_kv * q.cost();
+            if (rem < w) {
+                s_seq = s;
+                s_rem = rem;
+                s_q = q;
+                break;
             }
-            dot[u] = 0.0f;
-            if (seen[u]) {
-                float k[N];
-                q8_ld_row(a.kv.k + paged_offset(a.kv, page[u], (uint32_t)j, kh) + lane * N, k);
+            rem -= w;
+        }
+    }
+    __syncthreads();
+    PaWalk<PROMPT> cw, lw;  // the compute walk and the copies ahead of it
+    cw.s = s_seq;
+    cw.q = s_q;
+    cw.unit = (uint32_t)div_small(s_rem, cw.q.cost());
+    cw.tile = (uint32_t)(s_rem - (uint64_t)cw.unit * cw.q.cost());
+    if (cw.tile >= cw.q.tiles) {  // in what the unit before costs beyond its tiles
+        f0 += cw.q.cost() - cw.tile;
+        if (f0 >= f1) return;
+        cw.template next_unit<TILE>(a);
+    } else {
+        cw.set_unit(a);
+    }
+    lw = cw;
+    uint64_t lf = f0;  // lw's place in the count
+
+    // a unit's queries: warp w takes rows 2 w and 2 w + 1, a lane 4 consecutive elements of each 128
+    constexpr int QV = HD == 256 ? 2 : 1;
+    float4 qv[2][QV];
+    auto load_q = [&]() {
+        const uint32_t rows = min((uint32_t)kPaRows, cw.q.nq * a.group - cw.rb * kPaRows);
 #pragma unroll
-                for (int e = 0; e < N; e++) dot[u] = fmaf(x[e], k[e], dot[u]);
+        for (int rr = 0; rr < 2; rr++) {
+            const uint32_t r = warp * 2 + rr, R = cw.rb * kPaRows + r;
+            const float *src = a.q + (uint64_t)(cw.q.q0 + R / a.group) * a.q_stride + (uint64_t)(cw.kh * a.group + R % a.group) * HD;
+#pragma unroll
+            for (int e = 0; e < QV; e++)
+                qv[rr][e] = r < rows && (HD != 64 || lane < 16) ? *reinterpret_cast<const float4 *>(src + 128 * e + 4 * lane)
+                                                              : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        }
+    };
+    load_q();
+
+    // The piece to copy next: a page for each of its groups.  Whole groups are copied, what lies outside the
+    // unit's positions too (codes may be anything, scores there are masked); groups wholly outside are not.
+    constexpr int CH = HD / 16, STEP = 32 / CH;  // columns of a row, rows per copy instruction
+    const uint32_t row0 = lane / CH, col0 = lane % CH;
+    struct Job {
+        uint32_t page[NG], key, kh;
+        bool there;
+    };
+    auto look = [&]() {
+        Job j;
+        j.there = true;
+        j.key = lw.base + lw.tile * TILE + warp * KB;
+        j.kh = lw.kh;
+#pragma unroll
+        for (int n = 0; n < NG; n++) {
+            const uint32_t key = j.key + 16 * n;
+            j.page[n] = 0xffffffffu;
+            if (key < lw.hi && key + 16 > lw.lo) {
+                const uint32_t page = a.table[(uint64_t)lw.s * a.kv.max_pages + page_of(a.kv, key)];
+                if (page < a.kv.n_pages)
+                    j.page[n] = page;
+                else
+                    atomicExch(a.err, DEV_ERR_BAD_INDEX);
             }
         }
+        return j;
+    };
+    auto copy = [&](const Job &j, int stage) {
+        const uint32_t dst = ring_u + stage * S::PIECE;
 #pragma unroll
-        for (int w = 16; w > 0; w >>= 1) {
+        for (int n = 0; n < NG; n++) {
+            const bool take = j.page[n] != 0xffffffffu;
+            const uint32_t key = j.key + 16 * n;
+            const uint64_t o = take ? paged_offset(a.kv, j.page[n], key, j.kh) + row0 * a.kv.slot_stride + col0 * 16 : 0;
+            const uint8_t *pk = a.kv.k + o, *pv = a.kv.v + o;
 #pragma unroll
-            for (int u = 0; u < U; u++) dot[u] += __shfl_xor_sync(0xffffffffu, dot[u], w);
+            for (int r = 0; r < 16; r += STEP) {
+                const uint32_t at = dst + n * 16 * HD + q8_at<HD>(r + row0, col0);
+                cp_async16(at, pk, take);
+                cp_async16(at + S::HALF, pv, take);
+                pk += STEP * a.kv.slot_stride;
+                pv += STEP * a.kv.slot_stride;
+            }
+            if (lane < 2) {
+                const float *sc = (lane ? a.kv.v_scale : a.kv.k_scale) + (take ? q8_scale_at(a.kv, j.page[n], key, j.kh) : 0);
+                cp_async4(scale_u + stage * S::SCALES + n * 8 + lane * 4, sc, take);
+            }
         }
+    };
+    // all pages of the first pieces are looked up before the first copy waits for its own
+    Job jobs[S::STAGES];
+    auto look_next = [&](Job &j) {
+        j.there = lf < f1;
+        if (!j.there) return;
+        j = look();
+        if (++lw.tile < lw.q.tiles) {
+            lf++;
+        } else {
+            lf += 1 + kUnitCost;
+            if (lf < f1) lw.template next_unit<TILE>(a);
+        }
+    };
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            if (!seen[u]) continue;
-            const uint32_t j = (uint32_t)(j0 + u);
-            const uint64_t at = q8_scale_at(a.kv, page[u], j, kh);
-            const Q8Scale sc = q8_scale(a.kv.k_scale[at], a.kv.v_scale[at]);
-            float v[N];
-            q8_ld_row(a.kv.v + paged_offset(a.kv, page[u], j, kh) + lane * N, v);
-            const float y = score_log2(dot[u] * sc.k, f, a.softcap, slope, fabsf((float)(i - (int64_t)j))) + sc.v_log2;
-            const float mn = fmaxf(m, y), base = mn == -INFINITY ? 0.0f : mn;
-            const float al = ex2(m - base), p = ex2(y - base);
+    for (int st = 0; st < S::STAGES; st++) look_next(jobs[st]);
+#pragma unroll
+    for (int st = 0; st < S::STAGES - 1; st++) {
+        if (jobs[st].there) copy(jobs[st], st);
+        cp_async_commit();
+    }
+    Job job = jobs[S::STAGES - 1];
+
+    uint64_t f = f0;
+    int stage = 0;
+    while (f < f1) {
+        // ── one segment: this CTA's tiles of one unit ──
+        const uint32_t seg = (uint32_t)min((uint64_t)(cw.q.tiles - cw.tile), f1 - f);
+        const uint64_t unit_f0 = f - cw.tile;
+        const uint32_t rows = min((uint32_t)kPaRows, cw.q.nq * a.group - cw.rb * kPaRows);
+        // queries to digits
+#pragma unroll
+        for (int rr = 0; rr < 2; rr++) {
+            const uint32_t r = warp * 2 + rr;
+            uint32_t top = 0;  // bits: NaN above infinity above every number
+#pragma unroll
+            for (int e = 0; e < QV; e++) {
+                const float4 &v = qv[rr][e];
+                top = max(max(top, max(__float_as_uint(v.x) & 0x7fffffffu, __float_as_uint(v.y) & 0x7fffffffu)),
+                          max(__float_as_uint(v.z) & 0x7fffffffu, __float_as_uint(v.w) & 0x7fffffffu));
+            }
+            top = __reduce_max_sync(0xffffffffu, top);
+            const int ex = min(max(29 - (int)(top >> 23) + 127, -126), 126);
+            const float up = __uint_as_float((uint32_t)(ex + 127) << 23);
+            const float f1 = a.softcap != 0.0f ? a.scale / a.softcap : a.scale * 1.4426950408889634f;
+            if (lane == 0) rowf[r] = top < 0x7f800000u ? f1 / up : __int_as_float(0x7fffffff);
+#pragma unroll
+            for (int e = 0; e < QV; e++) {
+                const float4 &v = qv[rr][e];
+                uint32_t d[4];
+                const float x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int i = 0; i < 4; i++) d[i] = ((uint32_t)__float2int_rn(x[i] * up) + 0x00808080u) ^ 0x00808080u;
+                // digit p of four elements to a register
+                const uint32_t l01 = __byte_perm(d[0], d[1], 0x5140), l23 = __byte_perm(d[2], d[3], 0x5140);
+                const uint32_t h01 = __byte_perm(d[0], d[1], 0x7362), h23 = __byte_perm(d[2], d[3], 0x7362);
+                const uint32_t p0 = __byte_perm(l01, l23, 0x5410), p1 = __byte_perm(l01, l23, 0x7632);
+                const uint32_t p2 = __byte_perm(h01, h23, 0x5410), p3 = __byte_perm(h01, h23, 0x7632);
+                const uint32_t k = 128 * e + 4 * lane;  // element: step k / 32, its half (k / 16) % 2, column (k / 4) % 4
+                if (HD != 64 || lane < 16) {
+                    uint8_t *at = qm + (k / 32) * 1024 + (r * 4 + (k / 4) % 4) * 16 + (k / 16) % 2 * 8;
+                    *reinterpret_cast<uint2 *>(at) = make_uint2(p3, p2);
+                    *reinterpret_cast<uint2 *>(at + 512) = make_uint2(p1, p0);
+                }
+            }
+        }
+        __syncthreads();
+        // this thread's row g: factor, bias slope, what it sees
+        const uint32_t R = cw.rb * kPaRows + g;
+        const float rf = rowf[g];
+        const uint32_t head = cw.kh * a.group + R % a.group;
+        const float slope = a.slopes && (uint32_t)g < rows ? a.slopes[head] : 0.0f;
+        // positions are 32 bits wide here, and so are their differences: a length is at most 2^30, and a query that
+        // far before position 0 is clamped
+        const int row_i = (int)max((int64_t)cw.q.len - cw.q.nq + R / a.group, -((int64_t)1 << 30));
+        int row_lo = cw.q.lo, row_hi = cw.q.len;
+        uint32_t my_doc = 0;
+        const uint32_t *docs = nullptr;
+        if (PROMPT) {
+            if (a.causal) {
+                row_hi = min(row_i + 1, (int)cw.q.len);
+                if (a.prefix) row_hi = max(row_hi, (int)min(a.prefix[cw.s], cw.q.len));
+            }
+            row_lo = a.window ? (int)max((int64_t)0, (int64_t)row_i - a.window + 1) : 0;
+            if (a.docs) {
+                docs = a.docs + (uint64_t)cw.s * a.doc_stride;
+                if ((uint32_t)g < rows && row_i >= 0)
+                    my_doc = docs[row_i];
+                else
+                    row_hi = 0;
+            }
+        }
+        // Sums in registers; each piece's product is computed from zero and added here: the tensor core
+        // truncates where it accumulates.
+        float2 o[NB];
+#pragma unroll
+        for (int n = 0; n < NB; n++) o[n] = make_float2(0.0f, 0.0f);
+        float m = -INFINITY, l = 0.0f;
+
+        for (uint32_t it = 0; it < seg; it++) {
+            cp_async_wait<S::STAGES - 2>();
+            __syncwarp();
+            const uint32_t k0 = cw.base + cw.tile * TILE + warp * KB;  // the piece's first position
+            if (k0 < cw.hi && k0 + KB > cw.lo) {
+                const uint32_t kb = ring_u + stage * S::PIECE, vb = kb + S::HALF;
+                float sc[4 * NG];  // positions k0 + 16 (i / 4) + 4 j4 + i % 4
+                {
+                    int s0[2 * NG][4], s1[2 * NG][4];
+#pragma unroll
+                    for (int n = 0; n < 2 * NG; n++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) s0[n][e] = s1[n][e] = 0;
+                    // column x of product 2 n + h is key 16 n + 4 (x / 2) + 2 h + x % 2
+                    const uint32_t x = lane & 7, key = 4 * (x >> 1) + (x & 1) + 2 * (lane >> 4), half = (lane >> 3) & 1;
+#pragma unroll
+                    for (int i = 0; i < S::QSTEPS; i++) {
+                        const uint4 q0 = lds_u4(qm_u + i * 1024 + lane * 16), q1 = lds_u4(qm_u + i * 1024 + 512 + lane * 16);
+#pragma unroll
+                        for (int n = 0; n < NG; n++) {
+                            uint32_t b[4];
+                            ldsm4(b, kb + n * 16 * HD + q8_at<HD>(key, 2 * i + half));
+                            mma_s8(s0[2 * n], q0, b[0], b[1]);
+                            mma_s8(s1[2 * n], q1, b[0], b[1]);
+                            mma_s8(s0[2 * n + 1], q0, b[2], b[3]);
+                            mma_s8(s1[2 * n + 1], q1, b[2], b[3]);
+                        }
+                    }
+#pragma unroll
+                    for (int n = 0; n < 2 * NG; n++)
+#pragma unroll
+                        for (int e = 0; e < 2; e++)
+                            sc[4 * (n / 2) + 2 * (n % 2) + e] =
+                                fmaf((float)(s0[n][e] * 256 + s0[n][2 + e]), 65536.0f, (float)(s1[n][e] * 256 + s1[n][2 + e]));
+                }
+                float top = -INFINITY, v_inv[NG];
+                const bool whole = !PROMPT && k0 >= cw.lo && k0 + KB <= cw.hi;
+                const float dist = (float)(row_i - (int)(k0 + 4 * j4));
+#pragma unroll
+                for (int n = 0; n < NG; n++) {
+                    float ks, vs;
+                    asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(ks), "=f"(vs) : "r"(scale_u + stage * S::SCALES + n * 8) : "memory");
+                    const Q8Scale z = q8_scale(ks, vs);
+                    const float rk = rf * z.k;
+                    v_inv[n] = z.v_inv;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        float &t = sc[4 * n + e];
+                        const int j = (int)k0 + 16 * n + 4 * j4 + e;
+                        t = PLAIN ? fmaf(t, rk, z.v_log2)
+                                  : score_log2(t, rk, a.softcap, slope, fabsf(dist - (float)(16 * n + e))) + z.v_log2;
+                        if (PROMPT) {
+                            bool seen = j >= row_lo && j < row_hi;
+                            if (docs && seen) seen = docs[j] == my_doc;
+                            if (!seen) t = -INFINITY;
+                        } else if (!whole && (j < row_lo || j >= row_hi)) {
+                            t = -INFINITY;
+                        }
+                        top = fmaxf(top, t);
+                    }
+                }
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                const float mn = fmaxf(m, top);
+                const float al = mn > m ? ex2(m - mn) : 1.0f;  // m = -inf: 0
+                l *= al;
+                m = mn;
+                // weights scaled by 2^10 so that small ones keep their f16 bits; l carries the same factor
+                const float base = m == -INFINITY ? 0.0f : m - 10.0f;
+                uint32_t pa[NG][4];
+#pragma unroll
+                for (int n = 0; n < NG; n++) {
+                    float sum = 0.0f;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        sc[4 * n + e] = ex2(sc[4 * n + e] - base);
+                        sum += sc[4 * n + e];
+                    }
+                    l = fmaf(sum, v_inv[n], l);
+                    split_f16x2(sc[4 * n], sc[4 * n + 1], pa[n][0], pa[n][1]);
+                    split_f16x2(sc[4 * n + 2], sc[4 * n + 3], pa[n][2], pa[n][3]);
+                }
+                const float2 al2 = make_float2(al, al);
+#pragma unroll
+                for (int i = 0; i < HD / 32; i++) {
+                    float p[4][4] = {};  // dims 32 i + 8 x ..
+#pragma unroll
+                    for (int n = 0; n < NG; n++) {
+                        uint32_t w[4];
+                        ldsm_t8(w, vb + n * 16 * HD + q8_at<HD>(lane & 15, 2 * i + (lane >> 4)));
+#pragma unroll
+                        for (int x = 0; x < 4; x++) {
+                            uint32_t b0, b1;
+                            s8_to_f16(w[x], b0, b1);
+                            mma_f16(p[x], pa[n], b0, b1);
+                        }
+                    }
+#pragma unroll
+                    for (int x = 0; x < 4; x++)
+                        o[4 * i + x] = ffma2(o[4 * i + x], al2, fadd2(make_float2(p[x][0], p[x][1]), make_float2(p[x][2], p[x][3])));
+                }
+            }
+            __syncwarp();
+            int fill = stage + S::STAGES - 1;
+            if (fill >= S::STAGES) fill -= S::STAGES;
+            if (job.there) {
+                copy(job, fill);
+                look_next(job);
+            }
+            cp_async_commit();
+            if (++stage == S::STAGES) stage = 0;
+            if (it + 1 < seg) cw.tile++;
+        }
+
+        // ── merge the warps: the upper half into the lower, or one after the other into warp 0 ──
+        l += __shfl_xor_sync(0xffffffffu, l, 1);
+        l += __shfl_xor_sync(0xffffffffu, l, 2);
+        __syncthreads();  // every warp is done with the query fragments
+        auto give = [&](int rec) {
+            float *to = reinterpret_cast<float *>(qm) + (rec * kPaRows + g) * (HD + 2);
+#pragma unroll
+            for (int n = 0; n < NB; n++) *reinterpret_cast<float2 *>(to + 8 * n + 2 * j4) = o[n];
+            if (j4 == 0) *reinterpret_cast<float2 *>(to + HD) = make_float2(m, l);
+        };
+        auto take = [&](int rec) {
+            const float *from = reinterpret_cast<const float *>(qm) + (rec * kPaRows + g) * (HD + 2);
+            const float2 ml = *reinterpret_cast<const float2 *>(from + HD);
+            const float mn = fmaxf(m, ml.x);
+            const float w1 = m == -INFINITY ? 0.0f : ex2(m - mn), w2 = ml.x == -INFINITY ? 0.0f : ex2(ml.x - mn);
+            l = l * w1 + ml.y * w2;
             m = mn;
-            l = fmaf(l, al, p * sc.v_inv);
 #pragma unroll
-            for (int e = 0; e < N; e++) o[e] = fmaf(o[e], al, p * v[e]);
+            for (int n = 0; n < NB; n++) {
+                const float2 t = *reinterpret_cast<const float2 *>(from + 8 * n + 2 * j4);
+                o[n].x = o[n].x * w1 + t.x * w2;
+                o[n].y = o[n].y * w1 + t.y * w2;
+            }
+        };
+        if constexpr (S::RECS == 2) {
+#pragma unroll
+            for (int half = kPaWarps / 2; half >= 1; half /= 2) {
+                if (warp >= half && warp < 2 * half) give(warp - half);
+                __syncthreads();
+                if (warp < half) take(warp);
+                __syncthreads();
+            }
+        } else {
+#pragma unroll
+            for (int w = 1; w < kPaWarps; w++) {
+                if (warp == w) give(0);
+                __syncthreads();
+                if (warp == 0) take(0);
+                __syncthreads();
+            }
+        }
+        if (warp == 0) {
+            const uint32_t first = share.owner(unit_f0), last = share.owner(unit_f0 + cw.q.tiles - 1);
+            const uint64_t u = pa_unit(a, cw.s, cw.kh, cw.rb);
+            if (unit_f0 == f && lane == 0) {
+                a.unit_info[2 * u] = first;
+                a.unit_info[2 * u + 1] = last - first + 1;
+            }
+            if (first == last) {
+                const float inv = l > 0.0f ? __fdiv_rn(1.0f, l) : (l == 0.0f ? 0.0f : l);
+                if ((uint32_t)g < rows) {
+                    float *dst = a.out + (uint64_t)(cw.q.q0 + R / a.group) * a.out_stride + (uint64_t)head * HD;
+#pragma unroll
+                    for (int n = 0; n < NB; n++)
+                        *reinterpret_cast<float2 *>(dst + 8 * n + 2 * j4) = make_float2(o[n].x * inv, o[n].y * inv);
+                }
+            } else {
+                const uint64_t p = 2 * (uint64_t)c + (unit_f0 == f ? 1 : 0);
+                float *dst = a.part_o + (p * kPaRows + g) * HD;
+#pragma unroll
+                for (int n = 0; n < NB; n++) *reinterpret_cast<float2 *>(dst + 8 * n + 2 * j4) = o[n];
+                if (j4 == 0) {
+                    a.part_ml[p * 16 + g] = m;
+                    a.part_ml[p * 16 + 8 + g] = l;
+                }
+            }
+        }
+        __syncthreads();  // the merge records are read before the next queries overwrite them
+        f = unit_f0 + cw.q.cost();  // the next unit, unless this one goes on elsewhere
+        if (f < f1) {
+            cw.template next_unit<TILE>(a);
+            load_q();
         }
     }
-    float *out = a.out + (uint64_t)row * a.out_stride + (uint64_t)head * HD + lane * N;
-#pragma unroll
-    for (int e = 0; e < N; e++) out[e] = l == 0.0f ? 0.0f : (l == l ? o[e] / l : l);
+    cp_async_wait<0>();
 }
 
-size_t paged_q8_attn_scratch(const PagedAttnArgs &, int) { return 0; }
+// Rows of units that several CTAs share.
+template <int HD, bool PROMPT>
+__global__ void __launch_bounds__(128) k_paged_q8_join(const __grid_constant__ PagedAttnArgs a) {
+    pdl_launch_dependents();
+    pdl_wait();
+    if constexpr (PROMPT) {  // many units, few of them shared: a CTA looks at one unit
+        if (a.unit_info[2 * (uint64_t)blockIdx.x + 1] < 2) return;
+        for (uint32_t r = 0; r < kPaRows; r++) {
+            pa_join_row<HD, PROMPT, false>(a, blockIdx.x, r);
+            __syncthreads();
+        }
+    } else {
+        pa_join_row<HD, PROMPT, false>(a, blockIdx.x / kPaRows, blockIdx.x % kPaRows);
+    }
+}
 
-cudaError_t launch_paged_q8_attn(const LaunchCfg &c, PagedAttnArgs a, uint8_t *) {
+namespace {
+
+size_t up256(size_t v) { return (v + 255) & ~(size_t)255; }
+
+struct Q8Scratch {
+    size_t part_o, part_ml, unit_info, total;
+};
+uint32_t q8_grid(uint32_t hd, int num_sms) {
+    return min((uint32_t)num_sms * (hd == 256 ? Q8Shape<256>::CTAS : hd == 128 ? Q8Shape<128>::CTAS : Q8Shape<64>::CTAS), kPaMaxParts);
+}
+uint32_t q8_row_blocks(const PagedAttnArgs &a) {
+    return (uint32_t)(((uint64_t)(a.cu ? a.max_q : 1) * a.group + kPaRows - 1) / kPaRows);
+}
+Q8Scratch q8_layout(const PagedAttnArgs &a, uint32_t G) {
+    Q8Scratch s;
+    s.part_o = 0;
+    s.part_ml = up256((size_t)2 * G * kPaRows * a.kv.hd * 4);
+    s.unit_info = s.part_ml + up256((size_t)2 * G * 16 * 4);
+    s.total = s.unit_info + up256((size_t)a.n_seq * a.kv.n_kv * q8_row_blocks(a) * 8);
+    return s;
+}
+
+template <int HD, bool PROMPT>
+cudaError_t q8_launch(const LaunchCfg &c, const PagedAttnArgs &a) {
+    const char *label = PROMPT ? "paged_q8_attn_rows" : "paged_q8_attn";
+    const dim3 grid(q8_grid(HD, c.num_sms)), block(kPaThreads);
+    cudaError_t e;
+    if (a.softcap == 0.0f && !a.slopes)
+        e = launch_k(c, label, k_paged_q8<HD, PROMPT, true>, grid, block, Q8Shape<HD>::SMEM, a);
+    else
+        e = launch_k(c, label, k_paged_q8<HD, PROMPT, false>, grid, block, Q8Shape<HD>::SMEM, a);
+    if (e != cudaSuccess) return e;
+    const uint64_t units = (uint64_t)a.n_seq * a.kv.n_kv * a.row_blocks, join = PROMPT ? units : units * kPaRows;
+    if (join > 0x7fffffffull) return cudaErrorInvalidValue;
+    return launch_k(c, "paged_q8_join", k_paged_q8_join<HD, PROMPT>, dim3((uint32_t)join), dim3(128), 0, a);
+}
+
+}  // namespace
+
+size_t paged_q8_attn_scratch(const PagedAttnArgs &a, int num_sms) { return q8_layout(a, q8_grid(a.kv.hd, num_sms)).total; }
+
+cudaError_t launch_paged_q8_attn(const LaunchCfg &c, PagedAttnArgs a, uint8_t *scratch) {
+    const Q8Scratch s = q8_layout(a, q8_grid(a.kv.hd, c.num_sms));
+    a.part_o = (float *)(scratch + s.part_o);
+    a.part_ml = (float *)(scratch + s.part_ml);
+    a.unit_info = (uint32_t *)(scratch + s.unit_info);
     a.err = c.dev_err;
-    const uint64_t rows = (uint64_t)a.n_seq * a.max_q * a.n_heads, ctas = (rows + kQrWarps - 1) / kQrWarps;
-    if (ctas > 0x7fffffffull) return cudaErrorInvalidValue;
-    const dim3 grid((uint32_t)ctas), block(kQrWarps * 32);
+    a.row_blocks = q8_row_blocks(a);
     switch (a.kv.hd) {
-    case 64: return launch_k(c, "paged_q8_attn", k_paged_q8_rows<64>, grid, block, 0, a, rows);
-    case 128: return launch_k(c, "paged_q8_attn", k_paged_q8_rows<128>, grid, block, 0, a, rows);
-    case 256: return launch_k(c, "paged_q8_attn", k_paged_q8_rows<256>, grid, block, 0, a, rows);
+    case 64: return a.cu ? q8_launch<64, true>(c, a) : q8_launch<64, false>(c, a);
+    case 128: return a.cu ? q8_launch<128, true>(c, a) : q8_launch<128, false>(c, a);
+    case 256: return a.cu ? q8_launch<256, true>(c, a) : q8_launch<256, false>(c, a);
     default: return cudaErrorInvalidValue;
     }
 }
