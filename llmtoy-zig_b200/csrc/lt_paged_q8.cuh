@@ -33,8 +33,10 @@ LT_DEVINL Q8Scale q8_scale(float ks, float vs) {
     const bool ok = ks >= 0.0f && ks <= 3.402823466e38f && vs >= 0.0f && vs <= kQ8Most;
     const float v = ok ? fmaxf(vs, kQ8Least) : 1.0f;
     r.k = ok ? ks : __int_as_float(0x7fffffff);
-    r.v_log2 = log2f(v);
-    r.v_inv = __fdiv_rn(1.0f, v);
+    // the approximations are off by 2^-22 (lg2, absolute between 1/2 and 2) and one unit in the last place, of f32: as much as a weight's
+    // two terms; log2 and inverse need not agree better
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(r.v_log2) : "f"(v));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.v_inv) : "f"(v));
     return r;
 }
 

@@ -6,7 +6,7 @@
 //
 // Bound: memory (K and V are read once per 8 query heads of a KV head); the work is
 // shared as lt_paged_walk.cuh says.
-// - Each warp owns KB keys of a tile and a ring of kStages such pieces in shared memory,
+// - Each warp owns KB keys of a tile and a ring of STAGES such pieces in shared memory,
 //   filled by 16-byte asynchronous copies, with the pieces' scales beside them.  Rows of
 //   codes lie one behind the other, their 16-byte columns permuted so that neither matrix
 //   load meets a bank conflict.
@@ -35,13 +35,14 @@ struct Q8Shape {
     static constexpr int SCALES = NG * 8;                   // bytes per piece: K and V scale of each group
     static constexpr int QSTEPS = HD / 32;
     static constexpr int QBYTES = QSTEPS * 1024;
-    static constexpr int RECS = HD == 256 ? 1 : 2;          // merge records at a time
-    static constexpr int MERGE = RECS * kPaRows * (HD + 2) * 4;
+    static constexpr int RECS = HD == 256 ? 2 : kPaWarps;   // merge records
+    static constexpr int MERGE = RECS * kPaRows * HD * 4;
     static constexpr int UNION = QBYTES > MERGE ? QBYTES : MERGE;
     static constexpr int OFF_SCALES = RING + UNION;
-    static constexpr int OFF_ROWF = OFF_SCALES + SCALES * STAGES * kPaWarps;
+    static constexpr int OFF_ML = OFF_SCALES + SCALES * STAGES * kPaWarps;  // (m, l) of each warp's rows
+    static constexpr int OFF_ROWF = OFF_ML + kPaWarps * kPaRows * 8;
     static constexpr int SMEM = OFF_ROWF + kPaRows * 4;
-    static constexpr int CTAS = HD == 64 ? 4 : 2;
+    static constexpr int CTAS = HD == 64 ? 3 : 2;
 };
 
 // Place of 16-byte column c of row r of a piece.  Eight rows of a matrix load are 0-7 or 8-15 (V), or the 8
@@ -53,12 +54,24 @@ LT_DEVINL uint32_t q8_at(uint32_t r, uint32_t c) {
     return r * HD + ((c ^ f) << 4);
 }
 
-// C[16x8] += A[16x32] B[32x8], signed bytes, exact.
+// C[16x8] += A[16x32] B[32x8], signed bytes, exact.  Not volatile, as the f16 product: products may
+// move between loads (which keep their order).
 LT_DEVINL void mma_s8(int (&c)[4], const uint4 &a, uint32_t b0, uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
         : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+}
+LT_DEVINL void mma_w(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// Byte p of four words to a register each: d[p] = bytes p of x[0], x[1], x[2], x[3].
+LT_DEVINL void bytes_across(const uint32_t (&x)[4], uint32_t (&d)[4]) {
+    const uint32_t l01 = __byte_perm(x[0], x[1], 0x5140), l23 = __byte_perm(x[2], x[3], 0x5140);
+    const uint32_t h01 = __byte_perm(x[0], x[1], 0x7362), h23 = __byte_perm(x[2], x[3], 0x7362);
+    d[0] = __byte_perm(l01, l23, 0x5410), d[1] = __byte_perm(l01, l23, 0x7632);
+    d[2] = __byte_perm(h01, h23, 0x5410), d[3] = __byte_perm(h01, h23, 0x7632);
 }
 // Two 16x16 matrices of bytes, transposed: lanes 0-15 give the first's rows, 16-31 the second's.
 // Register i: bytes 4 (lane % 4) .. + 3 of column lane / 4 + 8 (i % 2) of matrix i / 2.
@@ -98,11 +111,21 @@ __global__ void __launch_bounds__(kPaThreads, Q8Shape<HD>::CTAS) k_paged_q8(cons
     __shared__ PaSeq s_q;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, j4 = lane & 3;
     uint8_t *qm = smem + S::RING;  // query fragments, then the merge records
+    float *rec = reinterpret_cast<float *>(qm);
+    float2 *ml = reinterpret_cast<float2 *>(smem + S::OFF_ML);
     float *rowf = reinterpret_cast<float *>(smem + S::OFF_ROWF);
     const uint32_t ring_u = smem_u32(smem) + warp * (S::PIECE * S::STAGES), qm_u = smem_u32(qm);
     const uint32_t scale_u = smem_u32(smem) + S::OFF_SCALES + warp * (S::SCALES * S::STAGES);
     const uint32_t c = blockIdx.x;
     pdl_launch_dependents();
+    // Lengths, page table and queries towards L2 while the kernel before still runs (hints only: the values
+    // are read after the wait).
+    {
+        const uint64_t line = ((uint64_t)c * kPaThreads + tid) * 32, entries = (uint64_t)a.n_seq * a.kv.max_pages;
+        if (line < entries) prefetch_l2(a.table + line);
+        if (tid < 32 && tid * 32 < a.n_seq) prefetch_l2(a.lens + tid * 32);
+        if (tid == 32) prefetch_l2(a.q);
+    }
     pdl_wait();
 
     // the tiles of all sequences, and where this CTA's share begins
@@ -208,21 +231,26 @@ __global__ void __launch_bounds__(kPaThreads, Q8Shape<HD>::CTAS) k_paged_q8(cons
         }
         return j;
     };
+    // Row row0 + i STEP of a group: its column's permutation is row0's, xored by what i adds to the row's number
+    // (STEP is 4, 8 or 2 rows: bits 2 and 3, bit 3, or bits 1 to 3).
+    uint32_t row_at[16 / STEP];
+#pragma unroll
+    for (int i = 0; i < 16 / STEP; i++) row_at[i] = q8_at<HD>(row0 + i * STEP, col0);
+    const uint64_t lane_off = row0 * a.kv.slot_stride + col0 * 16, step_off = STEP * a.kv.slot_stride;
+    const uint64_t v_off = a.kv.v - a.kv.k;
     auto copy = [&](const Job &j, int stage) {
         const uint32_t dst = ring_u + stage * S::PIECE;
 #pragma unroll
         for (int n = 0; n < NG; n++) {
             const bool take = j.page[n] != 0xffffffffu;
             const uint32_t key = j.key + 16 * n;
-            const uint64_t o = take ? paged_offset(a.kv, j.page[n], key, j.kh) + row0 * a.kv.slot_stride + col0 * 16 : 0;
-            const uint8_t *pk = a.kv.k + o, *pv = a.kv.v + o;
+            const uint8_t *pk = a.kv.k + (take ? paged_offset(a.kv, j.page[n], key, j.kh) + lane_off : 0);
 #pragma unroll
-            for (int r = 0; r < 16; r += STEP) {
-                const uint32_t at = dst + n * 16 * HD + q8_at<HD>(r + row0, col0);
+            for (int i = 0; i < 16 / STEP; i++) {
+                const uint32_t at = dst + n * 16 * HD + row_at[i];
                 cp_async16(at, pk, take);
-                cp_async16(at + S::HALF, pv, take);
-                pk += STEP * a.kv.slot_stride;
-                pv += STEP * a.kv.slot_stride;
+                cp_async16(at + S::HALF, pk + v_off, take);
+                pk += step_off;
             }
             if (lane < 2) {
                 const float *sc = (lane ? a.kv.v_scale : a.kv.k_scale) + (take ? q8_scale_at(a.kv, j.page[n], key, j.kh) : 0);
@@ -282,16 +310,13 @@ __global__ void __launch_bounds__(kPaThreads, Q8Shape<HD>::CTAS) k_paged_q8(cons
                 const float x[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
                 for (int i = 0; i < 4; i++) d[i] = ((uint32_t)__float2int_rn(x[i] * up) + 0x00808080u) ^ 0x00808080u;
-                // digit p of four elements to a register
-                const uint32_t l01 = __byte_perm(d[0], d[1], 0x5140), l23 = __byte_perm(d[2], d[3], 0x5140);
-                const uint32_t h01 = __byte_perm(d[0], d[1], 0x7362), h23 = __byte_perm(d[2], d[3], 0x7362);
-                const uint32_t p0 = __byte_perm(l01, l23, 0x5410), p1 = __byte_perm(l01, l23, 0x7632);
-                const uint32_t p2 = __byte_perm(h01, h23, 0x5410), p3 = __byte_perm(h01, h23, 0x7632);
+                uint32_t p[4];
+                bytes_across(d, p);
                 const uint32_t k = 128 * e + 4 * lane;  // element: step k / 32, its half (k / 16) % 2, column (k / 4) % 4
                 if (HD != 64 || lane < 16) {
                     uint8_t *at = qm + (k / 32) * 1024 + (r * 4 + (k / 4) % 4) * 16 + (k / 16) % 2 * 8;
-                    *reinterpret_cast<uint2 *>(at) = make_uint2(p3, p2);
-                    *reinterpret_cast<uint2 *>(at + 512) = make_uint2(p1, p0);
+                    *reinterpret_cast<uint2 *>(at) = make_uint2(p[3], p[2]);
+                    *reinterpret_cast<uint2 *>(at + 512) = make_uint2(p[1], p[0]);
                 }
             }
         }
@@ -422,7 +447,7 @@ __global__ void __launch_bounds__(kPaThreads, Q8Shape<HD>::CTAS) k_paged_q8(cons
                         for (int x = 0; x < 4; x++) {
                             uint32_t b0, b1;
                             s8_to_f16(w[x], b0, b1);
-                            mma_f16(p[x], pa[n], b0, b1);
+                            mma_w(p[x], pa[n], b0, b1);
                         }
                     }
 #pragma unroll
@@ -442,72 +467,79 @@ __global__ void __launch_bounds__(kPaThreads, Q8Shape<HD>::CTAS) k_paged_q8(cons
             if (it + 1 < seg) cw.tile++;
         }
 
-        // ── merge the warps: the upper half into the lower, or one after the other into warp 0 ──
+        // ── merge the warps: each leaves its sums, then every thread adds up dims of its own, row by row.  This runs
+        // once per unit: short loops, since fetching its instructions is most of its time (unrolled in registers, from
+        // half the warps to the other half: 2.7 us) ──
         l += __shfl_xor_sync(0xffffffffu, l, 1);
         l += __shfl_xor_sync(0xffffffffu, l, 2);
+        if (j4 == 0) ml[warp * kPaRows + g] = make_float2(m, l);
+        // column of a record's row: 8 floats apart in the rows that a store of a warp's half touches
+        auto rec_at = [](uint32_t w, uint32_t r, uint32_t d) { return (w * kPaRows + r) * HD + (d ^ ((r & 3) << 3)); };
         __syncthreads();  // every warp is done with the query fragments
-        auto give = [&](int rec) {
-            float *to = reinterpret_cast<float *>(qm) + (rec * kPaRows + g) * (HD + 2);
+        if constexpr (S::RECS == kPaWarps) {
 #pragma unroll
-            for (int n = 0; n < NB; n++) *reinterpret_cast<float2 *>(to + 8 * n + 2 * j4) = o[n];
-            if (j4 == 0) *reinterpret_cast<float2 *>(to + HD) = make_float2(m, l);
-        };
-        auto take = [&](int rec) {
-            const float *from = reinterpret_cast<const float *>(qm) + (rec * kPaRows + g) * (HD + 2);
-            const float2 ml = *reinterpret_cast<const float2 *>(from + HD);
-            const float mn = fmaxf(m, ml.x);
-            const float w1 = m == -INFINITY ? 0.0f : ex2(m - mn), w2 = ml.x == -INFINITY ? 0.0f : ex2(ml.x - mn);
-            l = l * w1 + ml.y * w2;
-            m = mn;
+            for (int n = 0; n < NB; n++) *reinterpret_cast<float2 *>(rec + rec_at(warp, g, 8 * n + 2 * j4)) = o[n];
+        } else {  // two records: the upper warps' sums, to which the lower ones add theirs
+            if (warp >= 2)
 #pragma unroll
-            for (int n = 0; n < NB; n++) {
-                const float2 t = *reinterpret_cast<const float2 *>(from + 8 * n + 2 * j4);
-                o[n].x = o[n].x * w1 + t.x * w2;
-                o[n].y = o[n].y * w1 + t.y * w2;
-            }
-        };
-        if constexpr (S::RECS == 2) {
+                for (int n = 0; n < NB; n++) *reinterpret_cast<float2 *>(rec + rec_at(warp - 2, g, 8 * n + 2 * j4)) = o[n];
+            __syncthreads();
+            if (warp < 2) {
+                const float m2 = ml[(warp + 2) * kPaRows + g].x, mn = fmaxf(m, m2), from = mn == -INFINITY ? 0.0f : mn;
+                const float w1 = ex2(m - from), w2 = ex2(m2 - from);
 #pragma unroll
-            for (int half = kPaWarps / 2; half >= 1; half /= 2) {
-                if (warp >= half && warp < 2 * half) give(warp - half);
-                __syncthreads();
-                if (warp < half) take(warp);
-                __syncthreads();
-            }
-        } else {
-#pragma unroll
-            for (int w = 1; w < kPaWarps; w++) {
-                if (warp == w) give(0);
-                __syncthreads();
-                if (warp == 0) take(0);
-                __syncthreads();
+                for (int n = 0; n < NB; n++) {
+                    float2 *at = reinterpret_cast<float2 *>(rec + rec_at(warp, g, 8 * n + 2 * j4));
+                    const float2 t = *at;
+                    *at = make_float2(o[n].x * w1 + t.x * w2, o[n].y * w1 + t.y * w2);
+                }
             }
         }
-        if (warp == 0) {
-            const uint32_t first = share.owner(unit_f0), last = share.owner(unit_f0 + cw.q.tiles - 1);
-            const uint64_t u = pa_unit(a, cw.s, cw.kh, cw.rb);
-            if (unit_f0 == f && lane == 0) {
-                a.unit_info[2 * u] = first;
-                a.unit_info[2 * u + 1] = last - first + 1;
-            }
-            if (first == last) {
-                const float inv = l > 0.0f ? __fdiv_rn(1.0f, l) : (l == 0.0f ? 0.0f : l);
-                if ((uint32_t)g < rows) {
-                    float *dst = a.out + (uint64_t)(cw.q.q0 + R / a.group) * a.out_stride + (uint64_t)head * HD;
+        const uint32_t first = share.owner(unit_f0), last = share.owner(unit_f0 + cw.q.tiles - 1);
+        const bool whole_unit = first == last, begins = unit_f0 == f;
+        const uint64_t u = pa_unit(a, cw.s, cw.kh, cw.rb), part = 2 * (uint64_t)c + (begins ? 1 : 0);
+        if (begins && tid == 0) {
+            a.unit_info[2 * u] = first;
+            a.unit_info[2 * u + 1] = last - first + 1;
+        }
+        __syncthreads();
+        constexpr int D = HD / 4, RSTEP = kPaThreads / D;  // threads to a row, rows at a time
+#pragma unroll 1
+        for (uint32_t r = tid / D; r < rows; r += RSTEP) {
+            const int d = tid % D * 4;
+            float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            float top = ml[r].x, all = 0.0f;
 #pragma unroll
-                    for (int n = 0; n < NB; n++)
-                        *reinterpret_cast<float2 *>(dst + 8 * n + 2 * j4) = make_float2(o[n].x * inv, o[n].y * inv);
-                }
+            for (int w = 1; w < kPaWarps; w++) top = fmaxf(top, ml[w * kPaRows + r].x);
+            const float from = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+            for (int w = 0; w < kPaWarps; w++) {
+                const float2 x = ml[w * kPaRows + r];
+                all = fmaf(x.y, ex2(x.x - from), all);  // m = -inf: times 0, and l and the sums are 0 or NaN
+                if (w >= S::RECS) continue;
+                // a record's reference: its warp's, or the larger of the two that are in it
+                const float y = S::RECS == kPaWarps ? x.x : fmaxf(x.x, ml[(w + 2) * kPaRows + r].x);
+                const float f = ex2(y - from);
+                const float4 v = *reinterpret_cast<const float4 *>(rec + rec_at(w, r, d));
+                sum.x = fmaf(v.x, f, sum.x);
+                sum.y = fmaf(v.y, f, sum.y);
+                sum.z = fmaf(v.z, f, sum.z);
+                sum.w = fmaf(v.w, f, sum.w);
+            }
+            float *dst;
+            if (whole_unit) {
+                const uint32_t row = cw.rb * kPaRows + r;
+                const float inv = all > 0.0f ? __fdiv_rn(1.0f, all) : (all == 0.0f ? 0.0f : all);
+                sum = make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv);
+                dst = a.out + (uint64_t)(cw.q.q0 + row / a.group) * a.out_stride + (uint64_t)(cw.kh * a.group + row % a.group) * HD;
             } else {
-                const uint64_t p = 2 * (uint64_t)c + (unit_f0 == f ? 1 : 0);
-                float *dst = a.part_o + (p * kPaRows + g) * HD;
-#pragma unroll
-                for (int n = 0; n < NB; n++) *reinterpret_cast<float2 *>(dst + 8 * n + 2 * j4) = o[n];
-                if (j4 == 0) {
-                    a.part_ml[p * 16 + g] = m;
-                    a.part_ml[p * 16 + 8 + g] = l;
+                dst = a.part_o + (part * kPaRows + r) * HD;
+                if (d == 0) {
+                    a.part_ml[part * 16 + r] = top;
+                    a.part_ml[part * 16 + 8 + r] = all;
                 }
             }
+            *reinterpret_cast<float4 *>(dst + d) = sum;
         }
         __syncthreads();  // the merge records are read before the next queries overwrite them
         f = unit_f0 + cw.q.cost();  // the next unit, unless this one goes on elsewhere
