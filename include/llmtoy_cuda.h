@@ -648,7 +648,7 @@ typedef struct lt_paged_q8 {
     uint32_t n_pages, max_pages;
     /* Bytes between pages, slots and KV heads of the codes; each row of head_dim
      * bytes is contiguous.  All 0: [page][head][slot][head_dim], so that what an
-     * attention head reads of a page is contiguous.  Multiples of 16, as the addresses. */
+     * attention head reads of a page is contiguous.  Below 2^32, multiples of 16, as the addresses. */
     uint64_t page_stride, slot_stride, head_stride;
     void *dev_k, *dev_v;
     float *dev_k_scale, *dev_v_scale;  /* [page][head][page_size / block] */

@@ -68,6 +68,8 @@ lt_status paged_q8(lt_ctx *ctx, const lt_paged_q8 *kv, const char *who, lt::Page
     d.page_stride = plain ? kv->n_kv_heads * d.head_stride : kv->page_stride;
     if (d.head_stride % 16 || d.slot_stride % 16 || d.page_stride % 16 || !aligned16(kv->dev_k) || !aligned16(kv->dev_v))
         return st_of(ctx_fail(ctx, LT_EINVAL, "%s: cache addresses and strides must be multiples of 16 bytes", who));
+    if ((d.head_stride | d.slot_stride | d.page_stride) >> 32 || (uint64_t)kv->n_kv_heads * (kv->page_size / kv->block) >> 32)
+        return st_of(ctx_fail(ctx, LT_EINVAL, "%s: strides must be below 2^32 bytes", who));
     if (((uintptr_t)kv->dev_k_scale | (uintptr_t)kv->dev_v_scale) & 3)
         return st_of(ctx_fail(ctx, LT_EINVAL, "%s: scales must be 4-byte aligned", who));
     d.k = (uint8_t *)kv->dev_k;

@@ -90,8 +90,8 @@ LT_DEVINL void s8_to_f16(uint32_t w, uint32_t &b0, uint32_t &b1) {
     b0 = *reinterpret_cast<const uint32_t *>(&u);
     b1 = *reinterpret_cast<const uint32_t *>(&v);
 }
-LT_DEVINL void cp_async4(uint32_t dst, const void *src, bool take) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(take ? 4 : 0) : "memory");
+LT_DEVINL void cp_async4(uint32_t dst, const void *src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
 }
 LT_DEVINL uint4 lds_u4(uint32_t addr) {
     uint4 v;
@@ -204,58 +204,71 @@ __global__ void __launch_bounds__(kPaThreads, Q8Shape<HD>::CTAS) k_paged_q8(cons
     };
     load_q();
 
-    // The piece to copy next: a page for each of its groups.  Whole groups are copied, what lies outside the
-    // unit's positions too (codes may be anything, scores there are masked); groups wholly outside are not.
+    // The piece to copy next: a page for each of its groups, and where its slots begin there.  Whole groups are copied,
+    // what lies outside the unit's positions too (codes may be anything, scores there are masked); groups wholly
+    // outside are not.  This is a third of the instructions of a piece if left to 64-bit products of strides:
+    // strides are below 2^32, and what the unit fixes is added up once per unit.
     constexpr int CH = HD / 16, STEP = 32 / CH;  // columns of a row, rows per copy instruction
     const uint32_t row0 = lane / CH, col0 = lane % CH;
-    struct Job {
-        uint32_t page[NG], key, kh;
-        bool there;
-    };
-    auto look = [&]() {
-        Job j;
-        j.there = true;
-        j.key = lw.base + lw.tile * TILE + warp * KB;
-        j.kh = lw.kh;
-#pragma unroll
-        for (int n = 0; n < NG; n++) {
-            const uint32_t key = j.key + 16 * n;
-            j.page[n] = 0xffffffffu;
-            if (key < lw.hi && key + 16 > lw.lo) {
-                const uint32_t page = a.table[(uint64_t)lw.s * a.kv.max_pages + page_of(a.kv, key)];
-                if (page < a.kv.n_pages)
-                    j.page[n] = page;
-                else
-                    atomicExch(a.err, DEV_ERR_BAD_INDEX);
-            }
-        }
-        return j;
-    };
-    // Row row0 + i STEP of a group: its column's permutation is row0's, xored by what i adds to the row's number
-    // (STEP is 4, 8 or 2 rows: bits 2 and 3, bit 3, or bits 1 to 3).
+    const uint32_t page_stride = (uint32_t)a.kv.page_stride, slot_stride = (uint32_t)a.kv.slot_stride;
+    const uint64_t v_off = a.kv.v - a.kv.k, step_off = (uint64_t)STEP * slot_stride;
     uint32_t row_at[16 / STEP];
 #pragma unroll
-    for (int i = 0; i < 16 / STEP; i++) row_at[i] = q8_at<HD>(row0 + i * STEP, col0);
-    const uint64_t lane_off = row0 * a.kv.slot_stride + col0 * 16, step_off = STEP * a.kv.slot_stride;
-    const uint64_t v_off = a.kv.v - a.kv.k;
-    auto copy = [&](const Job &j, int stage) {
-        const uint32_t dst = ring_u + stage * S::PIECE;
+    for (int i = 0; i < 16 / STEP; i++) row_at[i] = ring_u + q8_at<HD>(row0 + i * STEP, col0);
+    const uint32_t *row_table;   // of lw's unit: its sequence's page table,
+    const uint8_t *head_k;       // its head's codes, from this lane's row and column on,
+    const float *head_scale;     // and its head's scales, K's or (odd lanes) V's
+    auto unit_base = [&]() {
+        row_table = a.table + (uint64_t)lw.s * a.kv.max_pages;
+        head_k = a.kv.k + (uint64_t)lw.kh * (uint32_t)a.kv.head_stride + (uint64_t)row0 * slot_stride + col0 * 16;
+        head_scale = (lane & 1 ? a.kv.v_scale : a.kv.k_scale) + (uint64_t)lw.kh * a.kv.page_blocks;
+    };
+    unit_base();
+    const uint32_t scales_per_page = a.kv.n_kv * a.kv.page_blocks;  // below 2^32: checked on the host
+    struct Job {
+        uint32_t page[NG], slot[NG];
+        const uint8_t *k;
+        const float *scale;
+        bool there;
+    };
+    constexpr uint32_t kNone = 0xffffffffu;
+    auto look = [&](Job &j) {
+        const uint32_t key0 = lw.base + lw.tile * TILE + warp * KB;
 #pragma unroll
         for (int n = 0; n < NG; n++) {
-            const bool take = j.page[n] != 0xffffffffu;
-            const uint32_t key = j.key + 16 * n;
-            const uint8_t *pk = a.kv.k + (take ? paged_offset(a.kv, j.page[n], key, j.kh) + lane_off : 0);
+            const uint32_t key = key0 + 16 * n;
+            uint32_t at;
+            if (a.kv.page_shift != kNoShift) {
+                at = key >> a.kv.page_shift;
+                j.slot[n] = key & (a.kv.page_size - 1);
+            } else {
+                at = key / a.kv.page_size;
+                j.slot[n] = key - at * a.kv.page_size;
+            }
+            j.page[n] = key < lw.hi && key + 16 > lw.lo ? row_table[at] : kNone;
+        }
+        j.k = head_k;
+        j.scale = head_scale;
+    };
+    auto copy = [&](const Job &j, int stage) {
+#pragma unroll
+        for (int n = 0; n < NG; n++) {
+            const uint32_t page = j.page[n];
+            if (page >= a.kv.n_pages) {
+                if (page != kNone) atomicExch(a.err, DEV_ERR_BAD_INDEX);
+                continue;
+            }
+            const uint8_t *pk = j.k + (uint64_t)page * page_stride + (uint64_t)j.slot[n] * slot_stride;
+            const uint32_t to = stage * S::PIECE + n * 16 * HD;
 #pragma unroll
             for (int i = 0; i < 16 / STEP; i++) {
-                const uint32_t at = dst + n * 16 * HD + row_at[i];
-                cp_async16(at, pk, take);
-                cp_async16(at + S::HALF, pk + v_off, take);
+                cp_async16(to + row_at[i], pk, true);
+                cp_async16(to + row_at[i] + S::HALF, pk + v_off, true);
                 pk += step_off;
             }
-            if (lane < 2) {
-                const float *sc = (lane ? a.kv.v_scale : a.kv.k_scale) + (take ? q8_scale_at(a.kv, j.page[n], key, j.kh) : 0);
-                cp_async4(scale_u + stage * S::SCALES + n * 8 + lane * 4, sc, take);
-            }
+            if (lane < 2)
+                cp_async4(scale_u + stage * S::SCALES + n * 8 + lane * 4,
+                          j.scale + (uint64_t)page * scales_per_page + (j.slot[n] >> a.kv.block_shift));
         }
     };
     // all pages of the first pieces are looked up before the first copy waits for its own
@@ -263,12 +276,15 @@ __global__ void __launch_bounds__(kPaThreads, Q8Shape<HD>::CTAS) k_paged_q8(cons
     auto look_next = [&](Job &j) {
         j.there = lf < f1;
         if (!j.there) return;
-        j = look();
+        look(j);
         if (++lw.tile < lw.q.tiles) {
             lf++;
         } else {
             lf += 1 + kUnitCost;
-            if (lf < f1) lw.template next_unit<TILE>(a);
+            if (lf < f1) {
+                lw.template next_unit<TILE>(a);
+                unit_base();
+            }
         }
     };
 #pragma unroll
@@ -408,12 +424,18 @@ __global__ void __launch_bounds__(kPaThreads, Q8Shape<HD>::CTAS) k_paged_q8(cons
                             bool seen = j >= row_lo && j < row_hi;
                             if (docs && seen) seen = docs[j] == my_doc;
                             if (!seen) t = -INFINITY;
-                        } else if (!whole && (j < row_lo || j >= row_hi)) {
-                            t = -INFINITY;
                         }
-                        top = fmaxf(top, t);
                     }
                 }
+                if (!PROMPT && !whole) {
+#pragma unroll
+                    for (int i = 0; i < 4 * NG; i++) {
+                        const int j = (int)k0 + 16 * (i / 4) + 4 * j4 + i % 4;
+                        if (j < row_lo || j >= row_hi) sc[i] = -INFINITY;
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 4 * NG; i++) top = fmaxf(top, sc[i]);
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
                 const float mn = fmaxf(m, top);

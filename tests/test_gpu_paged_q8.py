@@ -336,7 +336,7 @@ def test_append_refusals(pkg, ctx):
 
     for kv in (dict(head_dim=96), dict(block=8), dict(block=24), dict(block=0), dict(block=256), dict(page_size=24), dict(page_size=0),
                dict(n_kv_heads=0), dict(n_pages=0), dict(max_pages=0), dict(slot_stride=64), dict(page_stride=4096, slot_stride=72, head_stride=64),
-               dict(k=c.dc[0].data_ptr() + 4), dict(v=None), dict(k_scale=None), dict(v_scale=c.ds[1].data_ptr() + 2)):
+               dict(page_stride=1 << 32, slot_stride=64, head_stride=64), dict(k=c.dc[0].data_ptr() + 4), dict(v=None), dict(k_scale=None), dict(v_scale=c.ds[1].data_ptr() + 2)):
         refused(kv=kv)
     for cfg in (dict(n_heads=0), dict(n_kv_heads=1), dict(head_dim=128), dict(rope_theta=0.0), dict(rope_theta=float("inf")),
                 dict(rope_theta=float("nan"))):
