@@ -1,5 +1,5 @@
-// lt_paged_prompt.cu — attention of many queries per sequence over a paged f16
-// cache, on the 5th-generation tensor cores.
+// lt_paged_prompt.cu — attention of many queries per sequence over a paged cache of
+// f16 values or 8-bit codes, on the 5th-generation tensor cores.
 //
 // Same formula as lt_paged_attn.cu.  Rows are (token, head of the KV head's
 // group) pairs, so all the heads that read a KV head share its tiles.  The f32
@@ -17,7 +17,10 @@
 //                    128-byte-swizzled rows: tiles that lie wholly within the
 //                    sequence by TMA, a box per page and 64 columns; the ragged
 //                    ends, and pages that are no multiple of 8 slots, by 16-byte
-//                    asynchronous copies with zero fill
+//                    asynchronous copies with zero fill.  8-bit codes: from their pages through
+//                    registers, where they become f16 numbers (exactly), the next stage's
+//                    codes on their way; scales enter as lt_paged_q8.cuh puts them, a
+//                    factor and a summand for 16 columns of scores
 // While one tile's softmax runs, the tensor cores work for the other: per tile
 // of keys the MMA order is PV0 QK0' PV1 QK1' (' the next keys), PV in two halves so
 // that the first can start while the softmax is at the second.  S and P share
@@ -36,7 +39,7 @@
 // (8192 tokens 1.15 ms, 1.00 without), as did one KV head after the other (1.01 ms).
 #include <cuda.h>  // CUtensorMap (encoded through the runtime's driver entry point)
 
-#include "lt_paged.cuh"
+#include "lt_paged_q8.cuh"
 #include "lt_umma.cuh"
 
 namespace lt {
@@ -46,7 +49,7 @@ constexpr int kPpThreads = 384, kPpProducers = 96;
 // the ring at head_dim 128.  Longer rows (512 K keys; 256 K at head_dim 256) go through every tile.
 constexpr int kPpSkipTiles = 4096;
 
-template <int HD>
+template <int HD, bool Q8 = false>
 struct PpShape {
     static constexpr int TILES = HD == 256 ? 1 : 2;       // row tiles of 128
     static constexpr int ROWS = TILES * 128;
@@ -62,8 +65,10 @@ struct PpShape {
     static constexpr int Q_BYTES = TILES * 2 * QPLANE;
     static constexpr int OFF_RING = Q_BYTES;
     static constexpr int OFF_OFFS = OFF_RING + STAGES * STAGE;
-    static constexpr int OFF_DOCS = OFF_OFFS + KT * 8;
-    static constexpr int OFF_SKIP = OFF_DOCS + DOCS * KT * 4;
+    static constexpr int GROUPS = KT / 16;                // of 16 keys, each within a page and a block
+    static constexpr int OFF_DOCS = OFF_OFFS + (Q8 ? GROUPS : KT) * 8;
+    static constexpr int OFF_SCALES = OFF_DOCS + DOCS * KT * 4;  // 8-bit codes: {k, log2 v, 1 / v} of each group
+    static constexpr int OFF_SKIP = OFF_SCALES + (Q8 ? DOCS * GROUPS * 16 : 0);
     static constexpr int OFF_BARS = OFF_SKIP + kPpSkipTiles / 8;
     static constexpr int SMEM = OFF_BARS + 256;
     static constexpr uint32_t S_COL(int i) { return (HD == 256 ? 64 : 128) * i; }
@@ -182,14 +187,15 @@ struct IntC {
     static constexpr int value = N;
 };
 
-template <int HD, bool EXTRA>
+template <int HD, bool EXTRA, bool Q8>
 __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_constant__ PagedAttnArgs a,
                                                                 const __grid_constant__ PpMaps maps) {
-    using S = PpShape<HD>;
+    using S = PpShape<HD, Q8>;
     constexpr int KT = S::KT, NS = S::STAGES;
     extern __shared__ __align__(1024) uint8_t smem[];
     uint64_t *offs = reinterpret_cast<uint64_t *>(smem + S::OFF_OFFS);
     uint32_t *docs_s = reinterpret_cast<uint32_t *>(smem + S::OFF_DOCS);
+    float4 *scales_s = reinterpret_cast<float4 *>(smem + S::OFF_SCALES);
     uint32_t *skip = reinterpret_cast<uint32_t *>(smem + S::OFF_SKIP);  // bit set: some row may see the tile
     uint64_t *full = reinterpret_cast<uint64_t *>(smem + S::OFF_BARS), *empty = full + NS;
     uint64_t *s_full = empty + NS, *p_full = s_full + 2, *o_full = p_full + 2, *p_half = o_full + 2;
@@ -225,7 +231,7 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
     if (a.causal) hi64 = min(hi64, max(i1 + 1, (int64_t)prefix));
     if (a.window) lo64 = max((int64_t)0, i0 - (int64_t)a.window + 1);
     const uint32_t hi = (uint32_t)max((int64_t)0, hi64), first = (uint32_t)min(lo64, (int64_t)hi);
-    const uint32_t lo = maps.rows ? first - first % maps.rows : first;  // tiles start on a box
+    const uint32_t lo = Q8 ? first & ~15u : maps.rows ? first - first % maps.rows : first;  // tiles start on a box, or a group
     const uint32_t all_tiles = (hi - lo + KT - 1) / KT, share = (all_tiles + a.nsplit - 1) / a.nsplit;
     const uint32_t begin = uniform(min(all_tiles, split * share)), tiles = uniform(min(all_tiles, begin + share));
     const uint32_t *table = a.table + (uint64_t)s * a.kv.max_pages;
@@ -304,123 +310,215 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
         if (warp > 8) {
             // ── K and V tiles into the ring ──
             const int pt = tid - 288, pw = warp - 9;
-            constexpr int CH = HD / 8, RPI = 32 / CH;  // 16-byte chunks per row, rows per warp and step
-            const int col = lane % CH;
-            constexpr int PER = (KT + kPpProducers - 1) / kPpProducers;
-            uint64_t mine[PER];  // pool offsets of this thread's rows, looked up one tile ahead
-            auto look = [&](uint32_t t) {
-#pragma unroll
-                for (int u = 0; u < PER; u++) {
-                    const uint32_t r = pt + u * kPpProducers, j = lo + t * KT + r;
-                    mine[u] = ~0ull;
-                    if (r < KT && j >= first && j < hi) {
-                        const uint32_t page = table[j / a.kv.page_size];
-                        if (page < a.kv.n_pages)
-                            mine[u] = paged_offset(a.kv, page, j, kh);
-                        else
-                            atomicExch(a.err, DEV_ERR_BAD_INDEX);
+            if constexpr (Q8) {
+                constexpr int CH = HD / 16, CHUNKS = KT * CH, PER = (CHUNKS + kPpProducers - 1) / kPpProducers;
+                uint4 v[PER];        // the next stage's codes: chunk c = pt + 96 i, column c % CH of row c / CH
+                uint64_t at = ~0ull; // threads pt < GROUPS: place of group pt of the next tile, and its scales
+                float ks = 0.0f, vs = 0.0f;
+                auto look = [&](uint32_t tt) {
+                    if (pt >= S::GROUPS) return;
+                    const uint32_t key = lo + tt * KT + 16 * pt;
+                    at = ~0ull;
+                    ks = vs = 0.0f;
+                    if (key >= hi || key + 16 <= first) return;
+                    const uint32_t page = table[page_of(a.kv, key)];
+                    if (page >= a.kv.n_pages) {
+                        atomicExch(a.err, DEV_ERR_BAD_INDEX);
+                        return;
                     }
-                }
-            };
-            auto landed = [&](uint32_t stage) {  // this thread's copies are in place: hand the stage on
-                fence_async_smem();
-                mbar_arrive(full + stage);
-            };
-            uint32_t jj = 0, st = 0, turn = 0;  // tile count; ring stage and how often it went round
-            uint32_t boxes_in = 0, boxes_phase = 0;  // bit per stage: last filled by TMA, and in which phase
-            uint32_t t = next_tile(begin);
-            bool owed = false;                // the stage before st is copied but not handed on
-            // tiles of whole boxes: every slot holds a cached position
-            auto boxed = [&](uint32_t tt) {
-                const uint32_t k0 = lo + tt * KT;
-                return maps.rows && k0 >= first && (uint64_t)k0 + KT <= len;
-            };
-            const uint32_t boxes = maps.rows ? KT / maps.rows : 0;  // per 64 columns
-            uint32_t box_page = 0;
-            auto look_boxed = [&](uint32_t tt) {  // lane l of warp 9: box l % boxes of column block l / boxes
-                if (pw == 0 && (uint32_t)lane < boxes * S::NBLK) {
-                    box_page = table[(lo + tt * KT + lane % boxes * maps.rows) / a.kv.page_size];
-                    if (box_page >= a.kv.n_pages) atomicExch(a.err, DEV_ERR_BAD_INDEX);
-                }
-            };
-            auto ahead = [&](uint32_t tt) {
-                if (tt >= tiles) return;
-                if (boxed(tt))
-                    look_boxed(tt);
-                else
-                    look(tt);
-            };
-            ahead(t);
-            while (t < tiles) {
-                const bool by_box = boxed(t);
-                if (!by_box) {
-                    named_sync<1, kPpProducers>();  // the last such tile's offsets are read
+                    at = paged_offset(a.kv, page, key, kh);
+                    const uint64_t sc = q8_scale_at(a.kv, page, key, kh);
+                    ks = a.kv.k_scale[sc];
+                    vs = a.kv.v_scale[sc];
+                };
+                auto fetch = [&](const uint8_t *pool) {
 #pragma unroll
-                    for (int u = 0; u < PER; u++)
-                        if (pt + u * kPpProducers < KT) offs[pt + u * kPpProducers] = mine[u];
-                    named_sync<1, kPpProducers>();
-                }
-                const uint32_t tn = next_tile(t + 1), page = box_page;
-#pragma unroll 1
-                for (int kv = 0; kv < 2; kv++) {
-                    if (owed && (by_box || !mbar_try_wait(empty + st, (turn & 1) ^ 1))) {
-                        cp_async_wait<0>();
-                        landed(st ? st - 1 : NS - 1);
-                        owed = false;
+                    for (int i = 0; i < PER; i++) {
+                        const int c = pt + i * kPpProducers, r = c / CH;
+                        const uint64_t o = c < CHUNKS ? offs[r / 16] : ~0ull;
+                        v[i] = make_uint4(0, 0, 0, 0);  // groups that are not there: zeros, which no weight of 0 makes NaN
+                        if (o != ~0ull)
+                            v[i] = *reinterpret_cast<const uint4 *>(pool + o + (uint64_t)(r % 16) * a.kv.slot_stride + c % CH * 16);
                     }
-                    if (!__all_sync(0xffffffffu, wait(empty + st, (turn & 1) ^ 1))) continue;
-                    const uint32_t bit = 1u << st;
-                    boxes_in = by_box ? boxes_in | bit : boxes_in & ~bit;
-                    boxes_phase = turn & 1 ? boxes_phase | bit : boxes_phase & ~bit;
-                    if (docs && kv == 0)
-                        for (int r = pt; r < KT; r += kPpProducers) {
-                            const uint32_t j = lo + t * KT + r;
-                            docs_s[(jj % S::DOCS) * KT + r] = j < hi ? docs[j] : 0;
-                        }
-                    const uint32_t stage = smem_u32(smem) + S::OFF_RING + st * S::STAGE;
-                    if (by_box) {
-                        if (pw == 0) {
-                            if (lane == 0) mbar_arrive_expect_tx(full + st, S::STAGE);
-                            __syncwarp();
-                            if ((uint32_t)lane < boxes * S::NBLK) {
-                                const uint32_t r = lane % boxes * maps.rows, blk = lane / boxes;
-                                tma_load_4d(stage + blk * (KT * 128) + r * 128, kv ? &maps.v : &maps.k, blk * 64,
-                                            (lo + t * KT + r) % a.kv.page_size, kh, page, full + st);
+                };
+                uint32_t st = 0, turn = 0;
+                // the stage's turn, then its codes as f16: 16 of them fill two 16-byte columns of a 128-byte-swizzled row
+                auto hand_over = [&](bool k_stage, uint32_t t, uint32_t jj) {
+                    const bool ok = __all_sync(0xffffffffu, wait(empty + st, (turn & 1) ^ 1));
+                    if (ok) {
+                        if (k_stage) {
+                            if (docs)
+                                for (int r = pt; r < KT; r += kPpProducers) {
+                                    const uint32_t j = lo + t * KT + r;
+                                    docs_s[(jj % S::DOCS) * KT + r] = j < hi ? docs[j] : 0;
+                                }
+                            if (pt < S::GROUPS) {
+                                const Q8Scale z = q8_scale(ks, vs);
+                                scales_s[(jj % S::DOCS) * S::GROUPS + pt] = make_float4(z.k, z.v_log2, z.v_inv, 0.0f);
                             }
-                            if (lane) mbar_arrive(full + st);
-                        } else {
-                            mbar_arrive(full + st);
                         }
-                        if (kv == 0) ahead(tn);
-                    } else {
-                        const uint8_t *src = (kv ? a.kv.v : a.kv.k) + col * 16;
-                        const uint32_t dst = stage + (col / 8) * (KT * 128);
-#pragma unroll 4
-                        for (int r = pw * RPI + lane / CH; r < KT; r += 3 * RPI) {
-                            const uint64_t o = offs[r];
-                            const bool take = o != ~0ull;
-                            cp_async16(dst + r * 128 + (((col & 7) ^ (r & 7)) << 4), src + (take ? o : 0), take);
+                        uint8_t *stage = smem + S::OFF_RING + st * S::STAGE;
+#pragma unroll
+                        for (int i = 0; i < PER; i++) {
+                            const int c = pt + i * kPpProducers, r = c / CH, col = 2 * (c % CH);
+                            if (c >= CHUNKS) break;
+                            uint4 h0, h1;
+                            s8_to_f16(v[i].x, h0.x, h0.y);
+                            s8_to_f16(v[i].y, h0.z, h0.w);
+                            s8_to_f16(v[i].z, h1.x, h1.y);
+                            s8_to_f16(v[i].w, h1.z, h1.w);
+                            uint8_t *row = stage + col / 8 * (KT * 128) + r * 128;
+                            *reinterpret_cast<uint4 *>(row + (((col & 7) ^ (r & 7)) << 4)) = h0;
+                            *reinterpret_cast<uint4 *>(row + ((((col & 7) + 1) ^ (r & 7)) << 4)) = h1;
                         }
-                        cp_async_commit();
-                        if (kv == 0) ahead(tn);
-                        if (owed) {
-                            cp_async_wait<1>();
-                            landed(st ? st - 1 : NS - 1);
-                        }
-                        owed = true;
+                        fence_async_smem();
+                        mbar_arrive(full + st);
                     }
                     if (++st == NS) st = 0, turn++;
+                };
+                auto publish = [&]() {  // the next tile's places, once everybody has the last one's codes on their way
+                    named_sync<1, kPpProducers>();
+                    if (pt < S::GROUPS) offs[pt] = at;
+                    named_sync<1, kPpProducers>();
+                };
+                uint32_t t = next_tile(begin), jj = 0;
+                if (t < tiles) {
+                    look(t);
+                    publish();
+                    fetch(a.kv.k);
                 }
-                t = tn;
-                jj++;
+                while (t < tiles) {
+                    const uint32_t tn = next_tile(t + 1);
+                    hand_over(true, t, jj);
+                    fetch(a.kv.v);
+                    if (tn < tiles) look(tn);
+                    hand_over(false, t, jj);
+                    if (tn < tiles) {
+                        publish();
+                        fetch(a.kv.k);
+                    }
+                    t = tn;
+                    jj++;
+                }
+            } else {
+                constexpr int CH = HD / 8, RPI = 32 / CH;  // 16-byte chunks per row, rows per warp and step
+                const int col = lane % CH;
+                constexpr int PER = (KT + kPpProducers - 1) / kPpProducers;
+                uint64_t mine[PER];  // pool offsets of this thread's rows, looked up one tile ahead
+                auto look = [&](uint32_t t) {
+#pragma unroll
+                    for (int u = 0; u < PER; u++) {
+                        const uint32_t r = pt + u * kPpProducers, j = lo + t * KT + r;
+                        mine[u] = ~0ull;
+                        if (r < KT && j >= first && j < hi) {
+                            const uint32_t page = table[j / a.kv.page_size];
+                            if (page < a.kv.n_pages)
+                                mine[u] = paged_offset(a.kv, page, j, kh);
+                            else
+                                atomicExch(a.err, DEV_ERR_BAD_INDEX);
+                        }
+                    }
+                };
+                auto landed = [&](uint32_t stage) {  // this thread's copies are in place: hand the stage on
+                    fence_async_smem();
+                    mbar_arrive(full + stage);
+                };
+                uint32_t jj = 0, st = 0, turn = 0;  // tile count; ring stage and how often it went round
+                uint32_t boxes_in = 0, boxes_phase = 0;  // bit per stage: last filled by TMA, and in which phase
+                uint32_t t = next_tile(begin);
+                bool owed = false;                // the stage before st is copied but not handed on
+                // tiles of whole boxes: every slot holds a cached position
+                auto boxed = [&](uint32_t tt) {
+                    const uint32_t k0 = lo + tt * KT;
+                    return maps.rows && k0 >= first && (uint64_t)k0 + KT <= len;
+                };
+                const uint32_t boxes = maps.rows ? KT / maps.rows : 0;  // per 64 columns
+                uint32_t box_page = 0;
+                auto look_boxed = [&](uint32_t tt) {  // lane l of warp 9: box l % boxes of column block l / boxes
+                    if (pw == 0 && (uint32_t)lane < boxes * S::NBLK) {
+                        box_page = table[(lo + tt * KT + lane % boxes * maps.rows) / a.kv.page_size];
+                        if (box_page >= a.kv.n_pages) atomicExch(a.err, DEV_ERR_BAD_INDEX);
+                    }
+                };
+                auto ahead = [&](uint32_t tt) {
+                    if (tt >= tiles) return;
+                    if (boxed(tt))
+                        look_boxed(tt);
+                    else
+                        look(tt);
+                };
+                ahead(t);
+                while (t < tiles) {
+                    const bool by_box = boxed(t);
+                    if (!by_box) {
+                        named_sync<1, kPpProducers>();  // the last such tile's offsets are read
+#pragma unroll
+                        for (int u = 0; u < PER; u++)
+                            if (pt + u * kPpProducers < KT) offs[pt + u * kPpProducers] = mine[u];
+                        named_sync<1, kPpProducers>();
+                    }
+                    const uint32_t tn = next_tile(t + 1), page = box_page;
+#pragma unroll 1
+                    for (int kv = 0; kv < 2; kv++) {
+                        if (owed && (by_box || !mbar_try_wait(empty + st, (turn & 1) ^ 1))) {
+                            cp_async_wait<0>();
+                            landed(st ? st - 1 : NS - 1);
+                            owed = false;
+                        }
+                        if (!__all_sync(0xffffffffu, wait(empty + st, (turn & 1) ^ 1))) continue;
+                        const uint32_t bit = 1u << st;
+                        boxes_in = by_box ? boxes_in | bit : boxes_in & ~bit;
+                        boxes_phase = turn & 1 ? boxes_phase | bit : boxes_phase & ~bit;
+                        if (docs && kv == 0)
+                            for (int r = pt; r < KT; r += kPpProducers) {
+                                const uint32_t j = lo + t * KT + r;
+                                docs_s[(jj % S::DOCS) * KT + r] = j < hi ? docs[j] : 0;
+                            }
+                        const uint32_t stage = smem_u32(smem) + S::OFF_RING + st * S::STAGE;
+                        if (by_box) {
+                            if (pw == 0) {
+                                if (lane == 0) mbar_arrive_expect_tx(full + st, S::STAGE);
+                                __syncwarp();
+                                if ((uint32_t)lane < boxes * S::NBLK) {
+                                    const uint32_t r = lane % boxes * maps.rows, blk = lane / boxes;
+                                    tma_load_4d(stage + blk * (KT * 128) + r * 128, kv ? &maps.v : &maps.k, blk * 64,
+                                                (lo + t * KT + r) % a.kv.page_size, kh, page, full + st);
+                                }
+                                if (lane) mbar_arrive(full + st);
+                            } else {
+                                mbar_arrive(full + st);
+                            }
+                            if (kv == 0) ahead(tn);
+                        } else {
+                            const uint8_t *src = (kv ? a.kv.v : a.kv.k) + col * 16;
+                            const uint32_t dst = stage + (col / 8) * (KT * 128);
+#pragma unroll 4
+                            for (int r = pw * RPI + lane / CH; r < KT; r += 3 * RPI) {
+                                const uint64_t o = offs[r];
+                                const bool take = o != ~0ull;
+                                cp_async16(dst + r * 128 + (((col & 7) ^ (r & 7)) << 4), src + (take ? o : 0), take);
+                            }
+                            cp_async_commit();
+                            if (kv == 0) ahead(tn);
+                            if (owed) {
+                                cp_async_wait<1>();
+                                landed(st ? st - 1 : NS - 1);
+                            }
+                            owed = true;
+                        }
+                        if (++st == NS) st = 0, turn++;
+                    }
+                    t = tn;
+                    jj++;
+                }
+                if (owed) {
+                    cp_async_wait<0>();
+                    landed(st ? st - 1 : NS - 1);
+                }
+                if (pw == 0)  // no copy of this CTA is under way when it ends
+                    for (int i = 0; i < NS; i++)
+                        if ((boxes_in >> i & 1u) && !wait_always(full + i, boxes_phase >> i & 1u)) break;
             }
-            if (owed) {
-                cp_async_wait<0>();
-                landed(st ? st - 1 : NS - 1);
-            }
-            if (pw == 0)  // no copy of this CTA is under way when it ends
-                for (int i = 0; i < NS; i++)
-                    if ((boxes_in >> i & 1u) && !wait_always(full + i, boxes_phase >> i & 1u)) break;
         } else {
             // ── MMAs ──
             constexpr uint32_t IQK = umma_idesc_f16_f32(128, KT);
@@ -676,6 +774,12 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
             // pass 1: the row's maximum; capped, biased or masked scores go back to tensor
             // memory.  Each load runs while the columns before it are worked on.
             float top = -INFINITY;
+            const float4 *zs = scales_s + (jj % S::DOCS) * S::GROUPS + half * 2;  // this thread's columns' scales, 16 to each
+            // the factor on 16 columns' raw scores: not 0, by which a masked score's -inf would become NaN; NaN stays
+            auto factor = [&](float k) {
+                const float f = rf * k;
+                return f < 1.17549435e-38f ? 1.17549435e-38f : f;
+            };
             {
                 uint32_t v[2][16];
                 tmem_ld16(s_addr, v[0]);
@@ -695,15 +799,22 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
                             x0 = fmaxf(fmaxf(x0, __uint_as_float(u[e])), __uint_as_float(u[e + 1]));
                             x1 = fmaxf(fmaxf(x1, __uint_as_float(u[e + 2])), __uint_as_float(u[e + 3]));
                         }
-                        top = fmaxf(top, fmaxf(x0, x1));
+                        if constexpr (Q8) {
+                            const float4 z = zs[c / 16];
+                            top = fmaxf(top, fmaf(fmaxf(x0, x1), factor(z.x), z.y));
+                        } else {
+                            top = fmaxf(top, fmaxf(x0, x1));
+                        }
                         continue;
                     }
+                    const float4 z = Q8 ? zs[c / 16] : make_float4(1.0f, 0.0f, 1.0f, 0.0f);
                     if (EXTRA) {  // score_log2, the usual case two at a time
                         constexpr float kLog2e = 1.4426950408889634f;
                         float big = 0.0f;
 #pragma unroll
                         for (int e = 0; e < 16; e++) big = fmaxf(big, fabsf(__uint_as_float(u[e])));
-                        const float2 f2 = make_float2(rf, rf);
+                        const float f1 = Q8 ? rf * z.x : rf;
+                        const float2 f2 = make_float2(f1, f1);
                         if (a.softcap == 0.0f) {
 #pragma unroll
                             for (int e = 0; e < 16; e += 2) {
@@ -711,7 +822,7 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
                                 u[e] = __float_as_uint(x.x);
                                 u[e + 1] = __float_as_uint(x.y);
                             }
-                        } else if (__all_sync(0xffffffffu, big * rf <= kTanhSmall)) {
+                        } else if (__all_sync(0xffffffffu, big * f1 <= kTanhSmall)) {
                             const float2 cl = make_float2(a.softcap * kLog2e, a.softcap * kLog2e);
 #pragma unroll
                             for (int e = 0; e < 16; e += 2) {
@@ -723,7 +834,7 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
                         } else {
 #pragma unroll
                             for (int e = 0; e < 16; e++)
-                                u[e] = __float_as_uint(tanh_any(__uint_as_float(u[e]) * rf) * (a.softcap * kLog2e));
+                                u[e] = __float_as_uint(tanh_any(__uint_as_float(u[e]) * f1) * (a.softcap * kLog2e));
                         }
                         if (a.slopes) {
                             const float sl = -row_slope * kLog2e;
@@ -733,6 +844,10 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
                         }
                     }
                     constexpr uint32_t kMinusInf = 0xff800000u;
+                    if (Q8 && !EXTRA && z.x != z.x) {  // no number: nor are the scores, but for those that the masks take
+#pragma unroll
+                        for (int e = 0; e < 16; e++) u[e] = 0x7fffffffu;
+                    }
                     if (!in_range) {
 #pragma unroll
                         for (int e = 0; e < 16; e++) u[e] = c + e >= from && c + e < to ? u[e] : kMinusInf;
@@ -748,14 +863,21 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
                             u[4 * e + 3] = d.w == row_doc ? u[4 * e + 3] : kMinusInf;
                         }
                     }
+                    if constexpr (Q8) {
+                        float x = -INFINITY;
 #pragma unroll
-                    for (int e = 0; e < 16; e++) top = fmaxf(top, __uint_as_float(u[e]));
+                        for (int e = 0; e < 16; e++) x = fmaxf(x, __uint_as_float(u[e]));
+                        top = fmaxf(top, fmaf(x, EXTRA || z.x != z.x ? 1.0f : factor(z.x), z.y));
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 16; e++) top = fmaxf(top, __uint_as_float(u[e]));
+                    }
                     tmem_st16(s_addr + c, u);
                 }
                 if (EXTRA || !plain) tmem_wait_st();
             }
             const float fs = EXTRA ? 1.0f : rf;
-            top = top == -INFINITY ? top : top * fs;
+            if (!Q8) top = top == -INFINITY ? top : top * fs;
             if constexpr (HD == 256) {  // the other half's maximum; the columns alternate with the tiles
                 const uint32_t x_addr = tmem + lane_base + S::X_COL + 2 * (jj & 1);
                 tmem_st1(x_addr + wg, top);
@@ -772,8 +894,9 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
             // weights times 2^10: small ones keep their f16 bits, and the sum carries the same factor
             const float base = m == -INFINITY ? 0.0f : 10.0f - m;
             float2 sum = make_float2(0.0f, 0.0f);
+            float weight = 0.0f;  // 8-bit codes: the columns' sums, each times its 1 / v
             {
-                const float2 fs2 = make_float2(fs, fs), base2 = make_float2(base, base);
+                float2 fs2 = make_float2(fs, fs), base2 = make_float2(base, base);
                 uint32_t v[2][16];
                 tmem_ld16(s_addr, v[0]);
 #pragma unroll
@@ -782,6 +905,14 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
                     uint32_t p[16];
                     tmem_wait_ld(u);
                     if (c + 16 < CW) tmem_ld16(s_addr + c + 16, v[(c / 16 + 1) & 1]);
+                    float4 z;
+                    if constexpr (Q8) {
+                        z = zs[c / 16];
+                        const float f1 = EXTRA ? 1.0f : z.x != z.x && !plain ? 1.0f : factor(z.x), b1 = base + z.y;
+                        fs2 = make_float2(f1, f1);
+                        base2 = make_float2(b1, b1);
+                        sum = make_float2(0.0f, 0.0f);
+                    }
 #pragma unroll
                     for (int e = 0; e < 16; e += 2) {
                         float2 x = ffma2(make_float2(__uint_as_float(u[e]), __uint_as_float(u[e + 1])), fs2, base2);
@@ -790,6 +921,7 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
                         sum = fadd2(sum, x);
                         split_weights(x.x, x.y, p[e / 2], p[8 + e / 2]);
                     }
+                    if constexpr (Q8) weight = fmaf(sum.x + sum.y, z.z, weight);
                     tmem_st16(s_addr + c, p);
                     if (HD != 256 && c + 16 == CW / 2) {
                         tmem_wait_st();
@@ -799,7 +931,7 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
                 }
             }
             tmem_wait_st();
-            l = fmaf(l, al, sum.x + sum.y);
+            l = fmaf(l, al, Q8 ? weight : sum.x + sum.y);
             if constexpr (HD == 256) {
                 // the last tile's product was computed while this softmax ran
                 if (jj) {
@@ -843,7 +975,7 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
         float off = l - l;
 #pragma unroll
         for (int e = 0; e < OW; e++) off += o[e] - o[e];
-        bool fine = off == 0.0f;
+        bool fine = Q8 || off == 0.0f;  // codes are always finite: a masked one is nothing times a weight of 0
         constexpr int PITCH = 36;
         float *st = reinterpret_cast<float *>(smem + tile * 2 * S::QPLANE) + (HD == 256 ? warp : warp & 3) * 32 * PITCH;
         uint64_t dst = reinterpret_cast<uint64_t>(a.out + (uint64_t)(c0 + token_of()) * a.out_stride + (uint64_t)head_of() * HD + half * 128);
@@ -873,8 +1005,10 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
                         *reinterpret_cast<const float4 *>(st + rr * PITCH + lane % 8 * 4);
             }
         }
-        uint32_t again = __ballot_sync(0xffffffffu, real && !fine && !*dead);
-        for (; again; again &= again - 1) slow_row<HD>(a, s, kh, R - lane + __ffs(again) - 1, half * 128, OW);
+        if constexpr (!Q8) {
+            uint32_t again = __ballot_sync(0xffffffffu, real && !fine && !*dead);
+            for (; again; again &= again - 1) slow_row<HD>(a, s, kh, R - lane + __ffs(again) - 1, half * 128, OW);
+        }
         tc_fence_before();
     }
     __syncthreads();
@@ -888,7 +1022,7 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
 // Grid (row steps, n_kv, n_seq).
 constexpr int kPpJoinRows = 8;
 
-template <int HD>
+template <int HD, bool Q8>
 __global__ void __launch_bounds__(kPpJoinRows * 32) k_paged_prompt_join(const __grid_constant__ PagedAttnArgs a) {
     using S = PpShape<HD>;
     constexpr int PER = HD / 64;  // float2 per lane
@@ -929,11 +1063,11 @@ __global__ void __launch_bounds__(kPpJoinRows * 32) k_paged_prompt_join(const __
     float off = l - l;
 #pragma unroll
     for (int e = 0; e < PER; e++) off += (acc[e].x - acc[e].x) + (acc[e].y - acc[e].y);
-    if (__all_sync(0xffffffffu, off == 0.0f)) {
+    if (Q8 || __all_sync(0xffffffffu, off == 0.0f)) {
         float *dst = a.out + (uint64_t)(c0 + R / a.group) * a.out_stride + (uint64_t)(kh * a.group + R % a.group) * HD + 2 * lane;
 #pragma unroll
         for (int e = 0; e < PER; e++) *reinterpret_cast<float2 *>(dst + 64 * e) = make_float2(acc[e].x * inv, acc[e].y * inv);
-    } else {
+    } else if constexpr (!Q8) {
         slow_row<HD>(a, s, kh, R, 0, HD);
     }
 }
@@ -1000,42 +1134,60 @@ uint64_t pp_records(const PagedAttnArgs &a) {  // rows of all records
 // Fewest rows for this kernel (see paged_prompt_supported).
 constexpr uint32_t kPpMinRows = 16, kPpMinRowsShort = 32;
 
-template <int HD, bool EXTRA>
+template <int HD, bool EXTRA, bool Q8>
 cudaError_t pp_launch(const LaunchCfg &c, const PagedAttnArgs &a) {
-    using S = PpShape<HD>;
+    using S = PpShape<HD, Q8>;
     PpMaps maps;
-    pp_maps(a.kv, S::KT, maps);
+    maps.rows = 0;
+    if (!Q8) pp_maps(a.kv, S::KT, maps);
     const uint64_t ctas = (uint64_t)a.row_blocks * a.nsplit * a.kv.n_kv * a.n_seq;
     if (ctas > 0x7fffffffull) return cudaErrorInvalidValue;
-    cudaError_t e = launch_k(c, "paged_prompt", k_paged_prompt<HD, EXTRA>, dim3((uint32_t)ctas), dim3(kPpThreads), S::SMEM, a,
+    cudaError_t e = launch_k(c, "paged_prompt", k_paged_prompt<HD, EXTRA, Q8>, dim3((uint32_t)ctas), dim3(kPpThreads), S::SMEM, a,
                              maps);
     if (e != cudaSuccess || a.nsplit == 1) return e;
     const uint32_t rows = a.max_q * a.group;
-    return launch_k(c, "paged_prompt_join", k_paged_prompt_join<HD>,
+    return launch_k(c, "paged_prompt_join", k_paged_prompt_join<HD, Q8>,
                     dim3((rows + kPpJoinRows - 1) / kPpJoinRows, a.kv.n_kv, a.n_seq), dim3(kPpJoinRows * 32), 0, a);
 }
 
 // The register split needs the registers that 168 per thread give a block.
-template <int HD, bool EXTRA>
+template <int HD, bool EXTRA, bool Q8>
 bool pp_regs() {
     cudaFuncAttributes f;
-    if (cudaFuncGetAttributes(&f, k_paged_prompt<HD, EXTRA>) == cudaSuccess) return f.numRegs >= 168;
+    if (cudaFuncGetAttributes(&f, k_paged_prompt<HD, EXTRA, Q8>) == cudaSuccess) return f.numRegs >= 168;
     cudaGetLastError();
     return false;
+}
+
+template <bool Q8>
+bool pp_regs_all() {
+    return pp_regs<64, false, Q8>() && pp_regs<64, true, Q8>() && pp_regs<128, false, Q8>() && pp_regs<128, true, Q8>() &&
+           pp_regs<256, false, Q8>() && pp_regs<256, true, Q8>();
+}
+
+template <bool Q8>
+cudaError_t pp_launch_hd(const LaunchCfg &c, const PagedAttnArgs &a) {
+    const bool extra = a.softcap != 0.0f || a.slopes;
+    switch (a.kv.hd) {
+    case 64: return extra ? pp_launch<64, true, Q8>(c, a) : pp_launch<64, false, Q8>(c, a);
+    case 128: return extra ? pp_launch<128, true, Q8>(c, a) : pp_launch<128, false, Q8>(c, a);
+    case 256: return extra ? pp_launch<256, true, Q8>(c, a) : pp_launch<256, false, Q8>(c, a);
+    default: return cudaErrorInvalidValue;
+    }
 }
 
 }  // namespace
 
 bool paged_prompt_supported(const PagedAttnArgs &a) {
-    static const bool regs = pp_regs<64, false>() && pp_regs<64, true>() && pp_regs<128, false>() &&
-                             pp_regs<128, true>() && pp_regs<256, false>() && pp_regs<256, true>();
+    static const bool regs = pp_regs_all<false>(), regs_q8 = pp_regs_all<true>();
     // Few rows: the kernel for single tokens reads the cache once per 8 rows.  Measured there and here,
     // over head_dim 64, 128 and 256: 8 rows of 8 sequences of 8000 cached tokens 23, 41 and 114 us and
     // 30, 65 and 206; 16 rows of them 33, 59 and 218 us and 30, 69 and 206; 32 rows 52, 99 and 424 us and
     // 30, 68 and 207.  A cache of 60 tokens: 28 to 32 rows 7.3, 7.8 and 19.5 us and 10.2, 12.6 and 13.7,
     // 56 rows 16, 18 and 20 us and 10, 13 and 14; of 200 tokens, 16 rows 16, 17 and 19 us and 13, 16 and 16.
     const uint64_t rows = (uint64_t)a.max_q * a.group;
-    return regs && a.kv.f16 && rows > (a.max_len > 256 ? kPpMinRows : kPpMinRowsShort);
+    if (a.kv.k_scale ? !regs_q8 : !regs || !a.kv.f16) return false;
+    return rows > (a.max_len > 256 ? kPpMinRows : kPpMinRowsShort);
 }
 
 size_t paged_prompt_scratch(PagedAttnArgs a, int num_sms) {
@@ -1050,7 +1202,8 @@ size_t paged_prompt_scratch_most(const PagedAttnArgs &a, int num_sms) {
     const size_t records = (size_t)num_sms * pp_rows(a) * (a.kv.hd + 2) * 4;
     PagedAttnArgs few = a;
     few.max_q = min(a.max_q, kPpMinRowsShort / a.group);
-    return few.max_q ? max(records, paged_attn_scratch(few, num_sms)) : records;
+    if (!few.max_q) return records;
+    return max(records, few.kv.k_scale ? paged_q8_attn_scratch(few, num_sms) : paged_attn_scratch(few, num_sms));
 }
 
 cudaError_t launch_paged_prompt(const LaunchCfg &c, PagedAttnArgs a, uint8_t *scratch) {
@@ -1058,13 +1211,7 @@ cudaError_t launch_paged_prompt(const LaunchCfg &c, PagedAttnArgs a, uint8_t *sc
     pp_split(a, c.num_sms);
     a.part_o = (float *)scratch;
     a.part_ml = a.part_o + (a.nsplit == 1 ? 0 : pp_records(a) * a.kv.hd);
-    const bool extra = a.softcap != 0.0f || a.slopes;
-    switch (a.kv.hd) {
-    case 64: return extra ? pp_launch<64, true>(c, a) : pp_launch<64, false>(c, a);
-    case 128: return extra ? pp_launch<128, true>(c, a) : pp_launch<128, false>(c, a);
-    case 256: return extra ? pp_launch<256, true>(c, a) : pp_launch<256, false>(c, a);
-    default: return cudaErrorInvalidValue;
-    }
+    return a.kv.k_scale ? pp_launch_hd<true>(c, a) : pp_launch_hd<false>(c, a);
 }
 
 }  // namespace lt

@@ -81,15 +81,6 @@ LT_DEVINL void ldsm_t8(uint32_t (&r)[4], uint32_t addr) {
                  : "r"(addr)
                  : "memory");
 }
-// Four signed bytes as f16.
-LT_DEVINL void s8_to_f16(uint32_t w, uint32_t &b0, uint32_t &b1) {
-    const uint32_t x = w ^ 0x80808080u;
-    const uint32_t p = __byte_perm(x, 0x64646464u, 0x4140), q = __byte_perm(x, 0x64646464u, 0x4342);
-    const __half2 off = __float2half2_rn(1152.0f);
-    const __half2 u = __hsub2(*reinterpret_cast<const __half2 *>(&p), off), v = __hsub2(*reinterpret_cast<const __half2 *>(&q), off);
-    b0 = *reinterpret_cast<const uint32_t *>(&u);
-    b1 = *reinterpret_cast<const uint32_t *>(&v);
-}
 LT_DEVINL void cp_async4(uint32_t dst, const void *src) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
 }
