@@ -13,7 +13,7 @@
 //   warps 0-3, 4-7   softmax of row tile 0 and 1, a thread per row.  head_dim 256:
 //                    both on the one row tile, each half of the keys and of O.
 //   warp 8           issues the MMAs
-//   warps 9-11       bring K and V tiles from their pages into a ring of stages of
+//   warps 9-11 (-15) bring K and V tiles from their pages into a ring of stages of
 //                    128-byte-swizzled rows: tiles that lie wholly within the
 //                    sequence by TMA, a box per page and 64 columns; the ragged
 //                    ends, and pages that are no multiple of 8 slots, by 16-byte
@@ -44,7 +44,6 @@
 
 namespace lt {
 
-constexpr int kPpThreads = 384, kPpProducers = 96;
 // Tiles whose documents are looked at beforehand: 512 bytes of bits, what shared memory leaves beside the queries and
 // the ring at head_dim 128.  Longer rows (512 K keys; 256 K at head_dim 256) go through every tile.
 constexpr int kPpSkipTiles = 4096;
@@ -58,17 +57,22 @@ struct PpShape {
     static constexpr int STAGE = KT * HD * 2;
     static constexpr int STAGES = HD == 64 ? 6 : 3;
     static constexpr int DOCS = HD == 64 ? 4 : 2;         // document-number buffers
-    // registers per thread after the split: 256 softmax threads and 128 others share the 384 x 168 of the launch
-    static constexpr int REGS_SOFTMAX = HD == 64 ? 200 : 208, REGS_REST = HD == 64 ? 104 : 88;
-    static_assert(256 * REGS_SOFTMAX + 128 * REGS_REST <= kPpThreads * 168, "more registers than the launch holds");
+    // 8-bit codes: seven copying warps instead of three, since a stage is refilled only as fast as its codes become f16
+    // (8192 tokens, 32/4 heads of 128: 1.22 ms with three, head_dim 256, 4096 tokens: 0.56)
+    static constexpr int THREADS = Q8 ? 512 : 384, REST = THREADS - 256, PRODUCERS = REST - 32;
+    // registers per thread after the split: 256 softmax threads and the others share those of the launch
+    static constexpr int REGS = Q8 ? 128 : 168;
+    static constexpr int REGS_SOFTMAX = HD == 64 ? 200 : 208, REGS_REST = Q8 ? (HD == 64 ? 56 : 48) : HD == 64 ? 104 : 88;
+    static_assert(256 * REGS_SOFTMAX + REST * REGS_REST <= THREADS * REGS, "more registers than the launch holds");
     static constexpr int QPLANE = 128 * HD * 2;
     static constexpr int Q_BYTES = TILES * 2 * QPLANE;
     static constexpr int OFF_RING = Q_BYTES;
     static constexpr int OFF_OFFS = OFF_RING + STAGES * STAGE;
     static constexpr int GROUPS = KT / 16;                // of 16 keys, each within a page and a block
-    static constexpr int OFF_DOCS = OFF_OFFS + (Q8 ? GROUPS : KT) * 8;
-    static constexpr int OFF_SCALES = OFF_DOCS + DOCS * KT * 4;  // 8-bit codes: {k, log2 v, 1 / v} of each group
-    static constexpr int OFF_SKIP = OFF_SCALES + (Q8 ? DOCS * GROUPS * 16 : 0);
+    // f16: places of a tile's rows; 8-bit codes: places and scales of the groups of two tiles
+    static constexpr int OFF_DOCS = OFF_OFFS + (Q8 ? 2 * GROUPS * 16 : KT * 8);
+    static constexpr int OFF_SCALES = OFF_DOCS + DOCS * KT * 4;  // 8-bit codes: k, log2 v and 1 / v of each group
+    static constexpr int OFF_SKIP = OFF_SCALES + (Q8 ? DOCS * GROUPS * 12 + 16 : 0);
     static constexpr int OFF_BARS = OFF_SKIP + kPpSkipTiles / 8;
     static constexpr int SMEM = OFF_BARS + 256;
     static constexpr uint32_t S_COL(int i) { return (HD == 256 ? 64 : 128) * i; }
@@ -188,14 +192,14 @@ struct IntC {
 };
 
 template <int HD, bool EXTRA, bool Q8>
-__global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_constant__ PagedAttnArgs a,
-                                                                const __grid_constant__ PpMaps maps) {
+__global__ void __launch_bounds__(PpShape<HD, Q8>::THREADS, 1) k_paged_prompt(const __grid_constant__ PagedAttnArgs a,
+                                                                              const __grid_constant__ PpMaps maps) {
     using S = PpShape<HD, Q8>;
-    constexpr int KT = S::KT, NS = S::STAGES;
+    constexpr int KT = S::KT, NS = S::STAGES, kPpThreads = S::THREADS, kPpProducers = S::PRODUCERS;
     extern __shared__ __align__(1024) uint8_t smem[];
     uint64_t *offs = reinterpret_cast<uint64_t *>(smem + S::OFF_OFFS);
     uint32_t *docs_s = reinterpret_cast<uint32_t *>(smem + S::OFF_DOCS);
-    float4 *scales_s = reinterpret_cast<float4 *>(smem + S::OFF_SCALES);
+    float *scales_s = reinterpret_cast<float *>(smem + S::OFF_SCALES);  // [DOCS][3][GROUPS]
     uint32_t *skip = reinterpret_cast<uint32_t *>(smem + S::OFF_SKIP);  // bit set: some row may see the tile
     uint64_t *full = reinterpret_cast<uint64_t *>(smem + S::OFF_BARS), *empty = full + NS;
     uint64_t *s_full = empty + NS, *p_full = s_full + 2, *o_full = p_full + 2, *p_half = o_full + 2;
@@ -282,7 +286,7 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
         regs_dec<S::REGS_REST>();
         if (skipping) {
             // a tile is left out when the ranges of document numbers do not meet
-            for (int i = tid - 256; i < kPpSkipTiles / 32; i += 128) skip[i] = 0;
+            for (int i = tid - 256; i < kPpSkipTiles / 32; i += S::REST) skip[i] = 0;
             uint32_t dmin = 0xffffffffu, dmax = 0;
             for (int64_t i = max((int64_t)0, i0) + lane; i <= i1; i += 32) {
                 dmin = min(dmin, docs[i]);
@@ -290,8 +294,8 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
             }
             dmin = __reduce_min_sync(0xffffffffu, dmin);
             dmax = __reduce_max_sync(0xffffffffu, dmax);
-            named_sync<4, 128>();
-            for (uint32_t t = begin + warp - 8; t < tiles; t += 4) {
+            named_sync<4, S::REST>();
+            for (uint32_t t = begin + warp - 8; t < tiles; t += S::REST / 32) {
                 uint32_t kmin = 0xffffffffu, kmax = 0;
     #pragma unroll
                 for (int e = 0; e < KT / 32; e++) {
@@ -312,33 +316,36 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
             const int pt = tid - 288, pw = warp - 9;
             if constexpr (Q8) {
                 constexpr int CH = HD / 16, CHUNKS = KT * CH, PER = (CHUNKS + kPpProducers - 1) / kPpProducers;
-                uint4 v[PER];        // the next stage's codes: chunk c = pt + 96 i, column c % CH of row c / CH
-                uint64_t at = ~0ull; // threads pt < GROUPS: place of group pt of the next tile, and its scales
-                float ks = 0.0f, vs = 0.0f;
-                auto look = [&](uint32_t tt) {
-                    if (pt >= S::GROUPS) return;
-                    const uint32_t key = lo + tt * KT + 16 * pt;
-                    at = ~0ull;
-                    ks = vs = 0.0f;
-                    if (key >= hi || key + 16 <= first) return;
-                    const uint32_t page = table[page_of(a.kv, key)];
-                    if (page >= a.kv.n_pages) {
-                        atomicExch(a.err, DEV_ERR_BAD_INDEX);
-                        return;
-                    }
-                    at = paged_offset(a.kv, page, key, kh);
-                    const uint64_t sc = q8_scale_at(a.kv, page, key, kh);
-                    ks = a.kv.k_scale[sc];
-                    vs = a.kv.v_scale[sc];
+                uint4 v[PER];  // the next stage's codes: chunk c = pt + i PRODUCERS, column c % CH of row c / CH
+                struct Group {
+                    uint64_t at;  // ~0: not there
+                    float k, v;
                 };
-                auto fetch = [&](const uint8_t *pool) {
+                Group *groups = reinterpret_cast<Group *>(offs);  // of two tiles
+                auto look = [&](uint32_t tt, uint32_t buf) {
+                    if (pt >= S::GROUPS) return;
+                    Group x = {~0ull, 0.0f, 0.0f};
+                    const uint32_t key = lo + tt * KT + 16 * pt;
+                    if (key < hi && key + 16 > first) {
+                        const uint32_t page = table[page_of(a.kv, key)];
+                        if (page < a.kv.n_pages) {
+                            const uint64_t sc = q8_scale_at(a.kv, page, key, kh);
+                            x = {paged_offset(a.kv, page, key, kh), a.kv.k_scale[sc], a.kv.v_scale[sc]};
+                        } else {
+                            atomicExch(a.err, DEV_ERR_BAD_INDEX);
+                        }
+                    }
+                    groups[buf * S::GROUPS + pt] = x;
+                };
+                auto fetch = [&](const uint8_t *pool, uint32_t buf) {
+                    pool += pt % CH * 16;
 #pragma unroll
                     for (int i = 0; i < PER; i++) {
-                        const int c = pt + i * kPpProducers, r = c / CH;
-                        const uint64_t o = c < CHUNKS ? offs[r / 16] : ~0ull;
+                        static_assert(kPpProducers % CH == 0, "one column per thread");
+                        const uint32_t r = pt / CH + i * (kPpProducers / CH);
+                        const uint64_t o = r < KT ? groups[buf * S::GROUPS + r / 16].at : ~0ull;
                         v[i] = make_uint4(0, 0, 0, 0);  // groups that are not there: zeros, which no weight of 0 makes NaN
-                        if (o != ~0ull)
-                            v[i] = *reinterpret_cast<const uint4 *>(pool + o + (uint64_t)(r % 16) * a.kv.slot_stride + c % CH * 16);
+                        if (o != ~0ull) v[i] = *reinterpret_cast<const uint4 *>(pool + o + (uint64_t)(r % 16) * (uint32_t)a.kv.slot_stride);
                     }
                 };
                 uint32_t st = 0, turn = 0;
@@ -353,15 +360,22 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
                                     docs_s[(jj % S::DOCS) * KT + r] = j < hi ? docs[j] : 0;
                                 }
                             if (pt < S::GROUPS) {
-                                const Q8Scale z = q8_scale(ks, vs);
-                                scales_s[(jj % S::DOCS) * S::GROUPS + pt] = make_float4(z.k, z.v_log2, z.v_inv, 0.0f);
+                                // Scales that cannot be used: weights above all others', and a sum that is NaN.  The factor on
+                                // scores stays a number: masked ones must stay -inf.
+                                const Group &x = groups[(jj & 1) * S::GROUPS + pt];
+                                const Q8Scale z = q8_scale(x.k, x.v);
+                                const bool good = z.k == z.k;
+                                float *to = scales_s + (jj % S::DOCS) * 3 * S::GROUPS + pt;
+                                to[0] = good ? z.k : 0.0f;
+                                to[S::GROUPS] = good ? z.v_log2 : 3e38f;
+                                to[2 * S::GROUPS] = good ? z.v_inv : __int_as_float(0x7fffffff);
                             }
                         }
                         uint8_t *stage = smem + S::OFF_RING + st * S::STAGE;
 #pragma unroll
                         for (int i = 0; i < PER; i++) {
-                            const int c = pt + i * kPpProducers, r = c / CH, col = 2 * (c % CH);
-                            if (c >= CHUNKS) break;
+                            const int r = pt / CH + i * (kPpProducers / CH), col = 2 * (pt % CH);
+                            if (r >= KT) break;
                             uint4 h0, h1;
                             s8_to_f16(v[i].x, h0.x, h0.y);
                             s8_to_f16(v[i].y, h0.z, h0.w);
@@ -376,26 +390,21 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
                     }
                     if (++st == NS) st = 0, turn++;
                 };
-                auto publish = [&]() {  // the next tile's places, once everybody has the last one's codes on their way
-                    named_sync<1, kPpProducers>();
-                    if (pt < S::GROUPS) offs[pt] = at;
-                    named_sync<1, kPpProducers>();
-                };
                 uint32_t t = next_tile(begin), jj = 0;
                 if (t < tiles) {
-                    look(t);
-                    publish();
-                    fetch(a.kv.k);
+                    look(t, 0);
+                    named_sync<1, kPpProducers>();
+                    fetch(a.kv.k, 0);
                 }
                 while (t < tiles) {
                     const uint32_t tn = next_tile(t + 1);
                     hand_over(true, t, jj);
-                    fetch(a.kv.v);
-                    if (tn < tiles) look(tn);
+                    fetch(a.kv.v, jj & 1);
+                    if (tn < tiles) look(tn, (jj + 1) & 1);  // its buffer's tile is fetched since the last barrier
                     hand_over(false, t, jj);
                     if (tn < tiles) {
-                        publish();
-                        fetch(a.kv.k);
+                        named_sync<1, kPpProducers>();
+                        fetch(a.kv.k, (jj + 1) & 1);
                     }
                     t = tn;
                     jj++;
@@ -774,12 +783,9 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
             // pass 1: the row's maximum; capped, biased or masked scores go back to tensor
             // memory.  Each load runs while the columns before it are worked on.
             float top = -INFINITY;
-            const float4 *zs = scales_s + (jj % S::DOCS) * S::GROUPS + half * 2;  // this thread's columns' scales, 16 to each
-            // the factor on 16 columns' raw scores: not 0, by which a masked score's -inf would become NaN; NaN stays
-            auto factor = [&](float k) {
-                const float f = rf * k;
-                return f < 1.17549435e-38f ? 1.17549435e-38f : f;
-            };
+            const float *zs = scales_s + (jj % S::DOCS) * 3 * S::GROUPS + half * 2;  // this thread's columns' scales, 16 to each
+            // the factor on 16 columns' raw scores: not 0, by which a masked score's -inf would become NaN
+            auto factor = [&](int c) { return fmaxf(rf * zs[c / 16], 1.17549435e-38f); };
             {
                 uint32_t v[2][16];
                 tmem_ld16(s_addr, v[0]);
@@ -800,20 +806,18 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
                             x1 = fmaxf(fmaxf(x1, __uint_as_float(u[e + 2])), __uint_as_float(u[e + 3]));
                         }
                         if constexpr (Q8) {
-                            const float4 z = zs[c / 16];
-                            top = fmaxf(top, fmaf(fmaxf(x0, x1), factor(z.x), z.y));
+                            top = fmaxf(top, fmaf(fmaxf(x0, x1), factor(c), zs[S::GROUPS + c / 16]));
                         } else {
                             top = fmaxf(top, fmaxf(x0, x1));
                         }
                         continue;
                     }
-                    const float4 z = Q8 ? zs[c / 16] : make_float4(1.0f, 0.0f, 1.0f, 0.0f);
                     if (EXTRA) {  // score_log2, the usual case two at a time
                         constexpr float kLog2e = 1.4426950408889634f;
                         float big = 0.0f;
 #pragma unroll
                         for (int e = 0; e < 16; e++) big = fmaxf(big, fabsf(__uint_as_float(u[e])));
-                        const float f1 = Q8 ? rf * z.x : rf;
+                        const float f1 = Q8 ? rf * zs[c / 16] : rf;
                         const float2 f2 = make_float2(f1, f1);
                         if (a.softcap == 0.0f) {
 #pragma unroll
@@ -844,10 +848,6 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
                         }
                     }
                     constexpr uint32_t kMinusInf = 0xff800000u;
-                    if (Q8 && !EXTRA && z.x != z.x) {  // no number: nor are the scores, but for those that the masks take
-#pragma unroll
-                        for (int e = 0; e < 16; e++) u[e] = 0x7fffffffu;
-                    }
                     if (!in_range) {
 #pragma unroll
                         for (int e = 0; e < 16; e++) u[e] = c + e >= from && c + e < to ? u[e] : kMinusInf;
@@ -867,7 +867,7 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
                         float x = -INFINITY;
 #pragma unroll
                         for (int e = 0; e < 16; e++) x = fmaxf(x, __uint_as_float(u[e]));
-                        top = fmaxf(top, fmaf(x, EXTRA || z.x != z.x ? 1.0f : factor(z.x), z.y));
+                        top = fmaxf(top, fmaf(x, EXTRA ? 1.0f : factor(c), zs[S::GROUPS + c / 16]));
                     } else {
 #pragma unroll
                         for (int e = 0; e < 16; e++) top = fmaxf(top, __uint_as_float(u[e]));
@@ -905,10 +905,8 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
                     uint32_t p[16];
                     tmem_wait_ld(u);
                     if (c + 16 < CW) tmem_ld16(s_addr + c + 16, v[(c / 16 + 1) & 1]);
-                    float4 z;
                     if constexpr (Q8) {
-                        z = zs[c / 16];
-                        const float f1 = EXTRA ? 1.0f : z.x != z.x && !plain ? 1.0f : factor(z.x), b1 = base + z.y;
+                        const float f1 = EXTRA ? 1.0f : factor(c), b1 = base + zs[S::GROUPS + c / 16];
                         fs2 = make_float2(f1, f1);
                         base2 = make_float2(b1, b1);
                         sum = make_float2(0.0f, 0.0f);
@@ -921,7 +919,10 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
                         sum = fadd2(sum, x);
                         split_weights(x.x, x.y, p[e / 2], p[8 + e / 2]);
                     }
-                    if constexpr (Q8) weight = fmaf(sum.x + sum.y, z.z, weight);
+                    if constexpr (Q8) {
+                        const float all = sum.x + sum.y;
+                        if (all != 0.0f) weight = fmaf(all, zs[2 * S::GROUPS + c / 16], weight);
+                    }
                     tmem_st16(s_addr + c, p);
                     if (HD != 256 && c + 16 == CW / 2) {
                         tmem_wait_st();
@@ -1142,7 +1143,7 @@ cudaError_t pp_launch(const LaunchCfg &c, const PagedAttnArgs &a) {
     if (!Q8) pp_maps(a.kv, S::KT, maps);
     const uint64_t ctas = (uint64_t)a.row_blocks * a.nsplit * a.kv.n_kv * a.n_seq;
     if (ctas > 0x7fffffffull) return cudaErrorInvalidValue;
-    cudaError_t e = launch_k(c, "paged_prompt", k_paged_prompt<HD, EXTRA, Q8>, dim3((uint32_t)ctas), dim3(kPpThreads), S::SMEM, a,
+    cudaError_t e = launch_k(c, "paged_prompt", k_paged_prompt<HD, EXTRA, Q8>, dim3((uint32_t)ctas), dim3(S::THREADS), S::SMEM, a,
                              maps);
     if (e != cudaSuccess || a.nsplit == 1) return e;
     const uint32_t rows = a.max_q * a.group;
@@ -1150,11 +1151,11 @@ cudaError_t pp_launch(const LaunchCfg &c, const PagedAttnArgs &a) {
                     dim3((rows + kPpJoinRows - 1) / kPpJoinRows, a.kv.n_kv, a.n_seq), dim3(kPpJoinRows * 32), 0, a);
 }
 
-// The register split needs the registers that 168 per thread give a block.
+// The register split needs the registers that a block is launched with.
 template <int HD, bool EXTRA, bool Q8>
 bool pp_regs() {
     cudaFuncAttributes f;
-    if (cudaFuncGetAttributes(&f, k_paged_prompt<HD, EXTRA, Q8>) == cudaSuccess) return f.numRegs >= 168;
+    if (cudaFuncGetAttributes(&f, k_paged_prompt<HD, EXTRA, Q8>) == cudaSuccess) return f.numRegs >= PpShape<HD, Q8>::REGS;
     cudaGetLastError();
     return false;
 }
