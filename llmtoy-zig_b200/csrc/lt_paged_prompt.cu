@@ -62,7 +62,8 @@ struct PpShape {
     static constexpr int THREADS = Q8 ? 512 : 384, REST = THREADS - 256, PRODUCERS = REST - 32;
     // registers per thread after the split: 256 softmax threads and the others share those of the launch
     static constexpr int REGS = Q8 ? 128 : 168;
-    static constexpr int REGS_SOFTMAX = HD == 64 ? 200 : 208, REGS_REST = Q8 ? (HD == 64 ? 56 : 48) : HD == 64 ? 104 : 88;
+    static constexpr int REGS_SOFTMAX = Q8 ? (HD == 64 ? 184 : HD == 128 ? 192 : 176) : HD == 64 ? 200 : 208;
+    static constexpr int REGS_REST = Q8 ? (HD == 64 ? 72 : HD == 128 ? 64 : 80) : HD == 64 ? 104 : 88;
     static_assert(256 * REGS_SOFTMAX + REST * REGS_REST <= THREADS * REGS, "more registers than the launch holds");
     static constexpr int QPLANE = 128 * HD * 2;
     static constexpr int Q_BYTES = TILES * 2 * QPLANE;
