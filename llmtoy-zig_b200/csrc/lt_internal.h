@@ -185,6 +185,7 @@ struct PagedAttnArgs {
     uint32_t *unit_info;
     uint32_t row_blocks;            // row blocks per (sequence, KV head) at most
     uint32_t nsplit;                // lt_paged_prompt.cu: CTAs that share a row block's keys
+    uint32_t join_units;            // lt_paged_q8_attn.cu: the join's list is by units
     int *err;
 };
 size_t paged_attn_scratch(const PagedAttnArgs &a, int num_sms);

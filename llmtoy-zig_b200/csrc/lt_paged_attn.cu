@@ -672,11 +672,11 @@ __global__ void __launch_bounds__(128) k_paged_finish(const __grid_constant__ Pa
     if constexpr (PROMPT) {  // many units, few of them shared: a CTA looks at one unit
         if (a.unit_info[2 * (uint64_t)blockIdx.x + 1] < 2) return;
         for (uint32_t r = 0; r < kPaRows; r++) {
-            pa_join_row<HD, PROMPT, PROMPT>(a, blockIdx.x, r);
+            pa_join_row<HD, PROMPT>(a, blockIdx.x, r);
             __syncthreads();
         }
     } else if (blockIdx.x < n_join) {  // few units: a CTA does one row
-        pa_join_row<HD, PROMPT, PROMPT>(a, blockIdx.x / kPaRows, blockIdx.x % kPaRows);
+        pa_join_row<HD, PROMPT>(a, blockIdx.x / kPaRows, blockIdx.x % kPaRows);
     } else {
         const uint32_t b = blockIdx.x - n_join, steps = (a.max_len + kMassKeys - 1) / kMassKeys;
         pa_mass(a, b / steps / a.kv.n_kv, b / steps % a.kv.n_kv, b % steps * kMassKeys);

@@ -90,6 +90,13 @@ LT_DEVINL uint4 lds_u4(uint32_t addr) {
     return v;
 }
 
+// What the join needs to know of a unit that CTAs first .. first + n - 1 share.  The list has a place per unit
+// (a.join_units: decode, where every unit is there) or, where there are more units than CTAs and for rows of prompts,
+// one per CTA, for the unit that begins there and goes on elsewhere (n = 0: none does).
+struct Q8Join {
+    uint32_t first, n, rows, kh, rb, q0, unused[2];
+};
+
 // PLAIN: neither cap nor distance bias.
 template <int HD, bool PROMPT, bool PLAIN>
 __global__ void __launch_bounds__(kPaThreads, Q8Shape<HD>::CTAS) k_paged_q8(const __grid_constant__ PagedAttnArgs a) {
@@ -144,7 +151,10 @@ __global__ void __launch_bounds__(kPaThreads, Q8Shape<HD>::CTAS) k_paged_q8(cons
     }
     // no more CTAs than tiles, so that every CTA of a unit leaves a record
     const uint32_t G = (uint32_t)min((uint64_t)gridDim.x, T);
-    if (c >= G) return;
+    if (c >= G) {
+        if (!a.join_units && tid == 0) reinterpret_cast<Q8Join *>(a.unit_info)[c].n = 0;
+        return;
+    }
     const PaShare share(T, G);
     uint64_t f0 = share.start(c);
     const uint64_t f1 = share.start(c + 1);
@@ -170,7 +180,10 @@ __global__ void __launch_bounds__(kPaThreads, Q8Shape<HD>::CTAS) k_paged_q8(cons
     cw.tile = (uint32_t)(s_rem - (uint64_t)cw.unit * cw.q.cost());
     if (cw.tile >= cw.q.tiles) {  // in what the unit before costs beyond its tiles
         f0 += cw.q.cost() - cw.tile;
-        if (f0 >= f1) return;
+        if (f0 >= f1) {
+            if (!a.join_units && tid == 0) reinterpret_cast<Q8Join *>(a.unit_info)[c].n = 0;
+            return;
+        }
         cw.template next_unit<TILE>(a);
     } else {
         cw.set_unit(a);
@@ -289,6 +302,7 @@ __global__ void __launch_bounds__(kPaThreads, Q8Shape<HD>::CTAS) k_paged_q8(cons
 
     uint64_t f = f0;
     int stage = 0;
+    bool continues = false;  // a unit begins here and goes on elsewhere
     while (f < f1) {
         // ── one segment: this CTA's tiles of one unit ──
         const uint32_t seg = (uint32_t)min((uint64_t)(cw.q.tiles - cw.tile), f1 - f);
@@ -511,10 +525,9 @@ __global__ void __launch_bounds__(kPaThreads, Q8Shape<HD>::CTAS) k_paged_q8(cons
         const uint32_t first = share.owner(unit_f0), last = share.owner(unit_f0 + cw.q.tiles - 1);
         const bool whole_unit = first == last, begins = unit_f0 == f;
         const uint64_t u = pa_unit(a, cw.s, cw.kh, cw.rb), part = 2 * (uint64_t)c + (begins ? 1 : 0);
-        if (begins && tid == 0) {
-            a.unit_info[2 * u] = first;
-            a.unit_info[2 * u + 1] = last - first + 1;
-        }
+        if (begins && tid == 0 && (a.join_units || !whole_unit))
+            reinterpret_cast<Q8Join *>(a.unit_info)[a.join_units ? u : c] = {first, last - first + 1, rows, cw.kh, cw.rb, cw.q.q0, {0, 0}};
+        continues |= begins && !whole_unit;
         __syncthreads();
         constexpr int D = HD / 4, RSTEP = kPaThreads / D;  // threads to a row, rows at a time
 #pragma unroll 1
@@ -562,22 +575,84 @@ __global__ void __launch_bounds__(kPaThreads, Q8Shape<HD>::CTAS) k_paged_q8(cons
         }
     }
     cp_async_wait<0>();
+    if (!a.join_units && !continues && tid == 0) reinterpret_cast<Q8Join *>(a.unit_info)[c].n = 0;
 }
 
-// Rows of units that several CTAs share.
-template <int HD, bool PROMPT>
-__global__ void __launch_bounds__(128) k_paged_q8_join(const __grid_constant__ PagedAttnArgs a) {
+// Row r of a unit that several CTAs share: out = sum_p 2^(m_p - m) o_p / sum_p 2^(m_p - m) l_p over its records
+// in CTA order.  Grid (8 rows of each entry of the list).  Few entries: 256 threads, so that nearly all records' sums
+// are on their way at once (74 records for each row: 31.8 us in all, 34.5 with 128); many, with few records each:
+// 128, of which more fit an SM (64 ragged sequences: 38.9 us, 43.0 with 256).
+template <int HD, int THREADS>
+__global__ void __launch_bounds__(THREADS) k_paged_q8_join(const __grid_constant__ PagedAttnArgs a) {
+    constexpr int LANES = HD / 4, GROUPS = THREADS / LANES, EARLY = THREADS == 256 ? 10 : 4, PER = kPaMaxParts / THREADS;
+    __shared__ float s_w[kPaMaxParts], s_top[THREADS / 32], s_sum[THREADS / 32];
+    __shared__ float4 s_o[THREADS];
     pdl_launch_dependents();
     pdl_wait();
-    if constexpr (PROMPT) {  // many units, few of them shared: a CTA looks at one unit
-        if (a.unit_info[2 * (uint64_t)blockIdx.x + 1] < 2) return;
-        for (uint32_t r = 0; r < kPaRows; r++) {
-            pa_join_row<HD, PROMPT, false>(a, blockIdx.x, r);
-            __syncthreads();
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, grp = tid / LANES, x = tid % LANES;
+    const uint32_t r = blockIdx.x % kPaRows;
+    const Q8Join in = reinterpret_cast<const Q8Join *>(a.unit_info)[blockIdx.x / kPaRows];
+    if (in.n < 2 || in.n > kPaMaxParts || r >= in.rows) return;
+    const auto sums = [&](uint32_t p) {
+        return *reinterpret_cast<const float4 *>(a.part_o + (pa_part(in.first, p) * kPaRows + r) * HD + 4 * x);
+    };
+    float4 v[EARLY];
+#pragma unroll
+    for (int i = 0; i < EARLY; i++)
+        if (grp + i * GROUPS < in.n) v[i] = sums(grp + i * GROUPS);
+    float pm[PER], pl[PER], m = -INFINITY, l = 0.0f;
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+        const uint32_t p = tid + THREADS * i;
+        pm[i] = -INFINITY;
+        pl[i] = 0.0f;
+        if (p < in.n) {
+            const float *ml = a.part_ml + pa_part(in.first, p) * 16 + r;
+            pm[i] = ml[0];
+            pl[i] = ml[8];
         }
-    } else {
-        pa_join_row<HD, PROMPT, false>(a, blockIdx.x / kPaRows, blockIdx.x % kPaRows);
+        m = fmaxf(m, pm[i]);
     }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if (lane == 0) s_top[warp] = m;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < THREADS / 32; w++) m = fmaxf(m, s_top[w]);
+    const float from = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+        const float w = ex2(pm[i] - from);
+        if (tid + THREADS * i < in.n) s_w[tid + THREADS * i] = w;
+        l = fmaf(pl[i], w, l);
+    }
+    l = warp_sum(l);
+    if (lane == 0) s_sum[warp] = l;
+    __syncthreads();
+    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    auto add = [&](const float4 &t, float w) {
+        acc.x = fmaf(t.x, w, acc.x);
+        acc.y = fmaf(t.y, w, acc.y);
+        acc.z = fmaf(t.z, w, acc.z);
+        acc.w = fmaf(t.w, w, acc.w);
+    };
+#pragma unroll
+    for (int i = 0; i < EARLY; i++)
+        if (grp + i * GROUPS < in.n) add(v[i], s_w[grp + i * GROUPS]);
+#pragma unroll 4
+    for (uint32_t p = grp + EARLY * GROUPS; p < in.n; p += GROUPS) add(sums(p), s_w[p]);
+    s_o[tid] = acc;
+    __syncthreads();
+    if (grp) return;
+    l = 0.0f;
+#pragma unroll
+    for (int w = 0; w < THREADS / 32; w++) l += s_sum[w];
+#pragma unroll
+    for (int i = 1; i < GROUPS; i++) add(s_o[i * LANES + x], 1.0f);
+    const float inv = l > 0.0f ? __fdiv_rn(1.0f, l) : (l == 0.0f ? 0.0f : l);
+    const uint32_t R = in.rb * kPaRows + r;
+    float *dst = a.out + (uint64_t)(in.q0 + R / a.group) * a.out_stride + (uint64_t)(in.kh * a.group + R % a.group) * HD + 4 * x;
+    *reinterpret_cast<float4 *>(dst) = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
 }
 
 namespace {
@@ -598,7 +673,7 @@ Q8Scratch q8_layout(const PagedAttnArgs &a, uint32_t G) {
     s.part_o = 0;
     s.part_ml = up256((size_t)2 * G * kPaRows * a.kv.hd * 4);
     s.unit_info = s.part_ml + up256((size_t)2 * G * 16 * 4);
-    s.total = s.unit_info + up256((size_t)a.n_seq * a.kv.n_kv * q8_row_blocks(a) * 8);
+    s.total = s.unit_info + up256((size_t)G * sizeof(Q8Join));
     return s;
 }
 
@@ -612,9 +687,10 @@ cudaError_t q8_launch(const LaunchCfg &c, const PagedAttnArgs &a) {
     else
         e = launch_k(c, label, k_paged_q8<HD, PROMPT, false>, grid, block, Q8Shape<HD>::SMEM, a);
     if (e != cudaSuccess) return e;
-    const uint64_t units = (uint64_t)a.n_seq * a.kv.n_kv * a.row_blocks, join = PROMPT ? units : units * kPaRows;
-    if (join > 0x7fffffffull) return cudaErrorInvalidValue;
-    return launch_k(c, "paged_q8_join", k_paged_q8_join<HD, PROMPT>, dim3((uint32_t)join), dim3(128), 0, a);
+    const uint32_t places = a.join_units ? a.n_seq * a.kv.n_kv * a.row_blocks : grid.x;
+    const dim3 rows(places * kPaRows);
+    if (rows.x <= 3u * (uint32_t)c.num_sms) return launch_k(c, "paged_q8_join", k_paged_q8_join<HD, 256>, rows, dim3(256), 0, a);
+    return launch_k(c, "paged_q8_join", k_paged_q8_join<HD, 128>, rows, dim3(128), 0, a);
 }
 
 }  // namespace
@@ -628,6 +704,7 @@ cudaError_t launch_paged_q8_attn(const LaunchCfg &c, PagedAttnArgs a, uint8_t *s
     a.unit_info = (uint32_t *)(scratch + s.unit_info);
     a.err = c.dev_err;
     a.row_blocks = q8_row_blocks(a);
+    a.join_units = !a.cu && (uint64_t)a.n_seq * a.kv.n_kv * a.row_blocks <= q8_grid(a.kv.hd, c.num_sms);
     switch (a.kv.hd) {
     case 64: return a.cu ? q8_launch<64, true>(c, a) : q8_launch<64, false>(c, a);
     case 128: return a.cu ? q8_launch<128, true>(c, a) : q8_launch<128, false>(c, a);

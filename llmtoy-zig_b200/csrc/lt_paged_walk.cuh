@@ -124,8 +124,7 @@ constexpr uint32_t kPaMaxParts = 512;  // CTAs of a launch at most (pa_grid), an
 
 // Row r of a unit that several CTAs share: out = sum_p 2^(m_p - m) o_p / sum_p 2^(m_p - m) l_p over
 // its records in CTA order.  The first records' sums are on their way while the weights are found.
-// AGAIN: a row that is not finite is done again by itself.
-template <int HD, bool PROMPT, bool AGAIN>
+template <int HD, bool PROMPT>
 LT_DEVINL void pa_join_row(const PagedAttnArgs &a, uint64_t u, uint32_t r) {
     constexpr int LANES = HD / 4, GROUPS = 128 / LANES, EARLY = 8;
     __shared__ float s_w[kPaMaxParts], s_red[4], s_red2[4];
@@ -205,9 +204,9 @@ LT_DEVINL void pa_join_row(const PagedAttnArgs &a, uint64_t u, uint32_t r) {
         const float inv = l > 0.0f ? __fdiv_rn(1.0f, l) : (l == 0.0f ? 0.0f : l);
         float *dst = a.out + (uint64_t)(q0 + R / a.group) * a.out_stride + (uint64_t)(kh * a.group + R % a.group) * HD + 4 * x;
         *reinterpret_cast<float4 *>(dst) = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
-        if (AGAIN && (acc.x - acc.x) + (acc.y - acc.y) + (acc.z - acc.z) + (acc.w - acc.w) + (l - l) != 0.0f) s_off = 1;
+        if (PROMPT && (acc.x - acc.x) + (acc.y - acc.y) + (acc.z - acc.z) + (acc.w - acc.w) + (l - l) != 0.0f) s_off = 1;
     }
-    if (AGAIN) {
+    if (PROMPT) {
         __syncthreads();
         if (s_off && warp == 0) slow_row<HD>(a, s, kh, R, 0, HD);
     }
