@@ -1133,8 +1133,14 @@ uint64_t pp_records(const PagedAttnArgs &a) {  // rows of all records
     return (uint64_t)a.n_seq * a.kv.n_kv * a.row_blocks * a.nsplit * pp_rows(a);
 }
 
-// Fewest rows for this kernel (see paged_prompt_supported).
-constexpr uint32_t kPpMinRows = 16, kPpMinRowsShort = 32;
+// Most rows for the kernel of single tokens, over a cache of more than 256 positions and of fewer (see paged_prompt_supported).
+struct PpFew {
+    uint32_t rows, rows_short;
+};
+PpFew pp_few(const PagedKvDev &kv) {
+    if (!kv.k_scale) return {16, 32};
+    return kv.hd == 64 ? PpFew{56, 56} : kv.hd == 128 ? PpFew{36, 80} : PpFew{26, 16};
+}
 
 template <int HD, bool EXTRA, bool Q8>
 cudaError_t pp_launch(const LaunchCfg &c, const PagedAttnArgs &a) {
@@ -1187,9 +1193,12 @@ bool paged_prompt_supported(const PagedAttnArgs &a) {
     // 30, 65 and 206; 16 rows of them 33, 59 and 218 us and 30, 69 and 206; 32 rows 52, 99 and 424 us and
     // 30, 68 and 207.  A cache of 60 tokens: 28 to 32 rows 7.3, 7.8 and 19.5 us and 10.2, 12.6 and 13.7,
     // 56 rows 16, 18 and 20 us and 10, 13 and 14; of 200 tokens, 16 rows 16, 17 and 19 us and 13, 16 and 16.
+    // 8-bit codes, the same shapes: 56 rows of 8000 tokens 34 and 34 us (head_dim 64), 32 and 48 rows 64, 90 and 70, 73 (128),
+    // 24 and 32 rows 165, 222 and 176, 176 (256); of 200 tokens, 64 and 96 rows 14, 20 and 18, 18.5 (128), 16 rows 18.5 and 18 (256).
     const uint64_t rows = (uint64_t)a.max_q * a.group;
     if (a.kv.k_scale ? !regs_q8 : !regs || !a.kv.f16) return false;
-    return rows > (a.max_len > 256 ? kPpMinRows : kPpMinRowsShort);
+    const PpFew few = pp_few(a.kv);
+    return rows > (a.max_len > 256 ? few.rows : few.rows_short);
 }
 
 size_t paged_prompt_scratch(PagedAttnArgs a, int num_sms) {
@@ -1203,7 +1212,7 @@ size_t paged_prompt_scratch(PagedAttnArgs a, int num_sms) {
 size_t paged_prompt_scratch_most(const PagedAttnArgs &a, int num_sms) {
     const size_t records = (size_t)num_sms * pp_rows(a) * (a.kv.hd + 2) * 4;
     PagedAttnArgs few = a;
-    few.max_q = min(a.max_q, kPpMinRowsShort / a.group);
+    few.max_q = min(a.max_q, max(pp_few(a.kv).rows, pp_few(a.kv).rows_short) / a.group);
     if (!few.max_q) return records;
     return max(records, few.kv.k_scale ? paged_q8_attn_scratch(few, num_sms) : paged_attn_scratch(few, num_sms));
 }
