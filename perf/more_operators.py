@@ -135,14 +135,15 @@ def _pkg():
     return importlib.import_module("llmtoy-zig_b200")
 
 
-_context = None
+_context = _stream = None
 
 
 def _ctx():
-    """The one device context that a program keeps."""
-    global _context
+    """The one device context that a program keeps, on a stream that it shares with torch."""
+    global _context, _stream
     if _context is None:
-        _context = _pkg().Context(0)
+        _context, _stream = _pkg().Context(0), torch.cuda.Stream()
+        _context.set_stream(_stream)
     return _context
 
 
@@ -282,7 +283,8 @@ def _own_plan(st):
 def _own_append(st):
     _ctx().paged_q8_append(st["cfg"], st["kvh"], st["qkv"], st["case"]["seqs"], st["cu"], st["total"], st["max_q"], st["qn"],
                            st["kn"], None, st["table"], st["lens"], st["q"])
-    return _append_outputs(st)
+    with torch.cuda.stream(_stream):  # behind the call
+        return _append_outputs(st)
 
 
 def _own_decode(st):
