@@ -11,19 +11,17 @@
 // sine and cosine: an angle in f32 alone is off by up to half a unit in its last place, 2e-4 at
 // position 4000.
 //
-// Bound: memory.  A CTA takes one block of one sequence; a warp one head vector of all of
-// the block's tokens, 16 at a time, so that a block of 16 stays in registers between its
-// maximum and its codes.  Longer blocks are read again (from L2).
+// Bound: memory (each value is read and written once).  A CTA takes one block of one
+// sequence; teams of its warps go through the head vectors, each warp with CHUNK of the block's
+// tokens in registers from the load to the codes, the team's maximum through shared
+// memory.  What costs instructions otherwise is shared among tokens: the sums of squares
+// of a chunk are reduced together (16 rows: 16 shuffles instead of 80, one square root per
+// lane instead of 16), and a code is the low byte of x / scale + 1.5 * 2^23, one operation.
 #include "lt_paged_q8.cuh"
 
 namespace lt {
 
-constexpr int kQaThreads = 256, kQaWarps = kQaThreads / 32, kQaChunk = 16;
-
-template <int N>
-struct QaInt {
-    static constexpr int value = N;
-};
+constexpr int kQaThreads = 256, kQaWarps = kQaThreads / 32;
 
 // A sequence's share of the call: n new rows from row c0 on, its first new position, and the blocks they lie in.
 struct QaSeq {
@@ -67,31 +65,47 @@ LT_DEVINL void qa_store(float *p, const float (&v)[N]) {
     else
         p[0] = v[0];
 }
-LT_DEVINL uint32_t qa_code(float x, float scale) {  // scale > 0
-    return (uint32_t)(int)fminf(fmaxf(rintf(__fdiv_rn(x, scale)), -127.0f), 127.0f) & 0xffu;
-}
+// Codes of N values times r: the low bytes of x r + 1.5 * 2^23, whose unit is 1 (|x r| is at most 127 and a bit).
 template <int N>
-LT_DEVINL void qa_store_codes(uint8_t *p, const float (&v)[N], float scale) {
-    uint32_t w = 0;
-    if (scale > 0.0f) {
+LT_DEVINL void qa_store_codes(uint8_t *p, const float (&v)[N], float r) {
+    uint32_t w[N];
 #pragma unroll
-        for (int e = 0; e < N; e++) w |= qa_code(v[e], scale) << (8 * e);
-    }
+    for (int e = 0; e < N; e++) w[e] = __float_as_uint(fmaf(v[e], r, 12582912.0f));
     if constexpr (N == 4)
-        *reinterpret_cast<uint32_t *>(p) = w;
+        *reinterpret_cast<uint32_t *>(p) = __byte_perm(__byte_perm(w[0], w[1], 0x0040), __byte_perm(w[2], w[3], 0x0040), 0x5410);
     else if constexpr (N == 2)
-        *reinterpret_cast<uint16_t *>(p) = (uint16_t)w;
+        *reinterpret_cast<uint16_t *>(p) = (uint16_t)__byte_perm(w[0], w[1], 0x0040);
     else
-        *p = (uint8_t)w;
+        *p = (uint8_t)w[0];
+}
+
+// Sums over the warp of NT values per lane (NT 1, 8 or 16): lane l returns that of value l % NT.
+template <int NT>
+LT_DEVINL float warp_sums(float (&v)[NT], int lane) {
+#pragma unroll
+    for (int n = NT / 2; n >= 1; n /= 2) {  // halves of the values change places between lanes n apart
+        const bool up = lane & n;
+#pragma unroll
+        for (int i = 0; i < n; i++) {
+            const float give = up ? v[i] : v[i + n], keep = up ? v[i + n] : v[i];
+            v[i] = keep + __shfl_xor_sync(0xffffffffu, give, n);
+        }
+    }
+    float x = v[0];
+#pragma unroll
+    for (int n = NT; n < 32; n *= 2) x += __shfl_xor_sync(0xffffffffu, x, n);
+    return x;
 }
 
 // Lane l holds N = HD / 64 rotation pairs as k_paged_append does: elements l N .. and HD / 2 + l N .. (consecutive
 // pairs of head_dim 64: 2 l and 2 l + 1).  Grid (blocks of all sequences at most, ceil(vectors / heads_per_cta)).
-template <int HD>
-__global__ void __launch_bounds__(kQaThreads) k_paged_q8_append(const __grid_constant__ PagedQ8AppendArgs a) {
+// CHUNK: tokens of a warp; 1: calls whose sequences have one row each.
+template <int HD, int CHUNK>
+__global__ void __launch_bounds__(kQaThreads, CHUNK == 1 ? 4 : HD * CHUNK >= 4096 ? 1 : 2) k_paged_q8_append(const __grid_constant__ PagedQ8AppendArgs a) {
     constexpr int N = HD / 64, HALF = HD / 2;
+    extern __shared__ __align__(16) float2 s_cs[];  // [tokens of the block][HALF]
     __shared__ double s_turn[HALF];  // turns of pi per position
-    __shared__ float2 s_cs[kQaChunk][HALF];
+    __shared__ uint32_t s_top[2][kQaWarps];
     __shared__ uint64_t s_scan[kQaWarps];
     __shared__ QaSeq s_q;
     __shared__ uint32_t s_seq, s_block;
@@ -149,25 +163,31 @@ __global__ void __launch_bounds__(kQaThreads) k_paged_q8_append(const __grid_con
     const bool split = neox || N > 1;
     const uint32_t e0 = split ? lane * N : 2 * lane, e1 = split ? HALF + lane * N : 2 * lane + 1;
 
-    // angles of tokens t0 .. of the block
-    auto angles = [&](uint32_t t0) {
-        __syncthreads();
-        const uint32_t n = min(ntok - t0, (uint32_t)kQaChunk);
-        for (uint32_t i = tid; i < n * HALF; i += kQaThreads) {
-            const uint32_t t = i / HALF, e = i % HALF;
-            const uint32_t pos = a.pos ? a.pos[row0 + t0 + t] : p0 + t0 + t;
-            const double turn = (double)pos * s_turn[e];
-            float s, c;
-            sincospif((float)(turn - 2.0 * rint(turn * 0.5)), &s, &c);
-            s_cs[t][e] = make_float2(c, s);
-        }
-        __syncthreads();
+    // angles of the block's new tokens
+    for (uint32_t i = tid; i < ntok * HALF; i += kQaThreads) {
+        const uint32_t t = i / HALF, e = i % HALF;
+        const uint32_t pos = a.pos ? a.pos[row0 + t] : p0 + t;
+        const double turn = (double)pos * s_turn[e];
+        float s, c;
+        sincospif((float)(turn - 2.0 * rint(turn * 0.5)), &s, &c);
+        s_cs[i] = make_float2(c, s);
+    }
+    __syncthreads();
+
+    // this warp's team and its tokens t0 .. t0 + n - 1
+    const uint32_t team_warps = CHUNK == 1 ? 1 : max(1u, size / CHUNK), teams = kQaWarps / team_warps;
+    const uint32_t team = warp / team_warps, t0 = warp % team_warps * CHUNK;
+    const uint32_t n = t0 < ntok ? min(ntok - t0, (uint32_t)CHUNK) : 0;
+    auto team_sync = [&]() {
+        __syncwarp();
+        if (team_warps > 1) asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "r"(team_warps * 32) : "memory");
     };
-    // head vector h of NT tokens from t0 on, of which n are there, normalised and rotated
-    auto fetch = [&](auto &x, auto &y, uint32_t h, uint32_t t0, uint32_t n) {
-        constexpr int NT = sizeof(x) / sizeof(x[0]);
+    uint32_t turn = 0;
+    for (uint32_t h = first + team; h < last; h += teams, turn ^= 1) {
+        const bool is_q = h < H, is_v = h >= H + KV;
+        float x[CHUNK][N], y[CHUNK][N];
 #pragma unroll
-        for (int t = 0; t < NT; t++) {
+        for (int t = 0; t < CHUNK; t++) {
             const float *src = a.qkv + ((uint64_t)(row0 + t0 + t) * vecs + h) * HD;
             if ((uint32_t)t < n) {
                 qa_load<N>(src + e0, x[t]);
@@ -177,190 +197,169 @@ __global__ void __launch_bounds__(kQaThreads) k_paged_q8_append(const __grid_con
                 for (int e = 0; e < N; e++) x[t][e] = y[t][e] = 0.0f;
             }
         }
-        const bool is_q = h < H, is_v = h >= H + KV;
         const float *w = is_q ? a.q_norm : is_v ? nullptr : a.k_norm;
         if (w || (is_v && a.v_norm)) {
-            float wx[N], wy[N];
+            float ss[CHUNK], wx[N], wy[N];
 #pragma unroll
             for (int e = 0; e < N; e++) {
                 wx[e] = w ? w[e0 + e] : 1.0f;
                 wy[e] = w ? w[e1 + e] : 1.0f;
             }
 #pragma unroll
-            for (int t = 0; t < NT; t++) {
-                float ss = 0.0f;
+            for (int t = 0; t < CHUNK; t++) {
+                ss[t] = 0.0f;
 #pragma unroll
-                for (int e = 0; e < N; e++) ss = fmaf(x[t][e], x[t][e], fmaf(y[t][e], y[t][e], ss));
-                ss = warp_sum(ss);
-                const float inv = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fdiv_rn(ss, (float)HD), a.eps)));
+                for (int e = 0; e < N; e++) ss[t] = fmaf(x[t][e], x[t][e], fmaf(y[t][e], y[t][e], ss[t]));
+            }
+            const float inv = __fdiv_rn(1.0f, __fsqrt_rn(fmaf(warp_sums<CHUNK>(ss, lane), 1.0f / HD, a.eps)));
+#pragma unroll
+            for (int t = 0; t < CHUNK; t++) {
+                const float f = __shfl_sync(0xffffffffu, inv, t);
 #pragma unroll
                 for (int e = 0; e < N; e++) {
-                    x[t][e] = x[t][e] * inv * wx[e];
-                    y[t][e] = y[t][e] * inv * wy[e];
+                    x[t][e] *= f * wx[e];
+                    y[t][e] *= f * wy[e];
                 }
             }
         }
-        if (is_v) return;
+        if (!is_v) {
 #pragma unroll
-        for (int t = 0; t < NT; t++) {
-            if ((uint32_t)t >= n) break;
-            if (neox) {
+            for (int t = 0; t < CHUNK; t++) {
+                const float2 *cs = s_cs + ((uint32_t)t < n ? t0 + t : 0) * HALF;
+                if (neox) {
 #pragma unroll
-                for (int e = 0; e < N; e++) {
-                    const float2 cs = s_cs[t][lane * N + e];
-                    const float p = x[t][e], r = y[t][e];
-                    x[t][e] = fmaf(p, cs.x, -r * cs.y);
-                    y[t][e] = fmaf(p, cs.y, r * cs.x);
+                    for (int e = 0; e < N; e++) {
+                        const float2 z = cs[lane * N + e];
+                        const float p = x[t][e], r = y[t][e];
+                        x[t][e] = fmaf(p, z.x, -r * z.y);
+                        y[t][e] = fmaf(p, z.y, r * z.x);
+                    }
+                } else if constexpr (N > 1) {
+#pragma unroll
+                    for (int e = 0; e < N; e += 2) {
+                        const float2 zx = cs[(lane * N + e) / 2], zy = cs[(HALF + lane * N + e) / 2];
+                        const float p = x[t][e], r = x[t][e + 1], u = y[t][e], v = y[t][e + 1];
+                        x[t][e] = fmaf(p, zx.x, -r * zx.y);
+                        x[t][e + 1] = fmaf(p, zx.y, r * zx.x);
+                        y[t][e] = fmaf(u, zy.x, -v * zy.y);
+                        y[t][e + 1] = fmaf(u, zy.y, v * zy.x);
+                    }
+                } else {
+                    const float2 z = cs[lane];
+                    const float p = x[t][0], r = y[t][0];
+                    x[t][0] = fmaf(p, z.x, -r * z.y);
+                    y[t][0] = fmaf(p, z.y, r * z.x);
                 }
-            } else if constexpr (N > 1) {
-#pragma unroll
-                for (int e = 0; e < N; e += 2) {
-                    const float2 cx = s_cs[t][(lane * N + e) / 2], cy = s_cs[t][(HALF + lane * N + e) / 2];
-                    const float p = x[t][e], r = x[t][e + 1], u = y[t][e], v = y[t][e + 1];
-                    x[t][e] = fmaf(p, cx.x, -r * cx.y);
-                    x[t][e + 1] = fmaf(p, cx.y, r * cx.x);
-                    y[t][e] = fmaf(u, cy.x, -v * cy.y);
-                    y[t][e + 1] = fmaf(u, cy.y, v * cy.x);
-                }
-            } else {
-                const float2 cs = s_cs[t][lane];
-                const float p = x[t][0], r = y[t][0];
-                x[t][0] = fmaf(p, cs.x, -r * cs.y);
-                y[t][0] = fmaf(p, cs.y, r * cs.x);
             }
         }
-    };
-    // the largest magnitude, as bits: NaN is above infinity, infinity above every number
-    auto top_of = [&](const auto &x, const auto &y) {
-        constexpr int NT = sizeof(x) / sizeof(x[0]);
+        if (is_q) {
+#pragma unroll
+            for (int t = 0; t < CHUNK; t++) {
+                if ((uint32_t)t >= n) break;
+                float *dst = a.q + ((uint64_t)(row0 + t0 + t) * H + h) * HD;
+                qa_store<N>(dst + e0, x[t]);
+                qa_store<N>(dst + e1, y[t]);
+            }
+            continue;
+        }
+        if (!there) continue;
+        // the largest magnitude, as bits: NaN is above infinity, infinity above every number
         uint32_t top = 0;
 #pragma unroll
-        for (int t = 0; t < NT; t++)
+        for (int t = 0; t < CHUNK; t++)
 #pragma unroll
             for (int e = 0; e < N; e++)
                 top = max(top, max(__float_as_uint(x[t][e]) & 0x7fffffffu, __float_as_uint(y[t][e]) & 0x7fffffffu));
-        return __reduce_max_sync(0xffffffffu, top);
-    };
-    // the block's scale for head vector h; codes that stay go onto it
-    auto rescale = [&](uint32_t h, uint32_t top) {
-        const bool is_v = h >= H + KV;
+        top = __reduce_max_sync(0xffffffffu, top);
+        if (team_warps > 1) {  // of the team; the two places take turns, so that one barrier does
+            if (lane == 0) s_top[turn][warp] = top;
+            team_sync();
+            for (uint32_t i = team * team_warps; i < (team + 1) * team_warps; i++) top = max(top, s_top[turn][i]);
+        }
+        // The block's scale.  Every warp of the team works it out; the first writes it, after all have read the old one,
+        // and puts the codes that stay onto it.
         const uint32_t kh = h - H - (is_v ? KV : 0);
         float *at = (is_v ? a.kv.v_scale : a.kv.k_scale) + q8_scale_at(a.kv, page, start, kh);
+        uint8_t *codes = (is_v ? a.kv.v : a.kv.k) + paged_offset(a.kv, page, start, kh);
         float scale = top > __float_as_uint(kQ8Most) ? __int_as_float(0x7fffffff) : __fdiv_rn(__uint_as_float(top), 127.0f);
         if (old) {
             const float was = *at;
-            __syncwarp();
             if (!(was >= 0.0f && was <= 3.402823466e38f)) scale = __int_as_float(0x7fffffff);
-            if (scale > was) {
+            team_sync();
+            if (scale > was && t0 == 0) {
                 const float f = __fdiv_rn(was, scale);
-                uint8_t *codes = (is_v ? a.kv.v : a.kv.k) + paged_offset(a.kv, page, start, kh);
                 for (uint32_t i = lane; i < old * (HD / 4); i += 32) {
                     uint32_t *p = reinterpret_cast<uint32_t *>(codes + (uint64_t)(i / (HD / 4)) * a.kv.slot_stride) + i % (HD / 4);
                     const uint32_t c = *p;
-                    uint32_t w = 0;
+                    uint32_t b = 0;
 #pragma unroll
                     for (int e = 0; e < 4; e++)
-                        w |= ((uint32_t)__float2int_rn((float)(int8_t)(c >> (8 * e)) * f) & 0xffu) << (8 * e);
-                    *p = w;
+                        b |= ((uint32_t)__float2int_rn((float)(int8_t)(c >> (8 * e)) * f) & 0xffu) << (8 * e);
+                    *p = b;
                 }
             }
             if (scale <= was) scale = was;
         }
-        if (lane == 0) *at = scale;
-        return scale;
-    };
-    auto put = [&](const auto &x, const auto &y, uint32_t h, uint32_t t0, uint32_t n, float scale) {
-        constexpr int NT = sizeof(x) / sizeof(x[0]);
-        const bool is_v = h >= H + KV;
-        uint8_t *dst = (is_v ? a.kv.v : a.kv.k) + paged_offset(a.kv, page, p0 + t0, h - H - (is_v ? KV : 0));
+        if (lane == 0 && t0 == 0) *at = scale;
+        // Codes: x / scale by its inverse (0: no codes).  Where that is not a normal number everything is scaled up first,
+        // and the values held to the codes' range: a scale of few bits may be far from top / 127.
+        const bool tiny = scale < 0x1p-100f;
+        const float r = scale > 0.0f ? __fdiv_rn(1.0f, tiny ? scale * 0x1p100f : scale) : 0.0f;
+        if (tiny) {
 #pragma unroll
-        for (int t = 0; t < NT; t++) {
+            for (int t = 0; t < CHUNK; t++)
+#pragma unroll
+                for (int e = 0; e < N; e++) {
+                    const float most = 127.0f * (scale * 0x1p100f);
+                    x[t][e] = fminf(fmaxf(x[t][e] * 0x1p100f, -most), most);
+                    y[t][e] = fminf(fmaxf(y[t][e] * 0x1p100f, -most), most);
+                }
+        }
+        const bool none = !(scale > 0.0f);  // zeros, or no numbers: codes of 0
+        codes += (uint64_t)(p0 - start + t0) * a.kv.slot_stride;
+#pragma unroll
+        for (int t = 0; t < CHUNK; t++) {
             if ((uint32_t)t >= n) break;
-            qa_store_codes<N>(dst + t * a.kv.slot_stride + e0, x[t], scale);
-            qa_store_codes<N>(dst + t * a.kv.slot_stride + e1, y[t], scale);
-        }
-    };
-    __shared__ uint32_t s_top[2048];  // of K and V heads of this CTA (n_kv <= 1024)
-    auto work = [&](auto nt) {
-        constexpr int NT = decltype(nt)::value;
-        float x[NT][N], y[NT][N];
-        if (ntok <= NT) {
-            angles(0);
-            for (uint32_t h = first + warp; h < last; h += kQaWarps) {
-                fetch(x, y, h, 0, ntok);
-                if (h < H) {
+            if (none) {
 #pragma unroll
-                    for (int t = 0; t < NT; t++) {
-                        if ((uint32_t)t >= ntok) break;
-                        float *dst = a.q + ((uint64_t)(row0 + t) * H + h) * HD;
-                        qa_store<N>(dst + e0, x[t]);
-                        qa_store<N>(dst + e1, y[t]);
-                    }
-                } else if (there) {
-                    const float scale = rescale(h, top_of(x, y));
-                    put(x, y, h, 0, ntok, scale);
-                }
+                for (int e = 0; e < N; e++) x[t][e] = y[t][e] = 0.0f;
             }
-            return;
+            qa_store_codes<N>(codes + t * a.kv.slot_stride + e0, x[t], r);
+            qa_store_codes<N>(codes + t * a.kv.slot_stride + e1, y[t], r);
         }
-        // more tokens than the registers hold: the maxima first, then everything again for the codes
-        for (uint32_t i = tid; i < 2 * KV; i += kQaThreads) s_top[i] = 0;
-        for (int pass = 0; pass < 2; pass++) {
-            for (uint32_t t0 = 0; t0 < ntok; t0 += NT) {
-                const uint32_t n = min(ntok - t0, (uint32_t)NT);
-                angles(t0);
-                for (uint32_t h = first + warp; h < last; h += kQaWarps) {
-                    if (pass && h < H) continue;
-                    fetch(x, y, h, t0, n);
-                    if (h < H) {
-#pragma unroll
-                        for (int t = 0; t < NT; t++) {
-                            if ((uint32_t)t >= n) break;
-                            float *dst = a.q + ((uint64_t)(row0 + t0 + t) * H + h) * HD;
-                            qa_store<N>(dst + e0, x[t]);
-                            qa_store<N>(dst + e1, y[t]);
-                        }
-                    } else if (!there) {
-                        continue;
-                    } else if (pass == 0) {
-                        const uint32_t top = max(s_top[h - H], top_of(x, y));
-                        __syncwarp();
-                        if (lane == 0) s_top[h - H] = top;
-                        __syncwarp();
-                    } else {
-                        const uint32_t top = s_top[h - H];
-                        __syncwarp();
-                        // s_top holds the scale's bits from the first chunk on
-                        float scale = __uint_as_float(top);
-                        if (t0 == 0) {
-                            scale = rescale(h, top);
-                            if (lane == 0) s_top[h - H] = __float_as_uint(scale);
-                        }
-                        __syncwarp();
-                        put(x, y, h, t0, n, scale);
-                    }
-                }
-            }
-        }
-    };
-    if (ntok == 1)
-        work(QaInt<1>());
-    else
-        work(QaInt<kQaChunk>());
+    }
 }
 
-cudaError_t launch_paged_q8_append(const LaunchCfg &c, PagedQ8AppendArgs a) {
-    const uint32_t vecs = a.n_heads + 2 * a.kv.n_kv;
-    a.err = c.dev_err;
+namespace {
+
+// Tokens of a warp: what its registers hold, and a block's tokens fill at most the CTA's warps.
+template <int HD>
+cudaError_t qa_launch(const LaunchCfg &c, PagedQ8AppendArgs a) {
+    const uint32_t vecs = a.n_heads + 2 * a.kv.n_kv, size = 1u << a.kv.block_shift;
     // blocks that the rows of all sequences can lie in: n rows touch at most n / size + 2, and n
     const uint64_t blocks = min((uint64_t)a.total_q, (uint64_t)(a.total_q >> a.kv.block_shift) + 2 * (uint64_t)a.n_seq);
-    const bool few = blocks < 4u * (uint32_t)c.num_sms;
-    a.heads_per_cta = few ? kQaWarps : vecs;
+    const uint32_t chunk = a.max_q == 1 ? 1 : HD == 256 && size < 128 ? 8 : 16;
+    const uint32_t teams = chunk == 1 ? kQaWarps : kQaWarps / max(1u, size / chunk);
+    // few blocks: several CTAs share one's heads, so that there are some six CTAs to an SM
+    const uint64_t want = max((uint64_t)1, (uint64_t)c.num_sms * 6 / blocks);
+    const uint32_t rounds = (uint32_t)max((uint64_t)1, (vecs + teams * want - 1) / (teams * want));
+    a.heads_per_cta = rounds * teams;
     const dim3 grid((uint32_t)blocks, (vecs + a.heads_per_cta - 1) / a.heads_per_cta);
+    const size_t smem = (size_t)min(a.max_q, size) * HD / 2 * sizeof(float2);
+    if (chunk == 1) return launch_k(c, "paged_q8_append", k_paged_q8_append<HD, 1>, grid, dim3(kQaThreads), smem, a);
+    if constexpr (HD == 256)
+        if (chunk == 8) return launch_k(c, "paged_q8_append", k_paged_q8_append<HD, 8>, grid, dim3(kQaThreads), smem, a);
+    return launch_k(c, "paged_q8_append", k_paged_q8_append<HD, 16>, grid, dim3(kQaThreads), smem, a);
+}
+
+}  // namespace
+
+cudaError_t launch_paged_q8_append(const LaunchCfg &c, PagedQ8AppendArgs a) {
+    a.err = c.dev_err;
     switch (a.kv.hd) {
-    case 64: return launch_k(c, "paged_q8_append", k_paged_q8_append<64>, grid, dim3(kQaThreads), 0, a);
-    case 128: return launch_k(c, "paged_q8_append", k_paged_q8_append<128>, grid, dim3(kQaThreads), 0, a);
-    case 256: return launch_k(c, "paged_q8_append", k_paged_q8_append<256>, grid, dim3(kQaThreads), 0, a);
+    case 64: return qa_launch<64>(c, a);
+    case 128: return qa_launch<128>(c, a);
+    case 256: return qa_launch<256>(c, a);
     default: return cudaErrorInvalidValue;
     }
 }
