@@ -12,11 +12,13 @@
 // the page returned from entry j lies at n' - 1 - (G(s) + j - stay), and entry j
 // takes the page at n' - 1 - (T(s) + j - stay): every page and token finds its place by itself.
 //
-// Bound: latency (the sums over the sequences, one block barrier after the other);
-// many tokens: the writes, 12 bytes each.  One CTA scans the sequences, refuses what
-// cannot be done before anything is changed, and puts the returned pages on the
-// stack.  Few tokens are then placed by the same CTA, many by a second launch over
-// all SMs.
+// Bound: latency (dependent loads and block barriers); many tokens: the writes, 12 bytes
+// each.  One CTA scans the sequences, a thread to each as far as they go round, refuses what
+// cannot be done before anything is changed, and puts the returned pages on the stack.  Few
+// tokens are then placed by the same CTA, many by a second launch over all SMs.  Pages and
+// tokens are dealt to threads one by one, wherever their sequences begin: a sequence after
+// another, its pages read together, made 512 sequences wait for as many reads (25 us).  Up to
+// 2048 sequences are kept in shared memory between the steps.
 #include "lt_launch.cuh"
 
 namespace lt {
@@ -40,24 +42,29 @@ LT_DEVINL uint32_t owner_of(const uint32_t *first, uint32_t n, uint32_t i) {
     return lo;
 }
 
+// What the steps know of sequence s: its first token among all, its first page among those taken, and how many
+// positions stay.
+struct PlanSeqs {
+    const uint32_t *cu, *take, *keep;
+};
+
 // Table entries and token rows, thread `at` of `step`.  Nothing that is read here is written here.
-LT_DEVINL void plan_fill(const PagedPlanArgs &a, uint32_t at, uint32_t step) {
-    const uint32_t top = a.head[0], takes = a.head[1], tokens = a.head[2], n = a.n_seq;
+LT_DEVINL void plan_fill(const PagedPlanArgs &a, const PlanSeqs &q, uint32_t at, uint32_t step, uint32_t top, uint32_t takes,
+                         uint32_t tokens) {
+    const uint32_t n = a.n_seq;
     for (uint32_t k = at; k < takes; k += step) {
-        const uint32_t s = owner_of(a.take, n, k);
-        const uint32_t kept = a.lens[s] - (a.cu[s + 1] - a.cu[s]);
-        a.table[(uint64_t)s * a.max_pages + pages_for(kept, a.page) + (k - a.take[s])] = a.free[top - 1 - k];
+        const uint32_t s = owner_of(q.take, n, k);
+        a.table[(uint64_t)s * a.max_pages + pages_for(q.keep[s], a.page) + (k - q.take[s])] = a.free[top - 1 - k];
     }
     if (!a.seq && !a.pos && !a.slot) return;
     for (uint32_t t = at; t < tokens; t += step) {
-        const uint32_t s = owner_of(a.cu, n, t);
-        const uint32_t kept = a.lens[s] - (a.cu[s + 1] - a.cu[s]), p = kept + (t - a.cu[s]);
+        const uint32_t s = owner_of(q.cu, n, t), kept = q.keep[s], p = kept + (t - q.cu[s]);
         if (a.seq) a.seq[t] = s;
         if (a.pos) a.pos[t] = p;
         if (a.slot) {
             const uint32_t stay = pages_for(kept, a.page), j = p / a.page;
-            const uint32_t id = j < stay ? a.table[(uint64_t)s * a.max_pages + j] : a.free[top - 1 - (a.take[s] + j - stay)];
-            a.slot[t] = id * a.page + p % a.page;
+            const uint32_t id = j < stay ? a.table[(uint64_t)s * a.max_pages + j] : a.free[top - 1 - (q.take[s] + j - stay)];
+            a.slot[t] = id * a.page + (p - j * a.page);
         }
     }
 }
@@ -66,23 +73,34 @@ struct PlanSum {
     uint64_t tokens, gone, take;
 };
 
+constexpr uint32_t kPlanInShared = 2048;  // sequences
+
 // FILL: the same CTA places the tokens.
 template <bool FILL>
 __global__ void __launch_bounds__(kPlanThreads) k_paged_plan(const __grid_constant__ PagedPlanArgs a) {
-    __shared__ PlanSum s_warp[kPlanWarps];
+    __shared__ PlanSum s_warp[kPlanWarps], s_all;
     __shared__ int s_bad, s_bad_page;
+    __shared__ uint32_t s_cu[kPlanInShared], s_take[kPlanInShared], s_gone[kPlanInShared], s_keep[kPlanInShared];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const bool in_shared = a.n_seq <= kPlanInShared;
+    uint32_t *const cu = in_shared ? s_cu : a.cu_copy, *const take = in_shared ? s_take : a.take;
+    uint32_t *const gone = in_shared ? s_gone : a.gone, *const keeps = in_shared ? s_keep : a.keeps;
     pdl_launch_dependents();
-    pdl_wait();
     if (tid == 0) s_bad = s_bad_page = DEV_ERR_NONE;
+    pdl_wait();
+    const uint32_t n_free = *a.n_free;
     __syncthreads();
     const uint32_t per = (a.n_seq + kPlanThreads - 1) / kPlanThreads;
     const uint32_t sa = min(a.n_seq, tid * per), sb = min(a.n_seq, sa + per);
     const uint64_t cap = min((uint64_t)a.max_pages * a.page, (uint64_t)kPlanMaxLen);
     PlanSum mine = {0, 0, 0};
     bool bad = false;
-    for (uint32_t s = sa; s < sb; s++) {
+    for (uint32_t s = sa; s < sb; s++) {  // within this thread for now, in what belongs to it alone
         const uint32_t len = a.lens[s], keep = a.keep ? a.keep[s] : len, add = a.add[s];
+        cu[s] = (uint32_t)mine.tokens;
+        take[s] = (uint32_t)mine.take;
+        gone[s] = (uint32_t)mine.gone;
+        keeps[s] = keep;
         if (len > cap || keep > len || (uint64_t)keep + add > cap) {
             bad = true;
             continue;
@@ -92,83 +110,77 @@ __global__ void __launch_bounds__(kPlanThreads) k_paged_plan(const __grid_consta
         mine.gone += pages_for(len, a.page) - stay;
         mine.take += pages_for((uint64_t)keep + add, a.page) - stay;
     }
-    PlanSum incl = mine;
+    auto scan = [&](PlanSum &v) {
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const uint64_t x = __shfl_up_sync(0xffffffffu, incl.tokens, o), y = __shfl_up_sync(0xffffffffu, incl.gone, o),
-                       z = __shfl_up_sync(0xffffffffu, incl.take, o);
-        if (lane >= o) incl.tokens += x, incl.gone += y, incl.take += z;
-    }
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint64_t x = __shfl_up_sync(0xffffffffu, v.tokens, o), y = __shfl_up_sync(0xffffffffu, v.gone, o),
+                           z = __shfl_up_sync(0xffffffffu, v.take, o);
+            if (lane >= o) v.tokens += x, v.gone += y, v.take += z;
+        }
+    };
+    PlanSum incl = mine;
+    scan(incl);
     if (lane == 31) s_warp[warp] = incl;
     if (bad) s_bad = DEV_ERR_BAD_INDEX;
     __syncthreads();
-    PlanSum at = {incl.tokens - mine.tokens, incl.gone - mine.gone, incl.take - mine.take}, all = {0, 0, 0};
-#pragma unroll 8
-    for (int w = 0; w < kPlanWarps; w++) {
-        const PlanSum x = s_warp[w];
-        if (w < warp) at.tokens += x.tokens, at.gone += x.gone, at.take += x.take;
-        all.tokens += x.tokens, all.gone += x.gone, all.take += x.take;
-    }
-    const uint32_t n_free = *a.n_free;
-    const uint64_t top = (uint64_t)n_free + all.gone;
-    if (tid == 0 && s_bad == DEV_ERR_NONE) {
-        if (all.tokens > a.total_q || n_free > a.n_pages || top > a.n_pages)
-            s_bad = DEV_ERR_BAD_INDEX;
-        else if (all.take > top)
-            s_bad = DEV_ERR_NO_PAGES;
-    }
-    __syncthreads();
-    // where each sequence's pages and tokens begin, and which pages go: of scratch, nothing of the caller's
-    if (s_bad == DEV_ERR_NONE) {
-        for (uint32_t s = sa; s < sb; s++) {
-            const uint32_t len = a.lens[s], keep = a.keep ? a.keep[s] : len, add = a.add[s];
-            const uint32_t stay = pages_for(keep, a.page), have = pages_for(len, a.page);
-            a.take[s] = (uint32_t)at.take;
-            a.gone[s] = (uint32_t)at.gone;
-            a.stay[s] = stay;
-            a.have[s] = have;
-            at.gone += have - stay;
-            at.take += pages_for((uint64_t)keep + add, a.page) - stay;
-        }
-    }
-    __syncthreads();
-    // the pages that go, 32 sequences to a warp: first their numbers are looked at, then they move
-    bool ok = s_bad == DEV_ERR_NONE;
-    for (int pass = 0; pass < 2 && ok; pass++) {
-        for (uint32_t s0 = warp * 32; s0 < a.n_seq; s0 += kPlanThreads) {
-            const uint32_t s = s0 + lane;
-            const bool in = s < a.n_seq;
-            const uint32_t stay = in ? a.stay[s] : 0, have = in ? a.have[s] : 0, first = in ? a.gone[s] : 0;
-            for (uint32_t some = __ballot_sync(0xffffffffu, have > stay); some; some &= some - 1) {
-                const int x = __ffs(some) - 1;
-                const uint32_t j0 = __shfl_sync(0xffffffffu, stay, x), j1 = __shfl_sync(0xffffffffu, have, x);
-                const uint32_t g = __shfl_sync(0xffffffffu, first, x);
-                uint32_t *row = a.table + (uint64_t)(s0 + x) * a.max_pages;
-#pragma unroll 4
-                for (uint32_t j = j0 + lane; j < j1; j += 32) {
-                    const uint32_t id = row[j];
-                    if (pass == 0) {
-                        if (id >= a.n_pages) s_bad_page = DEV_ERR_BAD_INDEX;
-                    } else {
-                        a.free[top - 1 - (g + j - j0)] = id;
-                        row[j] = kPlanNoPage;
-                    }
-                }
+    if (warp == 0) {
+        PlanSum v = s_warp[lane];
+        const PlanSum own = v;
+        scan(v);
+        s_warp[lane] = {v.tokens - own.tokens, v.gone - own.gone, v.take - own.take};
+        if (lane == 31) {
+            s_all = v;
+            if (s_bad == DEV_ERR_NONE) {
+                const uint64_t top = (uint64_t)n_free + v.gone;
+                if (v.tokens > a.total_q || n_free > a.n_pages || top > a.n_pages)
+                    s_bad = DEV_ERR_BAD_INDEX;
+                else if (v.take > top)
+                    s_bad = DEV_ERR_NO_PAGES;
             }
         }
-        __syncthreads();  // s_bad_page is written in the first pass only, and read after it
-        ok = s_bad_page == DEV_ERR_NONE;
+    }
+    __syncthreads();
+    const PlanSum all = s_all;
+    const uint32_t top = n_free + (uint32_t)all.gone;  // where it counts, nothing is bad
+    const PlanSum at = {s_warp[warp].tokens + incl.tokens - mine.tokens, s_warp[warp].gone + incl.gone - mine.gone,
+                        s_warp[warp].take + incl.take - mine.take};
+    for (uint32_t s = sa; s < sb; s++) {
+        cu[s] += (uint32_t)at.tokens;
+        take[s] += (uint32_t)at.take;
+        gone[s] += (uint32_t)at.gone;
+    }
+    bool ok = s_bad == DEV_ERR_NONE;
+    if (ok && all.gone) {
+        // the pages that go, one to a thread: first their numbers are looked at, then they move
+        __syncthreads();
+        for (int pass = 0; pass < 2 && ok; pass++) {
+            for (uint32_t r = tid; r < all.gone; r += kPlanThreads) {
+                const uint32_t s = owner_of(gone, a.n_seq, r);
+                uint32_t *entry = a.table + (uint64_t)s * a.max_pages + pages_for(keeps[s], a.page) + (r - gone[s]);
+                const uint32_t id = *entry;
+                if (pass == 0) {
+                    if (id >= a.n_pages) s_bad_page = DEV_ERR_BAD_INDEX;
+                } else {
+                    a.free[top - 1 - r] = id;
+                    *entry = kPlanNoPage;
+                }
+            }
+            __syncthreads();  // s_bad_page is written in the first pass only, and read after it
+            ok = s_bad_page == DEV_ERR_NONE;
+        }
     }
     for (uint32_t s = sa; s < sb; s++) {
-        a.cu[s] = ok ? (uint32_t)at.tokens : 0;
+        a.cu[s] = ok ? cu[s] : 0;
         if (!ok) continue;
-        const uint32_t keep = a.keep ? a.keep[s] : a.lens[s], add = a.add[s];
-        at.tokens += add;
-        a.lens[s] = keep + add;
+        a.lens[s] = keeps[s] + ((s + 1 < sb ? cu[s + 1] : (uint32_t)(at.tokens + mine.tokens)) - cu[s]);
+        if (!FILL) {  // for the second launch
+            a.take[s] = take[s];
+            a.keeps[s] = keeps[s];
+        }
     }
     if (tid == 0) {
         a.cu[a.n_seq] = ok ? (uint32_t)all.tokens : 0;
-        a.head[0] = ok ? (uint32_t)top : 0;
+        a.head[0] = ok ? top : 0;
         a.head[1] = ok ? (uint32_t)all.take : 0;
         a.head[2] = ok ? (uint32_t)all.tokens : 0;
         if (ok)
@@ -176,9 +188,10 @@ __global__ void __launch_bounds__(kPlanThreads) k_paged_plan(const __grid_consta
         else
             atomicExch(a.err, s_bad != DEV_ERR_NONE ? s_bad : s_bad_page);
     }
-    if (FILL) {
+    if (FILL && ok) {
         __syncthreads();
-        plan_fill(a, tid, kPlanThreads);
+        const PlanSeqs q = {cu, take, keeps};
+        plan_fill(a, q, tid, kPlanThreads, top, (uint32_t)all.take, (uint32_t)all.tokens);
     }
 }
 
@@ -187,7 +200,8 @@ constexpr int kPlanFillThreads = 256;
 __global__ void __launch_bounds__(kPlanFillThreads) k_paged_plan_fill(const __grid_constant__ PagedPlanArgs a) {
     pdl_launch_dependents();
     pdl_wait();
-    plan_fill(a, blockIdx.x * kPlanFillThreads + threadIdx.x, gridDim.x * kPlanFillThreads);
+    const PlanSeqs q = {a.cu, a.take, a.keeps};
+    plan_fill(a, q, blockIdx.x * kPlanFillThreads + threadIdx.x, gridDim.x * kPlanFillThreads, a.head[0], a.head[1], a.head[2]);
 }
 
 namespace {
@@ -202,8 +216,8 @@ cudaError_t launch_paged_plan(const LaunchCfg &c, PagedPlanArgs a, uint8_t *scra
     a.head = (uint32_t *)scratch;
     a.take = (uint32_t *)(scratch + kPlanHead);
     a.gone = a.take + plan_row(a) / 4;
-    a.stay = a.gone + plan_row(a) / 4;
-    a.have = a.stay + plan_row(a) / 4;
+    a.keeps = a.gone + plan_row(a) / 4;
+    a.cu_copy = a.keeps + plan_row(a) / 4;
     const uint64_t steps = ((uint64_t)a.total_q + kPlanFillThreads - 1) / kPlanFillThreads;
     if (steps <= 16) return launch_k(c, "paged_plan", k_paged_plan<true>, dim3(1), dim3(kPlanThreads), 0, a);
     cudaError_t e = launch_k(c, "paged_plan", k_paged_plan<false>, dim3(1), dim3(kPlanThreads), 0, a);
