@@ -237,7 +237,8 @@ struct PagedPlanArgs {
     const uint32_t *keep, *add;     // keep: nullptr, all stay
     uint32_t *lens, *table, *free, *n_free, *cu, *seq, *pos, *slot;
     // scratch, set by the launcher: {stack top before taking, pages taken, tokens}; [n_seq] each
-    uint32_t *head, *take, *gone, *keeps, *cu_copy;
+    uint32_t *head, *take, *gone, *keeps, *stay, *cu_copy;
+    uint32_t page_shift;            // log2 of page, or kNoShift; set by the launcher
     int *err;
 };
 size_t paged_plan_scratch(const PagedPlanArgs &a);

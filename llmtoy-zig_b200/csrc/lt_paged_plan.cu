@@ -27,7 +27,10 @@ constexpr int kPlanThreads = 1024, kPlanWarps = kPlanThreads / 32;
 constexpr uint32_t kPlanNoPage = 0xffffffffu;
 constexpr uint32_t kPlanMaxLen = 1u << 30;
 
-LT_DEVINL uint32_t pages_for(uint64_t n, uint32_t page) { return (uint32_t)((n + page - 1) / page); }
+// Divisions by the page size, in 32 bits (the 64-bit ones of a first version were most of its time: 10426 pages back and
+// 325661 tokens, 37 us).
+LT_DEVINL uint32_t page_of(const PagedPlanArgs &a, uint32_t n) { return a.page_shift != kNoShift ? n >> a.page_shift : n / a.page; }
+LT_DEVINL uint32_t pages_for(const PagedPlanArgs &a, uint32_t n) { return n ? page_of(a, n - 1) + 1 : 0; }
 
 // The last s with first[s] <= i, of n ascending entries whose first is 0.
 LT_DEVINL uint32_t owner_of(const uint32_t *first, uint32_t n, uint32_t i) {
@@ -42,10 +45,10 @@ LT_DEVINL uint32_t owner_of(const uint32_t *first, uint32_t n, uint32_t i) {
     return lo;
 }
 
-// What the steps know of sequence s: its first token among all, its first page among those taken, and how many
-// positions stay.
+// What the steps know of sequence s: its first token among all, its first page among those taken, how many
+// positions stay, and on how many pages.
 struct PlanSeqs {
-    const uint32_t *cu, *take, *keep;
+    const uint32_t *cu, *take, *keep, *stay;
 };
 
 // Table entries and token rows, thread `at` of `step`.  Nothing that is read here is written here.
@@ -54,7 +57,7 @@ LT_DEVINL void plan_fill(const PagedPlanArgs &a, const PlanSeqs &q, uint32_t at,
     const uint32_t n = a.n_seq;
     for (uint32_t k = at; k < takes; k += step) {
         const uint32_t s = owner_of(q.take, n, k);
-        a.table[(uint64_t)s * a.max_pages + pages_for(q.keep[s], a.page) + (k - q.take[s])] = a.free[top - 1 - k];
+        a.table[(uint64_t)s * a.max_pages + q.stay[s] + (k - q.take[s])] = a.free[top - 1 - k];
     }
     if (!a.seq && !a.pos && !a.slot) return;
     for (uint32_t t = at; t < tokens; t += step) {
@@ -62,7 +65,7 @@ LT_DEVINL void plan_fill(const PagedPlanArgs &a, const PlanSeqs &q, uint32_t at,
         if (a.seq) a.seq[t] = s;
         if (a.pos) a.pos[t] = p;
         if (a.slot) {
-            const uint32_t stay = pages_for(kept, a.page), j = p / a.page;
+            const uint32_t stay = q.stay[s], j = page_of(a, p);
             const uint32_t id = j < stay ? a.table[(uint64_t)s * a.max_pages + j] : a.free[top - 1 - (q.take[s] + j - stay)];
             a.slot[t] = id * a.page + (p - j * a.page);
         }
@@ -80,11 +83,11 @@ template <bool FILL>
 __global__ void __launch_bounds__(kPlanThreads) k_paged_plan(const __grid_constant__ PagedPlanArgs a) {
     __shared__ PlanSum s_warp[kPlanWarps], s_all;
     __shared__ int s_bad, s_bad_page;
-    __shared__ uint32_t s_cu[kPlanInShared], s_take[kPlanInShared], s_gone[kPlanInShared], s_keep[kPlanInShared];
+    __shared__ uint32_t s_cu[kPlanInShared], s_take[kPlanInShared], s_gone[kPlanInShared], s_keep[kPlanInShared], s_stay[kPlanInShared];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const bool in_shared = a.n_seq <= kPlanInShared;
     uint32_t *const cu = in_shared ? s_cu : a.cu_copy, *const take = in_shared ? s_take : a.take;
-    uint32_t *const gone = in_shared ? s_gone : a.gone, *const keeps = in_shared ? s_keep : a.keeps;
+    uint32_t *const gone = in_shared ? s_gone : a.gone, *const keeps = in_shared ? s_keep : a.keeps, *const stays = in_shared ? s_stay : a.stay;
     pdl_launch_dependents();
     if (tid == 0) s_bad = s_bad_page = DEV_ERR_NONE;
     pdl_wait();
@@ -105,10 +108,11 @@ __global__ void __launch_bounds__(kPlanThreads) k_paged_plan(const __grid_consta
             bad = true;
             continue;
         }
-        const uint32_t stay = pages_for(keep, a.page);
+        const uint32_t stay = pages_for(a, keep);
+        stays[s] = stay;
         mine.tokens += add;
-        mine.gone += pages_for(len, a.page) - stay;
-        mine.take += pages_for((uint64_t)keep + add, a.page) - stay;
+        mine.gone += pages_for(a, len) - stay;
+        mine.take += pages_for(a, keep + add) - stay;
     }
     auto scan = [&](PlanSum &v) {
 #pragma unroll
@@ -156,7 +160,7 @@ __global__ void __launch_bounds__(kPlanThreads) k_paged_plan(const __grid_consta
         for (int pass = 0; pass < 2 && ok; pass++) {
             for (uint32_t r = tid; r < all.gone; r += kPlanThreads) {
                 const uint32_t s = owner_of(gone, a.n_seq, r);
-                uint32_t *entry = a.table + (uint64_t)s * a.max_pages + pages_for(keeps[s], a.page) + (r - gone[s]);
+                uint32_t *entry = a.table + (uint64_t)s * a.max_pages + stays[s] + (r - gone[s]);
                 const uint32_t id = *entry;
                 if (pass == 0) {
                     if (id >= a.n_pages) s_bad_page = DEV_ERR_BAD_INDEX;
@@ -176,6 +180,7 @@ __global__ void __launch_bounds__(kPlanThreads) k_paged_plan(const __grid_consta
         if (!FILL) {  // for the second launch
             a.take[s] = take[s];
             a.keeps[s] = keeps[s];
+            a.stay[s] = stays[s];
         }
     }
     if (tid == 0) {
@@ -190,7 +195,7 @@ __global__ void __launch_bounds__(kPlanThreads) k_paged_plan(const __grid_consta
     }
     if (FILL && ok) {
         __syncthreads();
-        const PlanSeqs q = {cu, take, keeps};
+        const PlanSeqs q = {cu, take, keeps, stays};
         plan_fill(a, q, tid, kPlanThreads, top, (uint32_t)all.take, (uint32_t)all.tokens);
     }
 }
@@ -200,7 +205,7 @@ constexpr int kPlanFillThreads = 256;
 __global__ void __launch_bounds__(kPlanFillThreads) k_paged_plan_fill(const __grid_constant__ PagedPlanArgs a) {
     pdl_launch_dependents();
     pdl_wait();
-    const PlanSeqs q = {a.cu, a.take, a.keeps};
+    const PlanSeqs q = {a.cu, a.take, a.keeps, a.stay};
     plan_fill(a, q, blockIdx.x * kPlanFillThreads + threadIdx.x, gridDim.x * kPlanFillThreads, a.head[0], a.head[1], a.head[2]);
 }
 
@@ -209,7 +214,7 @@ constexpr size_t kPlanHead = 256;
 size_t plan_row(const PagedPlanArgs &a) { return ((size_t)a.n_seq * 4 + 255) & ~(size_t)255; }
 }  // namespace
 
-size_t paged_plan_scratch(const PagedPlanArgs &a) { return kPlanHead + 4 * plan_row(a); }
+size_t paged_plan_scratch(const PagedPlanArgs &a) { return kPlanHead + 5 * plan_row(a); }
 
 cudaError_t launch_paged_plan(const LaunchCfg &c, PagedPlanArgs a, uint8_t *scratch) {
     a.err = c.dev_err;
@@ -217,7 +222,11 @@ cudaError_t launch_paged_plan(const LaunchCfg &c, PagedPlanArgs a, uint8_t *scra
     a.take = (uint32_t *)(scratch + kPlanHead);
     a.gone = a.take + plan_row(a) / 4;
     a.keeps = a.gone + plan_row(a) / 4;
-    a.cu_copy = a.keeps + plan_row(a) / 4;
+    a.stay = a.keeps + plan_row(a) / 4;
+    a.cu_copy = a.stay + plan_row(a) / 4;
+    a.page_shift = kNoShift;
+    for (uint32_t i = 0; i < 32; i++)
+        if (a.page == 1u << i) a.page_shift = i;
     const uint64_t steps = ((uint64_t)a.total_q + kPlanFillThreads - 1) / kPlanFillThreads;
     if (steps <= 16) return launch_k(c, "paged_plan", k_paged_plan<true>, dim3(1), dim3(kPlanThreads), 0, a);
     cudaError_t e = launch_k(c, "paged_plan", k_paged_plan<false>, dim3(1), dim3(kPlanThreads), 0, a);
