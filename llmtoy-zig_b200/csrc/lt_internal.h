@@ -232,12 +232,20 @@ size_t paged_q8_attn_scratch(const PagedAttnArgs &a, int num_sms);
 cudaError_t launch_paged_q8_attn(const LaunchCfg &c, PagedAttnArgs a, uint8_t *scratch);
 
 // Pages and slots of the coming tokens (lt_paged_plan.cu).
+// What the scan of the sequences found: the stack's top before anything is taken, pages and tokens, what is wrong.
+struct PlanHead {
+    uint32_t top, gone, take, tokens;
+    int bad;
+    uint32_t n_free;
+    int bad_page;
+};
 struct PagedPlanArgs {
     uint32_t n_seq, page, n_pages, max_pages, total_q;
     const uint32_t *keep, *add;     // keep: nullptr, all stay
     uint32_t *lens, *table, *free, *n_free, *cu, *seq, *pos, *slot;
-    // scratch, set by the launcher: {stack top before taking, pages taken, tokens}; [n_seq] each
-    uint32_t *head, *take, *gone, *keeps, *stay, *cu_copy;
+    // scratch, set by the launcher: [n_seq] each, and [n_pages] page ids
+    PlanHead *head;
+    uint32_t *take, *gone, *keeps, *stay, *cu_copy, *ids;
     uint32_t page_shift;            // log2 of page, or kNoShift; set by the launcher
     int *err;
 };

@@ -13,12 +13,12 @@
 // takes the page at n' - 1 - (T(s) + j - stay): every page and token finds its place by itself.
 //
 // Bound: latency (dependent loads and block barriers); many tokens: the writes, 12 bytes
-// each.  One CTA scans the sequences, a thread to each as far as they go round, refuses what
-// cannot be done before anything is changed, and puts the returned pages on the stack.  Few
-// tokens are then placed by the same CTA, many by a second launch over all SMs.  Pages and
-// tokens are dealt to threads one by one, wherever their sequences begin: a sequence after
-// another, its pages read together, made 512 sequences wait for as many reads (25 us).  Up to
-// 2048 sequences are kept in shared memory between the steps.
+// each.  One CTA scans the sequences, a thread to each as far as they go round, and refuses
+// what cannot be done before anything is changed.  Few tokens: the same CTA moves the pages and
+// places the tokens.  Many: two more launches over all SMs, one that looks at the pages that
+// go, one that writes everything (one CTA alone for the pages of 512 prompts, 10426 back and as
+// many taken: 22 us, by its instructions).  Pages and tokens are dealt to threads one by one,
+// wherever their sequences begin.  Up to 2048 sequences are kept in shared memory between the steps.
 #include "lt_launch.cuh"
 
 namespace lt {
@@ -45,28 +45,33 @@ LT_DEVINL uint32_t owner_of(const uint32_t *first, uint32_t n, uint32_t i) {
     return lo;
 }
 
-// What the steps know of sequence s: its first token among all, its first page among those taken, how many
-// positions stay, and on how many pages.
+// What the steps know of sequence s: its first token among all, its first pages among those taken and among those that
+// go, how many positions stay, and on how many pages.  And of all: the stack's top before anything is taken.
 struct PlanSeqs {
-    const uint32_t *cu, *take, *keep, *stay;
+    const uint32_t *cu, *take, *gone, *keep, *stay;
+    uint32_t top, n_gone, n_take, n_tokens;
 };
 
+// The page that the k-th place among those taken gets; ids: of the pages that go, where they are not yet on the stack.
+LT_DEVINL uint32_t taken(const PagedPlanArgs &a, const PlanSeqs &q, const uint32_t *ids, uint32_t k) {
+    return ids && k < q.n_gone ? ids[k] : a.free[q.top - 1 - k];
+}
+
 // Table entries and token rows, thread `at` of `step`.  Nothing that is read here is written here.
-LT_DEVINL void plan_fill(const PagedPlanArgs &a, const PlanSeqs &q, uint32_t at, uint32_t step, uint32_t top, uint32_t takes,
-                         uint32_t tokens) {
+LT_DEVINL void plan_fill(const PagedPlanArgs &a, const PlanSeqs &q, const uint32_t *ids, uint32_t at, uint32_t step) {
     const uint32_t n = a.n_seq;
-    for (uint32_t k = at; k < takes; k += step) {
+    for (uint32_t k = at; k < q.n_take; k += step) {
         const uint32_t s = owner_of(q.take, n, k);
-        a.table[(uint64_t)s * a.max_pages + q.stay[s] + (k - q.take[s])] = a.free[top - 1 - k];
+        a.table[(uint64_t)s * a.max_pages + q.stay[s] + (k - q.take[s])] = taken(a, q, ids, k);
     }
     if (!a.seq && !a.pos && !a.slot) return;
-    for (uint32_t t = at; t < tokens; t += step) {
-        const uint32_t s = owner_of(q.cu, n, t), kept = q.keep[s], p = kept + (t - q.cu[s]);
+    for (uint32_t t = at; t < q.n_tokens; t += step) {
+        const uint32_t s = owner_of(q.cu, n, t), p = q.keep[s] + (t - q.cu[s]);
         if (a.seq) a.seq[t] = s;
         if (a.pos) a.pos[t] = p;
         if (a.slot) {
             const uint32_t stay = q.stay[s], j = page_of(a, p);
-            const uint32_t id = j < stay ? a.table[(uint64_t)s * a.max_pages + j] : a.free[top - 1 - (q.take[s] + j - stay)];
+            const uint32_t id = j < stay ? a.table[(uint64_t)s * a.max_pages + j] : taken(a, q, ids, q.take[s] + j - stay);
             a.slot[t] = id * a.page + (p - j * a.page);
         }
     }
@@ -78,8 +83,8 @@ struct PlanSum {
 
 constexpr uint32_t kPlanInShared = 2048;  // sequences
 
-// FILL: the same CTA places the tokens.
-template <bool FILL>
+// ALONE: the same CTA does everything.  Else it writes what it found to scratch, and nothing of the caller's.
+template <bool ALONE>
 __global__ void __launch_bounds__(kPlanThreads) k_paged_plan(const __grid_constant__ PagedPlanArgs a) {
     __shared__ PlanSum s_warp[kPlanWarps], s_all;
     __shared__ int s_bad, s_bad_page;
@@ -154,6 +159,17 @@ __global__ void __launch_bounds__(kPlanThreads) k_paged_plan(const __grid_consta
         gone[s] += (uint32_t)at.gone;
     }
     bool ok = s_bad == DEV_ERR_NONE;
+    if (!ALONE) {
+        for (uint32_t s = sa; in_shared && s < sb; s++) {
+            a.cu_copy[s] = cu[s];
+            a.take[s] = take[s];
+            a.gone[s] = gone[s];
+            a.keeps[s] = keeps[s];
+            a.stay[s] = stays[s];
+        }
+        if (tid == 0) *a.head = {top, (uint32_t)all.gone, (uint32_t)all.take, (uint32_t)all.tokens, s_bad, n_free};
+        return;
+    }
     if (ok && all.gone) {
         // the pages that go, one to a thread: first their numbers are looked at, then they move
         __syncthreads();
@@ -175,38 +191,62 @@ __global__ void __launch_bounds__(kPlanThreads) k_paged_plan(const __grid_consta
     }
     for (uint32_t s = sa; s < sb; s++) {
         a.cu[s] = ok ? cu[s] : 0;
-        if (!ok) continue;
-        a.lens[s] = keeps[s] + ((s + 1 < sb ? cu[s + 1] : (uint32_t)(at.tokens + mine.tokens)) - cu[s]);
-        if (!FILL) {  // for the second launch
-            a.take[s] = take[s];
-            a.keeps[s] = keeps[s];
-            a.stay[s] = stays[s];
-        }
+        if (ok) a.lens[s] = keeps[s] + ((s + 1 < sb ? cu[s + 1] : (uint32_t)(at.tokens + mine.tokens)) - cu[s]);
     }
     if (tid == 0) {
         a.cu[a.n_seq] = ok ? (uint32_t)all.tokens : 0;
-        a.head[0] = ok ? top : 0;
-        a.head[1] = ok ? (uint32_t)all.take : 0;
-        a.head[2] = ok ? (uint32_t)all.tokens : 0;
         if (ok)
             *a.n_free = (uint32_t)(top - all.take);
         else
             atomicExch(a.err, s_bad != DEV_ERR_NONE ? s_bad : s_bad_page);
     }
-    if (FILL && ok) {
-        __syncthreads();
-        const PlanSeqs q = {cu, take, keeps, stays};
-        plan_fill(a, q, tid, kPlanThreads, top, (uint32_t)all.take, (uint32_t)all.tokens);
-    }
+    if (!ok) return;
+    __syncthreads();
+    const PlanSeqs q = {cu, take, gone, keeps, stays, top, (uint32_t)all.gone, (uint32_t)all.take, (uint32_t)all.tokens};
+    plan_fill(a, q, nullptr, tid, kPlanThreads);
 }
 
 constexpr int kPlanFillThreads = 256;
 
+// The pages that go, looked at.
+__global__ void __launch_bounds__(kPlanFillThreads) k_paged_plan_gone(const __grid_constant__ PagedPlanArgs a) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const uint32_t n = a.head->bad == DEV_ERR_NONE ? a.head->gone : 0;
+    for (uint32_t r = blockIdx.x * kPlanFillThreads + threadIdx.x; r < n; r += gridDim.x * kPlanFillThreads) {
+        const uint32_t s = owner_of(a.gone, a.n_seq, r);
+        const uint32_t id = a.table[(uint64_t)s * a.max_pages + a.stay[s] + (r - a.gone[s])];
+        a.ids[r] = id;
+        if (id >= a.n_pages) a.head->bad_page = DEV_ERR_BAD_INDEX;
+    }
+}
+
+// Everything that is written.  Pages that go are read from ids: their table entries may be written here.
 __global__ void __launch_bounds__(kPlanFillThreads) k_paged_plan_fill(const __grid_constant__ PagedPlanArgs a) {
     pdl_launch_dependents();
     pdl_wait();
-    const PlanSeqs q = {a.cu, a.take, a.keeps, a.stay};
-    plan_fill(a, q, blockIdx.x * kPlanFillThreads + threadIdx.x, gridDim.x * kPlanFillThreads, a.head[0], a.head[1], a.head[2]);
+    const PlanHead h = *a.head;
+    const uint32_t at = blockIdx.x * kPlanFillThreads + threadIdx.x, step = gridDim.x * kPlanFillThreads;
+    const int bad = h.bad != DEV_ERR_NONE ? h.bad : h.bad_page;
+    if (bad != DEV_ERR_NONE) {
+        for (uint32_t s = at; s <= a.n_seq; s += step) a.cu[s] = 0;
+        if (at == 0) atomicExch(a.err, bad);
+        return;
+    }
+    for (uint32_t s = at; s <= a.n_seq; s += step) {
+        const uint32_t first = s < a.n_seq ? a.cu_copy[s] : h.tokens, next = s + 1 < a.n_seq ? a.cu_copy[s + 1] : h.tokens;
+        a.cu[s] = first;
+        if (s < a.n_seq) a.lens[s] = a.keeps[s] + (next - first);
+    }
+    if (at == 0) *a.n_free = h.top - h.take;
+    for (uint32_t r = at; r < h.gone; r += step) {
+        a.free[h.top - 1 - r] = a.ids[r];
+        const uint32_t s = owner_of(a.gone, a.n_seq, r), j = r - a.gone[s];
+        const uint32_t takes = (s + 1 < a.n_seq ? a.take[s + 1] : h.take) - a.take[s];
+        if (j >= takes) a.table[(uint64_t)s * a.max_pages + a.stay[s] + j] = kPlanNoPage;
+    }
+    const PlanSeqs q = {a.cu_copy, a.take, a.gone, a.keeps, a.stay, h.top, h.gone, h.take, h.tokens};
+    plan_fill(a, q, a.ids, at, step);
 }
 
 namespace {
@@ -214,16 +254,17 @@ constexpr size_t kPlanHead = 256;
 size_t plan_row(const PagedPlanArgs &a) { return ((size_t)a.n_seq * 4 + 255) & ~(size_t)255; }
 }  // namespace
 
-size_t paged_plan_scratch(const PagedPlanArgs &a) { return kPlanHead + 5 * plan_row(a); }
+size_t paged_plan_scratch(const PagedPlanArgs &a) { return kPlanHead + 5 * plan_row(a) + (size_t)a.n_pages * 4; }
 
 cudaError_t launch_paged_plan(const LaunchCfg &c, PagedPlanArgs a, uint8_t *scratch) {
     a.err = c.dev_err;
-    a.head = (uint32_t *)scratch;
+    a.head = (PlanHead *)scratch;
     a.take = (uint32_t *)(scratch + kPlanHead);
     a.gone = a.take + plan_row(a) / 4;
     a.keeps = a.gone + plan_row(a) / 4;
     a.stay = a.keeps + plan_row(a) / 4;
     a.cu_copy = a.stay + plan_row(a) / 4;
+    a.ids = a.cu_copy + plan_row(a) / 4;
     a.page_shift = kNoShift;
     for (uint32_t i = 0; i < 32; i++)
         if (a.page == 1u << i) a.page_shift = i;
@@ -232,6 +273,8 @@ cudaError_t launch_paged_plan(const LaunchCfg &c, PagedPlanArgs a, uint8_t *scra
     cudaError_t e = launch_k(c, "paged_plan", k_paged_plan<false>, dim3(1), dim3(kPlanThreads), 0, a);
     if (e != cudaSuccess) return e;
     const uint32_t grid = (uint32_t)min(steps, (uint64_t)c.num_sms * 8);
+    e = launch_k(c, "paged_plan_gone", k_paged_plan_gone, dim3(min(grid, (uint32_t)c.num_sms)), dim3(kPlanFillThreads), 0, a);
+    if (e != cudaSuccess) return e;
     return launch_k(c, "paged_plan_fill", k_paged_plan_fill, dim3(grid), dim3(kPlanFillThreads), 0, a);
 }
 

@@ -72,8 +72,9 @@ class Batch:
 @pytest.mark.parametrize("n_seq,page,top,most", [
     (1, 1, 5, 3), (1, 16, 40, 0), (3, 16, 40, 1), (64, 16, 300, 1), (64, 24, 300, 50), (33, 128, 3000, 700), (1024, 16, 60, 9),
     (1025, 8, 60, 9), (5000, 3, 20, 4), (7, 64, 20000, 20000), (2, 1, 3000, 2500), (65535, 1, 2, 2)])
-def test_steps(pkg, ctx, n_seq, page, top, most):
-    """Several steps in a row: grow, cut back, end, start again."""
+@pytest.mark.parametrize("room", [0, 5000])
+def test_steps(pkg, ctx, n_seq, page, top, most, room):
+    """Several steps in a row: grow, cut back, end, start again; with room for few tokens and for many, which take other launches."""
     rng = np.random.default_rng(n_seq * 131 + page)
     lens = rng.integers(0, top + 1, n_seq)
     width = -(-(top + 4 * max(1, most)) // page) + 1
@@ -86,7 +87,7 @@ def test_steps(pkg, ctx, n_seq, page, top, most):
         new = [int(x) for x in rng.integers(0, most + 1, n_seq)]
         if step == 3:
             new = [0] * n_seq
-        total = sum(new) + int(rng.integers(0, 5))
+        total = sum(new) + int(rng.integers(0, 5)) + room
         got = b.run(ctx, None if step == 2 else keep, new, total)
         want = b.want(keep, new)
         assert got[0].tolist() == want[0].tolist()
@@ -126,9 +127,16 @@ BAD = [("past the table and the pages", [5, 64, 0], [0, 0, 200], 200, 10, 1), ("
        ("a length that wraps", [5, 64, 0], [0xFFFFFFFF, 1, 0], 100, 0, 1)]
 
 
+@pytest.mark.parametrize("room", [0, 5000])
 @pytest.mark.parametrize("what,keep,new,total,less,status", BAD, ids=[b[0] for b in BAD])
-def test_refused_plans_change_nothing(pkg, ctx, what, keep, new, total, less, status):
-    b = Batch(pkg, np.random.default_rng(5), [5, 64, 0], 16, 25, 12)
+def test_refused_plans_change_nothing(pkg, ctx, what, keep, new, total, less, status, room):
+    if room and what == "more tokens than room":
+        new = [room, 3, 3]
+        total = room + 5
+        b = Batch(pkg, np.random.default_rng(5), [5, 64, 0], 16, 400, 350)
+    else:
+        total += room
+        b = Batch(pkg, np.random.default_rng(5), [5, 64, 0], 16, 25, 12)
     if less:
         b.dn.sub_(less)
         torch.cuda.synchronize()
@@ -146,8 +154,9 @@ def test_refused_plans_change_nothing(pkg, ctx, what, keep, new, total, less, st
     ctx.sync()  # reported once
 
 
+@pytest.mark.parametrize("room", [0, 5000])
 @pytest.mark.parametrize("what", ["page id", "stack too long", "stack overflows"])
-def test_broken_state_is_reported(pkg, ctx, what):
+def test_broken_state_is_reported(pkg, ctx, what, room):
     b = Batch(pkg, np.random.default_rng(6), [5, 64, 0], 16, 25, 12)
     if what == "page id":
         b.dtable[1, 3] = 25
@@ -158,7 +167,7 @@ def test_broken_state_is_reported(pkg, ctx, what):
     cu = torch.full((4,), 7, dtype=torch.int32, device="cuda")
     keep, new = dev([0, 0, 0] if what == "stack overflows" else [5, 40, 0]), dev([1, 1, 1])
     torch.cuda.synchronize()
-    ctx.paged_plan(b.state, keep, new, 3, cu)
+    ctx.paged_plan(b.state, keep, new, 3 + room, cu)
     with pytest.raises(pkg.LtError) as e:
         ctx.sync()
     assert e.value.status == 1
@@ -167,17 +176,18 @@ def test_broken_state_is_reported(pkg, ctx, what):
         assert (x == host(t)).all()
 
 
-def test_captured_steps(pkg, ctx):
+@pytest.mark.parametrize("room", [0, 5000])
+def test_captured_steps(pkg, ctx, room):
     """One captured plan replayed: a token more of every sequence each time."""
     b = Batch(pkg, np.random.default_rng(7), [5, 64, 0, 31], 16, 40, 12)
     one = dev([1, 1, 1, 1])
-    cu, seq, pos, slot = (torch.zeros(5, dtype=torch.int32, device="cuda") for _ in range(4))
+    cu, seq, pos, slot = (torch.zeros(5 + room, dtype=torch.int32, device="cuda") for _ in range(4))
     torch.cuda.synchronize()
-    ctx.paged_plan(b.state, None, one, 4, cu, seq, pos, slot)
+    ctx.paged_plan(b.state, None, one, 4 + room, cu, seq, pos, slot)
     ctx.sync()
     b.want(list(b.lens), [1] * 4)
     ctx.capture_begin()
-    ctx.paged_plan(b.state, None, one, 4, cu, seq, pos, slot)
+    ctx.paged_plan(b.state, None, one, 4 + room, cu, seq, pos, slot)
     g = ctx.capture_end()
     for _ in range(20):
         g.launch()
