@@ -192,11 +192,10 @@ struct IntC {
     static constexpr int value = N;
 };
 
-template <int HD, bool EXTRA, bool Q8>
-__global__ void __launch_bounds__(PpShape<HD, Q8>::THREADS, 1) k_paged_prompt(const __grid_constant__ PagedAttnArgs a,
-                                                                              const __grid_constant__ PpMaps maps) {
+template <int HD, bool EXTRA, bool Q8, int kPpThreads = PpShape<HD, Q8>::THREADS>
+__global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_constant__ PagedAttnArgs a, const __grid_constant__ PpMaps maps) {
     using S = PpShape<HD, Q8>;
-    constexpr int KT = S::KT, NS = S::STAGES, kPpThreads = S::THREADS, kPpProducers = S::PRODUCERS;
+    constexpr int KT = S::KT, NS = S::STAGES, kPpProducers = S::PRODUCERS;
     extern __shared__ __align__(1024) uint8_t smem[];
     uint64_t *offs = reinterpret_cast<uint64_t *>(smem + S::OFF_OFFS);
     uint32_t *docs_s = reinterpret_cast<uint32_t *>(smem + S::OFF_DOCS);
