@@ -11,13 +11,17 @@ cut to its heaviest and newest positions (lt_kv_evict), whose weights the decode
 steps accumulate.  The models are those of decoder.ModelSpec's LLAMA family with
 stacked Q/K/V rows (Qwen2, Qwen3, Qwen3-MoE shapes); every other op is the one
 the single-sequence decoder uses, on several rows.
+
+Q8BatchDecoder is the same over a cache in 8 bits (lt_paged_q8_append and its
+attention), half the bytes of an f16 one, whose page tables and lengths live on
+the device: each call plans its pages and places there (lt_paged_plan).
 """
 from __future__ import annotations
 
 from contextlib import contextmanager
 from dataclasses import dataclass, field
 
-from . import AttnCfg, Context, LogitRule, NO_MASK, PagedAttnCfg, PagedKV
+from . import AttnCfg, Context, LogitRule, NO_MASK, PagedAttnCfg, PagedKV, PagedQ8, PagedState
 from .decoder import LLAMA, ModelSpec
 
 
@@ -65,8 +69,6 @@ class BatchDecoder:
         self.n_pages = n_pages or max_seqs * self.width
         self.pool = PagePool(self.n_pages)
         self.pages = []  # of each sequence
-        kind = torch.float16 if s.kv_f16 else torch.float32
-        shape = (self.n_pages, page_size, s.n_kv_heads, s.head_dim)
         torch.cuda.synchronize()
         self.emb = torch.empty(s.vocab, s.d_model, device="cuda")
         ctx.dequant(s.token_emb, 0, s.vocab, self.emb)
@@ -74,14 +76,22 @@ class BatchDecoder:
         self.attn = PagedAttnCfg(n_heads=s.n_heads, causal=1, scale=s.head_dim ** -0.5)
         self.caches, self.mass, self.biases = [], [], []
         for L in s.layers:
-            k, v = torch.zeros(shape, dtype=kind, device="cuda"), torch.zeros(shape, dtype=kind, device="cuda")
-            kv = PagedKV(n_kv_heads=s.n_kv_heads, head_dim=s.head_dim, kv_f16=int(s.kv_f16), page_size=page_size,
-                         n_pages=self.n_pages, max_pages=self.width, k=k.data_ptr(), v=v.data_ptr())
-            self.caches.append((kv, k, v))
+            self.caches.append(self._cache())
             self.mass.append(torch.zeros(max_seqs, s.n_kv_heads, max_len, device="cuda") if budget else None)
             b = None if L.qkv_bias is None else L.qkv_bias.contiguous()  # read 16 bytes at a time
             self.biases.append(b if b is None or b.data_ptr() % 16 == 0 else b.clone())
         torch.cuda.synchronize()
+
+    def _cache(self):
+        """One layer's cache: its descriptor and what it describes."""
+        import torch
+        s = self.spec
+        kind = torch.float16 if s.kv_f16 else torch.float32
+        shape = (self.n_pages, self.page, s.n_kv_heads, s.head_dim)
+        k, v = torch.zeros(shape, dtype=kind, device="cuda"), torch.zeros(shape, dtype=kind, device="cuda")
+        kv = PagedKV(n_kv_heads=s.n_kv_heads, head_dim=s.head_dim, kv_f16=int(s.kv_f16), page_size=self.page,
+                     n_pages=self.n_pages, max_pages=self.width, k=k.data_ptr(), v=v.data_ptr())
+        return kv, k, v
 
     @contextmanager
     def _between(self):
@@ -122,8 +132,7 @@ class BatchDecoder:
                     bias, zeros = torch.empty_like(qkv), self._dev([0] * ntok)
                 ctx.gather_rows(self.biases[i], nq + 2 * nkv, zeros, ntok, bias)  # its one row for every token
                 ctx.qmatvec_add(L.wqkv, xn, bias, qkv, ntok)
-            ctx.paged_append(self.cfg, self.caches[i][0], qkv, ntok, L.q_norm, L.k_norm, seq, pos, slot, self.table,
-                             self.n_seq, q)
+            self._append(i, qkv, ntok, seq, pos, slot, q)
             attend(i, q, att)
             ctx.qmatvec_add(L.wo, att, x, x, ntok)
             if L.router is None:
@@ -131,6 +140,11 @@ class BatchDecoder:
             else:
                 ctx.moe_block(L.router, L.exp_gate, L.exp_up, L.exp_down, s.act, s.norm_topk, None, L.ffn_norm, s.eps, x,
                               ntok, s.n_used, x)
+
+    def _append(self, i: int, qkv, ntok: int, seq, pos, slot, q) -> None:
+        """Rotated queries, keys and values of layer i: the queries to q, the others into the cache."""
+        L = self.spec.layers[i]
+        self.ctx.paged_append(self.cfg, self.caches[i][0], qkv, ntok, L.q_norm, L.k_norm, seq, pos, slot, self.table, self.n_seq, q)
 
     def _choose(self, x, rows) -> list[int]:
         """The next token of every sequence from rows `rows` of x."""
@@ -285,3 +299,68 @@ class BatchDecoder:
         finally:
             self.close()
         return out
+
+
+class Q8BatchDecoder(BatchDecoder):
+    """BatchDecoder over a cache in 8-bit codes, a scale for every `block` positions of a KV head (16, 32, 64 or 128;
+    page_size is a multiple).  No budget: a position does not leave its block's scale."""
+
+    def __init__(self, ctx: Context, spec: ModelSpec, max_seqs: int, max_len: int, page_size: int = 16, n_pages: int = 0, block: int = 16):
+        import torch
+        if block not in (16, 32, 64, 128) or page_size < 1 or page_size % block:
+            raise ValueError("block: 16, 32, 64 or 128 positions; page_size a multiple of it")
+        self.block = block
+        super().__init__(ctx, spec, max_seqs, max_len, page_size, n_pages)
+        # the batch's state on the device; which pages are whose is decided there, how many each has is known here too
+        self.dlens, self.cu = self._dev([0] * max_seqs), self._dev([0] * (max_seqs + 1))
+        self.table = self._dev([NO_MASK] * (max_seqs * self.width))
+        self.free, self.n_free = self._dev(range(self.n_pages)), self._dev([self.n_pages])
+        self.state = PagedState(n_seq=max_seqs, page_size=page_size, n_pages=self.n_pages, max_pages=self.width,
+                                lens=self.dlens.data_ptr(), page_table=self.table.data_ptr(), free=self.free.data_ptr(),
+                                n_free=self.n_free.data_ptr())
+        torch.cuda.synchronize()
+
+    def _cache(self):
+        import torch
+        s = self.spec
+        codes = torch.zeros(2, self.n_pages, s.n_kv_heads, self.page, s.head_dim, dtype=torch.int8, device="cuda")
+        scales = torch.zeros(2, self.n_pages, s.n_kv_heads, self.page // self.block, device="cuda")
+        kv = PagedQ8(n_kv_heads=s.n_kv_heads, head_dim=s.head_dim, page_size=self.page, block=self.block, n_pages=self.n_pages,
+                     max_pages=self.width, k=codes[0].data_ptr(), v=codes[1].data_ptr(), k_scale=scales[0].data_ptr(),
+                     v_scale=scales[1].data_ptr())
+        return kv, codes, scales
+
+    def _plan(self, keep, new: list[int]) -> None:
+        """Pages and places of new[r] more tokens behind keep (None: all) positions of every sequence."""
+        pad = [0] * (self.max_seqs - len(new))
+        dkeep = None if keep is None else self._dev(keep + pad)
+        self.ctx.paged_plan(self.state, dkeep, self._dev(list(new) + pad), sum(new), self.cu)
+        self.ctx.sync()  # a plan that was refused is reported before anything runs on it
+
+    def _append(self, i: int, qkv, ntok: int, seq, pos, slot, q) -> None:
+        L = self.spec.layers[i]
+        self.ctx.paged_q8_append(self.cfg, self.caches[i][0], qkv, self.n_seq, self.cu, ntok, self.most, L.q_norm, L.k_norm, None,
+                                 self.table, self.dlens, q)
+
+    def _prompts(self, new: list[int]) -> list[int]:
+        import torch
+        self._plan([0] * len(new), new)  # the batch before gives its pages back
+        total = sum(new)
+        self.most = most = max(new)
+        x = torch.empty(total, self.spec.d_model, device="cuda")
+        self.ctx.gather_rows(self.emb, self.spec.d_model, self._dev([t for s in self.tokens for t in s]), total, x)
+        self._layers(x, total, None, None, None, lambda i, q, out: self.ctx.paged_q8_attn_prompt(
+            self.attn, self.caches[i][0], q, self.n_seq, self.cu, total, most, self.table, self.dlens, most, out))
+        return self._choose(x, [sum(new[:i + 1]) - 1 for i in range(len(new))])
+
+    def _next(self) -> list[int]:
+        import torch
+        n, self.most = self.n_seq, 1
+        self._plan(None, [1] * n)
+        self.lens = [v + 1 for v in self.lens]
+        self.pos = [v + 1 for v in self.pos]
+        x = torch.empty(n, self.spec.d_model, device="cuda")
+        self.ctx.gather_rows(self.emb, self.spec.d_model, self._dev([t[-1] for t in self.tokens]), n, x)
+        self._layers(x, n, None, None, None, lambda i, q, out: self.ctx.paged_q8_attn_decode(
+            self.attn, self.caches[i][0], q, n, self.table, self.dlens, max(self.lens), out))
+        return self._choose(x, range(n))
