@@ -335,7 +335,6 @@ class Q8BatchDecoder(BatchDecoder):
         pad = [0] * (self.max_seqs - len(new))
         dkeep = None if keep is None else self._dev(keep + pad)
         self.ctx.paged_plan(self.state, dkeep, self._dev(list(new) + pad), sum(new), self.cu)
-        self.ctx.sync()  # a plan that was refused is reported before anything runs on it
 
     def _append(self, i: int, qkv, ntok: int, seq, pos, slot, q) -> None:
         L = self.spec.layers[i]
