@@ -12,8 +12,8 @@
 // the page returned from entry j lies at n' - 1 - (G(s) + j - stay), and entry j
 // takes the page at n' - 1 - (T(s) + j - stay): every page and token finds its place by itself.
 //
-// Bound: latency (dependent loads and block barriers); many tokens: the writes, 12 bytes
-// each.  One CTA scans the sequences, a thread to each as far as they go round, and refuses
+// Bound: latency (dependent loads and block barriers).  One B200: a token for each of 64 sequences
+// 5.3 us; prompts of 512 sequences (325661 tokens, 10426 pages back and as many taken) 15.9 us.  One CTA scans the sequences, a thread to each as far as they go round, and refuses
 // what cannot be done before anything is changed.  Few tokens: the same CTA moves the pages and
 // places the tokens.  Many: two more launches over all SMs, one that looks at the pages that
 // go, one that writes everything (one CTA alone for the pages of 512 prompts, 10426 back and as
@@ -27,8 +27,7 @@ constexpr int kPlanThreads = 1024, kPlanWarps = kPlanThreads / 32;
 constexpr uint32_t kPlanNoPage = 0xffffffffu;
 constexpr uint32_t kPlanMaxLen = 1u << 30;
 
-// Divisions by the page size, in 32 bits (the 64-bit ones of a first version were most of its time: 10426 pages back and
-// 325661 tokens, 37 us).
+// Divisions by the page size, in 32 bits and for powers of two as shifts.
 LT_DEVINL uint32_t page_of(const PagedPlanArgs &a, uint32_t n) { return a.page_shift != kNoShift ? n >> a.page_shift : n / a.page; }
 LT_DEVINL uint32_t pages_for(const PagedPlanArgs &a, uint32_t n) { return n ? page_of(a, n - 1) + 1 : 0; }
 

@@ -11,7 +11,10 @@
 // sine and cosine: an angle in f32 alone is off by up to half a unit in its last place, 2e-4 at
 // position 4000.
 //
-// Bound: memory (each value is read and written once).  A CTA takes one block of one
+// Bound: memory (each value is read once, and written once or as a quarter of its size).  One B200: 7003
+// prompt tokens (16/8 heads of 256, normalised values) 77.6 us, 4.8 TB/s, with a warp per row and no
+// teams 214; 8192 tokens of 32/4 heads of 128 62 us, 5.0 TB/s (blocks of 128: 73); one token of each
+// of 64 sequences 5.2 us, where launch and the lengths' scan count.  A CTA takes one block of one
 // sequence; teams of its warps go through the head vectors, each warp with CHUNK of the block's
 // tokens in registers from the load to the codes, the team's maximum through shared
 // memory.  What costs instructions otherwise is shared among tokens: the sums of squares

@@ -4,15 +4,21 @@
 // The formulas are lt_paged_attn.cu's, with the blocks' scales as lt_paged_q8.cuh puts
 // them, in one pass over the keys with the running maximum m and sum l.
 //
-// Bound: memory (K and V are read once per 8 query heads of a KV head); the work is
-// shared as lt_paged_walk.cuh says.
+// Bound: memory for many or long sequences (K and V are read once per 8 query heads of a
+// KV head), latency for few; the work is shared as lt_paged_walk.cuh says.  One B200: 64
+// sequences of 200 to 8192 positions (32/4 heads of 128) 36.6 us, 4.0 TB/s; one of 130001
+// 31.8 us, 4.2 TB/s; one of 8192 10.3 us; a window of 1024 (16/8 heads of 256) 10.7 us;
+// 64 sequences, 14/2 heads of 64, 17.3 us.  Some 11 us of the long ones are the start (2 us of launch,
+// lengths -> table -> codes), the merge and the join; while the codes stream, two warps to a scheduler
+// issue in 39% of the cycles and wait for their own results in most others.  Three CTAs to an SM instead of two at
+// head_dim 128, with pieces of 16 keys or rings of 2: 46.7 and 47.8 us.
 // - Each warp owns KB keys of a tile and a ring of STAGES such pieces in shared memory,
 //   filled by 16-byte asynchronous copies, with the pieces' scales beside them.  Rows of
 //   codes lie one behind the other, their 16-byte columns permuted so that neither matrix
 //   load meets a bank conflict.
-// - Scores are exact: a query row becomes 32-bit integers (a power of two times the row,
-//   its largest element in [2^29, 2^30)), those four signed 8-bit digits, in rows r and r + 8 of two
-//   operands of the integer tensor-core product with K's codes as they lie in memory.
+// - Scores are sums of exact products: a query row becomes 32-bit integers (a power of two times
+//   the row, its largest element in [2^29, 2^30)), those four signed 8-bit digits, in rows r and r + 8
+//   of two operands of the integer tensor-core product with K's codes as they lie in memory.
 // - Weights go in as two f16 terms (22 bits) in rows r and r + 8, against V's codes in
 //   f16, where they are exact: a transposing 8-bit matrix load gives 4 keys of a dimension,
 //   and a byte b next to 0x64 is the f16 number 1024 + b.

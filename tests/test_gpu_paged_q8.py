@@ -5,8 +5,9 @@ Bars, from the arithmetic.  Attention: codes are exact in the products, scales a
 terms of 11 bits each (2^-22), sums are f32, so a score of magnitude s is off by about s * 2^-21 and a weight by as much;
 the logarithm of V's scale, |log2 vs| <= 10 here, adds 10 * 2^-24.  With |s| up to about 10: 5e-6 at worst and less in a
 sum: rel-L2 < 1e-5.
-Append: a value is off by 1e-6 of the row's norm (the norm's f32 sum and quotients, 4 roundings, the angle's 2^-23), so by
-at most 1.2e-5 of a code's step times 127 ... a code is within 0.5 + 2e-3 steps of its value; a scale within 2e-6.
+Append: a value is off by 1e-6 of its block's largest (the norm's f32 sum and quotients, 4 roundings, the angle's 2^-23; what
+a rotation mixes is no larger than twice that), and that is 127 steps: 2.6e-4 steps, the quotient's rounding 127 * 2^-24 of one.
+A code is within 0.5 + 2e-3 steps of its value, a scale within 2e-6.
 """
 from __future__ import annotations
 
