@@ -12,13 +12,15 @@
 // the page returned from entry j lies at n' - 1 - (G(s) + j - stay), and entry j
 // takes the page at n' - 1 - (T(s) + j - stay): every page and token finds its place by itself.
 //
-// Bound: latency (dependent loads and block barriers).  One B200: a token for each of 64 sequences
-// 5.3 us; prompts of 512 sequences (325661 tokens, 10426 pages back and as many taken) 15.9 us.  One CTA scans the sequences, a thread to each as far as they go round, and refuses
-// what cannot be done before anything is changed.  Few tokens: the same CTA moves the pages and
-// places the tokens.  Many: two more launches over all SMs, one that looks at the pages that
-// go, one that writes everything (one CTA alone for the pages of 512 prompts, 10426 back and as
-// many taken: 22 us, by its instructions).  Pages and tokens are dealt to threads one by one,
-// wherever their sequences begin.  Up to 2048 sequences are kept in shared memory between the steps.
+// Bound: latency (dependent loads and block barriers).  One B200: a token for each of 64
+// sequences 5.3 us; prompts of 512 (325661 tokens, 10426 pages back and as many taken)
+// 15.9 us.  One CTA scans the sequences, a thread to each as far as they go round, and
+// refuses what cannot be done before anything is changed.  Few tokens: the same CTA moves
+// the pages and places the tokens.  Many: two more launches over all SMs, one that looks
+// at the pages that go, one that writes everything (one CTA alone for the pages of those
+// prompts: 22 us, by its instructions).  Pages and tokens are dealt to threads one by
+// one, wherever their sequences begin.  Up to 2048 sequences are kept in shared memory
+// between the steps.
 #include "lt_launch.cuh"
 
 namespace lt {

@@ -195,3 +195,48 @@ def test_captured_steps(pkg, ctx, room):
         want = b.want(list(b.lens), [1] * 4)
         b.same()
         assert host(slot)[:4].tolist() == want[3] and host(pos)[:4].tolist() == want[2]
+
+
+def test_rows_for_an_f16_cache(pkg, ctx):
+    """Sequence, position and pool slot as they come, for lt_paged_append: values lie where pool_slot says."""
+    rng = np.random.default_rng(11)
+    page, kv, hd, heads = 24, 2, 64, 6
+    b = Batch(pkg, rng, [0, 50, 7, 24], page, 40, 8)
+    new = [33, 1, 0, 25]
+    total = sum(new)
+    cu, seq, pos, slot = (torch.zeros(n, dtype=torch.int32, device="cuda") for n in (len(new) + 1, total, total, total))
+    k, v = (torch.zeros(40, page, kv, hd, dtype=torch.float16, device="cuda") for _ in range(2))
+    desc = pkg.PagedKV(n_kv_heads=kv, head_dim=hd, kv_f16=1, page_size=page, n_pages=40, max_pages=8, k=k.data_ptr(), v=v.data_ptr())
+    cfg = pkg.AttnCfg(n_heads=heads, n_kv_heads=kv, head_dim=hd, rope_neox=1, rope_theta=1e5, eps=1e-6, scale=1.0, kv_cap=1, kv_f16=1)
+    x = torch.from_numpy(rng.normal(0, 1, (total, heads + 2 * kv, hd)).astype(np.float32)).cuda()
+    q = torch.zeros(total, heads, hd, device="cuda")
+    want = b.want([0, 50, 3, 24], new)
+    keep, more = dev([0, 50, 3, 24]), dev(new)
+    torch.cuda.synchronize()
+    ctx.paged_plan(b.state, keep, more, total, cu, seq, pos, slot)
+    ctx.paged_append(cfg, desc, x, total, None, None, seq, pos, None, b.dtable, len(new), q)
+    ctx.sync()
+    for got, w in zip((cu, seq, pos, slot), want):
+        assert host(got).tolist() == list(w)
+    b.same()
+    rows = host(slot)
+    assert torch.equal(v.view(-1, kv, hd)[rows], x[:, heads + kv:].half())
+    left = np.setdiff1d(np.arange(40 * page), rows)
+    assert not v.view(-1, kv, hd)[left].any() and not k.view(-1, kv, hd)[left].any()
+
+
+@pytest.mark.parametrize("room", [65535, 70000])
+def test_most_sequences(pkg, ctx, room):
+    """As many sequences as there may be: ends, cuts and growth of each, three steps."""
+    rng = np.random.default_rng(12)
+    S, page = 65535, 3
+    lens = rng.integers(0, 10, S).tolist()
+    b = Batch(pkg, rng, lens, page, 4 * S, 8)
+    for _ in range(2):
+        keep = [int(rng.integers(0, n + 1)) if rng.random() < 0.5 else n for n in b.lens]
+        new = [1 if n < 20 else 0 for n in keep]
+        want = b.want(keep, new)
+        for got, w in zip(b.run(ctx, keep, new, room), want):
+            assert got[:len(w)].tolist() == list(w)
+            assert (got[len(w):] == MARK).all()
+        b.same()

@@ -767,6 +767,78 @@ def test_prompt_scales_of_many_sizes(pkg, ctx, heads, kv, hd):
     check_prompt(pkg, ctx, heads, kv, hd, 32, 32, [150, 17], [300, 64], cap=10.0, seed=9, spread=3.0, docs=lambda j: j // 40)
 
 
+def test_most_sequences(pkg, ctx):
+    """65535 sequences of one position each: appended, then attended to by one query (its result is the value), as single
+    tokens and as rows."""
+    rng = np.random.default_rng(22)
+    S, heads, kv, hd, page = 65535, 2, 1, 64, 16
+    codes = torch.zeros(2, S, kv, page, hd, dtype=torch.int8, device="cuda")
+    scales = torch.full((2, S, kv, 1), float("nan"), device="cuda")
+    desc = pkg.PagedQ8(n_kv_heads=kv, head_dim=hd, page_size=page, block=16, n_pages=S, max_pages=1, k=codes[0].data_ptr(),
+                       v=codes[1].data_ptr(), k_scale=scales[0].data_ptr(), v_scale=scales[1].data_ptr())
+    cfg = pkg.AttnCfg(n_heads=heads, n_kv_heads=kv, head_dim=hd, rope_neox=1, rope_theta=1e5, eps=1e-6, scale=1.0, kv_cap=1)
+    acfg = pkg.PagedAttnCfg(n_heads=heads, causal=1, scale=0.125)
+    x = torch.from_numpy(rng.normal(0, 1, (S, heads + 2 * kv, hd)).astype(np.float32)).cuda()
+    order = rng.permutation(S)
+    table, lens, cu = i32(order), i32(np.ones(S)), i32(np.arange(S + 1))
+    q, one, rows = (torch.full((S, heads, hd), 7.0, device="cuda") for _ in range(3))
+    torch.cuda.synchronize()
+    ctx.paged_q8_append(cfg, desc, x, S, cu, S, 1, None, None, None, table, lens, q)
+    ctx.paged_q8_attn_decode(acfg, desc, q, S, table, lens, 1, one)
+    ctx.paged_q8_attn_prompt(acfg, desc, q, S, cu, S, 1, table, lens, 1, rows)
+    ctx.sync()
+    at = torch.from_numpy(order).cuda()
+    held = codes[1, at, 0, 0].double() * scales[1, at, 0].double()
+    v = x[:, heads + kv].double()
+    assert ((held - v).abs() <= scales[1, at, 0].double() * CODE_BAR).all()
+    for got in (one, rows):
+        # one weight over itself: the scale's inverse, 1 / l and the product are off by 2^-23 each at most, times two
+        assert ((got.double() - held[:, None]).abs() <= held[:, None].abs() * 2.0 ** -20).all()
+
+
+def test_two_contexts_at_once(pkg, ctx):
+    """A second context on a stream of its own, both with decode and prompt calls in flight: workspaces are a context's."""
+    rng = np.random.default_rng(23)
+    heads, kv, hd, lens = 32, 4, 128, [3000, 17, 900, 2500]
+    other, streams = pkg.Context(0), [torch.cuda.Stream() for _ in range(2)]
+    other.set_stream(streams[1])
+    ctx.set_stream(streams[0])
+    try:
+        sides = []
+        for k, c0 in enumerate((ctx, other)):
+            c = Cache(pkg, rng, lens, kv, hd, 16, 16)
+            n = sum(min(x, 200) for x in lens)
+            cu = np.concatenate([[0], np.cumsum([min(x, 200) for x in lens])])
+            q, o = torch.from_numpy(rng.normal(0, 1.5, (n, heads, hd)).astype(np.float32)).cuda(), torch.zeros(n, heads, hd, device="cuda")
+            sides.append((c0, c, q, o, torch.zeros(4, heads, hd, device="cuda"), i32(cu), i32(lens), n))
+        cfg = pkg.PagedAttnCfg(n_heads=heads, causal=1, scale=1 / math.sqrt(hd))
+
+        def calls(side):
+            c0, c, q, o, d, cu, ln, n = side
+            c0.paged_q8_attn_decode(cfg, c.desc, q, 4, c.dtable, ln, 3000, d)
+            c0.paged_q8_attn_prompt(cfg, c.desc, q, 4, cu, n, 200, c.dtable, ln, 3000, o)
+
+        alone = []
+        for side in sides:
+            torch.cuda.synchronize()
+            calls(side)
+            torch.cuda.synchronize()
+            alone.append((side[3].clone(), side[4].clone()))
+            side[3].zero_()
+            side[4].zero_()
+        torch.cuda.synchronize()
+        for _ in range(30):
+            for side in sides:
+                calls(side)
+        torch.cuda.synchronize()
+        for side, (o, d) in zip(sides, alone):
+            assert torch.equal(side[3], o) and torch.equal(side[4], d) and o.any() and d.any()
+            side[0].sync()
+    finally:
+        ctx.set_stream(None)
+        other.close()
+
+
 # ── together ─────────────────────────────────────────────────────────────────
 
 @pytest.mark.parametrize("heads,kv,hd", SHAPES[:3])
