@@ -12,7 +12,7 @@
 // position 4000.
 //
 // Bound: memory (each value is read once, and written once or as a quarter of its size).  One B200: 7003
-// prompt tokens (16/8 heads of 256, normalised values) 77.6 us, 4.8 TB/s, with a warp per row and no
+// prompt tokens (16/8 heads of 256, normalised values) 74.9 us, 5.0 TB/s, with a warp per row and no
 // teams 214; 8192 tokens of 32/4 heads of 128 62 us, 5.0 TB/s (blocks of 128: 73); one token of each
 // of 64 sequences 5.2 us, where launch and the lengths' scan count.  A CTA takes one block of one
 // sequence; teams of its warps go through the head vectors, each warp with CHUNK of the block's
@@ -199,6 +199,14 @@ __global__ void __launch_bounds__(kQaThreads, CHUNK == 1 ? 4 : HD * CHUNK >= 409
 #pragma unroll
                 for (int e = 0; e < N; e++) x[t][e] = y[t][e] = 0.0f;
             }
+        }
+        // The next head's rows towards L2 meanwhile.  head_dim 256, whose chunks are the fewest tokens: 77.9 -> 74.9 us; 128 loses
+        // more to the registers that the addresses take (62.2 -> 64.6).
+        if (HD == 256 && CHUNK > 1 && h + teams < last) {
+            constexpr uint32_t LINES = HD / 32;
+#pragma unroll
+            for (uint32_t i = lane; i < CHUNK * LINES; i += 32)
+                if (i / LINES < n) prefetch_l2(a.qkv + ((uint64_t)(row0 + t0 + i / LINES) * vecs + h + teams) * HD + i % LINES * 32);
         }
         const float *w = is_q ? a.q_norm : is_v ? nullptr : a.k_norm;
         if (w || (is_v && a.v_norm)) {
