@@ -767,6 +767,30 @@ def test_prompt_scales_of_many_sizes(pkg, ctx, heads, kv, hd):
     check_prompt(pkg, ctx, heads, kv, hd, 32, 32, [150, 17], [300, 64], cap=10.0, seed=9, spread=3.0, docs=lambda j: j // 40)
 
 
+@pytest.mark.parametrize("heads,kv,hd", SHAPES[:3])
+@pytest.mark.parametrize("scale", [-0.1, 0.0])
+@pytest.mark.parametrize("cap", [0.0, 20.0])
+def test_scale_of_any_sign(pkg, ctx, heads, kv, hd, scale, cap):
+    """A scale below zero turns the scores round, 0 makes all weights alike; a block of zeros for keys among the others."""
+    rng = np.random.default_rng(24)
+    n = 150
+    c = Cache(pkg, rng, [n], kv, hd, 16, 16)
+    c.hs[0][c.table[0, 3]] = 0.0
+    c.upload(pkg)
+    K, V = c.seq(0)
+    rows = rng.normal(0, 1.0, (n, heads, hd)).astype(np.float32)
+    qd, out, one = torch.from_numpy(rows).cuda(), torch.zeros(n, heads, hd, device="cuda"), torch.zeros(1, heads, hd, device="cuda")
+    cu, ln, cfg = i32([0, n]), i32([n]), pkg.PagedAttnCfg(n_heads=heads, causal=1, scale=scale, softcap=cap)
+    torch.cuda.synchronize()
+    ctx.paged_q8_attn_prompt(cfg, c.desc, qd, 1, cu, n, n, c.dtable, ln, n, out)
+    ctx.paged_q8_attn_decode(cfg, c.desc, qd[n - 1:], 1, c.dtable, ln, n, one)
+    ctx.sync()
+    i = np.arange(n)
+    want = attend(rows, K, V, i, i[None] <= i[:, None], scale, cap)
+    assert rel(out.cpu(), want) < ATTN_BAR
+    assert rel(one.cpu(), want[n - 1:]) < ATTN_BAR
+
+
 def test_most_sequences(pkg, ctx):
     """65535 sequences of one position each: appended, then attended to by one query (its result is the value), as single
     tokens and as rows."""
