@@ -245,7 +245,8 @@ struct PagedPlanArgs {
     uint32_t *lens, *table, *free, *n_free, *cu, *seq, *pos, *slot;
     // scratch, set by the launcher: [n_seq] each, and [n_pages] page ids
     PlanHead *head;
-    uint32_t *take, *gone, *keeps, *stay, *cu_copy, *ids;
+    uint32_t *take, *gone, *keeps, *stay, *cu_copy, *ids, *flags;
+    uint32_t n_flags;               // one of each CTA that looked at pages
     uint32_t page_shift;            // log2 of page, or kNoShift; set by the launcher
     int *err;
 };

@@ -16,11 +16,12 @@
 // sequences 5.3 us; prompts of 512 (325661 tokens, 10426 pages back and as many taken)
 // 15.9 us.  One CTA scans the sequences, a thread to each as far as they go round, and
 // refuses what cannot be done before anything is changed.  Few tokens: the same CTA moves
-// the pages and places the tokens.  Many: two more launches over all SMs, one that looks
-// at the pages that go, one that writes everything (one CTA alone for the pages of those
-// prompts: 22 us, by its instructions).  Pages and tokens are dealt to threads one by
-// one, wherever their sequences begin.  Up to 2048 sequences are kept in shared memory
-// between the steps.
+// the pages and places the tokens.  Many: all SMs, in two launches (one CTA alone for the
+// pages of those prompts: 22 us, by its instructions): every CTA scans the sequences
+// for itself and looks at its share of the pages that go, then everything is written.
+// Pages and tokens are dealt to threads one by one, wherever their sequences begin.  Up to
+// 2048 sequences are kept in shared memory between the steps; more are scanned by one CTA,
+// and the pages looked at in a launch of their own.
 #include "lt_launch.cuh"
 
 namespace lt {
@@ -84,7 +85,8 @@ struct PlanSum {
 
 constexpr uint32_t kPlanInShared = 2048;  // sequences
 
-// ALONE: the same CTA does everything.  Else it writes what it found to scratch, and nothing of the caller's.
+// ALONE: the one CTA does everything.  Else what was found goes to scratch, by CTA 0, and nothing to the caller's; all CTAs
+// look at the pages that go where the sequences are in shared memory.
 template <bool ALONE>
 __global__ void __launch_bounds__(kPlanThreads) k_paged_plan(const __grid_constant__ PagedPlanArgs a) {
     __shared__ PlanSum s_warp[kPlanWarps], s_all;
@@ -161,14 +163,25 @@ __global__ void __launch_bounds__(kPlanThreads) k_paged_plan(const __grid_consta
     }
     bool ok = s_bad == DEV_ERR_NONE;
     if (!ALONE) {
-        for (uint32_t s = sa; in_shared && s < sb; s++) {
+        for (uint32_t s = sa; in_shared && blockIdx.x == 0 && s < sb; s++) {
             a.cu_copy[s] = cu[s];
             a.take[s] = take[s];
             a.gone[s] = gone[s];
             a.keeps[s] = keeps[s];
             a.stay[s] = stays[s];
         }
-        if (tid == 0) *a.head = {top, (uint32_t)all.gone, (uint32_t)all.take, (uint32_t)all.tokens, s_bad, n_free};
+        if (blockIdx.x == 0 && tid == 0) *a.head = {top, (uint32_t)all.gone, (uint32_t)all.take, (uint32_t)all.tokens, s_bad, n_free};
+        if (!in_shared) return;
+        __syncthreads();
+        bool off = false;
+        for (uint32_t r = blockIdx.x * kPlanThreads + tid; ok && r < all.gone; r += gridDim.x * kPlanThreads) {
+            const uint32_t s = owner_of(gone, a.n_seq, r);
+            const uint32_t id = a.table[(uint64_t)s * a.max_pages + stays[s] + (r - gone[s])];
+            a.ids[r] = id;
+            off |= id >= a.n_pages;
+        }
+        off = __syncthreads_or(off);
+        if (tid == 0) a.flags[blockIdx.x] = off;
         return;
     }
     if (ok && all.gone) {
@@ -209,7 +222,7 @@ __global__ void __launch_bounds__(kPlanThreads) k_paged_plan(const __grid_consta
 
 constexpr int kPlanFillThreads = 256;
 
-// The pages that go, looked at.
+// The pages that go, looked at: of more sequences than shared memory holds.
 __global__ void __launch_bounds__(kPlanFillThreads) k_paged_plan_gone(const __grid_constant__ PagedPlanArgs a) {
     pdl_launch_dependents();
     pdl_wait();
@@ -228,7 +241,10 @@ __global__ void __launch_bounds__(kPlanFillThreads) k_paged_plan_fill(const __gr
     pdl_wait();
     const PlanHead h = *a.head;
     const uint32_t at = blockIdx.x * kPlanFillThreads + threadIdx.x, step = gridDim.x * kPlanFillThreads;
-    const int bad = h.bad != DEV_ERR_NONE ? h.bad : h.bad_page;
+    bool off = false;
+    for (uint32_t i = threadIdx.x; i < a.n_flags; i += kPlanFillThreads) off |= a.flags[i] != 0;
+    off = __syncthreads_or(off) || h.bad_page != DEV_ERR_NONE;
+    const int bad = h.bad != DEV_ERR_NONE ? h.bad : off ? DEV_ERR_BAD_INDEX : DEV_ERR_NONE;
     if (bad != DEV_ERR_NONE) {
         for (uint32_t s = at; s <= a.n_seq; s += step) a.cu[s] = 0;
         if (at == 0) atomicExch(a.err, bad);
@@ -251,7 +267,8 @@ __global__ void __launch_bounds__(kPlanFillThreads) k_paged_plan_fill(const __gr
 }
 
 namespace {
-constexpr size_t kPlanHead = 256;
+constexpr size_t kPlanHead = 4096;  // and the flags behind it
+constexpr uint32_t kPlanMostFlags = (4096 - 256) / 4;
 size_t plan_row(const PagedPlanArgs &a) { return ((size_t)a.n_seq * 4 + 255) & ~(size_t)255; }
 }  // namespace
 
@@ -260,6 +277,7 @@ size_t paged_plan_scratch(const PagedPlanArgs &a) { return kPlanHead + 5 * plan_
 cudaError_t launch_paged_plan(const LaunchCfg &c, PagedPlanArgs a, uint8_t *scratch) {
     a.err = c.dev_err;
     a.head = (PlanHead *)scratch;
+    a.flags = (uint32_t *)(scratch + 256);
     a.take = (uint32_t *)(scratch + kPlanHead);
     a.gone = a.take + plan_row(a) / 4;
     a.keeps = a.gone + plan_row(a) / 4;
@@ -271,11 +289,15 @@ cudaError_t launch_paged_plan(const LaunchCfg &c, PagedPlanArgs a, uint8_t *scra
         if (a.page == 1u << i) a.page_shift = i;
     const uint64_t steps = ((uint64_t)a.total_q + kPlanFillThreads - 1) / kPlanFillThreads;
     if (steps <= 16) return launch_k(c, "paged_plan", k_paged_plan<true>, dim3(1), dim3(kPlanThreads), 0, a);
-    cudaError_t e = launch_k(c, "paged_plan", k_paged_plan<false>, dim3(1), dim3(kPlanThreads), 0, a);
+    const uint32_t grid = (uint32_t)min(steps, (uint64_t)c.num_sms * 8), look = min(grid, min((uint32_t)c.num_sms, kPlanMostFlags));
+    const bool in_shared = a.n_seq <= kPlanInShared;
+    a.n_flags = in_shared ? look : 0;
+    cudaError_t e = launch_k(c, "paged_plan", k_paged_plan<false>, dim3(in_shared ? look : 1), dim3(kPlanThreads), 0, a);
     if (e != cudaSuccess) return e;
-    const uint32_t grid = (uint32_t)min(steps, (uint64_t)c.num_sms * 8);
-    e = launch_k(c, "paged_plan_gone", k_paged_plan_gone, dim3(min(grid, (uint32_t)c.num_sms)), dim3(kPlanFillThreads), 0, a);
-    if (e != cudaSuccess) return e;
+    if (!in_shared) {
+        e = launch_k(c, "paged_plan_gone", k_paged_plan_gone, dim3(look), dim3(kPlanFillThreads), 0, a);
+        if (e != cudaSuccess) return e;
+    }
     return launch_k(c, "paged_plan_fill", k_paged_plan_fill, dim3(grid), dim3(kPlanFillThreads), 0, a);
 }
 
