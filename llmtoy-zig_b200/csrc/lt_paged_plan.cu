@@ -13,8 +13,8 @@
 // takes the page at n' - 1 - (T(s) + j - stay): every page and token finds its place by itself.
 //
 // Bound: latency (dependent loads and block barriers).  One B200: a token for each of 64
-// sequences 5.3 us; prompts of 512 (325661 tokens, 10426 pages back and as many taken)
-// 15.9 us.  One CTA scans the sequences, a thread to each as far as they go round, and
+// sequences 4.9 us; prompts of 512 (325661 tokens, 10426 pages back and as many taken)
+// 10.4 us (in three launches, threads with pages and tokens to place alike, 15.9).  One CTA scans the sequences, a thread to each as far as they go round, and
 // refuses what cannot be done before anything is changed.  Few tokens: the same CTA moves
 // the pages and places the tokens.  Many: all SMs, in two launches (one CTA alone for the
 // pages of those prompts: 22 us, by its instructions): every CTA scans the sequences
@@ -59,10 +59,11 @@ LT_DEVINL uint32_t taken(const PagedPlanArgs &a, const PlanSeqs &q, const uint32
     return ids && k < q.n_gone ? ids[k] : a.free[q.top - 1 - k];
 }
 
-// Table entries and token rows, thread `at` of `step`.  Nothing that is read here is written here.
+// Table entries and token rows, thread `at` of `step`; entries from the middle thread on, so that few threads have
+// both.  Nothing that is read here is written here.
 LT_DEVINL void plan_fill(const PagedPlanArgs &a, const PlanSeqs &q, const uint32_t *ids, uint32_t at, uint32_t step) {
     const uint32_t n = a.n_seq;
-    for (uint32_t k = at; k < q.n_take; k += step) {
+    for (uint32_t k = at < step / 2 ? at + step - step / 2 : at - step / 2; k < q.n_take; k += step) {
         const uint32_t s = owner_of(q.take, n, k);
         a.table[(uint64_t)s * a.max_pages + q.stay[s] + (k - q.take[s])] = taken(a, q, ids, k);
     }
@@ -256,7 +257,7 @@ __global__ void __launch_bounds__(kPlanFillThreads) k_paged_plan_fill(const __gr
         if (s < a.n_seq) a.lens[s] = a.keeps[s] + (next - first);
     }
     if (at == 0) *a.n_free = h.top - h.take;
-    for (uint32_t r = at; r < h.gone; r += step) {
+    for (uint32_t r = step - 1 - at; r < h.gone; r += step) {  // from the last thread on
         a.free[h.top - 1 - r] = a.ids[r];
         const uint32_t s = owner_of(a.gone, a.n_seq, r), j = r - a.gone[s];
         const uint32_t takes = (s + 1 < a.n_seq ? a.take[s + 1] : h.take) - a.take[s];
