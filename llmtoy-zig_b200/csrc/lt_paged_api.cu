@@ -382,13 +382,14 @@ lt_status lt_paged_q8_attn_prompt(lt_ctx *ctx, const lt_paged_attn_cfg *cfg, con
     a.doc_stride = (uint32_t)doc_stride;
     const lt::LaunchCfg c = lt::ctx_cfg(ctx);
     uint8_t *scratch = nullptr;
+    const size_t most = lt::paged_prompt_scratch_most(a, c.num_sms);
     if (lt::paged_prompt_supported(a)) {
-        const size_t need = lt::paged_prompt_scratch(a, c.num_sms), most = lt::paged_prompt_scratch_most(a, c.num_sms);
+        const size_t need = lt::paged_prompt_scratch(a, c.num_sms);
         if ((st = st_of(lt::ctx_scratch(ctx, most, need, &scratch))) != LT_OK) return st;
         return st_of(lt::ctx_launched(ctx, lt::launch_paged_prompt(c, a, scratch), "8-bit paged prompt attention"));
     }
     const size_t need = lt::paged_q8_attn_scratch(a, c.num_sms);
-    if ((st = st_of(lt::ctx_scratch(ctx, need, need, &scratch))) != LT_OK) return st;
+    if ((st = st_of(lt::ctx_scratch(ctx, most > need ? most : need, need, &scratch))) != LT_OK) return st;
     return st_of(lt::ctx_launched(ctx, lt::launch_paged_q8_attn(c, a, scratch), "8-bit paged prompt attention"));
 }
 

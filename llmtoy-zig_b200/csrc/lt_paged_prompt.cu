@@ -1212,11 +1212,13 @@ size_t paged_prompt_scratch(PagedAttnArgs a, int num_sms) {
 
 // Enough for this call and for every smaller one, so that an op run once at its largest sizes has its scratch when a
 // smaller call is recorded.  Only smaller calls may share their keys, and there are records only where a launch has no
-// more CTAs than SMs; the fewest rows take the other kernel with its own scratch.
+// more CTAs than SMs; the fewest rows take the other kernel with its own scratch (a call that does so itself may have
+// smaller ones of as many rows here, where a shorter cache has the lower bound).
 size_t paged_prompt_scratch_most(const PagedAttnArgs &a, int num_sms) {
-    const size_t records = (size_t)num_sms * pp_rows(a) * (a.kv.hd + 2) * 4;
+    const uint32_t least = min(pp_few(a.kv).rows, pp_few(a.kv).rows_short), most = max(pp_few(a.kv).rows, pp_few(a.kv).rows_short);
+    const size_t records = (uint64_t)a.max_q * a.group > least ? (size_t)num_sms * pp_rows(a) * (a.kv.hd + 2) * 4 : 0;
     PagedAttnArgs few = a;
-    few.max_q = min(a.max_q, max(pp_few(a.kv).rows, pp_few(a.kv).rows_short) / a.group);
+    few.max_q = min(a.max_q, most / a.group);
     if (!few.max_q) return records;
     return max(records, few.kv.k_scale ? paged_q8_attn_scratch(few, num_sms) : paged_attn_scratch(few, num_sms));
 }

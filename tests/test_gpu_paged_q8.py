@@ -768,6 +768,52 @@ def test_prompt_scales_of_many_sizes(pkg, ctx, heads, kv, hd):
 
 
 @pytest.mark.parametrize("heads,kv,hd", SHAPES[:3])
+@pytest.mark.parametrize("largest", [300, 13, 10, 5])
+def test_smaller_calls_need_no_more_scratch(pkg, heads, kv, hd, largest):
+    """Each op run once with its largest sizes, then recorded with smaller ones: fewer rows, or shorter caches, go to another
+    kernel or are shared among more CTAs, and the arena has to hold what either needs.  Each graph is launched, too."""
+    rng = np.random.default_rng(25)
+    S, n, most = 9, 250, 4096
+    c = Cache(pkg, rng, [n] * S, kv, hd, 16, 16, spare=most // 16)
+    cfg = pkg.PagedAttnCfg(n_heads=heads, causal=1, scale=1 / math.sqrt(hd))
+    q, out, ln = torch.randn(S * 300, heads * hd, device="cuda"), torch.zeros(S * 300, heads * hd, device="cuda"), i32([n] * S)
+    ms = [m for m in (300, 64, 13, 10, 9, 5, 3, 1) if m <= largest]
+    cus = {(s, m): i32(np.arange(s + 1) * m) for s in (S, 3, 1) for m in ms}
+    torch.cuda.synchronize()
+
+    def prompt(ctx, s, m, max_len):
+        ctx.paged_q8_attn_prompt(cfg, c.desc, q, s, cus[s, m], s * m, m, c.dtable, ln, max_len, out)
+
+    calls = [(s, m, l) for s in (S, 3, 1) for m in ms for l in (n, 600, most)]
+    want = []
+    with pkg.Context(0) as ctx:
+        prompt(ctx, S, largest, most)
+        ctx.paged_q8_attn_decode(cfg, c.desc, q, S, c.dtable, ln, most, out)
+        ctx.sync()
+        for a in calls:
+            ctx.capture_begin()
+            prompt(ctx, *a)
+            ctx.paged_q8_attn_decode(cfg, c.desc, q, a[0], c.dtable, ln, a[2], out)
+            ctx.capture_end().free()
+            ctx.capture_begin()
+            prompt(ctx, *a)
+            graph = ctx.capture_end()
+            out.zero_()
+            torch.cuda.synchronize()
+            graph.launch()
+            ctx.sync()
+            want.append(out.clone())
+            graph.free()
+    with pkg.Context(0) as ctx:  # and they compute what they do without a graph
+        for a, w in zip(calls, want):
+            out.zero_()
+            torch.cuda.synchronize()
+            prompt(ctx, *a)
+            ctx.sync()
+            assert torch.equal(out, w), a
+
+
+@pytest.mark.parametrize("heads,kv,hd", SHAPES[:3])
 @pytest.mark.parametrize("scale", [-0.1, 0.0])
 @pytest.mark.parametrize("cap", [0.0, 20.0])
 def test_scale_of_any_sign(pkg, ctx, heads, kv, hd, scale, cap):
