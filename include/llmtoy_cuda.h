@@ -87,10 +87,11 @@ int         lt_api_version(void);
 lt_status   lt_init(int device, lt_ctx **out);
 void        lt_free(lt_ctx *ctx);
 /* Use an existing cudaStream_t (passed as void*); NULL selects the
- * context's own stream (non-blocking).  The legacy default stream is
- * cudaStreamLegacy ((void *)1), the per-thread one cudaStreamPerThread
- * ((void *)2); on those two the kernels launch without programmatic
- * dependent launch. */
+ * context's own stream, a blocking one: its work and the legacy default
+ * stream's run in the order in which they were issued.  The legacy default
+ * stream itself is cudaStreamLegacy ((void *)1), the per-thread one
+ * cudaStreamPerThread ((void *)2); on those two the kernels launch without
+ * programmatic dependent launch. */
 lt_status   lt_set_stream(lt_ctx *ctx, void *cuda_stream);
 lt_status   lt_sync(lt_ctx *ctx);
 const char *lt_last_error(const lt_ctx *ctx);
@@ -242,9 +243,10 @@ lt_status lt_profile_reset(lt_ctx *ctx);
 /* ── CUDA graph capture ───────────────────────────────────────────────────
  * Records the device ops issued between begin and end on the context stream
  * into a graph that lt_graph_launch replays (one launch per decode token
- * instead of one per kernel).  The stream must not be the legacy default
- * stream; call lt_reserve, or each op once at its largest sizes, first so no op
- * allocates while capturing.  An op that needs a larger arena later gets a new
+ * instead of one per kernel).  Where that is the context's own stream or a
+ * default one, the recording itself is on a stream apart, and work that anyone
+ * issues to the default stream meanwhile goes on.  Call lt_reserve, or each op
+ * once at its largest sizes, first so no op allocates while capturing.  An op that needs a larger arena later gets a new
  * one: what graphs were recorded with stays allocated until lt_free, and they
  * may be launched as before.  The same holds where the owner of the stream
  * records it. */

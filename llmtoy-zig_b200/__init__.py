@@ -322,8 +322,9 @@ class Context:
 
     def set_stream(self, stream) -> None:
         """Run ops on a cudaStream_t (int handle or torch.cuda.Stream); None: the context's own
-        stream.  Handle 0, torch's default stream, means the legacy default stream
-        (cudaStreamLegacy), so work torch queues there orders with these ops."""
+        stream, which a context starts on.  Handle 0, torch's default stream, means the legacy
+        default stream (cudaStreamLegacy).  On either, work that torch queues on its default stream
+        orders with these ops; work on other streams of torch's does not."""
         if stream is None:
             handle = None
         else:

@@ -23,7 +23,7 @@ struct lt_tensor {
 
 struct lt_ctx {
     int device = 0;
-    cudaStream_t own = nullptr;
+    cudaStream_t own = nullptr;      // takes turns with the legacy default stream
     cudaStream_t stream = nullptr;
     std::string err;
     int num_sms = 0;
@@ -50,8 +50,11 @@ struct lt_ctx {
     // replaced by a larger one without being freed, and lt_free frees it.
     bool scratch_recorded = false, counters_recorded = false, consts_recorded = false;
     std::vector<void *> kept;
-    cudaStream_t cap_user = nullptr; // the caller's stream while a capture runs on `own`
-    cudaEvent_t cap_ev = nullptr;    // joins `own` to the caller's stream for such a capture
+    // A stream that records what is called between lt_capture_begin and _end where `stream` is `own` or a default
+    // stream, and `stream` meanwhile.  It is no one's turn with the legacy stream: a stream that takes turns with it would
+    // make every launch there, any thread's, fail and the recording with it.
+    cudaStream_t cap = nullptr;
+    cudaStream_t cap_user = nullptr;
     lt::Profiler prof;
 };
 
@@ -365,8 +368,10 @@ lt_status lt_init(int device, lt_ctx **out) {
     const char *tc = getenv("LLMTOY_TC_MIN_TOKENS");  // 0 turns the tensor-core expert GEMM off
     if (tc) ctx->tc_min_tokens = (uint32_t)strtoul(tc, nullptr, 10);
     lt_status st = LT_OK;
+    // The own stream is one that the legacy default stream waits for and that waits for it: callers whose other work is
+    // there, torch's by default, need no waits of their own.
     if (cudaSetDevice(device) != cudaSuccess ||
-        cudaStreamCreateWithFlags(&ctx->own, cudaStreamNonBlocking) != cudaSuccess ||
+        cudaStreamCreateWithFlags(&ctx->own, cudaStreamDefault) != cudaSuccess ||
         cudaMalloc(&ctx->dev_err, 4) != cudaSuccess || cudaMemset(ctx->dev_err, 0, 4) != cudaSuccess ||
         cudaMalloc(&ctx->dec_sync, lt::kDecodeSyncBytes) != cudaSuccess ||
         cudaMemset(ctx->dec_sync, 0, lt::kDecodeSyncBytes) != cudaSuccess ||
@@ -391,6 +396,7 @@ void lt_free(lt_ctx *ctx) {
         cudaGraph_t g = nullptr;
         cudaStreamEndCapture(ctx->stream, &g);
         if (g) cudaGraphDestroy(g);
+        if (ctx->cap_user) ctx->stream = ctx->cap_user;
     }
     if (ctx->stream) cudaStreamSynchronize(ctx->stream);
     ctx->prof.destroy();
@@ -403,7 +409,7 @@ void lt_free(lt_ctx *ctx) {
     if (ctx->ones) cudaFree(ctx->ones);
     if (ctx->zeros) cudaFree(ctx->zeros);
     if (ctx->pinned) cudaFreeHost(ctx->pinned);
-    if (ctx->cap_ev) cudaEventDestroy(ctx->cap_ev);
+    if (ctx->cap) cudaStreamDestroy(ctx->cap);
     if (ctx->own) cudaStreamDestroy(ctx->own);
     delete ctx;
 }
@@ -453,14 +459,11 @@ lt_status lt_capture_begin(lt_ctx *ctx) {
     if (ctx->capturing) return fail(ctx, LT_EINVAL, "lt_capture_begin: already capturing");
     if (ctx->prof.on) return fail(ctx, LT_EINVAL, "lt_capture_begin: turn profiling off first");
     ctx->cap_user = nullptr;
-    if (ctx->stream == cudaStreamLegacy || ctx->stream == cudaStreamPerThread) {
-        // the default streams cannot be captured: capture on the context's own
-        // stream, ordered after the caller's work; the graph launches on any stream
-        if (!ctx->cap_ev) LT_CUDA(ctx, cudaEventCreateWithFlags(&ctx->cap_ev, cudaEventDisableTiming), "cudaEventCreate");
-        LT_CUDA(ctx, cudaEventRecord(ctx->cap_ev, ctx->stream), "cudaEventRecord");
-        LT_CUDA(ctx, cudaStreamWaitEvent(ctx->own, ctx->cap_ev, 0), "cudaStreamWaitEvent");
+    if (ctx->stream == cudaStreamLegacy || ctx->stream == cudaStreamPerThread || ctx->stream == ctx->own) {
+        // recorded on a stream apart (nothing runs there); the graph launches on the context's
+        if (!ctx->cap) LT_CUDA(ctx, cudaStreamCreateWithFlags(&ctx->cap, cudaStreamNonBlocking), "cudaStreamCreate");
         ctx->cap_user = ctx->stream;
-        ctx->stream = ctx->own;
+        ctx->stream = ctx->cap;
     }
     cudaError_t e = cudaStreamBeginCapture(ctx->stream, cudaStreamCaptureModeThreadLocal);
     if (e != cudaSuccess) {

@@ -229,6 +229,16 @@ def test_append_token_by_token(pkg, ctx, block):
         a.check([1], [n], scale_of=1.0 + (n % 7))
 
 
+@pytest.mark.parametrize("heads,kv,hd,page,block,new,past", [
+    (4, 8, 256, 32, 32, [4001, 1001, 2001], [0, 700, 41]), (6, 2, 64, 128, 128, [6000], [3]), (2, 4, 128, 48, 16, [3000, 1], [7, 15])])
+def test_append_long(pkg, ctx, heads, kv, hd, page, block, new, past):
+    """More blocks than the device runs at once, thousands of rows to a sequence."""
+    rng = np.random.default_rng(31)
+    lens = [a + b for a, b in zip(new, past)]
+    c = Cache(pkg, rng, lens, kv, hd, page, block)
+    Appends(pkg, ctx, c, rng, heads, neox=hd != 256, v_norm=hd != 128, theta=1e6).check(new, lens)
+
+
 def test_append_twice_changes_nothing(pkg, ctx):
     rng = np.random.default_rng(1)
     heads, kv, hd, new, lens = 8, 2, 128, [5, 33, 1], [21, 40, 64]
