@@ -25,32 +25,32 @@ EPS = 1e-6
 def listed():
     return [
         # one step of a batch of chats: a token each, a few chats cut back or ended before it
-        dict(name="plan one step", op="plan", seqs=64, new_lo=1, new_hi=1, past_lo=100, past_hi=4000, cut=0.2, page=16),
+        dict(name="plan, one step", op="plan", seqs=64, new_lo=1, new_hi=1, past_lo=100, past_hi=4000, cut=0.2, page=16),
         # a wave of prompts: pages and slots of a quarter of a million tokens
-        dict(name="plan prompts", op="plan", seqs=512, new_lo=100, new_hi=2000, past_lo=0, past_hi=1000, cut=0.5, page=32),
+        dict(name="plan, prompts", op="plan", seqs=512, new_lo=100, new_hi=2000, past_lo=0, past_hi=1000, cut=0.5, page=32),
         # one decode step of a batch of chats: a token each, most into a block that holds others already
-        dict(name="append 64 sequences", op="append", seqs=64, new_lo=1, new_hi=1, past_lo=16, past_hi=250, heads=32,
+        dict(name="append, 64 sequences", op="append", seqs=64, new_lo=1, new_hi=1, past_lo=16, past_hi=250, heads=32,
              kv=4, hd=128, page=16, block=16, v_norm=False, neox=True),
         # three prompts of uneven length with normalised values, behind cached conversations
-        dict(name="append prompts", op="append", seqs=3, new_lo=1001, new_hi=4001, past_lo=0, past_hi=700, heads=16,
+        dict(name="append, prompts", op="append", seqs=3, new_lo=1001, new_hi=4001, past_lo=0, past_hi=700, heads=16,
              kv=8, hd=256, page=32, block=32, v_norm=True, neox=False),
         # one chat on a sliding-window layer with capped scores: the call's latency is what counts
-        dict(name="decode one window", op="decode", seqs=1, lo=2345, hi=2345, heads=16, kv=8, hd=256, page=32, block=32,
+        dict(name="decode, one window", op="decode", seqs=1, lo=2345, hi=2345, heads=16, kv=8, hd=256, page=32, block=32,
              softcap=50.0, window=1024, alibi=False),
         # a batch of chats with histories of very different lengths
-        dict(name="decode 64 ragged", op="decode", seqs=64, lo=200, hi=8192, heads=32, kv=4, hd=128, page=16, block=16,
+        dict(name="decode, 64 ragged", op="decode", seqs=64, lo=200, hi=8192, heads=32, kv=4, hd=128, page=16, block=16,
              softcap=0.0, window=0, alibi=False),
         # one long document
-        dict(name="decode one long", op="decode", seqs=1, lo=130001, hi=130001, heads=32, kv=4, hd=128, page=64, block=64,
+        dict(name="decode, one long", op="decode", seqs=1, lo=130001, hi=130001, heads=32, kv=4, hd=128, page=64, block=64,
              softcap=0.0, window=0, alibi=False),
         # a short follow-up question on a cached conversation
-        dict(name="prompt follow-up", op="prompt", seqs=1, new_lo=257, new_hi=257, past_lo=1243, past_hi=1243, heads=14,
+        dict(name="prompt, follow-up", op="prompt", seqs=1, new_lo=257, new_hi=257, past_lo=1243, past_hi=1243, heads=14,
              kv=2, hd=64, page=16, block=16, causal=True, softcap=0.0, window=0, alibi=False, prefix=0, doc=0),
         # one long prompt from its first token
-        dict(name="prompt 8192", op="prompt", seqs=1, new_lo=8192, new_hi=8192, past_lo=0, past_hi=0, heads=32, kv=4,
+        dict(name="prompt, 8192", op="prompt", seqs=1, new_lo=8192, new_hi=8192, past_lo=0, past_hi=0, heads=32, kv=4,
              hd=128, page=16, block=16, causal=True, softcap=0.0, window=0, alibi=False, prefix=0, doc=0),
         # packed documents, the first tokens seen in both directions, capped scores and a distance bias
-        dict(name="prompt documents", op="prompt", seqs=3, new_lo=1501, new_hi=2777, past_lo=0, past_hi=515, heads=16,
+        dict(name="prompt, documents", op="prompt", seqs=3, new_lo=1501, new_hi=2777, past_lo=0, past_hi=515, heads=16,
              kv=8, hd=256, page=32, block=32, causal=True, softcap=50.0, window=1024, alibi=True, prefix=300, doc=900),
     ]
 
@@ -135,15 +135,14 @@ def _pkg():
     return importlib.import_module("llmtoy-zig_b200")
 
 
-_context = _stream = None
+_context = None
 
 
 def _ctx():
-    """The one device context that a program keeps, on a stream that it shares with torch."""
-    global _context, _stream
+    """The one device context that a program keeps."""
+    global _context
     if _context is None:
-        _context, _stream = _pkg().Context(0), torch.cuda.Stream()
-        _context.set_stream(_stream)
+        _context = _pkg().Context(0)
     return _context
 
 
@@ -283,8 +282,7 @@ def _own_plan(st):
 def _own_append(st):
     _ctx().paged_q8_append(st["cfg"], st["kvh"], st["qkv"], st["case"]["seqs"], st["cu"], st["total"], st["max_q"], st["qn"],
                            st["kn"], None, st["table"], st["lens"], st["q"])
-    with torch.cuda.stream(_stream):  # behind the call
-        return _append_outputs(st)
+    return _append_outputs(st)
 
 
 def _own_decode(st):
