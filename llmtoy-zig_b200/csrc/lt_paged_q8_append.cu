@@ -222,7 +222,10 @@ __global__ void __launch_bounds__(kQaThreads, CHUNK == 1 ? 4 : HD * CHUNK >= 409
 #pragma unroll
                 for (int e = 0; e < N; e++) ss[t] = fmaf(x[t][e], x[t][e], fmaf(y[t][e], y[t][e], ss[t]));
             }
-            const float inv = __fdiv_rn(1.0f, __fsqrt_rn(fmaf(warp_sums<CHUNK>(ss, lane), 1.0f / HD, a.eps)));
+            // 0 for rows that are not there, which stay 0 and out of the block's maximum: with eps = 0 their own inverse
+            // would be infinite
+            const float mean = fmaf(warp_sums<CHUNK>(ss, lane), 1.0f / HD, a.eps);
+            const float inv = (uint32_t)lane % CHUNK < n ? __fdiv_rn(1.0f, __fsqrt_rn(mean)) : 0.0f;
 #pragma unroll
             for (int t = 0; t < CHUNK; t++) {
                 const float f = __shfl_sync(0xffffffffu, inv, t);

@@ -239,6 +239,20 @@ def test_append_long(pkg, ctx, heads, kv, hd, page, block, new, past):
     Appends(pkg, ctx, c, rng, heads, neox=hd != 256, v_norm=hd != 128, theta=1e6).check(new, lens)
 
 
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("block", [16, 32, 64, 128])
+def test_append_without_eps(pkg, ctx, hd, block):
+    """eps = 0: rows that a warp's share of a block lacks are no rows of zeros to be normalised.  Sequences that end at every
+    kind of place in their blocks, shares of a block with some rows, one and none; begun blocks, too."""
+    rng = np.random.default_rng(32)
+    heads, kv, new = 3, 2, [17, 1, 0, 31, 7, 130]
+    c = Cache(pkg, rng, [20, 1, 5, 32, 70, 131], kv, hd, 128, block)
+    a = Appends(pkg, ctx, c, rng, heads, v_norm=True)
+    a.eps = a.cfg.eps = 0.0
+    a.check(new, c.lens)
+    a.check([2, 1, 0, 15, 1, 9], c.lens, scale_of=5.0)
+
+
 def test_append_twice_changes_nothing(pkg, ctx):
     rng = np.random.default_rng(1)
     heads, kv, hd, new, lens = 8, 2, 128, [5, 33, 1], [21, 40, 64]
