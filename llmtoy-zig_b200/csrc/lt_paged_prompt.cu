@@ -53,6 +53,9 @@ namespace lt {
 // the ring at head_dim 128.  Longer rows (512 K keys; 256 K at head_dim 256) go through every tile.
 constexpr int kPpSkipTiles = 4096;
 
+// 8-bit codes: above every sum of a score and a logarithm of V's scale, where twice it stands for a scale that cannot be used.
+constexpr float kQ8LogMost = 1.5e38f;
+
 template <int HD, bool Q8 = false>
 struct PpShape {
     static constexpr int TILES = HD == 256 ? 1 : 2;       // row tiles of 128
@@ -365,14 +368,14 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
                                     docs_s[(jj % S::DOCS) * KT + r] = j < hi ? docs[j] : 0;
                                 }
                             if (pt < S::GROUPS) {
-                                // Scales that cannot be used: weights above all others', and a sum that is NaN.  The factor on
-                                // scores stays a number: masked ones must stay -inf.
+                                // Scales that cannot be used: scores above all others', by which their rows' sums become NaN.
+                                // The factor on scores stays a number: masked ones must stay -inf.
                                 const Group &x = groups[(jj & 1) * S::GROUPS + pt];
                                 const Q8Scale z = q8_scale(x.k, x.v);
                                 const bool good = z.k == z.k;
                                 float *to = scales_s + (jj % S::DOCS) * 3 * S::GROUPS + pt;
                                 to[0] = good ? z.k : 0.0f;
-                                to[S::GROUPS] = good ? z.v_log2 : 3e38f;
+                                to[S::GROUPS] = good ? z.v_log2 : 2.0f * kQ8LogMost;
                                 to[2 * S::GROUPS] = good ? z.v_inv : __int_as_float(0x7fffffff);
                             }
                         }
@@ -899,7 +902,10 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
             // weights times 2^10: small ones keep their f16 bits, and the sum carries the same factor
             const float base = m == -INFINITY ? 0.0f : 10.0f - m;
             float2 sum = make_float2(0.0f, 0.0f);
-            float weight = 0.0f;  // 8-bit codes: the columns' sums, each times its 1 / v
+            // 8-bit codes: the columns' sums, each times its 1 / v.  NaN where the row sees a scale that cannot be used, whatever
+            // the distance bias leaves of the weights there (asked of every 16 columns: 8-bit 4096 tokens with a bias,
+            // 32/4 heads of 128, 311 -> 323 us; so 311)
+            float weight = Q8 && top > kQ8LogMost ? __int_as_float(0x7fffffff) : 0.0f;
             {
                 float2 fs2 = make_float2(fs, fs), base2 = make_float2(base, base);
                 uint32_t v[2][16];

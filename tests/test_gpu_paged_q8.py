@@ -520,6 +520,35 @@ def test_scales_that_are_no_numbers_are_seen(pkg, ctx, which, value):
     assert np.isfinite(got[:32]).all() and np.isfinite(got[:, :4]).all() and np.isnan(got[32:, 4:]).all()
 
 
+@pytest.mark.parametrize("heads,kv,hd", [(4, 2, 64), (8, 2, 128), (4, 2, 256)])
+@pytest.mark.parametrize("seqs,rows", [(1, 100), (90, 100), (3, 3)])
+@pytest.mark.parametrize("cap,slope", [(0.0, 0.7), (20.0, 0.7), (0.0, 3e4), (0.0, 0.0), (20.0, 0.0)])
+def test_scales_that_are_no_numbers_are_seen_from_far(pkg, ctx, heads, kv, hd, seqs, rows, cap, slope):
+    """A distance bias that leaves nothing of a far block's weights leaves the NaN of its scale; prompts that share their keys
+    among CTAs (one sequence), that do not (many), and few rows; a row whose window has passed the block is as without it."""
+    rng = np.random.default_rng(33)
+    n, group = 700, heads // kv
+    c = Cache(pkg, rng, [n], kv, hd, 16, 16)
+    c.hs[0][c.table[0, 2], 1] = np.nan        # positions 32 .. 47 of KV head 1
+    c.hs[1][c.table[0, 20], 0] = np.inf       # positions 320 .. 335 of KV head 0
+    c.upload(pkg)
+    table = c.dtable.repeat(seqs, 1).contiguous()
+    q, out = torch.randn(seqs * rows, heads, hd, device="cuda"), torch.zeros(seqs * rows, heads, hd, device="cuda")
+    cu, ln, sl = i32(np.arange(seqs + 1) * rows), i32([n] * seqs), torch.full((heads,), slope, device="cuda")
+    for window in (0, 330, 400):
+        cfg = pkg.PagedAttnCfg(n_heads=heads, causal=1, window=window, scale=1 / math.sqrt(hd), softcap=cap, slopes=sl.data_ptr())
+        out.fill_(7.0)
+        torch.cuda.synchronize()
+        ctx.paged_q8_attn_prompt(cfg, c.desc, q, seqs, cu, seqs * rows, rows, table, ln, n, out)
+        ctx.sync()
+        got = out.cpu().numpy().reshape(seqs, rows, heads, hd)
+        lo = np.maximum(0, np.arange(n - rows, n) - window + 1) if window else np.zeros(rows, np.int64)
+        for h, end in ((0, 336), (1, 48)):
+            part = got[:, :, h * group:(h + 1) * group]
+            assert np.isnan(part[:, lo < end]).all(), (window, h)
+            assert np.isfinite(part[:, lo >= end]).all(), (window, h)
+
+
 def test_decode_extreme_queries(pkg, ctx):
     """Query rows of very small and very large magnitude keep their relative precision."""
     rng = np.random.default_rng(8)
