@@ -729,7 +729,8 @@ typedef struct lt_paged_state {
  *
  * All or nothing: a plan that wants more pages than there are is reported by
  * lt_sync as LT_ENOMEM, one with keep > lens, more positions than a table row (or
- * 2^30) holds, more tokens than total_q, or a page id or stack past n_pages, as
+ * 2^30) holds, more tokens than total_q, or a stack or page id past n_pages (of a
+ * page that goes, comes, or is filled further; no other is looked at), as
  * LT_EINVAL; the state then stays as it was and dev_cu_q is all 0: the ops that
  * follow find no new rows. */
 lt_status lt_paged_plan(lt_ctx *ctx, const lt_paged_state *state, const uint32_t *dev_keep, const uint32_t *dev_new,

@@ -15,7 +15,8 @@
 // Bound: latency (dependent loads and block barriers).  One B200: a token for each of 64
 // sequences 4.9 us; prompts of 512 (325661 tokens, 10426 pages back and as many taken)
 // 10.4 us (in three launches, threads with pages and tokens to place alike, 15.9).  One CTA scans the sequences, a thread to each as far as they go round, and
-// refuses what cannot be done before anything is changed.  Few tokens: the same CTA moves
+// refuses what cannot be done before anything is changed: page numbers past the pool, too, wherever the plan makes a table
+// entry or a slot of them.  Few tokens: the same CTA moves
 // the pages and places the tokens.  Many: all SMs, in two launches (one CTA alone for the
 // pages of those prompts: 22 us, by its instructions): every CTA scans the sequences
 // for itself and looks at its share of the pages that go, then everything is written.
@@ -59,6 +60,25 @@ LT_DEVINL uint32_t taken(const PagedPlanArgs &a, const PlanSeqs &q, const uint32
     return ids && k < q.n_gone ? ids[k] : a.free[q.top - 1 - k];
 }
 
+// Whether one of the pages that go, or that come from the stack as it was, has a number past the pool; thread `at` of
+// `step` looks at its share.  gone, stay: of each sequence.  ids: where the numbers of those that go are left.
+LT_DEVINL bool plan_look(const PagedPlanArgs &a, const uint32_t *gone, const uint32_t *stay, uint32_t top, uint32_t n_gone, uint32_t n_take,
+                         uint32_t *ids, uint32_t at, uint32_t step) {
+    bool off = false;
+    const uint32_t more = n_take > n_gone ? n_take - n_gone : 0, n = max(n_gone, more);
+    for (uint32_t i = at; i < n; i += step) {
+        const uint32_t comes = i < more ? a.free[top - 1 - n_gone - i] : 0;  // on its way during the search
+        if (i < n_gone) {
+            const uint32_t s = owner_of(gone, a.n_seq, i);
+            const uint32_t id = a.table[(uint64_t)s * a.max_pages + stay[s] + (i - gone[s])];
+            if (ids) ids[i] = id;
+            off |= id >= a.n_pages;
+        }
+        off |= comes >= a.n_pages;
+    }
+    return off;
+}
+
 // Table entries and token rows, thread `at` of `step`; entries from the middle thread on, so that few threads have
 // both.  Nothing that is read here is written here.
 LT_DEVINL void plan_fill(const PagedPlanArgs &a, const PlanSeqs &q, const uint32_t *ids, uint32_t at, uint32_t step) {
@@ -89,7 +109,7 @@ constexpr uint32_t kPlanInShared = 2048;  // sequences
 // ALONE: the one CTA does everything.  Else what was found goes to scratch, by CTA 0, and nothing to the caller's; all CTAs
 // look at the pages that go where the sequences are in shared memory.
 template <bool ALONE>
-__global__ void __launch_bounds__(kPlanThreads) k_paged_plan(const __grid_constant__ PagedPlanArgs a) {
+__global__ void __launch_bounds__(kPlanThreads, 1) k_paged_plan(const __grid_constant__ PagedPlanArgs a) {
     __shared__ PlanSum s_warp[kPlanWarps], s_all;
     __shared__ int s_bad, s_bad_page;
     __shared__ uint32_t s_cu[kPlanInShared], s_take[kPlanInShared], s_gone[kPlanInShared], s_keep[kPlanInShared], s_stay[kPlanInShared];
@@ -106,7 +126,8 @@ __global__ void __launch_bounds__(kPlanThreads) k_paged_plan(const __grid_consta
     const uint32_t sa = min(a.n_seq, tid * per), sb = min(a.n_seq, sa + per);
     const uint64_t cap = min((uint64_t)a.max_pages * a.page, (uint64_t)kPlanMaxLen);
     PlanSum mine = {0, 0, 0};
-    bool bad = false;
+    bool bad = false, off = false;  // off: a page number past the pool
+    uint32_t held = 0;              // one that is on its way, looked at only when the sums are scanned
     for (uint32_t s = sa; s < sb; s++) {  // within this thread for now, in what belongs to it alone
         const uint32_t len = a.lens[s], keep = a.keep ? a.keep[s] : len, add = a.add[s];
         cu[s] = (uint32_t)mine.tokens;
@@ -119,6 +140,10 @@ __global__ void __launch_bounds__(kPlanThreads) k_paged_plan(const __grid_consta
         }
         const uint32_t stay = pages_for(a, keep);
         stays[s] = stay;
+        if (add && stay * a.page != keep && (ALONE || !in_shared || s % gridDim.x == blockIdx.x)) {
+            off |= held >= a.n_pages;
+            held = a.table[(uint64_t)s * a.max_pages + stay - 1];  // the page that the coming tokens go on with
+        }
         mine.tokens += add;
         mine.gone += pages_for(a, len) - stay;
         mine.take += pages_for(a, keep + add) - stay;
@@ -152,6 +177,8 @@ __global__ void __launch_bounds__(kPlanThreads) k_paged_plan(const __grid_consta
             }
         }
     }
+    off |= held >= a.n_pages;
+    if (ALONE && off) s_bad_page = DEV_ERR_BAD_INDEX;
     __syncthreads();
     const PlanSum all = s_all;
     const uint32_t top = n_free + (uint32_t)all.gone;  // where it counts, nothing is bad
@@ -171,37 +198,31 @@ __global__ void __launch_bounds__(kPlanThreads) k_paged_plan(const __grid_consta
             a.keeps[s] = keeps[s];
             a.stay[s] = stays[s];
         }
-        if (blockIdx.x == 0 && tid == 0) *a.head = {top, (uint32_t)all.gone, (uint32_t)all.take, (uint32_t)all.tokens, s_bad, n_free};
+        int wrong = s_bad;
+        if (!in_shared && __syncthreads_or(off) && ok) wrong = DEV_ERR_BAD_INDEX;
+        if (blockIdx.x == 0 && tid == 0) *a.head = {top, (uint32_t)all.gone, (uint32_t)all.take, (uint32_t)all.tokens, wrong, n_free};
         if (!in_shared) return;
         __syncthreads();
-        bool off = false;
-        for (uint32_t r = blockIdx.x * kPlanThreads + tid; ok && r < all.gone; r += gridDim.x * kPlanThreads) {
-            const uint32_t s = owner_of(gone, a.n_seq, r);
-            const uint32_t id = a.table[(uint64_t)s * a.max_pages + stays[s] + (r - gone[s])];
-            a.ids[r] = id;
-            off |= id >= a.n_pages;
-        }
+        if (ok)
+            off |= plan_look(a, gone, stays, top, (uint32_t)all.gone, (uint32_t)all.take, a.ids, blockIdx.x * kPlanThreads + tid,
+                             gridDim.x * kPlanThreads);
         off = __syncthreads_or(off);
         if (tid == 0) a.flags[blockIdx.x] = off;
         return;
     }
-    if (ok && all.gone) {
-        // the pages that go, one to a thread: first their numbers are looked at, then they move
-        __syncthreads();
-        for (int pass = 0; pass < 2 && ok; pass++) {
+    ok = ok && s_bad_page == DEV_ERR_NONE;  // written before the barrier above only
+    if (ok && (all.gone || all.take)) {
+        // the pages that go and those from the stack, one to a thread: their numbers are looked at before any moves
+        if (all.gone) __syncthreads();
+        ok = !__syncthreads_or(plan_look(a, gone, stays, top, (uint32_t)all.gone, (uint32_t)all.take, nullptr, tid, kPlanThreads));
+        if (ok && all.gone) {
             for (uint32_t r = tid; r < all.gone; r += kPlanThreads) {
                 const uint32_t s = owner_of(gone, a.n_seq, r);
                 uint32_t *entry = a.table + (uint64_t)s * a.max_pages + stays[s] + (r - gone[s]);
-                const uint32_t id = *entry;
-                if (pass == 0) {
-                    if (id >= a.n_pages) s_bad_page = DEV_ERR_BAD_INDEX;
-                } else {
-                    a.free[top - 1 - r] = id;
-                    *entry = kPlanNoPage;
-                }
+                a.free[top - 1 - r] = *entry;
+                *entry = kPlanNoPage;
             }
-            __syncthreads();  // s_bad_page is written in the first pass only, and read after it
-            ok = s_bad_page == DEV_ERR_NONE;
+            __syncthreads();
         }
     }
     for (uint32_t s = sa; s < sb; s++) {
@@ -213,7 +234,7 @@ __global__ void __launch_bounds__(kPlanThreads) k_paged_plan(const __grid_consta
         if (ok)
             *a.n_free = (uint32_t)(top - all.take);
         else
-            atomicExch(a.err, s_bad != DEV_ERR_NONE ? s_bad : s_bad_page);
+            atomicExch(a.err, s_bad != DEV_ERR_NONE ? s_bad : DEV_ERR_BAD_INDEX);
     }
     if (!ok) return;
     __syncthreads();
@@ -223,17 +244,14 @@ __global__ void __launch_bounds__(kPlanThreads) k_paged_plan(const __grid_consta
 
 constexpr int kPlanFillThreads = 256;
 
-// The pages that go, looked at: of more sequences than shared memory holds.
+// The pages that go and those from the stack, looked at: of more sequences than shared memory holds.
 __global__ void __launch_bounds__(kPlanFillThreads) k_paged_plan_gone(const __grid_constant__ PagedPlanArgs a) {
     pdl_launch_dependents();
     pdl_wait();
-    const uint32_t n = a.head->bad == DEV_ERR_NONE ? a.head->gone : 0;
-    for (uint32_t r = blockIdx.x * kPlanFillThreads + threadIdx.x; r < n; r += gridDim.x * kPlanFillThreads) {
-        const uint32_t s = owner_of(a.gone, a.n_seq, r);
-        const uint32_t id = a.table[(uint64_t)s * a.max_pages + a.stay[s] + (r - a.gone[s])];
-        a.ids[r] = id;
-        if (id >= a.n_pages) a.head->bad_page = DEV_ERR_BAD_INDEX;
-    }
+    const PlanHead h = *a.head;
+    if (h.bad != DEV_ERR_NONE) return;
+    const uint32_t at = blockIdx.x * kPlanFillThreads + threadIdx.x, step = gridDim.x * kPlanFillThreads;
+    if (plan_look(a, a.gone, a.stay, h.top, h.gone, h.take, a.ids, at, step)) a.head->bad_page = DEV_ERR_BAD_INDEX;
 }
 
 // Everything that is written.  Pages that go are read from ids: their table entries may be written here.

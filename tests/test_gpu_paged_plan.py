@@ -240,3 +240,50 @@ def test_most_sequences(pkg, ctx, room):
             assert got[:len(w)].tolist() == list(w)
             assert (got[len(w):] == MARK).all()
         b.same()
+
+
+@pytest.mark.parametrize("room", [0, 5000])
+@pytest.mark.parametrize("n_seq", [3, 2100])
+@pytest.mark.parametrize("what", ["stack", "stack's deepest", "kept page", "kept page behind others that go"])
+def test_page_ids_that_a_plan_would_use(pkg, ctx, what, n_seq, room):
+    """A page number past the pool is refused wherever the plan would make a table entry or a slot of it: among the pages to
+    be taken, and on the page that a sequence goes on with.  Where the plan has no use for it, it is nobody's business."""
+    b = Batch(pkg, np.random.default_rng(13), [5, 64, 0] + [9] * (n_seq - 3), 16, n_seq + 30, 12)
+    keep, new = [5, 64, 0] + [9] * (n_seq - 3), [20, 33, 1] + [1] * (n_seq - 3)   # takes 1 + 3 + 1 pages
+    n = len(b.free)
+    if what == "stack":
+        at = b.dfree[n - 2:n - 1]
+    elif what == "stack's deepest":
+        at = b.dfree[n - 5:n - 4]
+    elif what == "kept page":
+        at = b.dtable[n_seq - 1 if n_seq > 3 else 0, 0:1]
+    else:
+        keep[1] = 33                                           # a page goes, the one before it holds one position of 16
+        at = b.dtable[1, 2:3]
+    good = at.clone()
+    at.fill_(b.n_pages)
+    torch.cuda.synchronize()
+    before = [host(t).copy() for t in (b.dlens, b.dtable, b.dfree, b.dn)]
+    total = sum(new) + room
+    cu, seq, pos, slot = (torch.full((m,), 7, dtype=torch.int32, device="cuda") for m in (n_seq + 1, total, total, total))
+    dkeep, dnew = dev(keep), dev(new)
+    torch.cuda.synchronize()
+    ctx.paged_plan(b.state, dkeep, dnew, total, cu, seq, pos, slot)
+    with pytest.raises(pkg.LtError) as e:
+        ctx.sync()
+    assert e.value.status == 1
+    assert not host(cu).any()
+    assert all((host(t) == 7).all() for t in (seq, pos, slot))
+    for x, t in zip(before, (b.dlens, b.dtable, b.dfree, b.dn)):
+        assert (x == host(t)).all()
+    # the same page number where this plan does not look
+    at.copy_(good)
+    b.dfree[0] = b.n_pages                                     # deeper in the stack than what is taken
+    b.dtable[1, 0] = b.n_pages                                 # a page that stays and gets nothing
+    torch.cuda.synchronize()
+    got = b.run(ctx, keep, new, total)
+    b.free[0] = b.n_pages
+    b.pages[1][0] = b.n_pages
+    for g, w in zip(got, b.want(keep, new)):
+        assert g[:len(w)].tolist() == list(w)
+    b.same()
