@@ -409,7 +409,8 @@ lt_status lt_paged_plan(lt_ctx *ctx, const lt_paged_state *state, const uint32_t
     if (state->n_seq > 65535 || total_q > kMaxLen)
         return st_of(ctx_fail(ctx, LT_EINVAL, "lt_paged_plan: %u sequences (at most 65535), %u tokens (at most %u)",
                               state->n_seq, total_q, kMaxLen));
-    if (state->n_seq == 0) return LT_OK;
+    if (state->n_seq == 0)  // the sums of nothing: one 0
+        return st_of(lt::ctx_launched(ctx, cudaMemsetAsync(dev_cu_q, 0, sizeof(uint32_t), lt::ctx_stream(ctx)), "page plan"));
     lt::PagedPlanArgs a = {};
     a.n_seq = state->n_seq;
     a.page = state->page_size;

@@ -287,3 +287,23 @@ def test_page_ids_that_a_plan_would_use(pkg, ctx, what, n_seq, room):
     for g, w in zip(got, b.want(keep, new)):
         assert g[:len(w)].tolist() == list(w)
     b.same()
+
+
+def test_no_sequences(pkg, ctx):
+    """The running sums of nothing: one 0, recorded or not."""
+    b = Batch(pkg, np.random.default_rng(14), [5], 16, 10, 4)
+    b.state.n_seq = 0
+    cu, new = torch.full((2,), 7, dtype=torch.int32, device="cuda"), dev([1])
+    torch.cuda.synchronize()
+    ctx.paged_plan(b.state, None, new, 4, cu)
+    ctx.sync()
+    assert host(cu).tolist() == [0, 7]
+    cu.fill_(7)
+    torch.cuda.synchronize()
+    ctx.capture_begin()
+    ctx.paged_plan(b.state, None, new, 4, cu)
+    g = ctx.capture_end()
+    g.launch()
+    ctx.sync()
+    assert host(cu).tolist() == [0, 7]
+    b.same()
