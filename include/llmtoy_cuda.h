@@ -665,8 +665,9 @@ typedef struct lt_paged_q8 {
  *
  * A block whose first slot is written starts afresh, on scale = max |x| / 127.  In
  * others the codes before the new rows stay; where the new rows need a larger scale they
- * are rounded to it again.  code = x / scale to nearest.  A value that is not finite or
- * exceeds 2^60 makes its block's scale NaN, until the block starts afresh.
+ * are rounded to it again.  code = x / scale to nearest (within 2e-5 of the middle
+ * between two codes, either).  A value that is not finite or exceeds 2^60 makes its
+ * block's scale NaN, until the block starts afresh.
  * Pages written to must not be shared.  Repeating a call changes nothing. */
 lt_status lt_paged_q8_append(lt_ctx *ctx, const lt_attn_cfg *cfg, const lt_paged_q8 *kv, const float *dev_qkv,
                              uint32_t n_seq, const uint32_t *dev_cu_q, uint32_t total_q, uint32_t max_q,

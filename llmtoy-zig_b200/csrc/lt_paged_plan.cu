@@ -12,14 +12,15 @@
 // the page returned from entry j lies at n' - 1 - (G(s) + j - stay), and entry j
 // takes the page at n' - 1 - (T(s) + j - stay): every page and token finds its place by itself.
 //
-// Bound: latency (dependent loads and block barriers).  One B200: a token for each of 64
-// sequences 4.9 us; prompts of 512 (325661 tokens, 10426 pages back and as many taken)
-// 10.4 us (in three launches, threads with pages and tokens to place alike, 15.9).  One CTA scans the sequences, a thread to each as far as they go round, and
-// refuses what cannot be done before anything is changed: page numbers past the pool, too, wherever the plan makes a table
-// entry or a slot of them.  Few tokens: the same CTA moves
-// the pages and places the tokens.  Many: all SMs, in two launches (one CTA alone for the
-// pages of those prompts: 22 us, by its instructions): every CTA scans the sequences
-// for itself and looks at its share of the pages that go, then everything is written.
+// Bound: latency (dependent loads and block barriers).  One B200, calls of a recorded graph: a
+// token for each of 64 sequences 4.5 us; prompts of 512 (325661 tokens, 10426 pages back and as
+// many taken) 10.6 us (in three launches, threads with pages and tokens to place alike, 15.9).
+// One CTA scans the sequences, a thread to each as far as they go round, and refuses what
+// cannot be done before anything is changed: page numbers past the pool, too, wherever the plan
+// makes a table entry or a slot of them.  Few tokens: the same CTA moves the pages and places
+// the tokens.  Many: all SMs, in two launches (one CTA alone for the pages of those prompts:
+// 22 us, by its instructions): every CTA scans the sequences for itself and looks at its share
+// of the pages that go or come, then everything is written.
 // Pages and tokens are dealt to threads one by one, wherever their sequences begin.  Up to
 // 2048 sequences are kept in shared memory between the steps; more are scanned by one CTA,
 // and the pages looked at in a launch of their own.
@@ -107,7 +108,8 @@ struct PlanSum {
 constexpr uint32_t kPlanInShared = 2048;  // sequences
 
 // ALONE: the one CTA does everything.  Else what was found goes to scratch, by CTA 0, and nothing to the caller's; all CTAs
-// look at the pages that go where the sequences are in shared memory.
+// look at the pages that go or come where the sequences are in shared memory.  One CTA to an SM, said to the compiler: without it
+// it keeps to 32 registers and spills (prompts of 512: 12.0 us instead of 11.4, both by events around calls from the host).
 template <bool ALONE>
 __global__ void __launch_bounds__(kPlanThreads, 1) k_paged_plan(const __grid_constant__ PagedPlanArgs a) {
     __shared__ PlanSum s_warp[kPlanWarps], s_all;

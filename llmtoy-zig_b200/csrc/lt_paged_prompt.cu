@@ -41,7 +41,8 @@
 // 8-bit codes, the same cases: 8192 tokens 0.95 to 0.98 ms, the follow-up 20.4 us, the packed documents 241 us,
 // 4096 tokens of 16/8 heads of 256 0.31 ms (f16 0.35): half the bytes, and the copying warps' conversion instead.  With
 // three copying warps 1.27 ms and 351 us; with seven, whose registers the softmax warps gave, 1.00 and 299; with each
-// head_dim's own split of the registers (PpShape) what stands above.
+// head_dim's own split of the registers (PpShape) what stands above.  Spills at head_dim 256: 152 bytes with cap or bias, 140
+// without; at 128 36 and 8.
 #include <cuda.h>  // CUtensorMap (encoded through the runtime's driver entry point)
 
 #include "lt_paged_q8.cuh"

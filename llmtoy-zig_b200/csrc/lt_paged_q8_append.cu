@@ -4,17 +4,21 @@
 // Per head vector what lt_paged_append.cu does (norm, rotation); then, for K and V of
 // one KV head and one block of slots that the call writes to,
 //   top = max |x| over the new rows' elements,  scale = max(top / 127, scale of the codes that stay),
-//   code = x / scale to nearest,  a code that stays: code * (old scale / scale) to nearest.
+//   code = x / scale to nearest,  a code that stays: code * (old scale / scale) to nearest,
+// where the quotient is a product with a rounded inverse or quotient, off by 127 * 2^-23 = 1.5e-5 at most: nearer than
+// that to the middle between two codes it may go to either.
 // A maximum does not depend on order, so neither do scales and codes.
 //
 // Angles: p / theta^(2i/hd) in units of pi, reduced to [-1, 1] in f64, before the f32
 // sine and cosine: an angle in f32 alone is off by up to half a unit in its last place, 2e-4 at
 // position 4000.
 //
-// Bound: memory (each value is read once, and written once or as a quarter of its size).  One B200: 7003
-// prompt tokens (16/8 heads of 256, normalised values) 74.9 us, 5.0 TB/s, with a warp per row and no
-// teams 214; 8192 tokens of 32/4 heads of 128 62 us, 5.0 TB/s (blocks of 128: 73); one token of each
-// of 64 sequences 5.2 us, where launch and the lengths' scan count.  A CTA takes one block of one
+// Bound: memory (each value is read once, and written once or as a quarter of its size).  One B200, calls by
+// themselves in a row (three sets of inputs larger than L2): 7003 prompt tokens (16/8 heads of 256,
+// normalised values) 75.2 us, 5.0 TB/s, with a warp per row and no teams 214; 8192 tokens of 32/4 heads
+// of 128 62 us, 5.0 TB/s (blocks of 128: 73); one token of each of 64 sequences 3.8 us from a graph and 5.1
+// launched by the host, where launch and the lengths' scan count.  Spills: 100 bytes at head_dim 256 with
+// blocks of 128 (255 registers), 84 at 128, 28 at 256 with smaller blocks.  A CTA takes one block of one
 // sequence; teams of its warps go through the head vectors, each warp with CHUNK of the block's
 // tokens in registers from the load to the codes, the team's maximum through shared
 // memory.  What costs instructions otherwise is shared among tokens: the sums of squares
