@@ -417,7 +417,8 @@ void lt_free(lt_ctx *ctx) {
 lt_status lt_set_stream(lt_ctx *ctx, void *cuda_stream) {
     lt_status st = enter(ctx);
     if (st != LT_OK) return st;
-    ctx->stream = cuda_stream ? (cudaStream_t)cuda_stream : ctx->own;
+    // a recording on the stream apart goes on there, and the context changes streams when it ends
+    (ctx->cap_user ? ctx->cap_user : ctx->stream) = cuda_stream ? (cudaStream_t)cuda_stream : ctx->own;
     return LT_OK;
 }
 

@@ -135,6 +135,38 @@ def test_torch_works_on_while_a_context_records(pkg, default):
         g.free()
 
 
+def test_streams_changed_while_a_context_records(pkg):
+    """The recording goes on and ends; the context is on the new stream then, also where that is the one it was on."""
+    op = Append(pkg, n=200)
+    with pkg.Context(0) as ctx:
+        op.fill(0)
+        op.call(ctx)
+        ctx.sync()
+        want = op.read()
+        torch.cuda.synchronize()
+        for stream in (None, torch.cuda.current_stream(), None, torch.cuda.Stream(), None):
+            op.q.zero_()
+            own = pkg.Context(0)
+            try:
+                own.capture_begin()
+                own.set_stream(stream)
+                op.call(own)
+                g = own.capture_end()
+                torch.cuda.synchronize()
+                assert not op.q.any()
+                g.launch()
+                own.sync()
+                assert torch.equal(op.q, want[0])
+                g.free()
+                op.q.zero_()
+                torch.cuda.synchronize()
+                op.call(own)
+                own.sync()
+                assert torch.equal(op.q, want[0])
+            finally:
+                own.close()
+
+
 def test_a_context_closed_while_it_records(pkg):
     """An open recording ends with its context; the next context is none the worse."""
     op = Append(pkg, n=200)
