@@ -54,8 +54,10 @@ namespace lt {
 // the ring at head_dim 128.  Longer rows (512 K keys; 256 K at head_dim 256) go through every tile.
 constexpr int kPpSkipTiles = 4096;
 
-// 8-bit codes: above every sum of a score and a logarithm of V's scale, where twice it stands for a scale that cannot be used.
-constexpr float kQ8LogMost = 1.5e38f;
+// 8-bit codes: what stands for the logarithm of V's scale where a scale cannot be used.  With a score and its distance bias it is
+// still above kQ8NoScore, which the sums of numbers stay below (scores near f32's largest number, 3.4e38, aside); it is finite, so
+// that a masked score, -inf, stays that.
+constexpr float kQ8NoScale = 3.3e38f, kQ8NoScore = 3.2e38f;
 
 template <int HD, bool Q8 = false>
 struct PpShape {
@@ -376,7 +378,7 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
                                 const bool good = z.k == z.k;
                                 float *to = scales_s + (jj % S::DOCS) * 3 * S::GROUPS + pt;
                                 to[0] = good ? z.k : 0.0f;
-                                to[S::GROUPS] = good ? z.v_log2 : 2.0f * kQ8LogMost;
+                                to[S::GROUPS] = good ? z.v_log2 : kQ8NoScale;
                                 to[2 * S::GROUPS] = good ? z.v_inv : __int_as_float(0x7fffffff);
                             }
                         }
@@ -906,7 +908,7 @@ __global__ void __launch_bounds__(kPpThreads, 1) k_paged_prompt(const __grid_con
             // 8-bit codes: the columns' sums, each times its 1 / v.  NaN where the row sees a scale that cannot be used, whatever
             // the distance bias leaves of the weights there (asked of every 16 columns: 8-bit 4096 tokens with a bias,
             // 32/4 heads of 128, 311 -> 323 us; so 311)
-            float weight = Q8 && top > kQ8LogMost ? __int_as_float(0x7fffffff) : 0.0f;
+            float weight = Q8 && top > kQ8NoScore ? __int_as_float(0x7fffffff) : 0.0f;
             {
                 float2 fs2 = make_float2(fs, fs), base2 = make_float2(base, base);
                 uint32_t v[2][16];

@@ -549,6 +549,31 @@ def test_scales_that_are_no_numbers_are_seen_from_far(pkg, ctx, heads, kv, hd, s
             assert np.isfinite(part[:, lo >= end]).all(), (window, h)
 
 
+@pytest.mark.parametrize("heads,kv,hd", [(4, 2, 64), (8, 2, 128), (4, 2, 256)])
+@pytest.mark.parametrize("alibi", [False, True])
+def test_prompt_scores_near_the_largest_numbers(pkg, ctx, heads, kv, hd, alibi):
+    """A score of 2e38 in units of log2 is a number like others: its value is the row.  All keys but that one are zeros, and its
+    product is a power of two times the factor, so that it is exact."""
+    rng = np.random.default_rng(34)
+    n = 300
+    c = Cache(pkg, rng, [n], kv, hd, 16, 16)
+    for s in (c.hs[0], c.hc[0]):
+        s[c.table[0, :-(-n // 16)]] = 0
+    p = c.table[0, 5]                          # position 80: a key of ones
+    c.hs[0][p], c.hc[0][p, :, 0] = 1.0, 1
+    c.upload(pkg)
+    q, sl = torch.ones(n, heads, hd, device="cuda"), torch.full((heads,), 1e-3, device="cuda")
+    cfg = pkg.PagedAttnCfg(n_heads=heads, causal=1, scale=2e38 / 1.4426950408889634 / hd, slopes=sl.data_ptr() if alibi else None)
+    out, cu, ln = torch.zeros(n, heads, hd, device="cuda"), i32([0, n]), i32([n])
+    torch.cuda.synchronize()
+    ctx.paged_q8_attn_prompt(cfg, c.desc, q, 1, cu, n, n, c.dtable, ln, n, out)
+    ctx.sync()
+    got, V = out.cpu().numpy(), c.seq(0)[1]
+    want = np.broadcast_to(V[80].repeat(heads // kv, 0), (n - 80, heads, hd))
+    assert np.isfinite(got).all()
+    assert rel(got[80:], want) < ATTN_BAR
+
+
 def test_decode_extreme_queries(pkg, ctx):
     """Query rows of very small and very large magnitude keep their relative precision."""
     rng = np.random.default_rng(8)
